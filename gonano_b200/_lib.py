@@ -49,6 +49,37 @@ class GnAttentionParams(C.Structure):
     ]
 
 
+class GnView(C.Structure):
+    _fields_ = [("data", vp), ("batch_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
+class GnSinkParams(C.Structure):
+    _fields_ = [
+        ("query", GnView), ("key", GnView), ("value", GnView),
+        ("batch", C.c_int32), ("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("seq", C.c_int32), ("head_dim", C.c_int32),
+        ("sinks", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("lengths", vp),
+    ]
+
+
+class GnPagedParams(C.Structure):
+    _fields_ = [
+        ("query", GnView), ("new_key", GnView), ("new_value", GnView), ("key_pages", vp), ("value_pages", vp), ("page_table", vp),
+        ("query_starts", vp), ("context_lens", vp), ("mass", vp), ("mass_out", vp), ("rows", C.c_int32), ("tokens", C.c_int32),
+        ("max_query", C.c_int32), ("max_context", C.c_int32), ("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32),
+        ("page_size", C.c_int32), ("pages", C.c_int32), ("table_width", C.c_int32), ("sinks", C.c_int32), ("window", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class GnEvictParams(C.Structure):
+    _fields_ = [
+        ("key_pages", vp), ("value_pages", vp), ("mass", vp), ("page_table", vp), ("new_table", vp), ("context_lens", vp),
+        ("rows", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
+        ("table_width", C.c_int32), ("new_width", C.c_int32), ("mass_stride", C.c_int32), ("max_context", C.c_int32),
+        ("budget", C.c_int32), ("sinks", C.c_int32), ("recent", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/gonano_cuda.h declares.
 I, L, F, U32 = C.c_int, C.c_int64, C.c_float, C.c_uint32
 SIGNATURES = {
@@ -89,6 +120,13 @@ SIGNATURES = {
     "gn_attention_forward_split": (I, [C.POINTER(GnAttentionParams), I, I, vp, vp, vp]),
     "gn_attention_combine": (I, [vp, vp, vp, I, I, I, vp, vp]),
     "gn_attention_backward": (I, [C.POINTER(GnAttentionParams), vp, vp, vp, vp, vp, vp, vp]),
+    "gn_attention_sink_workspace": (I, [C.POINTER(GnSinkParams), I, C.POINTER(L)]),
+    "gn_attention_sink_forward": (I, [C.POINTER(GnSinkParams), C.POINTER(GnView), vp, vp, L, vp]),
+    "gn_attention_sink_backward": (I, [C.POINTER(GnSinkParams), C.POINTER(GnView), C.POINTER(GnView), vp, C.POINTER(GnView), C.POINTER(GnView),
+                                       C.POINTER(GnView), I, vp, L, vp]),
+    "gn_attention_paged_workspace": (I, [C.POINTER(GnPagedParams), C.POINTER(L)]),
+    "gn_attention_paged": (I, [C.POINTER(GnPagedParams), C.POINTER(GnView), vp, vp, L, vp]),
+    "gn_cache_evict": (I, [C.POINTER(GnEvictParams), vp, vp, vp, vp]),
     "gn_sample_next_token": (I, [vp, I, I, vp, vp, I, U32, F, I, vp]),
     "gn_group_advantage": (I, [vp, I, I, I, vp]),
     "gn_adamw_step": (I, [vp, vp, vp, vp, L, I, F, F, F, F, F]),

@@ -1,0 +1,469 @@
+// Streaming attention: C entry points and the float32 kernels (a warp per row of the result).
+#include <algorithm>
+
+#include "streaming.cuh"
+
+namespace gn {
+
+namespace {
+
+constexpr int kE = 4;   // channels of a lane: head_dim <= 128
+
+template <bool PAGED>
+__device__ __forceinline__ void load_lane(const float* p, int D, float (&x)[kE]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) x[e] = (p && lane + 32 * e < D) ? p[lane + 32 * e] : 0.0f;
+}
+__device__ __forceinline__ float dot_lane(const float (&a)[kE], const float (&b)[kE]) {
+  float d = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) d = fmaf(a[e], b[e], d);
+  return warp_sum(d);
+}
+template <bool PAGED>
+__device__ __forceinline__ const float* key_ptr(const StreamRows& s, bool value, int r, int hk, int j) {
+  const int64_t off = key_offset<PAGED>(s, value ? s.v : s.k, r, hk, j);
+  if (off < 0 && PAGED) return nullptr;
+  return (PAGED ? (value ? s.pages_v : s.pages_k) : (value ? s.v.data : s.k.data)) + off;
+}
+
+// A warp per (row, query head, token): online softmax over the keys the query sees.
+template <bool PAGED>
+__global__ void __launch_bounds__(128) stream_forward_kernel(StreamRows s, gn_view out, float* __restrict__ lse) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * 4 + warp, h = blockIdx.y, r = blockIdx.z;
+  const RowSpan sp = row_span<PAGED>(s, r);
+  if (t >= (PAGED ? sp.q_len : s.seq)) return;
+  const int token = sp.q_begin + t;
+  float o[kE] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
+  if (t < sp.q_len) {
+    const int pos = PAGED ? sp.ctx - sp.q_len + t : t;
+    float q[kE];
+    load_lane<PAGED>(s.q.data + token_offset<PAGED>(s.q, r, h, token), s.D, q);
+    const Seen see = seen_by(s, pos);
+    for (int j = see.sink_end > 0 ? 0 : see.begin; j <= pos; j = (j + 1 == see.sink_end) ? max(see.begin, j + 1) : j + 1) {
+      const float* kp = key_ptr<PAGED>(s, false, r, h / s.G, j);
+      if (PAGED && !kp) continue;
+      float k[kE], v[kE];
+      load_lane<PAGED>(kp, s.D, k);
+      load_lane<PAGED>(key_ptr<PAGED>(s, true, r, h / s.G, j), s.D, v);
+      const float x = dot_lane(q, k) * s.scale, mn = fmaxf(m, x), a = m == -INFINITY ? 0.0f : expf(m - mn), p = x == -INFINITY ? 0.0f : expf(x - mn);
+      l = fmaf(l, a, p);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) o[e] = fmaf(o[e], a, p * v[e]);
+      m = mn;
+    }
+  }
+  float* op = out.data + token_offset<PAGED>(out, r, h, token);
+#pragma unroll
+  for (int e = 0; e < kE; ++e)
+    if (lane + 32 * e < s.D) op[lane + 32 * e] = l == 0.0f ? 0.0f : o[e] / l;
+  if (lane == 0) lse[stat_offset<PAGED>(s, r, h, token)] = l == 0.0f ? -INFINITY : m + logf(l);
+}
+
+// A warp per (row, query head, token): dq = scale sum_j p (do.v - delta) k, and delta = do.o for the kernel below.
+__global__ void __launch_bounds__(128) stream_dq_kernel(StreamRows s, gn_view out, gn_view dout, const float* __restrict__ lse, float* __restrict__ delta,
+                                                        gn_view dq, int accumulate) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * 4 + warp, h = blockIdx.y, r = blockIdx.z;
+  const RowSpan sp = row_span<false>(s, r);
+  if (t >= s.seq) return;
+  float acc[kE] = {0, 0, 0, 0};
+  if (t < sp.q_len) {
+    float q[kE], g[kE], o[kE];
+    load_lane<false>(s.q.data + token_offset<false>(s.q, r, h, t), s.D, q);
+    load_lane<false>(dout.data + token_offset<false>(dout, r, h, t), s.D, g);
+    load_lane<false>(out.data + token_offset<false>(out, r, h, t), s.D, o);
+    const float dl = dot_lane(g, o), L = lse[stat_offset<false>(s, r, h, t)];
+    if (lane == 0) delta[stat_offset<false>(s, r, h, t)] = dl;
+    const Seen see = seen_by(s, t);
+    for (int j = see.sink_end > 0 ? 0 : see.begin; j <= t; j = (j + 1 == see.sink_end) ? max(see.begin, j + 1) : j + 1) {
+      float k[kE], v[kE];
+      load_lane<false>(key_ptr<false>(s, false, r, h / s.G, j), s.D, k);
+      load_lane<false>(key_ptr<false>(s, true, r, h / s.G, j), s.D, v);
+      const float ds = expf(dot_lane(q, k) * s.scale - L) * (dot_lane(g, v) - dl) * s.scale;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[e] = fmaf(ds, k[e], acc[e]);
+    }
+  }
+  float* p = dq.data + token_offset<false>(dq, r, h, t);
+#pragma unroll
+  for (int e = 0; e < kE; ++e)
+    if (lane + 32 * e < s.D) p[lane + 32 * e] = (accumulate ? p[lane + 32 * e] : 0.0f) + acc[e];
+}
+// A warp per (row, kv head, key): sums over the queries of every head of the group that see the key.
+__global__ void __launch_bounds__(128) stream_dkv_kernel(StreamRows s, gn_view dout, const float* __restrict__ lse, const float* __restrict__ delta, gn_view dk,
+                                                         gn_view dv, int accumulate) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int j = blockIdx.x * 4 + warp, hk = blockIdx.y, r = blockIdx.z;
+  const RowSpan sp = row_span<false>(s, r);
+  if (j >= s.seq) return;
+  float ak[kE] = {0, 0, 0, 0}, av[kE] = {0, 0, 0, 0};
+  if (j < sp.ctx) {
+    float k[kE], v[kE];
+    load_lane<false>(key_ptr<false>(s, false, r, hk, j), s.D, k);
+    load_lane<false>(key_ptr<false>(s, true, r, hk, j), s.D, v);
+    const int end = (s.window < 0 || j < s.sinks) ? sp.q_len : min((int64_t)sp.q_len, (int64_t)j + s.window + 1);
+    for (int h = hk * s.G; h < (hk + 1) * s.G; ++h)
+      for (int t = j; t < end; ++t) {
+        float q[kE], g[kE];
+        load_lane<false>(s.q.data + token_offset<false>(s.q, r, h, t), s.D, q);
+        load_lane<false>(dout.data + token_offset<false>(dout, r, h, t), s.D, g);
+        const int64_t at = stat_offset<false>(s, r, h, t);
+        const float p = expf(dot_lane(q, k) * s.scale - lse[at]), ds = p * (dot_lane(g, v) - delta[at]) * s.scale;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) { ak[e] = fmaf(ds, q[e], ak[e]); av[e] = fmaf(p, g[e], av[e]); }
+      }
+  }
+  float* pk = dk.data + token_offset<false>(dk, r, hk, j); float* pv = dv.data + token_offset<false>(dv, r, hk, j);
+#pragma unroll
+  for (int e = 0; e < kE; ++e)
+    if (lane + 32 * e < s.D) {
+      pk[lane + 32 * e] = (accumulate ? pk[lane + 32 * e] : 0.0f) + ak[e];
+      pv[lane + 32 * e] = (accumulate ? pv[lane + 32 * e] : 0.0f) + av[e];
+    }
+}
+
+// A warp per (row, new token, kv head): the new token's key and value go to its slot.
+__global__ void __launch_bounds__(128) stream_append_kernel(StreamRows s, gn_view nk, gn_view nv) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * 4 + warp, hk = blockIdx.y, r = blockIdx.z;
+  const RowSpan sp = row_span<true>(s, r);
+  if (t >= sp.q_len) return;
+  const int pos = sp.ctx - sp.q_len + t;
+  if (pos < 0) return;
+  const int64_t to = key_offset<true>(s, s.k, r, hk, pos);
+  if (to < 0) return;
+  const float* a = nk.data + token_offset<true>(nk, r, hk, sp.q_begin + t); const float* b = nv.data + token_offset<true>(nv, r, hk, sp.q_begin + t);
+  for (int c = lane; c < s.D; c += 32) { s.pages_k[to + c] = a[c]; s.pages_v[to + c] = b[c]; }
+}
+// A warp per (row, kv head, key): the weight that this call's queries gave the key.
+__global__ void __launch_bounds__(128) stream_mass_kernel(StreamRows s, const float* __restrict__ lse, const float* mass, float* mass_out) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int j = blockIdx.x * 4 + warp, hk = blockIdx.y, r = blockIdx.z;
+  const RowSpan sp = row_span<true>(s, r);
+  if (j >= sp.ctx) return;
+  const int first = sp.ctx - sp.q_len;
+  float sum = 0.0f;
+  const float* kp = key_ptr<true>(s, false, r, hk, j);
+  if (kp) {
+    float k[kE];
+    load_lane<true>(kp, s.D, k);
+    for (int t = max(0, j - first); t < sp.q_len; ++t) {
+      if (!sees(s, first + t, j)) continue;
+      for (int h = hk * s.G; h < (hk + 1) * s.G; ++h) {
+        float q[kE];
+        load_lane<true>(s.q.data + token_offset<true>(s.q, r, h, sp.q_begin + t), s.D, q);
+        sum += expf(dot_lane(q, k) * s.scale - lse[stat_offset<true>(s, r, h, sp.q_begin + t)]);
+      }
+    }
+  }
+  if (lane == 0) {
+    const int64_t at = ((int64_t)r * s.Hkv + hk) * s.width * s.page_size + j;
+    mass_out[at] = (mass && j < first ? mass[at] : 0.0f) + sum;
+  }
+}
+
+// ------------------------------------------------------------------ eviction
+struct Evict {
+  gn_evict_params p;
+  int32_t* kept; int32_t* new_lens; float* mass_out;
+};
+// Mass as an integer that orders like it: equal values (both zeros too) alike, NaN below everything.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (isnan(x)) return 0u;
+  const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ int evict_len(const gn_evict_params& p, int r) { return min(max(p.context_lens[r], 0), p.max_context); }
+
+// A CTA per (row, kv head).  The threshold (the smallest kept order key of the middle) by four radix passes of 8 bits, then the
+// kept indices by a stable scan; of the keys equal to the threshold the first ones.
+__global__ void __launch_bounds__(256) evict_select_kernel(Evict e) {
+  const gn_evict_params& p = e.p;
+  const int hk = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = evict_len(p, r), keep = min(n, p.budget), lo = p.sinks, hi = n - p.recent;
+  const int64_t head = (int64_t)r * p.n_kv_head + hk;
+  const float* mass = p.mass + head * p.mass_stride;
+  __shared__ int hist[256];
+  __shared__ uint32_t prefix_s;
+  __shared__ int want_s, warp_keep[8], warp_tie[8];
+  uint32_t prefix = 0;
+  int want = n <= p.budget ? 0 : p.budget - p.sinks - p.recent;   // of the middle
+  const int wanted = want;
+  if (wanted > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      hist[tid] = 0;
+      __syncthreads();
+      for (int j = lo + tid; j < hi; j += 256) {
+        const uint32_t k = order_key(mass[j]);
+        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255u], 1);
+      }
+      __syncthreads();
+      if (tid == 0) {
+        int b = 255, left = want;
+        while (b > 0 && hist[b] < left) left -= hist[b--];
+        prefix_s = prefix | ((uint32_t)b << shift); want_s = left;
+      }
+      __syncthreads();
+      prefix = prefix_s; want = want_s;
+      __syncthreads();
+    }
+  }
+  // now `want` of the keys equal to `prefix` are kept, and all above it
+  int base = 0, ties = 0;
+  for (int j0 = 0; j0 < n; j0 += 256) {
+    const int j = j0 + tid;
+    bool take = false, tie = false;
+    if (j < n) {
+      if (n <= p.budget || j < lo || j >= hi) take = true;
+      else if (wanted > 0) { const uint32_t k = order_key(mass[j]); take = k > prefix; tie = k == prefix; }
+    }
+    const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
+    if (lane == 0) warp_tie[warp] = __popc(tie_mask);
+    __syncthreads();
+    int before = ties, all = 0;
+    for (int w = 0; w < 8; ++w) { if (w < warp) before += warp_tie[w]; all += warp_tie[w]; }
+    ties += all;
+    if (tie) take = before + __popc(tie_mask & ((1u << lane) - 1u)) < want;
+    const uint32_t mask = __ballot_sync(0xffffffffu, take);
+    if (lane == 0) warp_keep[warp] = __popc(mask);
+    __syncthreads();
+    int at = base; all = 0;
+    for (int w = 0; w < 8; ++w) { if (w < warp) at += warp_keep[w]; all += warp_keep[w]; }
+    base += all;
+    if (take) e.kept[head * p.budget + at + __popc(mask & ((1u << lane) - 1u))] = j;
+    __syncthreads();
+  }
+  for (int i = keep + tid; i < p.budget; i += 256) e.kept[head * p.budget + i] = -1;
+  if (hk == 0 && tid == 0) e.new_lens[r] = keep;
+  __syncthreads();
+  if (e.mass_out)   // mass_out is an array of its own: the indices were written by this CTA
+    for (int i = tid; i < p.budget; i += 256) e.mass_out[head * p.budget + i] = i < keep ? mass[e.kept[head * p.budget + i]] : 0.0f;
+}
+// A CTA per (32 channels, kv head, row x {key, value}): kept key i goes to slot i.  Slots are filled in ascending order, 256 at
+// a time, every read of a group before its writes: slot i <= kept[i], so in place a group writes only what it or earlier groups read.
+__global__ void __launch_bounds__(256) evict_move_kernel(Evict e) {
+  const gn_evict_params& p = e.p;
+  const int hk = blockIdx.y, r = blockIdx.z >> 1, c0 = blockIdx.x * 32, tid = threadIdx.x;
+  float* pages = (blockIdx.z & 1) ? p.value_pages : p.key_pages;
+  const int keep = min(evict_len(p, r), p.budget), lane = tid & 31, warp = tid >> 5;
+  const int32_t* kept = e.kept + ((int64_t)r * p.n_kv_head + hk) * p.budget;
+  const bool in = c0 + lane < p.head_dim;
+  auto slot = [&](const int32_t* table, int width, int j) -> int64_t {
+    const int page = table[(int64_t)r * width + j / p.page_size];
+    if ((unsigned)page >= (unsigned)p.pages) return -1;
+    return (((int64_t)page * p.n_kv_head + hk) * p.page_size + j % p.page_size) * p.head_dim;
+  };
+  for (int i0 = 0; i0 < keep; i0 += 256) {
+    float x[32];
+#pragma unroll
+    for (int u = 0; u < 32; ++u) {
+      const int i = i0 + warp * 32 + u;
+      x[u] = 0.0f;
+      if (i < keep && in) { const int64_t from = slot(p.page_table, p.table_width, kept[i]); if (from >= 0) x[u] = pages[from + c0 + lane]; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 32; ++u) {
+      const int i = i0 + warp * 32 + u;
+      if (i < keep && in) { const int64_t to = slot(p.new_table, p.new_width, i); if (to >= 0) pages[to + c0 + lane] = x[u]; }
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ checks
+int on_this_device(const void* p, const char* what) {
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) { cudaGetLastError(); set_error("no CUDA device available: %s", cudaGetErrorString(err)); return GN_ERR_CUDA; }
+  cudaPointerAttributes at;
+  err = cudaPointerGetAttributes(&at, p);
+  if (err != cudaSuccess) { cudaGetLastError(); set_error("%s: %s", what, cudaGetErrorString(err)); return GN_ERR_CUDA; }
+  GN_REQUIRE(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, "%s: not device memory", what);
+  if (at.type == cudaMemoryTypeDevice && at.device != device) {
+    set_error("%s: memory of device %d, but device %d is current", what, at.device, device);
+    return GN_ERR_UNSUPPORTED;
+  }
+  return GN_OK;
+}
+// An output's elements must not share memory: sorted by stride, every dimension steps over the whole of the one inside it.
+bool apart(const gn_view& v, int64_t batch, int64_t heads, int64_t tokens, int64_t dim) {
+  int64_t n[3] = {batch, heads, tokens}, st[3] = {v.batch_stride, v.head_stride, v.token_stride};
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return st[a] < st[b]; });
+  int64_t extent = dim;
+  for (int i : order) {
+    if (n[i] <= 1) continue;
+    if (st[i] < extent) return false;
+    extent = st[i] * (n[i] - 1) + extent;
+  }
+  return true;
+}
+bool strides_ok(const gn_view& v) { return v.batch_stride >= 0 && v.head_stride >= 0 && v.token_stride >= 0; }
+
+int sink_rows(const gn_sink_params* p, StreamRows* s) {
+  GN_REQUIRE(p, "attention_sink: null parameters");
+  GN_REQUIRE(p->batch >= 0 && p->seq >= 0 && p->n_kv_head > 0 && p->n_head > 0 && p->n_head % p->n_kv_head == 0,
+             "attention_sink: batch %d, seq %d, %d heads on %d kv heads", p->batch, p->seq, p->n_head, p->n_kv_head);
+  GN_REQUIRE(p->head_dim > 0 && p->head_dim <= 128, "attention_sink: head_dim %d outside [1, 128]", p->head_dim);
+  GN_REQUIRE(p->batch <= 65535 && p->n_head <= 65535, "attention_sink: more than 65535 sequences or heads");
+  GN_REQUIRE(p->sinks >= 0 && p->scale == p->scale, "attention_sink: bad sinks or scale");
+  GN_REQUIRE(strides_ok(p->query) && strides_ok(p->key) && strides_ok(p->value), "attention_sink: negative stride");
+  GN_REQUIRE((int64_t)p->seq * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_sink: seq x heads of a group exceeds 2^30");
+  s->rows = p->batch; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->D = p->head_dim;
+  s->window = p->window; s->sinks = p->sinks; s->scale = p->scale; s->q = p->query; s->k = p->key; s->v = p->value; s->seq = p->seq; s->lengths = p->lengths;
+  return GN_OK;
+}
+int sink_pointers(const gn_sink_params* p) {
+  GN_REQUIRE(p->query.data && p->key.data && p->value.data, "attention_sink: null tensor");
+  GN_TRY(on_this_device(p->query.data, "attention_sink: query")); GN_TRY(on_this_device(p->key.data, "attention_sink: key"));
+  GN_TRY(on_this_device(p->value.data, "attention_sink: value"));
+  if (p->lengths) GN_TRY(on_this_device(p->lengths, "attention_sink: lengths"));
+  return GN_OK;
+}
+int workspace_ok(const void* w, int64_t have, int64_t need, const char* what) {
+  if (need == 0) return GN_OK;
+  GN_REQUIRE(w && have >= need, "%s: workspace of %lld bytes, %lld needed", what, (long long)(w ? have : 0), (long long)need);
+  GN_REQUIRE((reinterpret_cast<uintptr_t>(w) & 15) == 0, "%s: workspace not 16-byte aligned", what);
+  return on_this_device(w, what);
+}
+int64_t sink_bytes(const StreamRows& s, int backward) { return backward ? (int64_t)s.rows * s.Hq * s.seq * 4 : 0; }
+
+int paged_rows(const gn_paged_params* p, StreamRows* s) {
+  GN_REQUIRE(p, "attention_paged: null parameters");
+  GN_REQUIRE(p->rows >= 0 && p->tokens >= 0 && p->max_query >= 0 && p->n_kv_head > 0 && p->n_head > 0 && p->n_head % p->n_kv_head == 0,
+             "attention_paged: rows %d, tokens %d, max_query %d, %d heads on %d kv heads", p->rows, p->tokens, p->max_query, p->n_head, p->n_kv_head);
+  GN_REQUIRE(p->head_dim > 0 && p->head_dim <= 128, "attention_paged: head_dim %d outside [1, 128]", p->head_dim);
+  GN_REQUIRE(p->rows <= 65535 && p->n_head <= 65535, "attention_paged: more than 65535 rows or heads");
+  GN_REQUIRE(p->page_size > 0 && p->pages >= 0 && p->table_width >= 0 && (int64_t)p->table_width * p->page_size < (1ll << 31),
+             "attention_paged: pages %d of %d keys, table of %d", p->pages, p->page_size, p->table_width);
+  GN_REQUIRE(p->max_context >= 0 && (int64_t)p->max_context <= (int64_t)p->table_width * p->page_size, "attention_paged: max_context %d, but a row of the table holds %lld keys",
+             p->max_context, (long long)p->table_width * p->page_size);
+  GN_REQUIRE((int64_t)p->max_query * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_paged: max_query x heads of a group exceeds 2^30");
+  GN_REQUIRE(p->sinks >= 0 && p->scale == p->scale, "attention_paged: bad sinks or scale");
+  GN_REQUIRE(strides_ok(p->query) && strides_ok(p->new_key) && strides_ok(p->new_value), "attention_paged: negative stride");
+  s->rows = p->rows; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->D = p->head_dim;
+  s->window = p->window; s->sinks = p->sinks; s->scale = p->scale; s->q = p->query;
+  s->pages_k = p->key_pages; s->pages_v = p->value_pages; s->table = p->page_table; s->starts = p->query_starts; s->lens = p->context_lens;
+  s->tokens = p->tokens; s->max_query = std::min(p->max_query, p->tokens); s->max_context = p->max_context; s->page_size = p->page_size; s->pages = p->pages;
+  s->width = p->table_width;
+  return GN_OK;
+}
+
+}  // namespace
+}  // namespace gn
+
+using namespace gn;
+
+extern "C" {
+
+int gn_attention_sink_workspace(const gn_sink_params* p, int backward, int64_t* bytes) {
+  GN_REQUIRE(bytes, "attention_sink_workspace: null bytes");
+  StreamRows s;
+  GN_TRY(sink_rows(p, &s));
+  *bytes = s.rows && s.seq ? sink_bytes(s, backward) : 0;
+  return GN_OK;
+}
+
+int gn_attention_sink_forward(const gn_sink_params* p, const gn_view* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  StreamRows s;
+  GN_TRY(sink_rows(p, &s));
+  if (!s.rows || !s.seq) return GN_OK;
+  GN_TRY(sink_pointers(p));
+  GN_REQUIRE(out && out->data && lse, "attention_sink_forward: null output");
+  GN_REQUIRE(strides_ok(*out) && apart(*out, s.rows, s.Hq, s.seq, s.D), "attention_sink_forward: elements of out share memory");
+  GN_TRY(on_this_device(out->data, "attention_sink_forward: out")); GN_TRY(on_this_device(lse, "attention_sink_forward: lse"));
+  GN_TRY(workspace_ok(workspace, workspace_bytes, sink_bytes(s, 0), "attention_sink_forward"));
+  stream_forward_kernel<false><<<dim3(ceil_div(s.seq, 4), s.Hq, s.rows), 128, 0, (cudaStream_t)stream>>>(s, *out, lse);
+  GN_LAUNCH_CHECK();
+  return GN_OK;
+}
+
+int gn_attention_sink_backward(const gn_sink_params* p, const gn_view* out, const gn_view* out_grad, const float* lse, const gn_view* dq, const gn_view* dk,
+                               const gn_view* dv, int accumulate, void* workspace, int64_t workspace_bytes, void* stream) {
+  StreamRows s;
+  GN_TRY(sink_rows(p, &s));
+  if (!s.rows || !s.seq) return GN_OK;
+  GN_TRY(sink_pointers(p));
+  GN_REQUIRE(out && out->data && out_grad && out_grad->data && lse && dq && dq->data && dk && dk->data && dv && dv->data, "attention_sink_backward: null tensor");
+  GN_REQUIRE(strides_ok(*out) && strides_ok(*out_grad) && strides_ok(*dq) && strides_ok(*dk) && strides_ok(*dv), "attention_sink_backward: negative stride");
+  GN_REQUIRE(apart(*dq, s.rows, s.Hq, s.seq, s.D) && apart(*dk, s.rows, s.Hkv, s.seq, s.D) && apart(*dv, s.rows, s.Hkv, s.seq, s.D),
+             "attention_sink_backward: elements of a gradient share memory");
+  const void* ptrs[] = {out->data, out_grad->data, lse, dq->data, dk->data, dv->data};
+  for (const void* x : ptrs) GN_TRY(on_this_device(x, "attention_sink_backward"));
+  GN_TRY(workspace_ok(workspace, workspace_bytes, sink_bytes(s, 1), "attention_sink_backward"));
+  cudaStream_t st = (cudaStream_t)stream;
+  float* delta = static_cast<float*>(workspace);
+  stream_dq_kernel<<<dim3(ceil_div(s.seq, 4), s.Hq, s.rows), 128, 0, st>>>(s, *out, *out_grad, lse, delta, *dq, accumulate);
+  GN_LAUNCH_CHECK();
+  stream_dkv_kernel<<<dim3(ceil_div(s.seq, 4), s.Hkv, s.rows), 128, 0, st>>>(s, *out_grad, lse, delta, *dk, *dv, accumulate);
+  GN_LAUNCH_CHECK();
+  return GN_OK;
+}
+
+int gn_attention_paged_workspace(const gn_paged_params* p, int64_t* bytes) {
+  GN_REQUIRE(bytes, "attention_paged_workspace: null bytes");
+  StreamRows s;
+  GN_TRY(paged_rows(p, &s));
+  *bytes = 0;
+  return GN_OK;
+}
+
+int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  StreamRows s;
+  GN_TRY(paged_rows(p, &s));
+  if (!s.rows || !s.tokens || !s.max_query) return GN_OK;
+  (void)workspace; (void)workspace_bytes;
+  GN_REQUIRE(p->query.data && p->query_starts && p->context_lens && out && out->data && lse, "attention_paged: null argument");
+  GN_REQUIRE(p->max_context == 0 || (p->key_pages && p->value_pages && p->page_table), "attention_paged: null pages");
+  GN_REQUIRE((p->new_key.data == nullptr) == (p->new_value.data == nullptr), "attention_paged: new_key and new_value come together");
+  GN_REQUIRE(!p->mass || p->mass_out, "attention_paged: mass without mass_out");
+  GN_REQUIRE(strides_ok(*out) && apart(*out, 1, s.Hq, s.tokens, s.D), "attention_paged: elements of out share memory");
+  const void* ptrs[] = {p->query.data, p->query_starts, p->context_lens, out->data, lse, p->key_pages, p->value_pages, p->page_table, p->new_key.data,
+                        p->new_value.data, p->mass, p->mass_out};
+  for (const void* x : ptrs) if (x) GN_TRY(on_this_device(x, "attention_paged"));
+  cudaStream_t st = (cudaStream_t)stream;
+  if (p->new_key.data && s.max_context) {
+    stream_append_kernel<<<dim3(ceil_div(s.max_query, 4), s.Hkv, s.rows), 128, 0, st>>>(s, p->new_key, p->new_value);
+    GN_LAUNCH_CHECK();
+  }
+  stream_forward_kernel<true><<<dim3(ceil_div(s.max_query, 4), s.Hq, s.rows), 128, 0, st>>>(s, *out, lse);
+  GN_LAUNCH_CHECK();
+  if (p->mass_out && s.max_context) {
+    stream_mass_kernel<<<dim3(ceil_div(s.max_context, 4), s.Hkv, s.rows), 128, 0, st>>>(s, lse, p->mass, p->mass_out);
+    GN_LAUNCH_CHECK();
+  }
+  return GN_OK;
+}
+
+int gn_cache_evict(const gn_evict_params* p, int32_t* kept, int32_t* new_lens, float* mass_out, void* stream) {
+  GN_REQUIRE(p, "cache_evict: null parameters");
+  GN_REQUIRE(p->rows >= 0 && p->rows <= 32767 && p->n_kv_head > 0 && p->n_kv_head <= 65535 && p->head_dim > 0 && p->page_size > 0 && p->pages >= 0 && p->table_width >= 0 && p->new_width >= 0,
+             "cache_evict: bad shape");
+  GN_REQUIRE(p->budget >= 0 && p->sinks >= 0 && p->recent >= 0 && (int64_t)p->sinks + p->recent <= p->budget, "cache_evict: sinks %d + recent %d exceed the budget %d",
+             p->sinks, p->recent, p->budget);
+  GN_REQUIRE(p->max_context >= 0 && (int64_t)p->max_context <= (int64_t)p->table_width * p->page_size && p->max_context <= p->mass_stride,
+             "cache_evict: max_context %d, but a row holds %lld keys and %d masses", p->max_context, (long long)p->table_width * p->page_size, p->mass_stride);
+  GN_REQUIRE((int64_t)p->new_width * p->page_size >= std::min(p->budget, p->max_context), "cache_evict: new_table holds %lld keys a row, %d are kept",
+             (long long)p->new_width * p->page_size, std::min(p->budget, p->max_context));
+  if (!p->rows) return GN_OK;
+  GN_REQUIRE(p->context_lens && new_lens && (p->budget == 0 || kept), "cache_evict: null argument");
+  GN_REQUIRE(p->max_context == 0 || (p->key_pages && p->value_pages && p->mass && p->page_table && (p->new_table || p->budget == 0)), "cache_evict: null argument");
+  GN_REQUIRE(mass_out == nullptr || mass_out != p->mass, "cache_evict: mass_out must not be mass");
+  const void* ptrs[] = {p->context_lens, new_lens, kept, p->key_pages, p->value_pages, p->mass, p->page_table, p->new_table, mass_out};
+  for (const void* x : ptrs) if (x) GN_TRY(on_this_device(x, "cache_evict"));
+  cudaStream_t st = (cudaStream_t)stream;
+  const Evict e{*p, kept, new_lens, mass_out};
+  evict_select_kernel<<<dim3(p->n_kv_head, p->rows), 256, 0, st>>>(e);
+  GN_LAUNCH_CHECK();
+  if (p->budget && p->max_context) {
+    evict_move_kernel<<<dim3(ceil_div(p->head_dim, 32), p->n_kv_head, 2 * p->rows), 256, 0, st>>>(e);
+    GN_LAUNCH_CHECK();
+  }
+  return GN_OK;
+}
+
+}  // extern "C"

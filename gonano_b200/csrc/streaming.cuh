@@ -1,0 +1,63 @@
+// Streaming attention (include/gonano_cuda.h): what its kernels share.
+#pragma once
+#include "common.cuh"
+
+namespace gn {
+
+// The rows (sequences) of a call, padded batch or paged cache, as the kernels see them.
+struct StreamRows {
+  int rows = 0, Hq = 0, Hkv = 0, G = 0, D = 0, window = -1, sinks = 0;
+  float scale = 1.0f;
+  gn_view q{}, k{}, v{};            // k, v: padded batch
+  // padded batch: `seq` tokens a row, lengths nullable
+  int seq = 0;
+  const int32_t* lengths = nullptr;
+  // paged cache (pages_k != null)
+  float* pages_k = nullptr; float* pages_v = nullptr;
+  const int32_t* table = nullptr; const int32_t* starts = nullptr; const int32_t* lens = nullptr;
+  int tokens = 0, max_query = 0, max_context = 0, page_size = 1, pages = 0, width = 0;
+  bool paged() const { return pages_k != nullptr; }
+};
+
+#ifdef __CUDACC__
+struct RowSpan { int q_begin, q_len, ctx; };   // the row's first token, its new tokens, its keys
+
+template <bool PAGED>
+__device__ __forceinline__ RowSpan row_span(const StreamRows& s, int r) {
+  if (!PAGED) {
+    const int n = s.lengths ? min(max(s.lengths[r], 0), s.seq) : s.seq;
+    return {0, n, n};
+  }
+  // offsets and lengths are device data: cut to what the buffers hold
+  const int b = min(max(s.starts[r], 0), s.tokens), e = min(max(s.starts[r + 1], b), s.tokens);
+  return {b, min(e - b, s.max_query), min(max(s.lens[r], 0), s.max_context)};
+}
+// Key j of row r, kv head hk; null when its page does not exist.
+template <bool PAGED>
+__device__ __forceinline__ int64_t key_offset(const StreamRows& s, const gn_view& view, int r, int hk, int j) {
+  if (!PAGED) return (int64_t)r * view.batch_stride + (int64_t)hk * view.head_stride + (int64_t)j * view.token_stride;
+  const int page = s.table[(int64_t)r * s.width + j / s.page_size];
+  if ((unsigned)page >= (unsigned)s.pages) return -1;
+  return (((int64_t)page * s.Hkv + hk) * s.page_size + j % s.page_size) * s.D;
+}
+template <bool PAGED>
+__device__ __forceinline__ int64_t token_offset(const gn_view& view, int r, int h, int token) {
+  return (PAGED ? 0 : (int64_t)r * view.batch_stride) + (int64_t)h * view.head_stride + (int64_t)token * view.token_stride;
+}
+// lse and other per-(token, head) numbers: [batch, heads, seq] or [tokens, heads]
+template <bool PAGED>
+__device__ __forceinline__ int64_t stat_offset(const StreamRows& s, int r, int h, int token) {
+  return PAGED ? (int64_t)token * s.Hq + h : ((int64_t)r * s.Hq + h) * s.seq + token;
+}
+// The keys that a query at position pos sees: [0, sink_end) and [begin, pos].
+struct Seen { int sink_end, begin; };
+__device__ __forceinline__ Seen seen_by(const StreamRows& s, int pos) {
+  const int begin = s.window < 0 ? 0 : max(0, pos - s.window);
+  return {min(s.sinks, begin), begin};
+}
+__device__ __forceinline__ bool sees(const StreamRows& s, int pos, int j) {
+  return j <= pos && (s.window < 0 || pos - j <= s.window || j < s.sinks);
+}
+#endif
+
+}  // namespace gn

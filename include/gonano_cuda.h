@@ -221,6 +221,88 @@ int gn_attention_windowed_backward(const float* query, const float* key, const f
                                    float* dq, float* dk, float* dv);
 
 /* ===================================================================== *
+ * Streaming attention: a bounded context for long rollouts              *
+ * ===================================================================== */
+
+/* Attention with a sliding window in which the first keys stay visible ("sinks"), for training and prefill; attention of
+ * new tokens over a paged key / value cache; and eviction from that cache by accumulated attention weight.  No counterpart
+ * in the reference, whose caches grow with every token (model/kvcache.go:10-28).
+ *
+ * Query i sees key j when j <= i and (window < 0 or i - j <= window or j < sinks): the reference's window
+ * (kernels/backend.go:167-283) plus the sinks.  Scores are scale * q.k; the reference's is 1.  A query that sees no key
+ * gets zeros and lse = -inf.  A non-finite key or value reaches only the
+ * queries that see it (whose channels may then all be NaN).
+ *
+ * Unlike the calls above these take device memory of the current device only, read and written through views with strides,
+ * run asynchronously on `stream` (a cudaStream_t; NULL = the default stream), allocate nothing and may be captured into a
+ * CUDA graph.  The scratch memory is the caller's: gn_*_workspace gives the bytes for a call with the same parameters
+ * (pointers are not looked at), 16-byte aligned; calls that may overlap in time need workspaces of their own.  Data on the
+ * device (lengths, tables) cannot be refused: what lies outside its range is cut off or skipped as stated, never read. */
+
+/* float32 tensor [batch, heads, tokens, head_dim] with strides in elements; the channels of a head are contiguous. */
+typedef struct gn_view {
+  float* data;
+  int64_t batch_stride, head_stride, token_stride;
+} gn_view;
+
+typedef struct gn_sink_params {
+  gn_view query;      /* [batch, n_head, seq, head_dim] */
+  gn_view key, value; /* [batch, n_kv_head, seq, head_dim] */
+  int32_t batch, n_head, n_kv_head, seq, head_dim; /* n_head a multiple of n_kv_head, head_dim 1..128 */
+  int32_t sinks, window;
+  float scale;
+  const int32_t* lengths; /* NULL, or [batch] on the device: tokens behind a sequence's length (cut to [0, seq]) are padding: neither
+                             read nor seen, their outputs 0 and lse -inf */
+} gn_sink_params;
+
+int gn_attention_sink_workspace(const gn_sink_params* p, int backward, int64_t* bytes);
+/* out like query (own strides), lse [batch, n_head, seq]. */
+int gn_attention_sink_forward(const gn_sink_params* p, const gn_view* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+/* out and lse are the forward's.  accumulate = 0 overwrites dq, dk, dv, 1 adds to them (kernels/backend.go:217-220).  The
+ * same call gives the same bits every time: no atomics. */
+int gn_attention_sink_backward(const gn_sink_params* p, const gn_view* out, const gn_view* out_grad, const float* lse, const gn_view* dq, const gn_view* dk,
+                               const gn_view* dv, int accumulate, void* workspace, int64_t workspace_bytes, void* stream);
+
+typedef struct gn_paged_params {
+  gn_view query;              /* [tokens, n_head, head_dim] (batch_stride unused): the new tokens of all rows, one row after the other */
+  gn_view new_key, new_value; /* data NULL, or [tokens, n_kv_head, head_dim]: the new tokens' own keys and values, written to the pages first */
+  float *key_pages, *value_pages;  /* [pages, n_kv_head, page_size, head_dim], contiguous */
+  const int32_t* page_table;       /* [rows, table_width]: key j of row r is slot j % page_size of page page_table[r][j / page_size]; a key whose
+                                      page is outside [0, pages) is neither read, written nor seen */
+  const int32_t* query_starts;     /* [rows + 1], ascending: row r's new tokens are query_starts[r] .. query_starts[r + 1] - 1 */
+  const int32_t* context_lens;     /* [rows]: keys of the row, the new tokens' included; the new tokens stand at its end */
+  const float* mass;               /* mass_out NULL: unused.  NULL, or [rows, n_kv_head, table_width * page_size]: the weight that each key has */
+  float* mass_out;                 /*   gathered so far (summed over queries and the heads of its group); mass_out (may be mass) gets it with this call's
+                                      added.  The new tokens' own keys start from 0; entries behind the row's length are left as they are. */
+  int32_t rows, tokens, max_query; /* no row has more than max_query new tokens (further ones are left out) */
+  int32_t max_context;             /* no row has more keys (further ones are left out) */
+  int32_t n_head, n_kv_head, head_dim, page_size, pages, table_width, sinks, window;
+  float scale;
+} gn_paged_params;
+
+int gn_attention_paged_workspace(const gn_paged_params* p, int64_t* bytes);
+/* out [tokens, n_head, head_dim] with its own strides, lse [tokens, n_head]; entries behind the last row's tokens are left as they are. */
+int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Keeps, for every row and kv head on its own, the first `sinks` keys, the last `recent` and of the others those of the largest
+ * mass, `budget` in all (ties to the lower index, NaN below everything), in their order, and moves them to the front of the row's
+ * pages in new_table.  A row of at most `budget` keys is kept whole.  new_table may be page_table itself (compaction in place; no
+ * page may then belong to two rows) or name pages that page_table does not. */
+typedef struct gn_evict_params {
+  float *key_pages, *value_pages;  /* [pages, n_kv_head, page_size, head_dim] */
+  const float* mass;               /* [rows, n_kv_head, mass_stride] */
+  const int32_t* page_table;       /* [rows, table_width] */
+  const int32_t* new_table;        /* [rows, new_width], new_width * page_size >= budget */
+  const int32_t* context_lens;     /* [rows] */
+  int32_t rows, n_kv_head, head_dim, page_size, pages, table_width, new_width, mass_stride;
+  int32_t max_context, budget, sinks, recent; /* sinks + recent <= budget; max_context as above */
+} gn_evict_params;
+
+/* kept [rows, n_kv_head, budget]: the indices that the kept keys had (-1 behind them); new_lens [rows]; mass_out [rows, n_kv_head,
+ * budget] (0 behind them), nullable. */
+int gn_cache_evict(const gn_evict_params* p, int32_t* kept, int32_t* new_lens, float* mass_out, void* stream);
+
+/* ===================================================================== *
  * Stand-alone kernels of the RL step (host or device pointers)          *
  * ===================================================================== */
 
