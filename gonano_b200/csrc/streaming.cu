@@ -1,7 +1,7 @@
 // Streaming attention: C entry points and the float32 kernels (a warp per row of the result).
 #include <algorithm>
 
-#include "streaming.cuh"
+#include "streaming_tc.cuh"
 
 namespace gn {
 
@@ -309,7 +309,7 @@ int sink_rows(const gn_sink_params* p, StreamRows* s) {
   GN_REQUIRE(p->batch >= 0 && p->seq >= 0 && p->n_kv_head > 0 && p->n_head > 0 && p->n_head % p->n_kv_head == 0,
              "attention_sink: batch %d, seq %d, %d heads on %d kv heads", p->batch, p->seq, p->n_head, p->n_kv_head);
   GN_REQUIRE(p->head_dim > 0 && p->head_dim <= 128, "attention_sink: head_dim %d outside [1, 128]", p->head_dim);
-  GN_REQUIRE(p->batch <= 65535 && p->n_head <= 65535, "attention_sink: more than 65535 sequences or heads");
+  GN_REQUIRE(p->batch <= 32767 && p->n_head <= 65535, "attention_sink: more than 32767 sequences or 65535 heads");
   GN_REQUIRE(p->sinks >= 0 && p->scale == p->scale, "attention_sink: bad sinks or scale");
   GN_REQUIRE(strides_ok(p->query) && strides_ok(p->key) && strides_ok(p->value), "attention_sink: negative stride");
   GN_REQUIRE((int64_t)p->seq * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_sink: seq x heads of a group exceeds 2^30");
@@ -330,14 +330,16 @@ int workspace_ok(const void* w, int64_t have, int64_t need, const char* what) {
   GN_REQUIRE((reinterpret_cast<uintptr_t>(w) & 15) == 0, "%s: workspace not 16-byte aligned", what);
   return on_this_device(w, what);
 }
-int64_t sink_bytes(const StreamRows& s, int backward) { return backward ? (int64_t)s.rows * s.Hq * s.seq * 4 : 0; }
+int64_t sink_bytes(const StreamRows& s, int backward) { return backward ? (int64_t)s.rows * s.Hq * s.seq * 4 : stream_tc_forward_bytes(s); }
+// New tokens over a paged cache: a single token per row runs on the warp-per-row kernel, chunks on the tensor cores.
+bool paged_on_tensor_cores(const StreamRows& s) { return (int64_t)s.max_query * s.G > 16; }
 
 int paged_rows(const gn_paged_params* p, StreamRows* s) {
   GN_REQUIRE(p, "attention_paged: null parameters");
   GN_REQUIRE(p->rows >= 0 && p->tokens >= 0 && p->max_query >= 0 && p->n_kv_head > 0 && p->n_head > 0 && p->n_head % p->n_kv_head == 0,
              "attention_paged: rows %d, tokens %d, max_query %d, %d heads on %d kv heads", p->rows, p->tokens, p->max_query, p->n_head, p->n_kv_head);
   GN_REQUIRE(p->head_dim > 0 && p->head_dim <= 128, "attention_paged: head_dim %d outside [1, 128]", p->head_dim);
-  GN_REQUIRE(p->rows <= 65535 && p->n_head <= 65535, "attention_paged: more than 65535 rows or heads");
+  GN_REQUIRE(p->rows <= 32767 && p->n_head <= 65535, "attention_paged: more than 32767 rows or 65535 heads");
   GN_REQUIRE(p->page_size > 0 && p->pages >= 0 && p->table_width >= 0 && (int64_t)p->table_width * p->page_size < (1ll << 31),
              "attention_paged: pages %d of %d keys, table of %d", p->pages, p->page_size, p->table_width);
   GN_REQUIRE(p->max_context >= 0 && (int64_t)p->max_context <= (int64_t)p->table_width * p->page_size, "attention_paged: max_context %d, but a row of the table holds %lld keys",
@@ -377,9 +379,7 @@ int gn_attention_sink_forward(const gn_sink_params* p, const gn_view* out, float
   GN_REQUIRE(strides_ok(*out) && apart(*out, s.rows, s.Hq, s.seq, s.D), "attention_sink_forward: elements of out share memory");
   GN_TRY(on_this_device(out->data, "attention_sink_forward: out")); GN_TRY(on_this_device(lse, "attention_sink_forward: lse"));
   GN_TRY(workspace_ok(workspace, workspace_bytes, sink_bytes(s, 0), "attention_sink_forward"));
-  stream_forward_kernel<false><<<dim3(ceil_div(s.seq, 4), s.Hq, s.rows), 128, 0, (cudaStream_t)stream>>>(s, *out, lse);
-  GN_LAUNCH_CHECK();
-  return GN_OK;
+  return stream_tc_forward(s, *out, lse, workspace, (cudaStream_t)stream);
 }
 
 int gn_attention_sink_backward(const gn_sink_params* p, const gn_view* out, const gn_view* out_grad, const float* lse, const gn_view* dq, const gn_view* dk,
@@ -408,7 +408,7 @@ int gn_attention_paged_workspace(const gn_paged_params* p, int64_t* bytes) {
   GN_REQUIRE(bytes, "attention_paged_workspace: null bytes");
   StreamRows s;
   GN_TRY(paged_rows(p, &s));
-  *bytes = 0;
+  *bytes = s.rows && s.tokens && s.max_query && paged_on_tensor_cores(s) ? stream_tc_forward_bytes(s) : 0;
   return GN_OK;
 }
 
@@ -416,7 +416,6 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
   StreamRows s;
   GN_TRY(paged_rows(p, &s));
   if (!s.rows || !s.tokens || !s.max_query) return GN_OK;
-  (void)workspace; (void)workspace_bytes;
   GN_REQUIRE(p->query.data && p->query_starts && p->context_lens && out && out->data && lse, "attention_paged: null argument");
   GN_REQUIRE(p->max_context == 0 || (p->key_pages && p->value_pages && p->page_table), "attention_paged: null pages");
   GN_REQUIRE((p->new_key.data == nullptr) == (p->new_value.data == nullptr), "attention_paged: new_key and new_value come together");
@@ -425,13 +424,18 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
   const void* ptrs[] = {p->query.data, p->query_starts, p->context_lens, out->data, lse, p->key_pages, p->value_pages, p->page_table, p->new_key.data,
                         p->new_value.data, p->mass, p->mass_out};
   for (const void* x : ptrs) if (x) GN_TRY(on_this_device(x, "attention_paged"));
+  const bool tensor = paged_on_tensor_cores(s);
+  GN_TRY(workspace_ok(workspace, workspace_bytes, tensor ? stream_tc_forward_bytes(s) : 0, "attention_paged"));
   cudaStream_t st = (cudaStream_t)stream;
   if (p->new_key.data && s.max_context) {
     stream_append_kernel<<<dim3(ceil_div(s.max_query, 4), s.Hkv, s.rows), 128, 0, st>>>(s, p->new_key, p->new_value);
     GN_LAUNCH_CHECK();
   }
-  stream_forward_kernel<true><<<dim3(ceil_div(s.max_query, 4), s.Hq, s.rows), 128, 0, st>>>(s, *out, lse);
-  GN_LAUNCH_CHECK();
+  if (tensor) GN_TRY(stream_tc_forward(s, *out, lse, workspace, st));
+  else {
+    stream_forward_kernel<true><<<dim3(ceil_div(s.max_query, 4), s.Hq, s.rows), 128, 0, st>>>(s, *out, lse);
+    GN_LAUNCH_CHECK();
+  }
   if (p->mass_out && s.max_context) {
     stream_mass_kernel<<<dim3(ceil_div(s.max_context, 4), s.Hkv, s.rows), 128, 0, st>>>(s, lse, p->mass, p->mass_out);
     GN_LAUNCH_CHECK();

@@ -1,0 +1,92 @@
+// Streaming attention on the tensor cores: operands, tiles and instructions shared by its kernels.
+//
+// Precision.  kind::f16 multiplies at twice the rate of kind::tf32 with the same 11-bit significand, so a float32 operand x is
+// held as two halves of s x, s a power of two: hi = f16(s x), lo = f16(s x - hi).  Together they keep 22 bits, as the tf32 pair
+// does, in half the bytes.  What f16 lacks is range, hence s: the largest finite |x| of a plane (a sequence and key head) lands
+// in [2^14, 2^15), which leaves every x an absolute error of at most 2^-40 of that largest one (f16's smallest step is 2^-24) or
+// 2^-22 of x, whichever is more.  A product is hi*lo + lo*hi + hi*hi in float32 (lo*lo is below 2^-22), the small terms first: the tensor core
+// cuts each partial sum off instead of rounding it, and a cut of the small terms costs 2^-11 of one of the large ones.
+//
+// Layout.  A packed plane is [64-channel block][hi, lo][row][64 channels], rows of 128 bytes whose 16-byte chunk c sits at chunk
+// c ^ (row % 8): the 128-byte swizzle that tcgen05 reads, laid out by the packing kernel, so that any run of rows from a multiple
+// of 8 is one contiguous bulk copy (no tensor maps), and the same rows serve as K-major operand (contraction over channels) and as
+// MN-major operand (contraction over rows).
+#pragma once
+#include <cuda_fp16.h>
+
+#include "streaming.cuh"
+#include "tcgen05.cuh"
+
+namespace gn {
+
+// Packed planes of one tensor: `rows` = rows of a plane as stored (a multiple of 16, 16 more than the longest sequence rounded up).
+struct Packed {
+  uint8_t* data = nullptr;
+  int rows = 0;
+  __host__ __device__ int64_t plane_bytes(int blocks) const { return (int64_t)blocks * 2 * rows * 128; }
+};
+static inline int packed_rows(int64_t n) { return (int)((n + 15) / 16 * 16 + 16); }
+
+// Keys and values of every (row, kv head) plane, packed, and what the packing found.
+struct PackedKeys {
+  Packed k, v;
+  uint32_t* amax = nullptr;    // [plane][2]: bits of the largest finite |k|, |v|
+  int* odd = nullptr;          // [plane]: a key is non-finite or has no page
+  uint8_t* flags_k = nullptr;  // [plane][k.rows]: kOdd: a component is not finite (stored as 0), kAbsent: no such page
+  uint8_t* flags_v = nullptr;
+};
+constexpr uint8_t kOdd = 1, kAbsent = 2;
+
+// tcgen05 forward of a call (streaming_tc.cu): the workspace it wants, and the launches.
+int64_t stream_tc_forward_bytes(const StreamRows& s);
+int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t stream);
+
+#ifdef __CUDACC__
+namespace {
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// kind::f16, both operands f16, float32 accumulators: [4,6) D format 1, A and B formats 0, [17,23) N>>3, [24,29) M>>4, bit 16: B MN-major.
+__device__ __forceinline__ uint32_t instr_desc_f16(int m, int n, int b_mn) {
+  return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// A in tensor memory: lane = row, a 32-bit column holds two consecutive elements of the contraction index.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// MN-major operand, 128-byte swizzle: 64 channels a row of 128 bytes, 8 contraction rows 1024 bytes (stride offset), the next 64
+// channels `group` bytes on (leading offset).
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t group) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(group >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u; }
+
+// Two floats to hi and lo pairs (the first in the low half).
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// The power of two that brings `amax` (bits of the largest finite magnitude) to [2^14, 2^15), and its inverse.
+__device__ __forceinline__ void plane_scale(uint32_t amax, float& s, float& inverse) {
+  const int e = max((int)(amax >> 23), 27) - 127;   // 0 and what is below 2^-100 scale like 2^-100
+  s = amax == 0 ? 1.0f : __uint_as_float((uint32_t)(14 - e + 127) << 23);
+  inverse = amax == 0 ? 1.0f : __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+}
+
+}  // namespace
+#endif
+
+}  // namespace gn
