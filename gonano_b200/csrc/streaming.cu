@@ -29,25 +29,24 @@ __device__ __forceinline__ const float* key_ptr(const StreamRows& s, bool value,
 }
 
 // A warp per (row, query head, token): online softmax over the keys the query sees.
-template <bool PAGED>
 __global__ void __launch_bounds__(128) stream_forward_kernel(StreamRows s, gn_view out, float* __restrict__ lse) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * 4 + warp, h = blockIdx.y, r = blockIdx.z;
-  const RowSpan sp = row_span<PAGED>(s, r);
-  if (t >= (PAGED ? sp.q_len : s.seq)) return;
+  const RowSpan sp = row_span<true>(s, r);
+  if (t >= sp.q_len) return;
   const int token = sp.q_begin + t;
   float o[kE] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-  if (t < sp.q_len) {
-    const int pos = PAGED ? sp.ctx - sp.q_len + t : t;
+  {
+    const int pos = sp.ctx - sp.q_len + t;
     float q[kE];
-    load_lane<PAGED>(s.q.data + token_offset<PAGED>(s.q, r, h, token), s.D, q);
+    load_lane<true>(s.q.data + token_offset<true>(s.q, r, h, token), s.D, q);
     const Seen see = seen_by(s, pos);
     for (int j = see.sink_end > 0 ? 0 : see.begin; j <= pos; j = (j + 1 == see.sink_end) ? max(see.begin, j + 1) : j + 1) {
-      const float* kp = key_ptr<PAGED>(s, false, r, h / s.G, j);
-      if (PAGED && !kp) continue;
+      const float* kp = key_ptr<true>(s, false, r, h / s.G, j);
+      if (!kp) continue;
       float k[kE], v[kE];
-      load_lane<PAGED>(kp, s.D, k);
-      load_lane<PAGED>(key_ptr<PAGED>(s, true, r, h / s.G, j), s.D, v);
+      load_lane<true>(kp, s.D, k);
+      load_lane<true>(key_ptr<true>(s, true, r, h / s.G, j), s.D, v);
       const float x = dot_lane(q, k) * s.scale, mn = fmaxf(m, x), a = m == -INFINITY ? 0.0f : expf(m - mn), p = x == -INFINITY ? 0.0f : expf(x - mn);
       l = fmaf(l, a, p);
 #pragma unroll
@@ -55,74 +54,11 @@ __global__ void __launch_bounds__(128) stream_forward_kernel(StreamRows s, gn_vi
       m = mn;
     }
   }
-  float* op = out.data + token_offset<PAGED>(out, r, h, token);
+  float* op = out.data + token_offset<true>(out, r, h, token);
 #pragma unroll
   for (int e = 0; e < kE; ++e)
     if (lane + 32 * e < s.D) op[lane + 32 * e] = l == 0.0f ? 0.0f : o[e] / l;
-  if (lane == 0) lse[stat_offset<PAGED>(s, r, h, token)] = l == 0.0f ? -INFINITY : m + logf(l);
-}
-
-// A warp per (row, query head, token): dq = scale sum_j p (do.v - delta) k, and delta = do.o for the kernel below.
-__global__ void __launch_bounds__(128) stream_dq_kernel(StreamRows s, gn_view out, gn_view dout, const float* __restrict__ lse, float* __restrict__ delta,
-                                                        gn_view dq, int accumulate) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x * 4 + warp, h = blockIdx.y, r = blockIdx.z;
-  const RowSpan sp = row_span<false>(s, r);
-  if (t >= s.seq) return;
-  float acc[kE] = {0, 0, 0, 0};
-  if (t < sp.q_len) {
-    float q[kE], g[kE], o[kE];
-    load_lane<false>(s.q.data + token_offset<false>(s.q, r, h, t), s.D, q);
-    load_lane<false>(dout.data + token_offset<false>(dout, r, h, t), s.D, g);
-    load_lane<false>(out.data + token_offset<false>(out, r, h, t), s.D, o);
-    const float dl = dot_lane(g, o), L = lse[stat_offset<false>(s, r, h, t)];
-    if (lane == 0) delta[stat_offset<false>(s, r, h, t)] = dl;
-    const Seen see = seen_by(s, t);
-    for (int j = see.sink_end > 0 ? 0 : see.begin; j <= t; j = (j + 1 == see.sink_end) ? max(see.begin, j + 1) : j + 1) {
-      float k[kE], v[kE];
-      load_lane<false>(key_ptr<false>(s, false, r, h / s.G, j), s.D, k);
-      load_lane<false>(key_ptr<false>(s, true, r, h / s.G, j), s.D, v);
-      const float ds = expf(dot_lane(q, k) * s.scale - L) * (dot_lane(g, v) - dl) * s.scale;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) acc[e] = fmaf(ds, k[e], acc[e]);
-    }
-  }
-  float* p = dq.data + token_offset<false>(dq, r, h, t);
-#pragma unroll
-  for (int e = 0; e < kE; ++e)
-    if (lane + 32 * e < s.D) p[lane + 32 * e] = (accumulate ? p[lane + 32 * e] : 0.0f) + acc[e];
-}
-// A warp per (row, kv head, key): sums over the queries of every head of the group that see the key.
-__global__ void __launch_bounds__(128) stream_dkv_kernel(StreamRows s, gn_view dout, const float* __restrict__ lse, const float* __restrict__ delta, gn_view dk,
-                                                         gn_view dv, int accumulate) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int j = blockIdx.x * 4 + warp, hk = blockIdx.y, r = blockIdx.z;
-  const RowSpan sp = row_span<false>(s, r);
-  if (j >= s.seq) return;
-  float ak[kE] = {0, 0, 0, 0}, av[kE] = {0, 0, 0, 0};
-  if (j < sp.ctx) {
-    float k[kE], v[kE];
-    load_lane<false>(key_ptr<false>(s, false, r, hk, j), s.D, k);
-    load_lane<false>(key_ptr<false>(s, true, r, hk, j), s.D, v);
-    const int end = (s.window < 0 || j < s.sinks) ? sp.q_len : min((int64_t)sp.q_len, (int64_t)j + s.window + 1);
-    for (int h = hk * s.G; h < (hk + 1) * s.G; ++h)
-      for (int t = j; t < end; ++t) {
-        float q[kE], g[kE];
-        load_lane<false>(s.q.data + token_offset<false>(s.q, r, h, t), s.D, q);
-        load_lane<false>(dout.data + token_offset<false>(dout, r, h, t), s.D, g);
-        const int64_t at = stat_offset<false>(s, r, h, t);
-        const float p = expf(dot_lane(q, k) * s.scale - lse[at]), ds = p * (dot_lane(g, v) - delta[at]) * s.scale;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) { ak[e] = fmaf(ds, q[e], ak[e]); av[e] = fmaf(p, g[e], av[e]); }
-      }
-  }
-  float* pk = dk.data + token_offset<false>(dk, r, hk, j); float* pv = dv.data + token_offset<false>(dv, r, hk, j);
-#pragma unroll
-  for (int e = 0; e < kE; ++e)
-    if (lane + 32 * e < s.D) {
-      pk[lane + 32 * e] = (accumulate ? pk[lane + 32 * e] : 0.0f) + ak[e];
-      pv[lane + 32 * e] = (accumulate ? pv[lane + 32 * e] : 0.0f) + av[e];
-    }
+  if (lane == 0) lse[stat_offset<true>(s, r, h, token)] = l == 0.0f ? -INFINITY : m + logf(l);
 }
 
 // A warp per (row, new token, kv head): the new token's key and value go to its slot.
@@ -330,7 +266,7 @@ int workspace_ok(const void* w, int64_t have, int64_t need, const char* what) {
   GN_REQUIRE((reinterpret_cast<uintptr_t>(w) & 15) == 0, "%s: workspace not 16-byte aligned", what);
   return on_this_device(w, what);
 }
-int64_t sink_bytes(const StreamRows& s, int backward) { return backward ? (int64_t)s.rows * s.Hq * s.seq * 4 : stream_tc_forward_bytes(s); }
+int64_t sink_bytes(const StreamRows& s, int backward) { return backward ? stream_tc_backward_bytes(s) : stream_tc_forward_bytes(s); }
 // New tokens over a paged cache: a single token per row runs on the warp-per-row kernel, chunks on the tensor cores.
 bool paged_on_tensor_cores(const StreamRows& s) { return (int64_t)s.max_query * s.G > 16; }
 
@@ -395,13 +331,7 @@ int gn_attention_sink_backward(const gn_sink_params* p, const gn_view* out, cons
   const void* ptrs[] = {out->data, out_grad->data, lse, dq->data, dk->data, dv->data};
   for (const void* x : ptrs) GN_TRY(on_this_device(x, "attention_sink_backward"));
   GN_TRY(workspace_ok(workspace, workspace_bytes, sink_bytes(s, 1), "attention_sink_backward"));
-  cudaStream_t st = (cudaStream_t)stream;
-  float* delta = static_cast<float*>(workspace);
-  stream_dq_kernel<<<dim3(ceil_div(s.seq, 4), s.Hq, s.rows), 128, 0, st>>>(s, *out, *out_grad, lse, delta, *dq, accumulate);
-  GN_LAUNCH_CHECK();
-  stream_dkv_kernel<<<dim3(ceil_div(s.seq, 4), s.Hkv, s.rows), 128, 0, st>>>(s, *out_grad, lse, delta, *dk, *dv, accumulate);
-  GN_LAUNCH_CHECK();
-  return GN_OK;
+  return stream_tc_backward(s, *out, *out_grad, lse, *dq, *dk, *dv, accumulate, workspace, (cudaStream_t)stream);
 }
 
 int gn_attention_paged_workspace(const gn_paged_params* p, int64_t* bytes) {
@@ -433,7 +363,7 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
   }
   if (tensor) GN_TRY(stream_tc_forward(s, *out, lse, workspace, st));
   else {
-    stream_forward_kernel<true><<<dim3(ceil_div(s.max_query, 4), s.Hq, s.rows), 128, 0, st>>>(s, *out, lse);
+    stream_forward_kernel<<<dim3(ceil_div(s.max_query, 4), s.Hq, s.rows), 128, 0, st>>>(s, *out, lse);
     GN_LAUNCH_CHECK();
   }
   if (p->mass_out && s.max_context) {

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256) stream_amax_kernel(const __grid_constant_
 }
 
 template <int CB, bool PAGED>
-__global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, int vec) {
+__global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, uint32_t* norms, int vec) {
   const int hk = blockIdx.y, r = blockIdx.z >> 1, value = blockIdx.z & 1, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const RowSpan sp = row_span<PAGED>(s, r);
   const int begin = first_needed<PAGED>(s, sp), j0 = blockIdx.x * kPackRows;
@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
   uint8_t* flags = (value ? pk.flags_v : pk.flags_k) + plane * dst.rows;
   float sc, inv;
   plane_scale(pk.amax[plane * 2 + value], sc, inv);
+  float top = 0.0f;
 #pragma unroll 2
   for (int u = 0; u < kPackRows / 16; ++u) {
     const int j = j0 + u * 16 + half;
@@ -95,6 +96,14 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
     for (int e = 0; e < 4 * CB; ++e) if (!finite_bits(x[e])) { odd = true; x[e] = 0.0f; }
     const uint32_t odds = __ballot_sync(0xffffffffu, odd);
     if ((odds >> (threadIdx.x & 16)) & 0xffffu) flag |= kOdd;
+    if (norms && value) {
+      float sq = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4 * CB; ++e) sq = fmaf(x[e] * sc, x[e] * sc, sq);
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
+      top = fmaxf(top, sq);
+    }
     if (j >= last || (!needed && j < sp.ctx)) continue;
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
@@ -110,6 +119,10 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
       if (flag) pk.odd[plane] = 1;
     }
   }
+  if (norms && value) {
+    top = warp_max(top);
+    if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(norms + plane * 2, __float_as_uint(top));
+  }
 }
 
 // ------------------------------------------------------------------ forward
@@ -124,25 +137,11 @@ struct ForwardTc {
 
 constexpr int kRowsT = 128;      // query rows of a CTA = keys of a tile = UMMA M and N
 constexpr int kThreads = 320;    // 8 softmax warps, the issuing warp, the copying warp
-constexpr float kWeightShift = 12.0f;   // weights are held as 2^12 p: f16 pairs then reach 2^-37 of a row's largest
-
-// Registers of a key tile's place in the two runs of keys: virtual key c is key c below a_len and key c + shift from there.
-struct KeyRuns { int a_len, shift, total; };
-__device__ __forceinline__ KeyRuns key_runs(const StreamRows& s, int pos0, int pos1) {
-  KeyRuns k{0, 0, 0};
-  if (pos1 < 0) return k;
-  const int begin = (s.window < 0 ? 0 : max(0, pos0 - s.window)) & ~7, sinks8 = (min(s.sinks, pos1 + 1) + 7) & ~7;
-  if (sinks8 == 0) k.shift = begin;
-  else if (begin > sinks8) { k.a_len = sinks8; k.shift = begin - sinks8; }
-  k.total = pos1 + 1 - k.shift;
-  return k;
-}
-__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 // One CTA per (128 query rows, kv head, row, key split), 320 threads:
 //   warps 0-7  two threads per query row, 64 keys of a tile and half the channels each.  They convert Q once (raw float32 rows to
 //              the swizzled hi / lo tile), then per tile read S from tensor memory, take the running maximum, and write
-//              2^12 p as f16 pairs over the scores they came from: P is the A operand of O = P V straight from tensor memory.
+//              2^15 p as f16 pairs over the scores they came from: P is the A operand of O = P V straight from tensor memory.
 //              Each tile's O starts from zero in one of two buffers and is added to float32 registers one tile later, where the
 //              rescaling by the grown maximum costs nothing extra: sums over many keys are rounded, not cut off.
 //   warp 8     issues S_{j+1} = Q K^T (24 instructions of 128 x 128 x 16), then O_j = P_j V, so that the tensor pipe works on the
@@ -305,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       plane_scale(top, sq, iq);
       plane_scale(p.pk.amax[plane * 2], sk, ik);
       // a negative scale goes into Q, so that larger products are larger scores; a vanishing one stays a positive number
-      c = fmaxf(fabsf(s.scale) * 1.4426950408889634f * iq * ik, 1e-30f);
+      c = fmaxf(fabsf(s.scale) * kLog2e * iq * ik, 1e-30f);
       if (s.scale < 0.0f) sq = -sq;
 #pragma unroll
       for (int e = 0; e < HC; e += 8) {
@@ -432,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
           for (int i = 0; i < 4; ++i) if (ch + i < s.D) dst[ch + i] = o[e + i] * z;
         }
       }
-      if (half == 0) p.lse[stat_offset<PAGED>(s, r, hk * s.G + g, token)] = L * 0.6931471805599453f;
+      if (half == 0) p.lse[stat_offset<PAGED>(s, r, hk * s.G + g, token)] = L * kLn2;
     }
   }
   tc_fence_before();
@@ -466,18 +465,10 @@ __global__ void __launch_bounds__(256) stream_tc_combine_kernel(const __grid_con
   const float z = bad ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e) if (lane + 32 * e < s.D) dst[lane + 32 * e] = o[e] * z;
-  if (lane == 0) p.lse[stat_offset<PAGED>(s, r, h, token)] = bad ? NAN : sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+  if (lane == 0) p.lse[stat_offset<PAGED>(s, r, h, token)] = bad ? NAN : sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 // ------------------------------------------------------------------ host
-struct Carve {   // workspace layout; with a null base it only counts
-  uint8_t* base; int64_t used = 0;
-  template <typename T> T* take(int64_t n) {
-    T* at = base ? reinterpret_cast<T*>(base + used) : nullptr;
-    used += (n * (int64_t)sizeof(T) + 127) / 128 * 128;
-    return at;
-  }
-};
 struct Plan { int DP, tiles, splits; int64_t planes, max_q, max_k; };
 Plan plan_forward(const StreamRows& s) {
   Plan pl;
@@ -511,26 +502,27 @@ int64_t carve_forward(const StreamRows& s, const Plan& pl, void* workspace, Forw
   }
   return c.used;
 }
-bool vec_view(const gn_view& v, int D) {
-  return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && D % 4 == 0 && v.batch_stride % 4 == 0 && v.head_stride % 4 == 0 && v.token_stride % 4 == 0;
-}
 bool vec_keys(const StreamRows& s) {
   if (!s.paged()) return vec_view(s.k, s.D) && vec_view(s.v, s.D);
   return s.D % 4 == 0 && ((reinterpret_cast<uintptr_t>(s.pages_k) | reinterpret_cast<uintptr_t>(s.pages_v)) & 15) == 0;
+}
+
+template <int CB, bool PAGED>
+int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t st) {
+  const int vec = vec_keys(s), keys = pk.k.rows;
+  stream_amax_kernel<CB, PAGED><<<dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, vec);
+  GN_LAUNCH_CHECK();
+  stream_pack_kernel<CB, PAGED><<<dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, norms, vec);
+  GN_LAUNCH_CHECK();
+  return GN_OK;
 }
 
 template <int DP, bool PAGED>
 int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t st) {
   constexpr int CB = DP / 64, STAGES = DP == 64 ? 2 : 1;
   constexpr int kSmem = CB * 32768 * (1 + 2 * STAGES) + 256 + 2048 + 1024;
-  const int vec = vec_keys(s);
   GN_CUDA(cudaMemsetAsync(f.pk.amax, 0, pl.planes * 3 * sizeof(uint32_t), st));
-  if (pl.max_k > 0) {
-    stream_amax_kernel<CB, PAGED><<<dim3(ceil_div(pl.max_k, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, f.pk, vec);
-    GN_LAUNCH_CHECK();
-    stream_pack_kernel<CB, PAGED><<<dim3(ceil_div(f.pk.k.rows, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, f.pk, vec);
-    GN_LAUNCH_CHECK();
-  }
+  GN_TRY(stream_pack_keys(s, f.pk, nullptr, st));
   static PerDeviceOnce once;
   if (once.first()) GN_CUDA(cudaFuncSetAttribute(stream_tc_forward_kernel<DP, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   stream_tc_forward_kernel<DP, PAGED><<<dim3(pl.tiles * pl.splits, s.Hkv, s.rows), kThreads, kSmem, st>>>(f);
@@ -543,6 +535,11 @@ int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t s
 }
 
 }  // namespace
+
+int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t st) {
+  if (s.D <= 64) return s.paged() ? pack_go<1, true>(s, pk, norms, st) : pack_go<1, false>(s, pk, norms, st);
+  return s.paged() ? pack_go<2, true>(s, pk, norms, st) : pack_go<2, false>(s, pk, norms, st);
+}
 
 int64_t stream_tc_forward_bytes(const StreamRows& s) {
   ForwardTc f{};

@@ -37,9 +37,32 @@ struct PackedKeys {
 };
 constexpr uint8_t kOdd = 1, kAbsent = 2;
 
+constexpr float kWeightShift = 15.0f;   // weights are held as 2^15 p (p <= 1): f16 pairs then reach 2^-40
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Carve {   // workspace layout; with a null base it only counts
+  uint8_t* base; int64_t used = 0;
+  template <typename T> T* take(int64_t n) {
+    T* at = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += (n * (int64_t)sizeof(T) + 127) / 128 * 128;
+    return at;
+  }
+};
+// Whether float4 accesses fit a view of head_dim D.
+static inline bool vec_view(const gn_view& v, int D) {
+  return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && D % 4 == 0 && v.batch_stride % 4 == 0 && v.head_stride % 4 == 0 && v.token_stride % 4 == 0;
+}
+// Packs keys and values (amax and odd cleared by the caller on the stream).  norms: null, or [plane][2]: [0] receives the bits of the
+// largest squared norm of a scaled value row.
+int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t stream);
+
 // tcgen05 forward of a call (streaming_tc.cu): the workspace it wants, and the launches.
 int64_t stream_tc_forward_bytes(const StreamRows& s);
 int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t stream);
+// tcgen05 backward (streaming_tc_backward.cu), padded batches.
+int64_t stream_tc_backward_bytes(const StreamRows& s);
+int stream_tc_backward(const StreamRows& s, const gn_view& out, const gn_view& dout, const float* lse, const gn_view& dq, const gn_view& dk, const gn_view& dv,
+                       int accumulate, void* workspace, cudaStream_t stream);
 
 #ifdef __CUDACC__
 namespace {
@@ -84,6 +107,21 @@ __device__ __forceinline__ void plane_scale(uint32_t amax, float& s, float& inve
   const int e = max((int)(amax >> 23), 27) - 127;   // 0 and what is below 2^-100 scale like 2^-100
   s = amax == 0 ? 1.0f : __uint_as_float((uint32_t)(14 - e + 127) << 23);
   inverse = amax == 0 ? 1.0f : __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+}
+
+__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
+
+// The keys that the queries at positions pos0 .. pos1 see, as two runs: virtual key c is key c below a_len and key c + shift from
+// there.  Runs start at multiples of 8.
+struct KeyRuns { int a_len, shift, total; };
+__device__ __forceinline__ KeyRuns key_runs(const StreamRows& s, int pos0, int pos1) {
+  KeyRuns k{0, 0, 0};
+  if (pos1 < 0) return k;
+  const int begin = (s.window < 0 ? 0 : max(0, pos0 - s.window)) & ~7, sinks8 = (min(s.sinks, pos1 + 1) + 7) & ~7;
+  if (sinks8 == 0) k.shift = begin;
+  else if (begin > sinks8) { k.a_len = sinks8; k.shift = begin - sinks8; }
+  k.total = pos1 + 1 - k.shift;
+  return k;
 }
 
 }  // namespace

@@ -4,7 +4,12 @@ Tolerances.  A score is a product of head_dim terms: operands kept to 22 bits, t
 e = 2^-19 |scale| |q| |k| (22-bit operands 2 * 2^-22, the product of the parts below 22 bits 2^-22, at most 24 roundings of a
 partial sum 24 * 2^-24, together below 2^-19).  A weight is then off by at most 2 e relative (numerator and sum), an output by
 (2 e + 2^-18) sum p |v| with the same 2^-18 > 2^-19 + 2^-20 for its own product and the sum of the weights.  Gradients propagate
-these bounds term by term in `backward_bounds`.  The largest possible errors add up; measured ones are far below.
+these bounds term by term in `window_reference`.  The largest possible errors add up; measured ones are far below.
+
+Operands that go through f16 pairs (high and low part of a scaled value) have, beside the relative bound, a smallest step: f16's
+is 2^-24, so a pair is off by up to 2^-25.  A weight is held as 2^15 p: off by up to FLOOR = 2^-40, whatever p.  A tensor's entry is held
+times a power of two that brings its sequence's largest to 2^14 or more: off by up to 2^-39 of the largest.  dS is held times
+2^(14 - e), max|dO| max|V| < 2^e <= 2 max|dO| max|V|: off by up to 2^-25 2^(e - 14) <= 2^-38 max|dO| max|V|.
 """
 import itertools
 import math
@@ -17,6 +22,7 @@ from gonano_b200 import _lib, streaming  # noqa: E402
 from gonano_b200._lib import GonanoError  # noqa: E402
 
 PRODUCT = 2.0 ** -18
+FLOOR = 2.0 ** -40
 DEVICE = "cuda"
 
 
@@ -67,7 +73,8 @@ def window_reference(q, k, v, dout, lengths, window, sinks, scale):
         mine = slice(h * g, (h + 1) * g)
         qq, kk, vv, do = q[b, mine, :n], k[b, h, :n], v[b, h, :n], dout[b, mine, :n]
         at = torch.arange(n, device=q.device)
-        out, lse, w = attend64(qq, kk, vv, visible(at, at, window, sinks), scale)
+        see = visible(at, at, window, sinks)
+        out, lse, w = attend64(qq, kk, vv, see, scale)
         dp = torch.einsum("gnd,md->gnm", do, vv) - (do * out).sum(-1, keepdim=True)
         ds = w * dp
         res["out"][b, mine, :n], res["lse"][b, mine, :n] = out, lse
@@ -75,14 +82,17 @@ def window_reference(q, k, v, dout, lengths, window, sinks, scale):
         res["dk"][b, h, :n] = scale * torch.einsum("gnm,gnd->md", ds, qq)
         res["dv"][b, h, :n] = torch.einsum("gnm,gnd->md", w, do)
         e = 2 * score_bound(qq, kk, scale)
-        bounds["out"][b, mine, :n] = (e + PRODUCT) * torch.einsum("gnm,md->gnd", w, vv.abs())
+        big = [float(x.abs().max()) for x in (qq, kk, vv, do)]
+        seen = see.double().expand(w.shape)
+        bounds["out"][b, mine, :n] = (e + PRODUCT) * torch.einsum("gnm,md->gnd", w, vv.abs()) + FLOOR * (torch.einsum("gnm,md->gnd", seen, vv.abs()) + 2 * big[2])
         bounds["lse"][b, mine, :n] = (e + PRODUCT) * (1 + lse.abs())
         # ds: the weight's error, and that of dO.v - dO.o (a product each, and the error of o)
         reach = do.norm(dim=-1, keepdim=True) * float(vv.norm(dim=-1).max())
-        eds = w * (e * dp.abs() + (e + 2 * PRODUCT) * reach) + PRODUCT * ds.abs()
-        bounds["dq"][b, mine, :n] = abs(scale) * torch.einsum("gnm,md->gnd", eds, kk.abs())
-        bounds["dk"][b, h, :n] = abs(scale) * torch.einsum("gnm,gnd->md", eds, qq.abs())
-        bounds["dv"][b, h, :n] = (e + PRODUCT) * torch.einsum("gnm,gnd->md", w, do.abs())
+        eds = w * (e * dp.abs() + (e + 2 * PRODUCT) * reach) + PRODUCT * ds.abs() + seen * (FLOOR * dp.abs() + 4 * FLOOR * float(reach.max()))
+        bounds["dq"][b, mine, :n] = abs(scale) * torch.einsum("gnm,md->gnd", eds, kk.abs()) + abs(scale) * 2 * FLOOR * big[1] * ds.abs().sum(-1, keepdim=True)
+        bounds["dk"][b, h, :n] = abs(scale) * torch.einsum("gnm,gnd->md", eds, qq.abs()) + abs(scale) * 2 * FLOOR * big[0] * ds.abs().sum((0, 1))[:, None]
+        bounds["dv"][b, h, :n] = (e + PRODUCT) * torch.einsum("gnm,gnd->md", w, do.abs()) + FLOOR * torch.einsum("gnm,gnd->md", seen, do.abs()) \
+            + 2 * FLOOR * big[3] * w.sum((0, 1))[:, None]
     return res, bounds
 
 
@@ -309,7 +319,7 @@ def check_paged(counts, lens, heads, kv_heads, dim, page, window, sinks, mass=Tr
             qq = q[b:e, heads_of].double().transpose(0, 1)
             o, l, w = attend64(qq, k64[:, h], v64[:, h], see, scale)
             eb = 2 * score_bound(qq, k64[:, h], scale) if qq.numel() else 0.0
-            close(out[b:e, heads_of].transpose(0, 1), o, (eb + PRODUCT) * torch.einsum("gnm,md->gnd", w, v64[:, h].abs()), f"out of row {r}")
+            close(out[b:e, heads_of].transpose(0, 1), o, (eb + PRODUCT) * torch.einsum("gnm,md->gnd", w, v64[:, h].abs()) + FLOOR * (n + 2) * float(v64.abs().max() if n else 0), f"out of row {r}")
             close(lse[b:e, heads_of].transpose(0, 1), l, (eb + PRODUCT) * (1 + l.abs()), f"lse of row {r}")
             if mass:
                 added = w.sum((0, 1))
@@ -551,7 +561,7 @@ def test_rollout_with_eviction():
                 o, l, w = attend64(qq, held[r][h], held[r][kv_heads + h], visible(pos, torch.arange(n, device=DEVICE), -1, 0), 0.125)
                 if c:
                     e = 2 * score_bound(qq, held[r][h], 0.125) + PRODUCT
-                    close(out[at:at + c, h * g:(h + 1) * g].transpose(0, 1), o, e * torch.einsum("gnm,md->gnd", w, held[r][kv_heads + h].abs()), "out")
+                    close(out[at:at + c, h * g:(h + 1) * g].transpose(0, 1), o, e * torch.einsum("gnm,md->gnd", w, held[r][kv_heads + h].abs()) + FLOOR * (n + 2) * float(held[r][kv_heads + h].abs().max()), "out")
                     close(lse[at:at + c, h * g:(h + 1) * g].transpose(0, 1), l, e * (1 + l.abs()), "lse")
                 mass[r][h] = torch.cat([mass[r][h], torch.zeros(c, dtype=torch.float64, device=DEVICE)]) + w.sum((0, 1))
             at += c
