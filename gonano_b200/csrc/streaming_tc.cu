@@ -135,308 +135,376 @@ struct ForwardTc {
   float* part_o; float* part_l;   // splits > 1: [plane][tile][split][128] rows of DP channels, and their log2-sum-exps
 };
 
-constexpr int kRowsT = 128;      // query rows of a CTA = keys of a tile = UMMA M and N
-constexpr int kThreads = 320;    // 8 softmax warps, the issuing warp, the copying warp
+constexpr int kRowsT = 128;      // query rows of an item = keys of a tile = UMMA M and N
+constexpr int kThreads = 768;    // four softmax warpgroups, one that fetches Q, one with the issuing and the copying warp
+constexpr int kRegsSoftmax = 88, kRegsFetch = 72, kRegsOther = 56;   // shares of the launch's 6 x 80
 
-// One CTA per (128 query rows, kv head, row, key split), 320 threads:
-//   warps 0-7  two threads per query row, 64 keys of a tile and half the channels each.  They convert Q once (raw float32 rows to
-//              the swizzled hi / lo tile), then per tile read S from tensor memory, take the running maximum, and write
-//              2^15 p as f16 pairs over the scores they came from: P is the A operand of O = P V straight from tensor memory.
-//              Each tile's O starts from zero in one of two buffers and is added to float32 registers one tile later, where the
-//              rescaling by the grown maximum costs nothing extra: sums over many keys are rounded, not cut off.
-//   warp 8     issues S_{j+1} = Q K^T (24 instructions of 128 x 128 x 16), then O_j = P_j V, so that the tensor pipe works on the
-//              next scores while the softmax threads work on these;
-//   warp 9     copies K and V tiles (bulk copies of packed rows) as their buffers fall free.
-// Tensor memory: two score / weight buffers of 128 columns, two O buffers of 128.  Shared memory: Q, K, V tiles, hi and lo.
-// Bound: 48 instructions of 64 cycles a tile = 3072 cycles of tensor pipe.  Every wait is bounded; a kernel whose wait ran out
-// writes NaN.
+// What a CTA works on next: 128 query rows of a plane against a range of their key tiles.
+struct Item {
+  int r, hk, tile, split, f0, nf, first, q_begin, j0, n;   // first: position of the row's first new token; n key tiles from j0
+  bool inside;                                             // the rows exist (a padded batch's padding does)
+  int64_t plane;
+  KeyRuns runs;
+  __device__ __forceinline__ int rows16(int j) const { return min(kRowsT, (runs.total - (j0 + j) * kRowsT + 15) & ~15); }   // keys of tile j, in 16s
+};
+template <bool PAGED>
+__device__ __forceinline__ Item get_item(const ForwardTc& p, int64_t w) {
+  const StreamRows& s = p.s;
+  Item it;
+  const int64_t planes = (int64_t)s.rows * s.Hkv, level = w / planes;   // the last tiles first: under a causal mask they are the longest
+  it.plane = w - level * planes;
+  it.split = (int)(level % p.splits); it.tile = p.tiles - 1 - (int)(level / p.splits);
+  it.r = (int)(it.plane / s.Hkv); it.hk = (int)(it.plane - (int64_t)it.r * s.Hkv);
+  const RowSpan sp = row_span<PAGED>(s, it.r);
+  it.f0 = it.tile * kRowsT; it.nf = sp.q_len * s.G; it.first = sp.ctx - sp.q_len; it.q_begin = sp.q_begin;
+  it.inside = it.f0 < (PAGED ? it.nf : s.seq * s.G);
+  it.runs = KeyRuns{0, 0, 0};
+  if (it.f0 < it.nf) it.runs = key_runs(s, it.first + it.f0 / s.G, it.first + min(it.f0 + kRowsT - 1, it.nf - 1) / s.G);
+  const int all = (it.runs.total + kRowsT - 1) / kRowsT, per = (all + p.splits - 1) / p.splits;
+  it.j0 = it.split * per; it.n = max(0, min(all, it.j0 + per) - it.j0);
+  return it;
+}
+
+// A persistent CTA per SM walks the items; no role waits for an item to end before it begins the next:
+//   warps 0-15  four threads per query row, 32 keys of a tile and a quarter of the channels each: read S from tensor memory, take the
+//               running maximum, and write 2^15 p as f16 pairs over the scores they came from: P is the A operand of O = P V
+//               straight from tensor memory.  Each tile's O starts from zero and is added to float32 registers one tile later, where the
+//               rescaling by the grown maximum costs nothing extra: sums over many keys are rounded, not cut off.  An item's
+//               result is stored in the shadow of the next item's first products;
+//   warps 16-19 fetch the next item's Q rows (raw float32), scale, split and leave them in tensor memory (A operand of S = Q K^T);
+//   warps 20, 22  issue the instructions, 24 of 128 x 128 x 16 for a tile's S and 24 for its O: each a queue of its own, so that the
+//               waits of one pass while the other's instructions run;
+//   warp 21     copies K and V tiles (bulk copies of packed rows) through a ring of tile buffers.
+// Tensor memory: two score / weight buffers of 128 columns, O 128, Q hi and lo 128.  Code is kept short: warps that run through
+// long unrolled code once a tile wait for instructions most of the time.  Sixteen warps, because eight took 3360 cycles a tile
+// (read 530, meet 250, weights 1650, O 850) against the 3072 = 48 x 64 of the tensor pipe, which is the bound.  Every wait is
+// bounded; a kernel whose wait ran out writes NaN.
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __grid_constant__ ForwardTc p) {
-  constexpr int CB = DP / 64, HC = DP / 2, STAGES = DP == 64 ? 2 : 1;
-  constexpr uint32_t TILE = CB * 32768u, OFF_K = TILE, OFF_V = TILE + STAGES * TILE, BARS = OFF_V + STAGES * TILE, XCH = BARS + 256;
+  constexpr int CB = DP / 64, QC = DP / 4, RING = DP == 64 ? 6 : 3;
+  constexpr uint32_t TILE = CB * 32768u, BARS = RING * TILE, ROWC = BARS + 256, XCH = ROWC + 2048;
+  constexpr uint32_t COL_O = 256, COL_Q = 384;
   extern __shared__ uint8_t smem_raw[];
   const StreamRows& s = p.s;
-  const int hk = blockIdx.y, r = blockIdx.z, sp_i = blockIdx.x % p.splits, tile = p.tiles - 1 - (int)blockIdx.x / p.splits;   // the long tiles first
-  const RowSpan sp = row_span<PAGED>(s, r);
-  const int f0 = tile * kRowsT, nf = sp.q_len * s.G;
-  if (f0 >= (PAGED ? nf : s.seq * s.G)) return;
-  const int first = sp.ctx - sp.q_len;   // position of the row's first new token
-  KeyRuns runs{0, 0, 0};
-  if (f0 < nf) runs = key_runs(s, first + f0 / s.G, first + min(f0 + kRowsT - 1, nf - 1) / s.G);
-  const int all = (runs.total + kRowsT - 1) / kRowsT, per = (all + p.splits - 1) / p.splits;
-  const int j0 = sp_i * per, n = max(0, min(all, j0 + per) - j0);
-  const int64_t plane = (int64_t)r * s.Hkv + hk;
-
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bars = base + BARS;
-  const uint32_t q_full = bars;
-  auto k_full = [&](int i) { return bars + 8u + 8u * i; };
-  auto k_empty = [&](int i) { return bars + 24u + 8u * i; };
-  auto v_full = [&](int i) { return bars + 40u + 8u * i; };
-  auto v_empty = [&](int i) { return bars + 56u + 8u * i; };
-  auto s_full = [&](int i) { return bars + 72u + 8u * i; };
-  auto p_full = [&](int i) { return bars + 88u + 8u * i; };
-  auto o_full = [&](int i) { return bars + 104u + 8u * i; };
-  auto o_empty = [&](int i) { return bars + 120u + 8u * i; };
-  const uint32_t tmem_slot = bars + 136;
+  auto full = [&](int i) { return bars + 8u * i; };
+  auto empty = [&](int i) { return bars + 48u + 8u * i; };
+  auto s_full = [&](int i) { return bars + 96u + 8u * i; };
+  auto p_full = [&](int i) { return bars + 112u + 8u * i; };
+  const uint32_t o_full = bars + 128, o_empty = bars + 136, q_ready = bars + 144, q_free = bars + 152, tmem_slot = bars + 160;
+  auto s_free = [&](int i) { return bars + 168u + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 256);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(k_full(i), 1); mbar_init(k_empty(i), 1); mbar_init(v_full(i), 1); mbar_init(v_empty(i), 1);
-      mbar_init(s_full(i), 1); mbar_init(p_full(i), 256); mbar_init(o_full(i), 1); mbar_init(o_empty(i), 256);
-    }
+    for (int i = 0; i < RING; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(s_full(i), 1); mbar_init(p_full(i), 512); mbar_init(s_free(i), 1); }
+    mbar_init(o_full, 1); mbar_init(o_empty, 512); mbar_init(q_ready, 128); mbar_init(q_free, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 20) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 136);
-  auto rows16 = [&](int j) { return min(kRowsT, (runs.total - (j0 + j) * kRowsT + 15) & ~15); };   // keys of tile j, in 16s
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 160);
+  const int64_t items = (int64_t)s.rows * s.Hkv * p.tiles * p.splits;
 
-  if (warp == 9) {
-    // ------------------------------------------------------------- copies
-    if (lane == 0) {
+  if (warp >= 20) {
+    regs_dec<kRegsOther>();
+    if (warp == 21 && lane == 0) {
+      // ------------------------------------------------------------- copies: K_0, K_1, V_0, K_2, V_1, ... as they are used
       bool ok = true;
-      auto copy_tile = [&](const Packed& src, uint32_t dst, uint32_t bar, int j) {
-        const int c0 = (j0 + j) * kRowsT, rows = rows16(j), na = min(max(runs.a_len - c0, 0), rows), nb = rows - na;
-        const uint8_t* from = src.data + plane * src.plane_bytes(CB);
-        mbar_expect_tx(bar, (uint32_t)CB * 2u * rows * 128u);
-#pragma unroll
-        for (int b = 0; b < CB * 2; ++b) {
-          if (na) bulk_load(dst + b * 16384, from + ((int64_t)b * src.rows + c0) * 128, na * 128, bar);
-          if (nb) bulk_load(dst + b * 16384 + na * 128, from + ((int64_t)b * src.rows + c0 + na + runs.shift) * 128, nb * 128, bar);
+      int slot = 0; uint32_t turn = 0;
+      for (int64_t w = blockIdx.x; w < items && ok; w += gridDim.x) {
+        const Item it = get_item<PAGED>(p, w);
+        for (int m = 0; m < 2 * it.n && ok; ++m) {
+          const bool value = m == 2 * it.n - 1 || (m > 0 && (m & 1) == 0);
+          const int j = value ? (m == 2 * it.n - 1 ? it.n - 1 : (m >> 1) - 1) : (m + 1) >> 1;
+          if (turn > 0) ok = mbar_wait(empty(slot), (turn - 1) & 1);
+          if (!ok) break;
+          const Packed& src = value ? p.pk.v : p.pk.k;
+          const int c0 = (it.j0 + j) * kRowsT, rows = it.rows16(j), na = min(max(it.runs.a_len - c0, 0), rows), nb = rows - na;
+          const uint8_t* from = src.data + it.plane * src.plane_bytes(CB) + (int64_t)c0 * 128;
+          uint32_t dst = base + slot * TILE;
+          mbar_expect_tx(full(slot), (uint32_t)CB * 2u * rows * 128u);
+#pragma unroll 1
+          for (int b = 0; b < CB * 2; ++b) {
+            if (na) bulk_load(dst, from, na * 128, full(slot));
+            if (nb) bulk_load(dst + na * 128, from + (int64_t)(na + it.runs.shift) * 128, nb * 128, full(slot));
+            dst += 16384; from += (int64_t)src.rows * 128;
+          }
+          if (++slot == RING) { slot = 0; ++turn; }
         }
-      };
-      int jk = 0, jv = 0;
-      for (uint32_t idle = 0; jv < n && ok;) {   // whichever buffer is free next
-        bool did = false;
-        if (jk < n && (jk < STAGES || mbar_test(k_empty(jk % STAGES), (jk / STAGES - 1) & 1))) {
-          copy_tile(p.pk.k, base + OFF_K + (jk % STAGES) * TILE, k_full(jk % STAGES), jk);
-          ++jk; did = true;
-        }
-        if (jv < jk && (jv < STAGES || mbar_test(v_empty(jv % STAGES), (jv / STAGES - 1) & 1))) {
-          copy_tile(p.pk.v, base + OFF_V + (jv % STAGES) * TILE, v_full(jv % STAGES), jv);
-          ++jv; did = true;
-        }
-        if (did) idle = 0;
-        else if (++idle > kSpinLimit) ok = false;
-        else if (idle > 4096) __nanosleep(64);
       }
       if (!ok)   // copies in flight land before the CTA goes
-        for (int st = 0; st < STAGES; ++st)
-          for (int ph = 0; ph < 2; ++ph) { mbar_wait(k_full(st), ph); mbar_wait(v_full(st), ph); }
+        for (int i = 0; i < RING; ++i) { mbar_wait(full(i), 0); mbar_wait(full(i), 1); }
     }
-  } else if (warp == 8) {
-    // ------------------------------------------------------------- instructions
-    if (lane == 0 && n > 0) {
-      bool ok = mbar_wait(q_full, 0);
-      auto scores = [&](int j) {
-        const int st = j % STAGES;
-        ok = ok && mbar_wait(k_full(st), (j / STAGES) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t d = tmem + (j & 1) * 128, id = instr_desc_f16(128, rows16(j), 0);
-        const uint32_t q = base, k = base + OFF_K + st * TILE;
-        auto one = [&](int ks, int ql, int kl, uint32_t acc) {
-          const uint32_t in = (ks >> 2) * 32768u;
-          umma_f16(d, smem_desc_sw128(q + in + ql * 16384) + 2u * (ks & 3), smem_desc_sw128(k + in + kl * 16384) + 2u * (ks & 3), id, acc);
-        };
-#pragma unroll
-        for (int ks = 0; ks < CB * 4; ++ks) { one(ks, 1, 0, ks > 0); one(ks, 0, 1, 1); }
-#pragma unroll
-        for (int ks = 0; ks < CB * 4; ++ks) one(ks, 0, 0, 1);
-        umma_commit(k_empty(st));
-        umma_commit(s_full(j & 1));
-      };
-      scores(0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) scores(j + 1);
-        const int st = j % STAGES, b = j & 1;
-        ok = ok && mbar_wait(p_full(b), (j >> 1) & 1) && mbar_wait(v_full(st), (j / STAGES) & 1) && (j < 2 || mbar_wait(o_empty(b), ((j >> 1) - 1) & 1));
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t d = tmem + 256 + b * 128, w = tmem + b * 128, id = instr_desc_f16(128, DP, 1), v = base + OFF_V + st * TILE;
-        const int slices = rows16(j) >> 4;
-        auto one = [&](int ks, int wl, int vl, uint32_t acc) {
-          umma_f16_ts(d, w + (ks >> 2) * 64 + wl * 32 + (ks & 3) * 8, smem_desc_mn(v + vl * 16384 + ks * 2048, 32768), id, acc);
-        };
-        for (int ks = 0; ks < slices; ++ks) { one(ks, 1, 0, ks > 0); one(ks, 0, 1, 1); }
-        for (int ks = 0; ks < slices; ++ks) one(ks, 0, 0, 1);
-        umma_commit(v_empty(st));
-        umma_commit(o_full(b));
+    if (warp == 20 || warp == 22) {
+      // ------------------------------------------------------------- instructions
+      const uint32_t el = elect_lane();
+      const bool products = warp == 22;   // O = P V; the other warp S = Q K^T
+      bool ok = true;
+      uint32_t tile = 0, count = 0, ring = 0;   // tiles, items and copies so far
+      Item it = get_item<PAGED>(p, blockIdx.x);   // the grid is no larger than the number of items
+      for (int64_t w = blockIdx.x; w < items && ok;) {
+        const int n = it.n, last16 = n > 0 ? it.rows16(n - 1) : 0;
+        w += gridDim.x;
+        if (w < items) it = get_item<PAGED>(p, w);   // the next item's geometry is on its way while this one runs
+        if (n == 0) continue;
+        if (!products) ok = mbar_wait(q_ready, count & 1);
+        for (int j = 0; j < n && ok; ++j, ++tile) {
+          const int rows = j + 1 == n ? last16 : kRowsT, b = tile & 1;
+          const uint32_t m = ring + (products ? min(2 * j + 2, 2 * n - 1) : j == 0 ? 0 : 2 * j - 1), slot = m % RING;
+          ok = mbar_wait(full(slot), (m / RING) & 1);
+          if (products) ok = ok && mbar_wait(p_full(b), (tile >> 1) & 1) && (tile == 0 || mbar_wait(o_empty, (tile - 1) & 1));
+          else ok = ok && (tile < 2 || mbar_wait(s_free(b), ((tile >> 1) - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          if (products) {
+            const uint32_t id = instr_desc_f16(128, DP, 1), wt = tmem + b * 128;
+            const uint64_t v = smem_desc_mn(base + slot * TILE, 32768);
+            const int slices = rows >> 4;
+#pragma unroll 1
+            for (int ks = 0; ks < slices; ++ks) {
+              const uint32_t at = wt + (ks >> 1) * 32 + (ks & 1) * 8;
+              umma_f16_ts(el, tmem + COL_O, at + 16, v + ks * 128, id, ks > 0);
+              umma_f16_ts(el, tmem + COL_O, at, v + ks * 128 + 1024, id, 1);
+            }
+#pragma unroll 1
+            for (int ks = 0; ks < slices; ++ks) umma_f16_ts(el, tmem + COL_O, wt + (ks >> 1) * 32 + (ks & 1) * 8, v + ks * 128, id, 1);
+            commit_by(el, o_full);
+            commit_by(el, s_free(b));
+          } else {
+            const uint32_t d = tmem + b * 128, id = instr_desc_f16(128, rows, 0);
+            const uint64_t k = smem_desc_sw128(base + slot * TILE);
+#pragma unroll 2
+            for (int ks = 0; ks < CB * 4; ++ks) {
+              const uint32_t at = tmem + COL_Q + (ks >> 1) * 32 + (ks & 1) * 8, in = (ks >> 2) * 2048 + (ks & 3) * 2;
+              umma_f16_ts(el, d, at + 16, k + in, id, ks > 0);
+              umma_f16_ts(el, d, at, k + in + 1024, id, 1);
+            }
+#pragma unroll 2
+            for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, tmem + COL_Q + (ks >> 1) * 32 + (ks & 1) * 8, k + (ks >> 2) * 2048 + (ks & 3) * 2, id, 1);
+            commit_by(el, s_full(b));
+            if (j + 1 == n) commit_by(el, q_free);   // the item's last scores
+          }
+          commit_by(el, empty(slot));
+        }
+        ++count;
+        ring += 2 * n;
       }
     }
-  } else {
-    // ------------------------------------------------------------- softmax threads
-    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
-    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
-    float* xch = reinterpret_cast<float*>(gen + XCH);
-    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };   // the two warps of these 32 rows
-    const int f = f0 + row;
-    const bool live = f < nf;
-    const int t = f / s.G, g = f - t * s.G, token = sp.q_begin + t, pos = first + t;
-    float c = 0.0f;   // from products of scaled operands to log2 units
-    if (n > 0) {
-      float x[HC];
-      const float* src = s.q.data + token_offset<PAGED>(s.q, r, hk * s.G + g, token);
-#pragma unroll
-      for (int e = 0; e < HC; e += 4) {
-        const int ch = half * HC + e;
+  } else if (warp >= 16) {
+    // --------------------------------------------------------------- Q rows to tensor memory
+    regs_dec<kRegsFetch>();
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t q_addr = tmem + COL_Q + ((uint32_t)((warp & 3) * 32) << 16);
+    float* rowc = reinterpret_cast<float*>(gen + ROWC);
+    bool ok = true;
+    uint32_t count = 0;
+    for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
+      const Item it = get_item<PAGED>(p, w);
+      if (it.n == 0) continue;
+      const int f = it.f0 + row, t = f / s.G, g = f - t * s.G;
+      const bool live = f < it.nf;
+      const float* src = live ? s.q.data + token_offset<PAGED>(s.q, it.r, it.hk * s.G + g, it.q_begin + t) : nullptr;
+      // 32 channels of the row from ch on: with float4 accesses the lanes of eight rows read one row after the other
+      auto load = [&](int ch, float (&x)[32]) {
         if (p.vec_q) {
-          float4 v = make_float4(0, 0, 0, 0);
-          if (live && ch < s.D) v = *reinterpret_cast<const float4*>(src + ch);
-          x[e] = v.x; x[e + 1] = v.y; x[e + 2] = v.z; x[e + 3] = v.w;
+          const int mine = ch + (lane & 7) * 4;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float* at = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), (lane & 24) + k));
+            float4 v = make_float4(0, 0, 0, 0);
+            if (at && mine < s.D) v = *reinterpret_cast<const float4*>(at + mine);
+            x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[e + i] = (live && ch + i < s.D) ? src[ch + i] : 0.0f;
+          for (int e = 0; e < 32; ++e) x[e] = src && ch + e < s.D ? src[ch + e] : 0.0f;
         }
-      }
+      };
       uint32_t top = 0;
+#pragma unroll 1
+      for (int h = 0; h < DP / 32; ++h) {
+        float x[32];
+        load(h * 32, x);
+        if (p.vec_q) transpose_blocks<8>(x);
 #pragma unroll
-      for (int e = 0; e < HC; ++e) if (finite_bits(x[e])) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-      reinterpret_cast<uint32_t*>(xch)[half * 128 + row] = top;
-      meet();
-      top = max(top, reinterpret_cast<uint32_t*>(xch)[(half ^ 1) * 128 + row]);
+        for (int e = 0; e < 32; ++e) if (finite_bits(x[e])) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+      }
       float sq, iq, sk, ik;
       plane_scale(top, sq, iq);
-      plane_scale(p.pk.amax[plane * 2], sk, ik);
+      plane_scale(p.pk.amax[it.plane * 2], sk, ik);
       // a negative scale goes into Q, so that larger products are larger scores; a vanishing one stays a positive number
-      c = fmaxf(fabsf(s.scale) * kLog2e * iq * ik, 1e-30f);
+      const float c = fmaxf(fabsf(s.scale) * kLog2e * iq * ik, 1e-30f);
       if (s.scale < 0.0f) sq = -sq;
-#pragma unroll
-      for (int e = 0; e < HC; e += 8) {
-        uint4 hi, lo;
-        split_f16(x[e] * sq, x[e + 1] * sq, hi.x, lo.x); split_f16(x[e + 2] * sq, x[e + 3] * sq, hi.y, lo.y);
-        split_f16(x[e + 4] * sq, x[e + 5] * sq, hi.z, lo.z); split_f16(x[e + 6] * sq, x[e + 7] * sq, hi.w, lo.w);
-        const int ch = half * HC + e;
-        uint8_t* at = gen + (ch >> 6) * 32768 + row * 128 + ((((ch & 63) >> 3) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4*>(at) = hi;
-        *reinterpret_cast<uint4*>(at + 16384) = lo;
-      }
-      fence_async_smem();
-      mbar_arrive(q_full);
-      meet();   // xch is read before it is used again
-    }
-    // what the row sees, in virtual keys: [0, s_end) and [lo, hi]
-    const int s_end = live ? max(0, min(s.sinks, pos + 1)) : 0;
-    const int lo_key = live ? (s.window < 0 ? 0 : max(0, pos - s.window)) - runs.shift : 0, hi_key = live ? pos - runs.shift : -1;
-    const bool odd_plane = n > 0 && p.pk.odd[plane] != 0;
-    float m = -INFINITY, l = 0.0f, alpha_prev = 0.0f;
-    bool ok = true, poison = false;
-    float o[HC];
-#pragma unroll
-    for (int e = 0; e < HC; ++e) o[e] = 0.0f;
-    auto gather = [&](int j, float alpha) {   // O += tile j's, against the maximum that tile j used
-      ok = ok && mbar_wait(o_full(j & 1), (j >> 1) & 1);
-      tc_fence_after();
-#pragma unroll
-      for (int h = 0; h < HC / 32; ++h) {
+#pragma unroll 1
+      for (int h = 0; h < DP / 32; ++h) {
+        float x[32];
+        load(h * 32, x);
+        if (p.vec_q) transpose_blocks<8>(x);
         uint32_t y[32];
-        tmem_ld32(lane_addr + 256 + (j & 1) * 128 + half * HC + h * 32, y);
-        tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[h * 32 + e] = fmaf(o[h * 32 + e], alpha, __uint_as_float(y[e]));
+        for (int e = 0; e < 32; e += 2) split_f16(x[e] * sq, x[e + 1] * sq, y[e >> 1], y[16 + (e >> 1)]);
+        if (h == 0 && count > 0) { ok = ok && mbar_wait(q_free, (count - 1) & 1); tc_fence_after(); }
+        tmem_st32(q_addr + h * 32, y);
       }
+      rowc[(count & 3) * 128 + row] = c;   // four: the fetcher can be three items ahead of the softmax threads
+      tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(o_empty(j & 1));
+      mbar_arrive(q_ready);
+      ++count;
+    }
+  } else {
+    // --------------------------------------------------------------- softmax threads
+    regs_inc<kRegsSoftmax>();
+    const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;   // a warp reaches the tensor-memory lanes [32 * (warp % 4), +32)
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    float* xch = reinterpret_cast<float*>(gen + XCH);   // [2][4 parts][128] maxima, then [4 parts][128] sums
+    const float* rowc = reinterpret_cast<const float*>(gen + ROWC);
+    auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory"); };   // the four warps of these 32 rows
+    bool ok = true;
+    uint32_t tiles = 0, count = 0;
+    float m = -INFINITY, l = 0.0f, alpha = 0.0f;   // l of a poisoned row is not a number
+    float o[QC];
+#pragma unroll
+    for (int e = 0; e < QC; ++e) o[e] = 0.0f;
+    // where the row's result goes: out from this thread's channels on (null: nowhere), lse null in all but one of the row's threads
+    struct Target { float* out; float* lse; float iv; } to{nullptr, nullptr, 1.0f};
+
+    auto gather = [&]() {   // O of the last tile, against the maximum that it used
+      ok = ok && mbar_wait(o_full, (tiles - 1) & 1);
+      tc_fence_after();
+      uint32_t y[QC];
+      if constexpr (QC == 32) tmem_ld32(lane_addr + COL_O + part * QC, y);
+      else tmem_ld16(lane_addr + COL_O + part * QC, y);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(o_empty);
+#pragma unroll
+      for (int e = 0; e < QC; ++e) o[e] = fmaf(o[e], alpha, __uint_as_float(y[e]));
     };
-    for (int j = 0; j < n; ++j) {
-      ok = ok && mbar_wait(s_full(j & 1), (j >> 1) & 1);
-      tc_fence_after();
-      float x[64];
-      {
-        uint32_t y[32];
-        tmem_ld32(lane_addr + (j & 1) * 128 + half * 64, y);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(y[e]);
-        tmem_ld32(lane_addr + (j & 1) * 128 + half * 64 + 32, y);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[32 + e] = __uint_as_float(y[e]);
-      }
-      const int c0 = (j0 + j) * kRowsT + half * 64;
-      uint64_t see = bits_below(s_end - c0) | (bits_below(hi_key + 1 - c0) & ~bits_below(lo_key - c0));
-      if (odd_plane) {
-        for (int e = 0; e < 64; ++e)
-          if ((see >> e) & 1ull) {
-            const int key = c0 + e < runs.a_len ? c0 + e : c0 + e + runs.shift;
-            const uint8_t flag = p.pk.flags_k[plane * p.pk.k.rows + key] | p.pk.flags_v[plane * p.pk.v.rows + key];
-            if (flag & kAbsent) see &= ~(1ull << e);
-            else if (flag & kOdd) poison = true;
-          }
-      }
-      if (__any_sync(0xffffffffu, see != ~0ull)) {
-        const uint32_t s0 = (uint32_t)see, s1 = (uint32_t)(see >> 32);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) { if (!((s0 >> e) & 1u)) x[e] = -INFINITY; if (!((s1 >> e) & 1u)) x[32 + e] = -INFINITY; }
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 64; ++e) top = fmaxf(top, x[e]);
-      xch[half * 128 + row] = top;
+    auto store = [&]() {
+      float* mine = xch + 1024;
+      mine[part * 128 + row] = ok ? l : NAN;
       meet();
-      top = fmaxf(top, xch[(half ^ 1) * 128 + row]);
-      const float m_new = fmaxf(m, top == -INFINITY ? -INFINITY : top * c), m_use = m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = exp2_fast(m - m_use), off = kWeightShift - m_use;
-      m = m_new;
-      float sum = 0.0f;
-      {
-        uint32_t hi[32], lo[32];
+      const float sum = (mine[row] + mine[128 + row]) + (mine[256 + row] + mine[384 + row]);
+      const float z = sum == 0.0f ? 0.0f : to.iv / sum, L = sum == 0.0f ? -INFINITY : m - kWeightShift + log2f(sum);
+      meet();
+      if (to.lse) *to.lse = p.splits > 1 ? L : L * kLn2;
+      const int left = (p.splits > 1 ? DP : s.D) - part * QC;
+      if (p.vec_out) {
+        constexpr int N = QC / 4;
 #pragma unroll
-        for (int e = 0; e < 64; e += 2) {
-          const float a = exp2_fast(fmaf(x[e], c, off)), b = exp2_fast(fmaf(x[e + 1], c, off));
+        for (int e = 0; e < QC; ++e) o[e] *= z;
+        transpose_blocks<N>(o);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to.out), (lane & ~(N - 1)) + k));
+          const int e = (lane & (N - 1)) * 4;
+          if (dst && e < left) *reinterpret_cast<float4*>(dst + e) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        }
+      } else if (to.out) {
+#pragma unroll
+        for (int e = 0; e < QC; ++e) if (e < left) to.out[e] = o[e] * z;
+      }
+    };
+
+    for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
+      const Item it = get_item<PAGED>(p, w);
+      if (!it.inside) continue;
+      const int f = it.f0 + row, t = f / s.G, g = f - t * s.G, token = it.q_begin + t, pos = it.first + t;
+      const bool live = f < it.nf;
+      Target here;
+      if (p.splits > 1) {
+        const int64_t at = ((it.plane * p.tiles + it.tile) * p.splits + it.split) * kRowsT + row;
+        here.out = p.part_o + at * DP + part * QC;
+        here.lse = p.part_l + at;
+      } else {
+        here.out = f < (PAGED ? it.nf : s.seq * s.G) ? p.out.data + token_offset<PAGED>(p.out, it.r, it.hk * s.G + g, token) + part * QC : nullptr;
+        here.lse = p.lse + stat_offset<PAGED>(s, it.r, it.hk * s.G + g, token);
+      }
+      if (!here.out || part != 0) here.lse = nullptr;
+      if (it.n == 0) {   // rows that see nothing: padding, or tokens before the cache
+        if (here.lse) *here.lse = -INFINITY;
+        if (here.out) for (int e = 0; e < min(QC, p.splits > 1 ? QC : s.D - part * QC); ++e) here.out[e] = 0.0f;
+        continue;
+      }
+      float sv;
+      plane_scale(p.pk.amax[it.plane * 2 + 1], sv, here.iv);
+      // what the row sees, in virtual keys: [0, s_end) and [lo, hi]
+      const int s_end = live ? max(0, min(s.sinks, pos + 1)) : 0;
+      const int lo_key = live ? (s.window < 0 ? 0 : max(0, pos - s.window)) - it.runs.shift : 0, hi_key = live ? pos - it.runs.shift : -1;
+      const bool odd_plane = p.pk.odd[it.plane] != 0;
+      ok = ok && mbar_wait(q_ready, count & 1);
+      const float c = rowc[(count & 3) * 128 + row];
+      ++count;
+      float m_here = -INFINITY, l_here = 0.0f;
+#pragma unroll 1
+      for (int j = 0; j < it.n; ++j) {
+        const uint32_t buf = lane_addr + (tiles & 1) * 128 + part * 32;
+        const int c0 = (it.j0 + j) * kRowsT + part * 32;
+        uint32_t see = (uint32_t)(bits_below(s_end - c0) | (bits_below(hi_key + 1 - c0) & ~bits_below(lo_key - c0)));
+        if (odd_plane) {
+          for (int e = 0; e < 32; ++e)
+            if ((see >> e) & 1u) {
+              const int key = c0 + e < it.runs.a_len ? c0 + e : c0 + e + it.runs.shift;
+              const uint8_t flag = p.pk.flags_k[it.plane * p.pk.k.rows + key] | p.pk.flags_v[it.plane * p.pk.v.rows + key];
+              if (flag & kAbsent) see &= ~(1u << e);
+              else if (flag & kOdd) l_here = NAN;
+            }
+        }
+        ok = ok && mbar_wait(s_full(tiles & 1), (tiles >> 1) & 1);
+        tc_fence_after();
+        uint32_t y[32];
+        tmem_ld32(buf, y);
+        tmem_ld_wait();
+        if (!__all_sync(0xffffffffu, see == ~0u)) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) if (!((see >> e) & 1u)) y[e] = 0xff800000u;
+        }
+        float top = __uint_as_float(y[0]);
+#pragma unroll
+        for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(y[e]));
+        float* mine = xch + (tiles & 1) * 512 + row;
+        mine[part * 128] = top;
+        meet();
+        top = fmaxf(fmaxf(mine[0], mine[128]), fmaxf(mine[256], mine[384]));
+        const float m_new = fmaxf(m_here, top == -INFINITY ? -INFINITY : top * c), m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha_here = exp2_fast(m_here - m_use), off = kWeightShift - m_use;
+        m_here = m_new;
+        float sum = 0.0f;
+        uint32_t z[32];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float a = exp2_fast(fmaf(__uint_as_float(y[e]), c, off)), b = exp2_fast(fmaf(__uint_as_float(y[e + 1]), c, off));
           sum += a + b;
-          split_f16(a, b, hi[e >> 1], lo[e >> 1]);
+          split_f16(a, b, z[e >> 1], z[16 + (e >> 1)]);
         }
-        tmem_st32(lane_addr + (j & 1) * 128 + half * 64, hi);
-        tmem_st32(lane_addr + (j & 1) * 128 + half * 64 + 32, lo);
+        tmem_st32(buf, z);
         tmem_st_wait();
-      }
-      tc_fence_before();
-      mbar_arrive(p_full(j & 1));
-      l = fmaf(l, alpha, sum);
-      if (j > 0) gather(j - 1, alpha_prev);
-      alpha_prev = alpha;
-      meet();   // both have read xch
-    }
-    if (n > 0) gather(n - 1, alpha_prev);
-    // ------------------------------------------------------------- result
-    xch[half * 128 + row] = l;
-    xch[256 + half * 128 + row] = (poison || !ok) ? 1.0f : 0.0f;
-    meet();
-    const float sum = xch[row] + xch[128 + row];
-    const bool bad = xch[256 + row] + xch[384 + row] > 0.0f;
-    float sv, iv;
-    plane_scale(n > 0 ? p.pk.amax[plane * 2 + 1] : 0u, sv, iv);
-    const float z = bad ? NAN : sum == 0.0f ? 0.0f : iv / sum;
-    const float L = bad ? NAN : sum == 0.0f ? -INFINITY : m - kWeightShift + log2f(sum);
-    if (p.splits > 1) {
-      const int64_t at = ((plane * p.tiles + tile) * p.splits + sp_i) * kRowsT + row;
+        tc_fence_before();
+        mbar_arrive(p_full(tiles & 1));
+        l_here = fmaf(l_here, alpha_here, sum);
+        if (tiles > 0) {
+          gather();
+          if (j == 0) {
+            store();
 #pragma unroll
-      for (int e = 0; e < HC; e += 4) *reinterpret_cast<float4*>(p.part_o + at * DP + half * HC + e) = make_float4(o[e] * z, o[e + 1] * z, o[e + 2] * z, o[e + 3] * z);
-      if (half == 0) p.part_l[at] = L;
-    } else if (f < (PAGED ? nf : s.seq * s.G)) {
-      float* dst = p.out.data + token_offset<PAGED>(p.out, r, hk * s.G + g, token);
-#pragma unroll
-      for (int e = 0; e < HC; e += 4) {
-        const int ch = half * HC + e;
-        if (p.vec_out) {
-          if (ch < s.D) *reinterpret_cast<float4*>(dst + ch) = make_float4(o[e] * z, o[e + 1] * z, o[e + 2] * z, o[e + 3] * z);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) if (ch + i < s.D) dst[ch + i] = o[e + i] * z;
+            for (int e = 0; e < QC; ++e) o[e] = 0.0f;
+          }
         }
+        alpha = alpha_here;
+        ++tiles;
       }
-      if (half == 0) p.lse[stat_offset<PAGED>(s, r, hk * s.G + g, token)] = L * kLn2;
+      to = here; m = m_here; l = l_here;
     }
+    if (tiles > 0) { gather(); store(); }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 20) tmem_dealloc(tmem, 512);
 }
 
 // Joins the key splits of a row: a warp per query row.
@@ -519,13 +587,16 @@ int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStre
 
 template <int DP, bool PAGED>
 int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t st) {
-  constexpr int CB = DP / 64, STAGES = DP == 64 ? 2 : 1;
-  constexpr int kSmem = CB * 32768 * (1 + 2 * STAGES) + 256 + 2048 + 1024;
+  constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 1024;
   GN_CUDA(cudaMemsetAsync(f.pk.amax, 0, pl.planes * 3 * sizeof(uint32_t), st));
   GN_TRY(stream_pack_keys(s, f.pk, nullptr, st));
   static PerDeviceOnce once;
-  if (once.first()) GN_CUDA(cudaFuncSetAttribute(stream_tc_forward_kernel<DP, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  stream_tc_forward_kernel<DP, PAGED><<<dim3(pl.tiles * pl.splits, s.Hkv, s.rows), kThreads, kSmem, st>>>(f);
+  if (once.first()) {
+    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_forward_kernel<DP, PAGED>), kThreads, 512 * kRegsSoftmax + 128 * (kRegsFetch + kRegsOther)));
+    GN_CUDA(cudaFuncSetAttribute(stream_tc_forward_kernel<DP, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  }
+  const int64_t items = pl.planes * pl.tiles * pl.splits;
+  stream_tc_forward_kernel<DP, PAGED><<<(unsigned)std::min<int64_t>(items, num_sms()), kThreads, kSmem, st>>>(f);
   GN_LAUNCH_CHECK();
   if (pl.splits > 1) {
     stream_tc_combine_kernel<DP, PAGED><<<dim3(ceil_div(pl.max_q * s.G, 8), s.Hkv, s.rows), 256, 0, st>>>(f);
@@ -535,6 +606,16 @@ int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t s
 }
 
 }  // namespace
+
+int check_registers(const void* kernel, int threads, int shared_out) {
+  cudaFuncAttributes a{};
+  GN_CUDA(cudaFuncGetAttributes(&a, kernel));
+  if (a.numRegs * threads < shared_out) {
+    set_error("streaming attention: built with %d registers a thread, too few for the kernel's split", a.numRegs);
+    return GN_ERR_UNSUPPORTED;
+  }
+  return GN_OK;
+}
 
 int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t st) {
   if (s.D <= 64) return s.paged() ? pack_go<1, true>(s, pk, norms, st) : pack_go<1, false>(s, pk, norms, st);
@@ -550,7 +631,7 @@ int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void*
   ForwardTc f{};
   f.s = s; f.out = out; f.lse = lse; f.tiles = pl.tiles; f.splits = pl.splits;
   carve_forward(s, pl, workspace, &f);
-  f.vec_q = vec_view(s.q, s.D); f.vec_out = vec_view(out, s.D);
+  f.vec_q = vec_view(s.q, s.D); f.vec_out = pl.splits > 1 || vec_view(out, s.D);
   if (pl.DP == 64) return s.paged() ? forward_go<64, true>(s, pl, f, st) : forward_go<64, false>(s, pl, f, st);
   return s.paged() ? forward_go<128, true>(s, pl, f, st) : forward_go<128, false>(s, pl, f, st);
 }

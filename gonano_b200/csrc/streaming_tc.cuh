@@ -48,6 +48,8 @@ struct Carve {   // workspace layout; with a null base it only counts
     return at;
   }
 };
+// A register split needs the launch to hold what its warpgroups share out, or the wait for registers would not end.
+int check_registers(const void* kernel, int threads, int shared_out);
 // Whether float4 accesses fit a view of head_dim D.
 static inline bool vec_view(const gn_view& v, int D) {
   return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && D % 4 == 0 && v.batch_stride % 4 == 0 && v.head_stride % 4 == 0 && v.token_stride % 4 == 0;
@@ -74,23 +76,67 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 __device__ __forceinline__ uint32_t instr_desc_f16(int m, int n, int b_mn) {
   return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A whole warp runs the issuing code, so that its operands stay in uniform registers (24 instructions of 64 cycles then issue in 1533
+// cycles, against 1830 from one lane's branch); `el` is non-zero in the one lane that issues.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+  return x;
+}
+__device__ __forceinline__ void umma_f16(uint32_t el, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(el) : "memory");
 }
 // A in tensor memory: lane = row, a 32-bit column holds two consecutive elements of the contraction index.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_f16_ts(uint32_t el, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(el) : "memory");
 }
+__device__ __forceinline__ void commit_by(uint32_t el, uint32_t bar) { if (el) umma_commit(bar); }
 // MN-major operand, 128-byte swizzle: 64 channels a row of 128 bytes, 8 contraction rows 1024 bytes (stride offset), the next 64
 // channels `group` bytes on (leading offset).
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t group) {
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(group >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Transposes N x N blocks of four floats among groups of N lanes (N 4 or 8): block k of lane i becomes block i of lane k.  With
+// it a thread that owns a row moves its channels by whole 64- or 128-byte pieces: lanes i of a group access piece i of one row.
+// (A warp whose lanes access 16 bytes of 32 rows each took 10 000 cycles to store a 64 KB tile.)
+template <int N>
+__device__ __forceinline__ void transpose_blocks(float (&x)[4 * N]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < N; d <<= 1) {
+    const bool upper = lane & d;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (k & d) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = x[4 * k + e], b = x[4 * (k | d) + e], y = __shfl_xor_sync(0xffffffffu, upper ? a : b, d);
+        x[4 * k + e] = upper ? y : a;
+        x[4 * (k | d) + e] = upper ? b : y;
+      }
+    }
+  }
+}
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u; }
 
@@ -108,6 +154,10 @@ __device__ __forceinline__ void plane_scale(uint32_t amax, float& s, float& inve
   s = amax == 0 ? 1.0f : __uint_as_float((uint32_t)(14 - e + 127) << 23);
   inverse = amax == 0 ? 1.0f : __uint_as_float((uint32_t)(e - 14 + 127) << 23);
 }
+
+// Registers move between warpgroups inside what the launch holds (check_registers).
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 __device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 

@@ -165,10 +165,7 @@ __device__ __forceinline__ PlaneFactors plane_factors(const BackwardTc& p, int64
 
 constexpr int kThreadsB = 384;        // two warpgroups of softmax threads, one for the issuing and the copying warp
 constexpr int kRegsSoftmax = 224, kRegsOther = 56;
-constexpr int kFlush = 8;             // steps whose sums are left to the tensor core before they are rounded into registers
-template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
+constexpr int kFlush = 2;             // steps whose sums are left to the tensor core before they are rounded into registers
 // Adds 32 * N columns of an accumulator to registers.
 template <int N>
 __device__ __forceinline__ void add_columns(uint32_t taddr, float* acc) {
@@ -291,7 +288,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
           for (int ph = 0; ph < 2; ++ph) { mbar_wait(q_full(i), ph); mbar_wait(g_full(i), ph); }
       mbar_wait(v_full, 0);
     }
-    if (warp == 8 && lane == 0 && n > 0) {
+    if (warp == 8 && n > 0) {
+      const uint32_t el = elect_lane();
       // ----------------------------------------------------------- instructions: whichever product has its operands
       int is = 0, ip = 0, iv = 0, ik = 0, chunk = 0;   // next S, dP, dV, dK; the accumulation chunk that may be written
       bool ok = mbar_wait(v_full, 0) && mbar_wait(kh_ready, 0);
@@ -307,18 +305,18 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         const int slices = rows16(i) >> 4;
         const uint32_t fresh = i % kFlush == 0 ? 0u : 1u;
         auto one = [&](int ks, int al, int bl, uint32_t acc) {
-          umma_f16_ts(d, a + (ks >> 1) * 32 + al * 16 + (ks & 1) * 8, smem_desc_mn(slot + bl * 8192 + ks * 2048, 16384), id, acc);
+          umma_f16_ts(el, d, a + (ks >> 1) * 32 + al * 16 + (ks & 1) * 8, smem_desc_mn(slot + bl * 8192 + ks * 2048, 16384), id, acc);
         };
         for (int ks = 0; ks < slices; ++ks) { one(ks, 1, 0, ks > 0 ? 1u : fresh); one(ks, 0, 1, 1); }
         for (int ks = 0; ks < slices; ++ks) one(ks, 0, 0, 1);
       };
-      auto end_chunk = [&]() { if (iv == ik && (iv % kFlush == 0 || iv == n)) umma_commit(acc_full); };
+      auto end_chunk = [&]() { if (iv == ik && (iv % kFlush == 0 || iv == n)) commit_by(el, acc_full); };
       for (uint32_t idle = 0; (ik < n || iv < n) && ok;) {
         bool did = false;
         if (ik < ip && in_chunk(ik) && mbar_test(ds_full, ik & 1)) {
           tc_fence_after();
           accumulate(tmem + COL_DK, tmem + COL_DP, base + OFF_Q + (ik & 1) * SLOT, ik);
-          umma_commit(q_empty(ik & 1));
+          commit_by(el, q_empty(ik & 1));
           ++ik; did = true;
           end_chunk();
         }
@@ -326,20 +324,20 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
           tc_fence_after();
           const uint32_t id = instr_desc_f16(128, rows16(ip), 0), g = base + OFF_G + (ip & 1) * SLOT;
           auto one = [&](int ks, int vl, int gl, uint32_t acc) {
-            umma_f16(tmem + COL_DP, smem_desc_sw128(base + (ks >> 2) * 32768 + vl * 16384) + 2u * (ks & 3),
+            umma_f16(el, tmem + COL_DP, smem_desc_sw128(base + (ks >> 2) * 32768 + vl * 16384) + 2u * (ks & 3),
                      smem_desc_sw128(g + (ks >> 2) * 16384 + gl * 8192) + 2u * (ks & 3), id, acc);
           };
 #pragma unroll
           for (int ks = 0; ks < CB * 4; ++ks) { one(ks, 1, 0, ks > 0); one(ks, 0, 1, 1); }
 #pragma unroll
           for (int ks = 0; ks < CB * 4; ++ks) one(ks, 0, 0, 1);
-          umma_commit(dp_full);
+          commit_by(el, dp_full);
           ++ip; did = true;
         }
         if (iv < is && iv < ip && in_chunk(iv) && mbar_test(p_full(iv & 1), (iv >> 1) & 1)) {
           tc_fence_after();
           accumulate(tmem + COL_DV, tmem + COL_S + (iv & 1) * 64, base + OFF_G + (iv & 1) * SLOT, iv);
-          umma_commit(g_empty(iv & 1));
+          commit_by(el, g_empty(iv & 1));
           ++iv; did = true;
           end_chunk();
         }
@@ -349,12 +347,12 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
           auto b_of = [&](int ks, int ql) { return smem_desc_sw128(q + (ks >> 2) * 16384 + ql * 8192) + 2u * (ks & 3); };
 #pragma unroll
           for (int ks = 0; ks < CB * 4; ++ks) {
-            umma_f16(d, smem_desc_sw128(kl + (ks >> 2) * 16384) + 2u * (ks & 3), b_of(ks, 0), id, ks > 0);
-            umma_f16_ts(d, tmem + COL_KH + ks * 8, b_of(ks, 1), id, 1);
+            umma_f16(el, d, smem_desc_sw128(kl + (ks >> 2) * 16384) + 2u * (ks & 3), b_of(ks, 0), id, ks > 0);
+            umma_f16_ts(el, d, tmem + COL_KH + ks * 8, b_of(ks, 1), id, 1);
           }
 #pragma unroll
-          for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(d, tmem + COL_KH + ks * 8, b_of(ks, 0), id, 1);
-          umma_commit(s_full(is & 1));
+          for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, tmem + COL_KH + ks * 8, b_of(ks, 0), id, 1);
+          commit_by(el, s_full(is & 1));
           ++is; did = true;
         }
         if (did) idle = 0;
@@ -380,6 +378,15 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
 #pragma unroll
     for (int e = 0; e < HC; ++e) dv[e] = dk[e] = 0.0f;
     bool ok = true;
+    // a chunk's sums are fetched one step later, between that step's weights and its dS: the products that end the chunk run meanwhile
+    auto flush = [&](int chunk) {
+      ok = ok && mbar_wait(acc_full, chunk & 1);
+      tc_fence_after();
+      add_columns<HC / 32>(lane_addr + COL_DV + half * HC, dv);
+      add_columns<HC / 32>(lane_addr + COL_DK + half * HC, dk);
+      tc_fence_before();
+      mbar_arrive(acc_empty);
+    };
     for (int i = 0; i < n; ++i) {
       const int f0 = row0(i) + half * 32;
       const uint32_t see = (uint32_t)(bits_below(f_hi - f0) & ~bits_below(f_lo - f0));
@@ -397,6 +404,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       store_pairs(lane_addr + COL_S + (i & 1) * 64 + half * 32, w);
       tc_fence_before();
       mbar_arrive(p_full(i & 1));
+      if (i > 0 && i % kFlush == 0) flush(i / kFlush - 1);
       ok = ok && mbar_wait(dp_full, i & 1);
       tc_fence_after();
       {
@@ -409,15 +417,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       store_pairs(lane_addr + COL_DP + half * 32, w);
       tc_fence_before();
       mbar_arrive(ds_full);
-      if ((i + 1) % kFlush == 0 || i + 1 == n) {
-        ok = ok && mbar_wait(acc_full, (i / kFlush) & 1);
-        tc_fence_after();
-        add_columns<HC / 32>(lane_addr + COL_DV + half * HC, dv);
-        add_columns<HC / 32>(lane_addr + COL_DK + half * HC, dk);
-        tc_fence_before();
-        mbar_arrive(acc_empty);
-      }
     }
+    if (n > 0) flush((n - 1) / kFlush);
     const float zk = ok ? fc.dk : NAN, zv = ok ? fc.dv : NAN;
     if (parts > 1) {
       float* at = p.part + (((plane * p.units + x0) * 2) * 128 + row) * DP + half * HC;
@@ -559,7 +560,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
         }
       mbar_wait(lo_full, 0);
     }
-    if (warp == 8 && lane == 0 && n > 0) {
+    if (warp == 8 && n > 0) {
+      const uint32_t el = elect_lane();
       bool ok = mbar_wait(lo_full, 0) && mbar_wait(hi_ready, 0);
       tc_fence_after();
       auto scores = [&](int j) {
@@ -573,15 +575,15 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
           auto b_of = [&](int ks, int l) { return smem_desc_sw128(slot + (ks >> 2) * 16384 + l * 8192) + 2u * (ks & 3); };
 #pragma unroll
           for (int ks = 0; ks < CB * 4; ++ks) {
-            umma_f16(d, smem_desc_sw128(lo + (ks >> 2) * 16384) + 2u * (ks & 3), b_of(ks, 0), id, ks > 0);
-            umma_f16_ts(d, hi + ks * 8, b_of(ks, 1), id, 1);
+            umma_f16(el, d, smem_desc_sw128(lo + (ks >> 2) * 16384) + 2u * (ks & 3), b_of(ks, 0), id, ks > 0);
+            umma_f16_ts(el, d, hi + ks * 8, b_of(ks, 1), id, 1);
           }
 #pragma unroll
-          for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(d, hi + ks * 8, b_of(ks, 0), id, 1);
+          for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, hi + ks * 8, b_of(ks, 0), id, 1);
         }
         if (!ok) return;
-        umma_commit(v_empty(j & 1));
-        umma_commit(sp_full(j & 1));
+        commit_by(el, v_empty(j & 1));
+        commit_by(el, sp_full(j & 1));
       };
       if (ok) scores(0);
       for (int j = 0; j < n && ok; ++j) {
@@ -593,12 +595,12 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
         const int slices = rows16(j) >> 4;
         const uint32_t fresh = j % kFlush == 0 ? 0u : 1u;
         auto one = [&](int ks, int al, int bl, uint32_t acc) {
-          umma_f16_ts(tmem + COL_DQ, a + (ks >> 1) * 32 + al * 16 + (ks & 1) * 8, smem_desc_mn(slot + bl * 8192 + ks * 2048, 16384), id, acc);
+          umma_f16_ts(el, tmem + COL_DQ, a + (ks >> 1) * 32 + al * 16 + (ks & 1) * 8, smem_desc_mn(slot + bl * 8192 + ks * 2048, 16384), id, acc);
         };
         for (int ks = 0; ks < slices; ++ks) { one(ks, 1, 0, ks > 0 ? 1u : fresh); one(ks, 0, 1, 1); }
         for (int ks = 0; ks < slices; ++ks) one(ks, 0, 0, 1);
-        umma_commit(k_empty(j % 3));
-        if ((j + 1) % kFlush == 0 || j + 1 == n) umma_commit(acc_full);
+        commit_by(el, k_empty(j % 3));
+        if ((j + 1) % kFlush == 0 || j + 1 == n) commit_by(el, acc_full);
       }
     }
   } else {
@@ -626,6 +628,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
 #pragma unroll
     for (int e = 0; e < HC; ++e) acc[e] = 0.0f;
     bool ok = true;
+    auto flush = [&](int chunk) {   // one step later, as above
+      ok = ok && mbar_wait(acc_full, chunk & 1);
+      tc_fence_after();
+      add_columns<HC / 32>(lane_addr + COL_DQ + half * HC, acc);
+      tc_fence_before();
+      mbar_arrive(acc_empty);
+    };
     for (int j = 0; j < n; ++j) {
       const int c0 = j * 64 + half * 32;
       const uint32_t see = (uint32_t)(bits_below(s_end - c0) | (bits_below(hi_key + 1 - c0) & ~bits_below(lo_key - c0)));
@@ -646,14 +655,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       store_pairs(lane_addr + COL_DP + (j & 1) * 64 + half * 32, w);
       tc_fence_before();
       mbar_arrive(ds_full(j & 1));
-      if ((j + 1) % kFlush == 0 || j + 1 == n) {
-        ok = ok && mbar_wait(acc_full, (j / kFlush) & 1);
-        tc_fence_after();
-        add_columns<HC / 32>(lane_addr + COL_DQ + half * HC, acc);
-        tc_fence_before();
-        mbar_arrive(acc_empty);
-      }
+      if (j > 0 && j % kFlush == 0) flush(j / kFlush - 1);
     }
+    if (n > 0) flush((n - 1) / kFlush);
     if (f < s.seq * s.G) {
       const float z = ok ? fc.dq : NAN;
       float* dst = p.dq.data + token_offset<false>(p.dq, r, h, t);
@@ -715,26 +719,14 @@ int64_t carve_backward(const StreamRows& s, void* workspace, BackwardTc* b) {
   return c.used;
 }
 
-// The register split needs the launch to hold what its warpgroups share out, or the wait for registers would not end.
-template <typename K>
-int check_registers(K kernel) {
-  cudaFuncAttributes a{};
-  GN_CUDA(cudaFuncGetAttributes(&a, kernel));
-  if (a.numRegs * kThreadsB < 256 * kRegsSoftmax + 128 * kRegsOther) {
-    set_error("attention_sink_backward: built with %d registers a thread, too few for its split", a.numRegs);
-    return GN_ERR_UNSUPPORTED;
-  }
-  return GN_OK;
-}
-
 template <int DP>
 int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
   constexpr int CB = DP / 64;
   constexpr int kSmemKv = CB * (32768 + 16384 + 4 * 16384) + 1024 + 256 + 1024, kSmemQ = CB * (2 * 16384 + 5 * 16384) + 256 + 1024;
   static PerDeviceOnce once;
   if (once.first()) {
-    GN_TRY(check_registers(stream_tc_dkv_kernel<DP>));
-    GN_TRY(check_registers(stream_tc_dq_kernel<DP>));
+    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_dkv_kernel<DP>), kThreadsB, 256 * kRegsSoftmax + 128 * kRegsOther));
+    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_dq_kernel<DP>), kThreadsB, 256 * kRegsSoftmax + 128 * kRegsOther));
     GN_CUDA(cudaFuncSetAttribute(stream_tc_dkv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemKv));
     GN_CUDA(cudaFuncSetAttribute(stream_tc_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemQ));
   }

@@ -586,18 +586,19 @@ def test_two_graphs_at_once():
         q, k, v, dout = tensors(2, 8, 2, 300 + 100 * i, 128, seed=20 + i)
         mask = dict(sinks=4, window=90, scale=0.09)
         nk = torch.randn(2, 2, 128, device=DEVICE)
-        cache = Cache(2, 2, 128, 16, 40, seed=i)
+        cache = Cache(2, 2, 128, 16, 45, seed=i)
         cache.fill([500, 400 + i])
+        table, fresh = cache.table[:, :32].contiguous(), cache.table[:, 32:].contiguous()
         starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEVICE)
         lens = torch.tensor([501, 401 + i], dtype=torch.int32, device=DEVICE)
-        mass = torch.zeros(2, 2, 640, device=DEVICE)
+        mass = torch.zeros(2, 2, 512, device=DEVICE)
         q1 = torch.randn(2, 8, 128, device=DEVICE)
 
-        def call(q=q, k=k, v=v, dout=dout, q1=q1, nk=nk, cache=cache, starts=starts, lens=lens, mass=mass, mask=mask):
+        def call(q=q, k=k, v=v, dout=dout, q1=q1, nk=nk, cache=cache, table=table, fresh=fresh, starts=starts, lens=lens, mass=mass, mask=mask):
             out, lse = streaming.sink_attention_forward(q, k, v, **mask)
             grads = streaming.sink_attention_backward(q, k, v, out, dout, lse, **mask)
-            paged = streaming.paged_attention(q1, cache.k, cache.v, cache.table, starts, lens, 1, new_key=nk, new_value=nk, scale=0.09, mass=mass, mass_out=torch.zeros_like(mass))
-            kept = streaming.evict_pages(cache.k, cache.v, paged[2], cache.table, lens, 200, 4, 20, new_table=cache.table.flip(1).contiguous(), max_context=320)
+            paged = streaming.paged_attention(q1, cache.k, cache.v, table, starts, lens, 1, new_key=nk, new_value=nk, scale=0.09, mass=mass, mass_out=torch.zeros_like(mass))
+            kept = streaming.evict_pages(cache.k, cache.v, paged[2], table, lens, 200, 4, 20, new_table=fresh)
             return [out, lse, *grads, *paged, *kept]
         call()   # warm-up before the capture
         torch.cuda.synchronize()
