@@ -28,39 +28,6 @@ __device__ __forceinline__ const float* key_ptr(const StreamRows& s, bool value,
   return (PAGED ? (value ? s.pages_v : s.pages_k) : (value ? s.v.data : s.k.data)) + off;
 }
 
-// A warp per (row, query head, token): online softmax over the keys the query sees.
-__global__ void __launch_bounds__(128) stream_forward_kernel(StreamRows s, gn_view out, float* __restrict__ lse) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x * 4 + warp, h = blockIdx.y, r = blockIdx.z;
-  const RowSpan sp = row_span<true>(s, r);
-  if (t >= sp.q_len) return;
-  const int token = sp.q_begin + t;
-  float o[kE] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-  {
-    const int pos = sp.ctx - sp.q_len + t;
-    float q[kE];
-    load_lane<true>(s.q.data + token_offset<true>(s.q, r, h, token), s.D, q);
-    const Seen see = seen_by(s, pos);
-    for (int j = see.sink_end > 0 ? 0 : see.begin; j <= pos; j = (j + 1 == see.sink_end) ? max(see.begin, j + 1) : j + 1) {
-      const float* kp = key_ptr<true>(s, false, r, h / s.G, j);
-      if (!kp) continue;
-      float k[kE], v[kE];
-      load_lane<true>(kp, s.D, k);
-      load_lane<true>(key_ptr<true>(s, true, r, h / s.G, j), s.D, v);
-      const float x = dot_lane(q, k) * s.scale, mn = fmaxf(m, x), a = m == -INFINITY ? 0.0f : expf(m - mn), p = x == -INFINITY ? 0.0f : expf(x - mn);
-      l = fmaf(l, a, p);
-#pragma unroll
-      for (int e = 0; e < kE; ++e) o[e] = fmaf(o[e], a, p * v[e]);
-      m = mn;
-    }
-  }
-  float* op = out.data + token_offset<true>(out, r, h, token);
-#pragma unroll
-  for (int e = 0; e < kE; ++e)
-    if (lane + 32 * e < s.D) op[lane + 32 * e] = l == 0.0f ? 0.0f : o[e] / l;
-  if (lane == 0) lse[stat_offset<true>(s, r, h, token)] = l == 0.0f ? -INFINITY : m + logf(l);
-}
-
 // A warp per (row, new token, kv head): the new token's key and value go to its slot.
 __global__ void __launch_bounds__(128) stream_append_kernel(StreamRows s, gn_view nk, gn_view nv) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -267,8 +234,10 @@ int workspace_ok(const void* w, int64_t have, int64_t need, const char* what) {
   return on_this_device(w, what);
 }
 int64_t sink_bytes(const StreamRows& s, int backward) { return backward ? stream_tc_backward_bytes(s) : stream_tc_forward_bytes(s); }
-// New tokens over a paged cache: a single token per row runs on the warp-per-row kernel, chunks on the tensor cores.
+// New tokens over a paged cache: up to 16 query rows a kv head run on the kernel that streams the cache once, more on the tensor
+// cores, which pack the keys first (3 times the cache's bytes) but take 128 rows for one reading.
 bool paged_on_tensor_cores(const StreamRows& s) { return (int64_t)s.max_query * s.G > 16; }
+int64_t paged_bytes(const StreamRows& s, bool mass) { return paged_on_tensor_cores(s) ? stream_tc_forward_bytes(s) : stream_decode_bytes(s, mass); }
 
 int paged_rows(const gn_paged_params* p, StreamRows* s) {
   GN_REQUIRE(p, "attention_paged: null parameters");
@@ -338,7 +307,7 @@ int gn_attention_paged_workspace(const gn_paged_params* p, int64_t* bytes) {
   GN_REQUIRE(bytes, "attention_paged_workspace: null bytes");
   StreamRows s;
   GN_TRY(paged_rows(p, &s));
-  *bytes = s.rows && s.tokens && s.max_query && paged_on_tensor_cores(s) ? stream_tc_forward_bytes(s) : 0;
+  *bytes = s.rows && s.tokens && s.max_query ? paged_bytes(s, p->mass_out != nullptr) : 0;
   return GN_OK;
 }
 
@@ -354,18 +323,14 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
   const void* ptrs[] = {p->query.data, p->query_starts, p->context_lens, out->data, lse, p->key_pages, p->value_pages, p->page_table, p->new_key.data,
                         p->new_value.data, p->mass, p->mass_out};
   for (const void* x : ptrs) if (x) GN_TRY(on_this_device(x, "attention_paged"));
-  const bool tensor = paged_on_tensor_cores(s);
-  GN_TRY(workspace_ok(workspace, workspace_bytes, tensor ? stream_tc_forward_bytes(s) : 0, "attention_paged"));
+  GN_TRY(workspace_ok(workspace, workspace_bytes, paged_bytes(s, p->mass_out != nullptr), "attention_paged"));
   cudaStream_t st = (cudaStream_t)stream;
+  if (!paged_on_tensor_cores(s)) return stream_decode(s, p->new_key, p->new_value, *out, lse, p->mass, p->mass_out, workspace, st);
   if (p->new_key.data && s.max_context) {
     stream_append_kernel<<<dim3(ceil_div(s.max_query, 4), s.Hkv, s.rows), 128, 0, st>>>(s, p->new_key, p->new_value);
     GN_LAUNCH_CHECK();
   }
-  if (tensor) GN_TRY(stream_tc_forward(s, *out, lse, workspace, st));
-  else {
-    stream_forward_kernel<<<dim3(ceil_div(s.max_query, 4), s.Hq, s.rows), 128, 0, st>>>(s, *out, lse);
-    GN_LAUNCH_CHECK();
-  }
+  GN_TRY(stream_tc_forward(s, *out, lse, workspace, st));
   if (p->mass_out && s.max_context) {
     stream_mass_kernel<<<dim3(ceil_div(s.max_context, 4), s.Hkv, s.rows), 128, 0, st>>>(s, lse, p->mass, p->mass_out);
     GN_LAUNCH_CHECK();

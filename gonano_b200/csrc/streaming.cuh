@@ -19,6 +19,11 @@ struct StreamRows {
   bool paged() const { return pages_k != nullptr; }
 };
 
+// Few new tokens a row over a paged cache (streaming_decode.cu): max_query * G <= 16.  Appends, attends and gathers the mass.
+int64_t stream_decode_bytes(const StreamRows& s, bool mass);
+int stream_decode(const StreamRows& s, const gn_view& nk, const gn_view& nv, const gn_view& out, float* lse, const float* mass, float* mass_out, void* workspace,
+                  cudaStream_t st);
+
 #ifdef __CUDACC__
 struct RowSpan { int q_begin, q_len, ctx; };   // the row's first token, its new tokens, its keys
 
