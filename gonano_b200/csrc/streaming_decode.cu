@@ -1,9 +1,9 @@
 // Few new tokens a row (decode steps) over a paged cache, in float32.
 //
 // Bound: HBM, 8 D bytes a key and kv head, each read once for all query heads of the group.  A CTA takes a range of a (row, kv head)'s
-// keys; its warps walk tiles of 32 of them, each on its own.  Scores: lane = key, the K tile in shared memory (asynchronous copies
-// one tile ahead, 16-byte chunks swizzled so that 8 lanes reading 8 rows meet no bank twice), the queries broadcast from
-// shared memory: no shuffles, 4 multiplications per word read.  Output: lane = 4 channels, V rows straight from global memory
+// keys; its warps walk tiles of 16 of them, each on its own.  Scores: two lanes a key, half the channels each, the K tile in shared
+// memory (asynchronous copies one tile ahead, 16-byte chunks swizzled so that 8 lanes meet no bank twice), the queries broadcast
+// from shared memory: one shuffle a score, 4 multiplications per word read.  Output: lane = 4 channels, V rows straight from global memory
 // (8 ahead), the weights broadcast.  Ranges and warps are joined by their maxima; a range of its own CTA through memory.
 // New tokens' keys and values are read from where they are and written to their pages by the warp that meets them.
 #include <algorithm>
@@ -14,7 +14,8 @@ namespace gn {
 
 namespace {
 
-constexpr int kWarps = 3;   // 2 CTAs of 3 warps (32 KB of K tiles each) an SM: 130 KB in flight, where 45 cover the latency at full rate
+constexpr int kWarps = 4;   // 3 CTAs of 4 warps (16 KB of K tiles each) an SM; 2 of 3 with tiles of 32 keys: half as fast, a CTA's start and end show
+constexpr int kTile = 16;   // keys of a warp's tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Decode {
@@ -51,15 +52,15 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
   extern __shared__ __align__(16) float smem[];
   float* q_s = smem;                                           // [R][DP]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* p_s = smem + R * DP + warp * 32 * R;                  // [32][R]
-  float* k_s = smem + R * DP + kWarps * 32 * R + warp * 2 * 32 * DP;
+  float* p_s = smem + R * DP + warp * kTile * R;               // [kTile][R]
+  float* k_s = smem + R * DP + kWarps * kTile * R + warp * 2 * kTile * DP;
   const StreamRows& s = p.s;
   const int split = blockIdx.x, hk = blockIdx.y, r = blockIdx.z;
   const RowSpan sp = row_span<true>(s, r);
   if (sp.q_len == 0) return;
   const int nq = sp.q_len * s.G, first = sp.ctx - sp.q_len;
   const Range rg = seen_range(s, sp);
-  const int per = ((rg.total + p.splits - 1) / p.splits + 31) & ~31, c0 = split * per, c1 = min(rg.total, c0 + per);
+  const int per = ((rg.total + p.splits - 1) / p.splits + kTile - 1) / kTile * kTile, c0 = split * per, c1 = min(rg.total, c0 + per);
   const int64_t plane = (int64_t)r * s.Hkv + hk;
   for (int i = threadIdx.x; i < R * DP; i += 32 * kWarps) {
     const int qi = i / DP, ch = i % DP;
@@ -67,10 +68,10 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
   }
   __syncthreads();
 
-  // where key c + lane is: its K and V rows (null: none, or no such page)
+  // where key c + lane is (16 lanes): its K and V rows (null: none, or no such page)
   auto locate = [&](int c, const float*& kp, const float*& vp) {
     kp = vp = nullptr;
-    if (c + lane >= c1) return;
+    if (lane >= kTile || c + lane >= c1) return;
     const int key = key_of(rg, c + lane);
     const int64_t at = key_offset<true>(s, s.k, r, hk, key);
     if (at < 0) return;
@@ -82,9 +83,9 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
   };
   auto fetch = [&](int buf, int c, const float* kp) {
     if (c < c1) {
-    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(k_s + buf * 32 * DP);
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(k_s + buf * kTile * DP);
 #pragma unroll 8
-    for (int i = 0; i < 32; i += STEP) {
+    for (int i = 0; i < kTile; i += STEP) {
       const int row = i + lane / LANES, ch = lane % LANES;
       const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(kp), row));
       const uint32_t at = dst + row * ROWB + ((ch ^ (row & 7)) << 4);
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
           if (ch * 4 + 2 < s.D) v.z = src[ch * 4 + 2];
           if (ch * 4 + 3 < s.D) v.w = src[ch * 4 + 3];
         }
-        *reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(k_s) + buf * 32 * ROWB + row * ROWB + ((ch ^ (row & 7)) << 4)) = v;
+        *reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(k_s) + buf * kTile * ROWB + row * ROWB + ((ch ^ (row & 7)) << 4)) = v;
       }
     }
     }
@@ -109,8 +110,8 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
   for (int q = 0; q < R; ++q) { m[q] = -INFINITY; l[q] = 0.0f; o[q][0] = o[q][1] = o[q][2] = o[q][3] = 0.0f; }
   // rows are located two tiles ahead (the table's latency), K tiles copied one ahead
   const float *kp, *vrow, *k_next, *v_next, *k_after, *v_after;
-  constexpr int kStride = 32 * kWarps;
-  int c = c0 + warp * 32, buf = 0;
+  constexpr int kStride = kTile * kWarps;
+  int c = c0 + warp * kTile, buf = 0;
   locate(c, kp, vrow);
   locate(c + kStride, k_next, v_next);
   fetch(0, c, kp);
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
     fetch(buf ^ 1, c + kStride, k_next);
     locate(c + 2 * kStride, k_after, v_after);
     const bool valid = kp != nullptr;
-    const int key = key_of(rg, c + lane);
+    const int key = key_of(rg, c + lane);   // of the first 16 lanes, which locate
     if (p.nk.data) {   // the new tokens' own: to their slots
       for (uint32_t mine = __ballot_sync(0xffffffffu, valid && key >= first); mine; mine &= mine - 1) {
         const int i = __ffs(mine) - 1;
@@ -149,34 +150,43 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
     float x[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) x[q] = 0.0f;
-    const float4* kt = reinterpret_cast<const float4*>(k_s + buf * 32 * DP + lane * DP);
+    const int mine = lane >> 1, half = lane & 1;   // this lane's key and half of its channels
+    const float4* kt = reinterpret_cast<const float4*>(k_s + buf * kTile * DP + mine * DP);
 #pragma unroll 4
-    for (int ch = 0; ch < CH; ++ch) {
-      const float4 k = kt[ch ^ (lane & 7)];
+    for (int i = 0; i < CH / 2; ++i) {
+      const int ch = half ? CH / 2 + (i ^ 4) : i;   // the halves four chunks apart: other banks
+      const float4 k = kt[ch ^ (mine & 7)];
 #pragma unroll
       for (int q = 0; q < R; ++q) {
         const float4 y = *reinterpret_cast<const float4*>(q_s + q * DP + ch * 4);
         x[q] = fmaf(k.x, y.x, fmaf(k.y, y.y, fmaf(k.z, y.z, fmaf(k.w, y.w, x[q]))));
       }
     }
+    const bool there = __shfl_sync(0xffffffffu, (int)valid, mine) != 0;
+    const int my_key = MULTI ? __shfl_sync(0xffffffffu, key, mine) : 0;
     float alpha[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      bool see = valid;
-      if (MULTI) see = see && q < nq && sees(s, first + q / s.G, key);
+      x[q] += __shfl_xor_sync(0xffffffffu, x[q], 1);
+      bool see = there;
+      if (MULTI) see = see && q < nq && sees(s, first + q / s.G, my_key);
       if (!see) x[q] = -INFINITY;
       const float top = fmaxf(m[q], warp_max(x[q])), use = top == -INFINITY ? 0.0f : top;
       alpha[q] = ex2(m[q] - use);
       m[q] = top;
-      if (p.scores && c + lane < c1) p.scores[(plane * s.max_context + c + lane) * R + q] = x[q];
       const float w = ex2(x[q] - use);
-      l[q] = fmaf(l[q], alpha[q], w);
-      p_s[lane * R + q] = w;
+      l[q] = fmaf(l[q], alpha[q], half ? 0.0f : w);
+      if (!half) p_s[mine * R + q] = w;
+    }
+    if (p.scores && !half && c + mine < c1) {
+      float* to = p.scores + (plane * s.max_context + c + mine) * R;
+#pragma unroll
+      for (int q = 0; q < R; q += 4) *reinterpret_cast<float4*>(to + q) = make_float4(x[q], x[q + 1], x[q + 2], x[q + 3]);
     }
     __syncwarp();
 #pragma unroll
     for (int q = 0; q < R; ++q) { o[q][0] *= alpha[q]; o[q][1] *= alpha[q]; o[q][2] *= alpha[q]; o[q][3] *= alpha[q]; }
-    constexpr int LOADS = 32 / STEP;
+    constexpr int LOADS = kTile / STEP;
 #pragma unroll 1
     for (int i0 = 0; i0 < LOADS; i0 += AHEAD) {
 #pragma unroll
@@ -210,7 +220,7 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
       for (int e = 0; e < 4; ++e) o[q][e] += __shfl_xor_sync(0xffffffffu, o[q][e], d);
   }
   __syncthreads();   // the tiles are no longer read
-  float* o_s = smem + R * DP + kWarps * 32 * R;   // [warp][R][DP]
+  float* o_s = smem + R * DP + kWarps * kTile * R;   // [warp][R][DP]
   float* ml = p_s;                                 // [R] maxima, [R] sums
 #pragma unroll
   for (int q = 0; q < R; ++q) {
@@ -224,12 +234,12 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
     const float* all = smem + R * DP;
     float top = -INFINITY, sum = 0.0f, acc = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, all[w * 32 * R + q]);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, all[w * kTile * R + q]);
     const float use = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float a = ex2(all[w * 32 * R + q] - use);
-      sum = fmaf(all[w * 32 * R + R + q], a, sum);
+      const float a = ex2(all[w * kTile * R + q] - use);
+      sum = fmaf(all[w * kTile * R + R + q], a, sum);
       acc = fmaf(o_s[(w * R + q) * DP + ch], a, acc);
     }
     const float y = sum == 0.0f ? 0.0f : acc / sum, L = sum == 0.0f ? -INFINITY : top + log2f(sum);
@@ -305,11 +315,11 @@ __global__ void __launch_bounds__(256) stream_decode_mass_kernel(const __grid_co
 
 int queries_of(const StreamRows& s) { const int n = s.max_query * s.G; return n <= 4 ? 4 : n <= 8 ? 8 : 16; }
 int splits_of(const StreamRows& s) {
-  // a few waves of the 2 CTAs that an SM holds, and no range below two tiles a warp
+  // about as many CTAs as the machine holds at once, and no range below two tiles a warp
   int64_t seen = s.max_context;
   if (s.window >= 0) seen = std::min<int64_t>(seen, (int64_t)s.window + s.sinks + s.max_query);
   const int64_t ctas = (int64_t)s.rows * s.Hkv;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(4 * 2 * 148, ctas), seen / (2 * 32 * kWarps), 128}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(3 * 148 + ctas / 2) / ctas, seen / (2 * kTile * kWarps), 128}));
 }
 int64_t carve(const StreamRows& s, bool mass, uint8_t* base, Decode* d) {
   const int R = queries_of(s), DP = s.D <= 64 ? 64 : 128;
@@ -328,7 +338,7 @@ int64_t carve(const StreamRows& s, bool mass, uint8_t* base, Decode* d) {
 
 template <int R, int DP, bool MULTI>
 int go(const Decode& d, cudaStream_t st) {
-  constexpr int kSmem = (R * DP + kWarps * 32 * R + kWarps * 2 * 32 * DP) * 4;
+  constexpr int kSmem = (R * DP + kWarps * kTile * R + kWarps * 2 * kTile * DP) * 4;
   const StreamRows& s = d.s;
   static PerDeviceOnce once;
   if (once.first()) GN_CUDA(cudaFuncSetAttribute(stream_decode_kernel<R, DP, MULTI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
