@@ -247,6 +247,7 @@ int paged_rows(const gn_paged_params* p, StreamRows* s) {
   GN_REQUIRE(p->rows <= 32767 && p->n_head <= 65535, "attention_paged: more than 32767 rows or 65535 heads");
   GN_REQUIRE(p->page_size > 0 && p->pages >= 0 && p->table_width >= 0 && (int64_t)p->table_width * p->page_size < (1ll << 31),
              "attention_paged: pages %d of %d keys, table of %d", p->pages, p->page_size, p->table_width);
+  GN_REQUIRE((int64_t)p->pages * p->n_kv_head < (1ll << 31) / p->page_size, "attention_paged: more than 2^31 slots of keys");
   GN_REQUIRE(p->max_context >= 0 && (int64_t)p->max_context <= (int64_t)p->table_width * p->page_size, "attention_paged: max_context %d, but a row of the table holds %lld keys",
              p->max_context, (long long)p->table_width * p->page_size);
   GN_REQUIRE((int64_t)p->max_query * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_paged: max_query x heads of a group exceeds 2^30");

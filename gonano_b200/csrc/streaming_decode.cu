@@ -1,11 +1,13 @@
-// Few new tokens a row (decode steps) over a paged cache, in float32.
+// Few new tokens a row (decode steps) over a paged cache.
 //
 // Bound: HBM, 8 D bytes a key and kv head, each read once for all query heads of the group.  A CTA takes a range of a (row, kv head)'s
-// keys; its warps walk tiles of 16 of them, each on its own.  Scores: two lanes a key, half the channels each, the K tile in shared
-// memory (asynchronous copies one tile ahead, 16-byte chunks swizzled so that 8 lanes meet no bank twice), the queries broadcast
-// from shared memory: one shuffle a score, 4 multiplications per word read.  Output: lane = 4 channels, V rows straight from global memory
-// (8 ahead), the weights broadcast.  Ranges and warps are joined by their maxima; a range of its own CTA through memory.
-// New tokens' keys and values are read from where they are and written to their pages by the warp that meets them.
+// keys; its warps walk tiles of 16 of them, each on its own, K and V going from memory to registers and nowhere else.  The products
+// are m16n8k8 tf32 instructions with the keys (then the channels) as their 16 rows and the queries as their 8 columns, so that no
+// row is padding: S^T = K Q^T, O^T += V^T P^T.  The order of a contraction and of the rows is free, and is chosen so that what a
+// lane needs of a K or V row is contiguous.  Float32 through tf32: x = hi + lo, lo*hi + hi*lo + hi*hi; the instruction itself cuts x to hi.
+// (In float32 instructions the same kernel took 126 of them a key, 106 us for 512 rows of 384 keys, issue and latency bound.)
+// Ranges and warps are joined by their maxima; a range of its own CTA through memory.  New tokens' keys and values are read from
+// where they are and written to their pages by the warp that meets them.
 #include <algorithm>
 
 #include "streaming.cuh"
@@ -14,7 +16,7 @@ namespace gn {
 
 namespace {
 
-constexpr int kWarps = 4;   // 3 CTAs of 4 warps (16 KB of K tiles each) an SM; 2 of 3 with tiles of 32 keys: half as fast, a CTA's start and end show
+constexpr int kWarps = 4;
 constexpr int kTile = 16;   // keys of a warp's tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -41,19 +43,26 @@ __device__ __forceinline__ Range seen_range(const StreamRows& s, const RowSpan& 
 __device__ __forceinline__ int key_of(const Range& g, int c) { return c < g.sinks ? c : g.begin + c - g.sinks; }
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }   // what tf32 keeps
+__device__ __forceinline__ float nearest(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); }
+__device__ __forceinline__ void mma(float (&c)[4], float a0, float a1, float a2, float a3, float b0, float b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)), "r"(__float_as_uint(b0)),
+                 "r"(__float_as_uint(b1)));
 }
 
-template <int R, int DP, bool MULTI>
-__global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid_constant__ Decode p) {
-  constexpr int ROWB = DP * 4, CH = DP / 4, LANES = DP / 4;   // LANES lanes hold a row's channels
-  constexpr int STEP = 32 / LANES;                            // V rows of a load
-  extern __shared__ __align__(16) float smem[];
-  float* q_s = smem;                                           // [R][DP]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* p_s = smem + R * DP + warp * kTile * R;               // [kTile][R]
-  float* k_s = smem + R * DP + kWarps * kTile * R + warp * 2 * kTile * DP;
+// R = 8 NT query rows.  Lane = (g, t) = (lane / 4, lane % 4), as the instruction's fragments are laid out: rows g and g + 8, contraction
+// indices t and t + 4, columns g of the second operand and 2 t, 2 t + 1 of the result.
+template <int NT, int DP, bool MULTI>
+__global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __grid_constant__ Decode p) {
+  constexpr int R = 8 * NT, PAIRS = DP / 16, EACH = DP / 8;   // float4s of a K row in a lane; channels of a V row in a lane
+  __shared__ __align__(16) float room[kWarps * R * DP];
+  float (&q_s)[NT][PAIRS][2][32][4] = *reinterpret_cast<float (*)[NT][PAIRS][2][32][4]>(room);   // queries as fragments, hi and lo
+  float (&o_s)[kWarps][R][DP] = *reinterpret_cast<float (*)[kWarps][R][DP]>(room);               // at the end, the warps' results
+  __shared__ __align__(16) float p_s[kWarps][kTile * R];
+  __shared__ float m_s[kWarps][R], l_s[kWarps][R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const StreamRows& s = p.s;
   const int split = blockIdx.x, hk = blockIdx.y, r = blockIdx.z;
   const RowSpan sp = row_span<true>(s, r);
@@ -64,183 +73,207 @@ __global__ void __launch_bounds__(32 * kWarps) stream_decode_kernel(const __grid
   const int64_t plane = (int64_t)r * s.Hkv + hk;
   for (int i = threadIdx.x; i < R * DP; i += 32 * kWarps) {
     const int qi = i / DP, ch = i % DP;
-    q_s[i] = qi < nq && ch < s.D ? s.q.data[token_offset<true>(s.q, r, hk * s.G + qi % s.G, sp.q_begin + qi / s.G) + ch] * (s.scale * kLog2e) : 0.0f;
+    const float x = qi < nq && ch < s.D ? s.q.data[token_offset<true>(s.q, r, hk * s.G + qi % s.G, sp.q_begin + qi / s.G) + ch] * (s.scale * kLog2e) : 0.0f;
+    const int to = (qi & 7) * 4 + ((ch & 15) >> 2);
+    const float hi = nearest(x);
+    q_s[qi >> 3][ch >> 4][0][to][ch & 3] = hi;
+    q_s[qi >> 3][ch >> 4][1][to][ch & 3] = x - hi;
   }
   __syncthreads();
 
-  // where key c + lane is (16 lanes): its K and V rows (null: none, or no such page)
-  auto locate = [&](int c, const float*& kp, const float*& vp) {
-    kp = vp = nullptr;
-    if (lane >= kTile || c + lane >= c1) return;
+  // where key c + lane is (lanes 0 .. 15): a slot of the pages, -1 none, -2 - i the row's new token i
+  auto locate = [&](int c) {
+    if (lane >= kTile || c + lane >= c1) return -1;
     const int key = key_of(rg, c + lane);
-    const int64_t at = key_offset<true>(s, s.k, r, hk, key);
-    if (at < 0) return;
-    kp = s.pages_k + at; vp = s.pages_v + at;
-    if (p.nk.data && key >= first) {
-      kp = p.nk.data + token_offset<true>(p.nk, r, hk, sp.q_begin + key - first);
-      vp = p.nv.data + token_offset<true>(p.nv, r, hk, sp.q_begin + key - first);
+    const int page = s.table[(int64_t)r * s.width + key / s.page_size];
+    if ((unsigned)page >= (unsigned)s.pages) return -1;
+    if (p.nk.data && key >= first) return -2 - (key - first);
+    return (page * s.Hkv + hk) * s.page_size + key % s.page_size;
+  };
+  auto row_of = [&](int slot, const float* pages, const gn_view& fresh) -> const float* {
+    if (slot >= 0) return pages + (int64_t)slot * s.D;
+    return slot == -1 ? nullptr : fresh.data + token_offset<true>(fresh, r, hk, sp.q_begin - 2 - slot);
+  };
+  auto load4 = [&](const float* row, int ch, float* x) {
+    x[0] = x[1] = x[2] = x[3] = 0.0f;
+    if (!row) return;
+    if (p.vec) {
+      if (ch < s.D) { const float4 v = *reinterpret_cast<const float4*>(row + ch); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (ch + e < s.D) x[e] = row[ch + e];
     }
   };
-  auto fetch = [&](int buf, int c, const float* kp) {
-    if (c < c1) {
-    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(k_s + buf * kTile * DP);
-#pragma unroll 8
-    for (int i = 0; i < kTile; i += STEP) {
-      const int row = i + lane / LANES, ch = lane % LANES;
-      const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(kp), row));
-      const uint32_t at = dst + row * ROWB + ((ch ^ (row & 7)) << 4);
-      if (p.vec) {
-        copy16(at, src ? src + min(ch * 4, s.D - 4) : s.pages_k, src && ch * 4 < s.D ? 16 : 0);   // no bytes: zeros
-      } else {
-        float4 v = make_float4(0, 0, 0, 0);
-        if (src) {
-          if (ch * 4 < s.D) v.x = src[ch * 4];
-          if (ch * 4 + 1 < s.D) v.y = src[ch * 4 + 1];
-          if (ch * 4 + 2 < s.D) v.z = src[ch * 4 + 2];
-          if (ch * 4 + 3 < s.D) v.w = src[ch * 4 + 3];
+  float kr[2][PAIRS * 4];   // rows g and g + 8 of the tile, channels 16 i + 4 t ..
+  auto load_k = [&](int slots) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float* row = row_of(__shfl_sync(0xffffffffu, slots, g + 8 * u), s.pages_k, p.nk);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) load4(row, 16 * i + 4 * t, &kr[u][4 * i]);
+    }
+  };
+  float m[2 * NT], l[2 * NT], o[NT][PAIRS][4];
+#pragma unroll
+  for (int q = 0; q < 2 * NT; ++q) { m[q] = -INFINITY; l[q] = 0.0f; }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.0f;
+
+  constexpr int kStride = kTile * kWarps;
+  int c = c0 + warp * kTile;
+  int slots = locate(c), next = locate(c + kStride);   // the table is read two tiles ahead
+  load_k(slots);
+  for (; c < c1; c += kStride) {
+    const int after = locate(c + 2 * kStride);
+    float vr[4][EACH];   // V rows t, t + 4, t + 8, t + 12, channels EACH g ..
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* row = row_of(__shfl_sync(0xffffffffu, slots, t + 4 * u), s.pages_v, p.nv);
+#pragma unroll
+      for (int e = 0; e < EACH; e += 4) load4(row, EACH * g + e, &vr[u][e]);
+    }
+    // the instruction cuts its sums off: the small terms have sums of their own, and the large ones four that are then added rounded
+    float x[NT][4], big[NT][4][4], small[NT][2][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        big[nt][0][e] = big[nt][1][e] = big[nt][2][e] = big[nt][3][e] = 0.0f;
+        small[nt][0][e] = small[nt][1][e] = 0.0f;
+      }
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i)
+#pragma unroll
+      for (int h = 0; h < 4; h += 2) {
+        const float a0 = kr[0][4 * i + h], a1 = kr[1][4 * i + h], a2 = kr[0][4 * i + h + 1], a3 = kr[1][4 * i + h + 1];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float2 hi = *reinterpret_cast<const float2*>(&q_s[nt][i][0][lane][h]), lo = *reinterpret_cast<const float2*>(&q_s[nt][i][1][lane][h]);
+          mma(small[nt][0], a0 - cut(a0), a1 - cut(a1), a2 - cut(a2), a3 - cut(a3), hi.x, hi.y);
+          mma(small[nt][1], a0, a1, a2, a3, lo.x, lo.y);
+          mma(big[nt][(2 * i + h / 2) & 3], a0, a1, a2, a3, hi.x, hi.y);
         }
-        *reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(k_s) + buf * kTile * ROWB + row * ROWB + ((ch ^ (row & 7)) << 4)) = v;
+      }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[nt][e] = ((big[nt][0][e] + big[nt][1][e]) + (big[nt][2][e] + big[nt][3][e])) + (small[nt][0][e] + small[nt][1][e]);
+    load_k(next);   // the next tile's keys are on their way from here on
+    bool odd[2] = {false, false};
+    if (MULTI) {   // a value that is not finite must reach only the queries that see it
+      uint32_t bad = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) if ((__float_as_uint(vr[u][e]) & 0x7f800000u) == 0x7f800000u) { any = true; vr[u][e] = 0.0f; }
+        const uint32_t lanes = __ballot_sync(0xffffffffu, any);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) if (lanes & (0x11111111u << k)) bad |= 1u << (4 * u + k);
+      }
+      odd[0] = (bad >> g) & 1u; odd[1] = (bad >> (g + 8)) & 1u;
+    }
+    float shrink[NT][2];
+    const int slot_a = __shfl_sync(0xffffffffu, slots, g), slot_b = __shfl_sync(0xffffffffu, slots, g + 8);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int q = nt * 8 + 2 * t + h;
+        float a = x[nt][h], b = x[nt][2 + h];
+        bool see_a = slot_a != -1, see_b = slot_b != -1;
+        if (MULTI) {
+          const int pos = first + q / s.G;
+          see_a = see_a && q < nq && sees(s, pos, key_of(rg, c + g)); see_b = see_b && q < nq && sees(s, pos, key_of(rg, c + g + 8));
+        }
+        if (!see_a) a = -INFINITY;
+        if (!see_b) b = -INFINITY;
+        x[nt][h] = a; x[nt][2 + h] = b;
+        float top = fmaxf(a, b);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4)); top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(m[2 * nt + h], fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)));
+        const float use = top == -INFINITY ? 0.0f : top, alpha = ex2(m[2 * nt + h] - use);
+        m[2 * nt + h] = top;
+        a = ex2(a - use); b = ex2(b - use);
+        l[2 * nt + h] = fmaf(l[2 * nt + h], alpha, a + b);
+        if (MULTI && ((odd[0] && see_a) || (odd[1] && see_b))) l[2 * nt + h] = NAN;
+        p_s[warp][g * R + q] = a; p_s[warp][(g + 8) * R + q] = b;
+        shrink[nt][h] = alpha;
+      }
+      if (p.scores) {
+        float* to = p.scores + (plane * s.max_context + c + g) * R + nt * 8 + 2 * t;
+        if (c + g < c1) *reinterpret_cast<float2*>(to) = make_float2(x[nt][0], x[nt][1]);
+        if (c + g + 8 < c1) *reinterpret_cast<float2*>(to + 8 * R) = make_float2(x[nt][2], x[nt][3]);
       }
     }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  float m[R], l[R], o[R][4];
+    __syncwarp();
+    float hi[2][NT][2], lo[2][NT][2];
 #pragma unroll
-  for (int q = 0; q < R; ++q) { m[q] = -INFINITY; l[q] = 0.0f; o[q][0] = o[q][1] = o[q][2] = o[q][3] = 0.0f; }
-  // rows are located two tiles ahead (the table's latency), K tiles copied one ahead
-  const float *kp, *vrow, *k_next, *v_next, *k_after, *v_after;
-  constexpr int kStride = kTile * kWarps;
-  int c = c0 + warp * kTile, buf = 0;
-  locate(c, kp, vrow);
-  locate(c + kStride, k_next, v_next);
-  fetch(0, c, kp);
-  for (; c < c1; c += kStride, buf ^= 1, kp = k_next, vrow = v_next, k_next = k_after, v_next = v_after) {
-    fetch(buf ^ 1, c + kStride, k_next);
-    locate(c + 2 * kStride, k_after, v_after);
-    const bool valid = kp != nullptr;
-    const int key = key_of(rg, c + lane);   // of the first 16 lanes, which locate
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float w = p_s[warp][(8 * k + 4 * h + t) * R + nt * 8 + g];
+          hi[k][nt][h] = nearest(w); lo[k][nt][h] = w - hi[k][nt][h];
+        }
+    // a tile's products start from zero and are added to the rescaled output rounded
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float a0 = vr[2 * k][2 * j], a1 = vr[2 * k][2 * j + 1], a2 = vr[2 * k + 1][2 * j], a3 = vr[2 * k + 1][2 * j + 1];
+          mma(y, a0 - cut(a0), a1 - cut(a1), a2 - cut(a2), a3 - cut(a3), hi[k][nt][0], hi[k][nt][1]);
+          mma(y, a0, a1, a2, a3, lo[k][nt][0], lo[k][nt][1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) mma(y, vr[2 * k][2 * j], vr[2 * k][2 * j + 1], vr[2 * k + 1][2 * j], vr[2 * k + 1][2 * j + 1], hi[k][nt][0], hi[k][nt][1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][j][e] = fmaf(o[nt][j][e], shrink[nt][e & 1], y[e]);
+      }
+    __syncwarp();
     if (p.nk.data) {   // the new tokens' own: to their slots
-      for (uint32_t mine = __ballot_sync(0xffffffffu, valid && key >= first); mine; mine &= mine - 1) {
-        const int i = __ffs(mine) - 1;
-        const float* from_k = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(kp), i));
-        const float* from_v = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vrow), i));
-        const int64_t at = key_offset<true>(s, s.k, r, hk, __shfl_sync(0xffffffffu, key, i));
+      for (uint32_t mine = __ballot_sync(0xffffffffu, slots <= -2); mine; mine &= mine - 1) {
+        const int i = __ffs(mine) - 1, slot = __shfl_sync(0xffffffffu, slots, i);
+        const int64_t at = key_offset<true>(s, s.k, r, hk, key_of(rg, c + i));
+        const float* from_k = row_of(slot, nullptr, p.nk);
+        const float* from_v = row_of(slot, nullptr, p.nv);
         for (int e = lane; e < s.D; e += 32) { s.pages_k[at + e] = from_k[e]; s.pages_v[at + e] = from_v[e]; }
       }
     }
-    // V rows of the first loads are on their way while the scores are computed
-    constexpr int AHEAD = 8;
-    auto load_v = [&](int i, float4& v) {
-      const int row = i * STEP + lane / LANES, ch = (lane % LANES) * 4;
-      const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vrow), row));
-      v = make_float4(0, 0, 0, 0);
-      if (!src) return;
-      if (p.vec) { if (ch < s.D) v = __ldg(reinterpret_cast<const float4*>(src + ch)); return; }
-      if (ch < s.D) v.x = src[ch];
-      if (ch + 1 < s.D) v.y = src[ch + 1];
-      if (ch + 2 < s.D) v.z = src[ch + 2];
-      if (ch + 3 < s.D) v.w = src[ch + 3];
-    };
-    float4 v[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) load_v(i, v[i]);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    __syncwarp();
-    float x[R];
-#pragma unroll
-    for (int q = 0; q < R; ++q) x[q] = 0.0f;
-    const int mine = lane >> 1, half = lane & 1;   // this lane's key and half of its channels
-    const float4* kt = reinterpret_cast<const float4*>(k_s + buf * kTile * DP + mine * DP);
-#pragma unroll 4
-    for (int i = 0; i < CH / 2; ++i) {
-      const int ch = half ? CH / 2 + (i ^ 4) : i;   // the halves four chunks apart: other banks
-      const float4 k = kt[ch ^ (mine & 7)];
-#pragma unroll
-      for (int q = 0; q < R; ++q) {
-        const float4 y = *reinterpret_cast<const float4*>(q_s + q * DP + ch * 4);
-        x[q] = fmaf(k.x, y.x, fmaf(k.y, y.y, fmaf(k.z, y.z, fmaf(k.w, y.w, x[q]))));
-      }
-    }
-    const bool there = __shfl_sync(0xffffffffu, (int)valid, mine) != 0;
-    const int my_key = MULTI ? __shfl_sync(0xffffffffu, key, mine) : 0;
-    float alpha[R];
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      x[q] += __shfl_xor_sync(0xffffffffu, x[q], 1);
-      bool see = there;
-      if (MULTI) see = see && q < nq && sees(s, first + q / s.G, my_key);
-      if (!see) x[q] = -INFINITY;
-      const float top = fmaxf(m[q], warp_max(x[q])), use = top == -INFINITY ? 0.0f : top;
-      alpha[q] = ex2(m[q] - use);
-      m[q] = top;
-      const float w = ex2(x[q] - use);
-      l[q] = fmaf(l[q], alpha[q], half ? 0.0f : w);
-      if (!half) p_s[mine * R + q] = w;
-    }
-    if (p.scores && !half && c + mine < c1) {
-      float* to = p.scores + (plane * s.max_context + c + mine) * R;
-#pragma unroll
-      for (int q = 0; q < R; q += 4) *reinterpret_cast<float4*>(to + q) = make_float4(x[q], x[q + 1], x[q + 2], x[q + 3]);
-    }
-    __syncwarp();
-#pragma unroll
-    for (int q = 0; q < R; ++q) { o[q][0] *= alpha[q]; o[q][1] *= alpha[q]; o[q][2] *= alpha[q]; o[q][3] *= alpha[q]; }
-    constexpr int LOADS = kTile / STEP;
-#pragma unroll 1
-    for (int i0 = 0; i0 < LOADS; i0 += AHEAD) {
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const float4 y = v[i];
-        if (i0 + AHEAD < LOADS) load_v(i0 + AHEAD + i, v[i]);
-        const float* w = p_s + ((i0 + i) * STEP + lane / LANES) * R;
-#pragma unroll
-        for (int q = 0; q < R; q += 4) {
-          const float4 w4 = *reinterpret_cast<const float4*>(w + q);
-          const float ww[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (MULTI && ww[u] == 0.0f) continue;   // a query that does not see the key is not touched by what its value holds
-            o[q + u][0] = fmaf(ww[u], y.x, o[q + u][0]); o[q + u][1] = fmaf(ww[u], y.y, o[q + u][1]);
-            o[q + u][2] = fmaf(ww[u], y.z, o[q + u][2]); o[q + u][3] = fmaf(ww[u], y.w, o[q + u][3]);
-          }
-        }
-      }
-    }
-    __syncwarp();
+    slots = next; next = after;
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
   // ------------------------------------------------------------- join the lanes, the warps
+  __syncthreads();
 #pragma unroll
-  for (int q = 0; q < R; ++q) {
-    l[q] = warp_sum(l[q]);
+  for (int q = 0; q < 2 * NT; ++q) {
 #pragma unroll
-    for (int d = LANES; d < 32; d <<= 1)
+    for (int d = 4; d < 32; d <<= 1) l[q] += __shfl_xor_sync(0xffffffffu, l[q], d);
+    const int qi = (q >> 1) * 8 + 2 * t + (q & 1);
+    if (g == 0) { m_s[warp][qi] = m[q]; l_s[warp][qi] = l[q]; }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[q][e] += __shfl_xor_sync(0xffffffffu, o[q][e], d);
-  }
-  __syncthreads();   // the tiles are no longer read
-  float* o_s = smem + R * DP + kWarps * kTile * R;   // [warp][R][DP]
-  float* ml = p_s;                                 // [R] maxima, [R] sums
-#pragma unroll
-  for (int q = 0; q < R; ++q) {
-    if (lane < LANES) *reinterpret_cast<float4*>(o_s + (warp * R + q) * DP + lane * 4) = make_float4(o[q][0], o[q][1], o[q][2], o[q][3]);
-    if (lane == 0) { ml[q] = m[q]; ml[R + q] = l[q]; }
+    for (int j = 0; j < PAIRS; j += 2)
+      *reinterpret_cast<float4*>(&o_s[warp][qi][EACH * g + 2 * j]) =
+          make_float4(o[q >> 1][j][q & 1], o[q >> 1][j][2 + (q & 1)], o[q >> 1][j + 1][q & 1], o[q >> 1][j + 1][2 + (q & 1)]);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < R * DP; i += 32 * kWarps) {
     const int q = i / DP, ch = i % DP;
     if (q >= nq) break;
-    const float* all = smem + R * DP;
     float top = -INFINITY, sum = 0.0f, acc = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, all[w * kTile * R + q]);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_s[w][q]);
     const float use = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float a = ex2(all[w * kTile * R + q] - use);
-      sum = fmaf(all[w * kTile * R + R + q], a, sum);
-      acc = fmaf(o_s[(w * R + q) * DP + ch], a, acc);
+      const float a = ex2(m_s[w][q] - use);
+      sum = fmaf(l_s[w][q], a, sum);
+      acc = fmaf(o_s[w][q][ch], a, acc);
     }
     const float y = sum == 0.0f ? 0.0f : acc / sum, L = sum == 0.0f ? -INFINITY : top + log2f(sum);
     if (p.splits > 1) {
@@ -313,13 +346,13 @@ __global__ void __launch_bounds__(256) stream_decode_mass_kernel(const __grid_co
   p.mass_out[at] = (p.mass && key < first ? p.mass[at] : 0.0f) + sum;
 }
 
-int queries_of(const StreamRows& s) { const int n = s.max_query * s.G; return n <= 4 ? 4 : n <= 8 ? 8 : 16; }
+int queries_of(const StreamRows& s) { return s.max_query * s.G <= 8 ? 8 : 16; }
 int splits_of(const StreamRows& s) {
   // about as many CTAs as the machine holds at once, and no range below two tiles a warp
   int64_t seen = s.max_context;
   if (s.window >= 0) seen = std::min<int64_t>(seen, (int64_t)s.window + s.sinks + s.max_query);
   const int64_t ctas = (int64_t)s.rows * s.Hkv;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(3 * 148 + ctas / 2) / ctas, seen / (2 * kTile * kWarps), 128}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(2 * 148 + ctas / 2) / ctas, seen / (2 * kTile * kWarps), 128}));
 }
 int64_t carve(const StreamRows& s, bool mass, uint8_t* base, Decode* d) {
   const int R = queries_of(s), DP = s.D <= 64 ? 64 : 128;
@@ -336,13 +369,11 @@ int64_t carve(const StreamRows& s, bool mass, uint8_t* base, Decode* d) {
   return used;
 }
 
-template <int R, int DP, bool MULTI>
+template <int NT, int DP, bool MULTI>
 int go(const Decode& d, cudaStream_t st) {
-  constexpr int kSmem = (R * DP + kWarps * kTile * R + kWarps * 2 * kTile * DP) * 4;
+  constexpr int R = 8 * NT;
   const StreamRows& s = d.s;
-  static PerDeviceOnce once;
-  if (once.first()) GN_CUDA(cudaFuncSetAttribute(stream_decode_kernel<R, DP, MULTI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  stream_decode_kernel<R, DP, MULTI><<<dim3(d.splits, s.Hkv, s.rows), 32 * kWarps, kSmem, st>>>(d);
+  stream_decode_kernel<NT, DP, MULTI><<<dim3(d.splits, s.Hkv, s.rows), 32 * kWarps, 0, st>>>(d);
   GN_LAUNCH_CHECK();
   if (d.splits > 1) {
     stream_decode_join_kernel<R, DP><<<dim3(ceil_div(s.max_query * s.G, 4), s.Hkv, s.rows), 128, 0, st>>>(d);
@@ -354,11 +385,11 @@ int go(const Decode& d, cudaStream_t st) {
   }
   return GN_OK;
 }
-template <int R>
+template <int NT>
 int go_rows(const Decode& d, cudaStream_t st) {
   const bool multi = d.s.max_query > 1;
-  if (d.s.D <= 64) return multi ? go<R, 64, true>(d, st) : go<R, 64, false>(d, st);
-  return multi ? go<R, 128, true>(d, st) : go<R, 128, false>(d, st);
+  if (d.s.D <= 64) return multi ? go<NT, 64, true>(d, st) : go<NT, 64, false>(d, st);
+  return multi ? go<NT, 128, true>(d, st) : go<NT, 128, false>(d, st);
 }
 
 }  // namespace
@@ -374,11 +405,7 @@ int stream_decode(const StreamRows& s, const gn_view& nk, const gn_view& nv, con
   carve(s, mass_out != nullptr, static_cast<uint8_t*>(workspace), &d);
   auto wide = [&](const gn_view& v) { return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && v.head_stride % 4 == 0 && v.token_stride % 4 == 0; };
   d.vec = s.D % 4 == 0 && ((reinterpret_cast<uintptr_t>(s.pages_k) | reinterpret_cast<uintptr_t>(s.pages_v)) & 15) == 0 && (!nk.data || (wide(nk) && wide(nv)));
-  switch (queries_of(s)) {
-    case 4: return go_rows<4>(d, st);
-    case 8: return go_rows<8>(d, st);
-    default: return go_rows<16>(d, st);
-  }
+  return queries_of(s) == 8 ? go_rows<1>(d, st) : go_rows<2>(d, st);
 }
 
 }  // namespace gn
