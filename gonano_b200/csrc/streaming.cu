@@ -68,115 +68,6 @@ __global__ void __launch_bounds__(128) stream_mass_kernel(StreamRows s, const fl
   }
 }
 
-// ------------------------------------------------------------------ eviction
-struct Evict {
-  gn_evict_params p;
-  int32_t* kept; int32_t* new_lens; float* mass_out;
-};
-// Mass as an integer that orders like it: equal values (both zeros too) alike, NaN below everything.
-__device__ __forceinline__ uint32_t order_key(float x) {
-  if (isnan(x)) return 0u;
-  const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ int evict_len(const gn_evict_params& p, int r) { return min(max(p.context_lens[r], 0), p.max_context); }
-
-// A CTA per (row, kv head).  The threshold (the smallest kept order key of the middle) by four radix passes of 8 bits, then the
-// kept indices by a stable scan; of the keys equal to the threshold the first ones.
-__global__ void __launch_bounds__(256) evict_select_kernel(Evict e) {
-  const gn_evict_params& p = e.p;
-  const int hk = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n = evict_len(p, r), keep = min(n, p.budget), lo = p.sinks, hi = n - p.recent;
-  const int64_t head = (int64_t)r * p.n_kv_head + hk;
-  const float* mass = p.mass + head * p.mass_stride;
-  __shared__ int hist[256];
-  __shared__ uint32_t prefix_s;
-  __shared__ int want_s, warp_keep[8], warp_tie[8];
-  uint32_t prefix = 0;
-  int want = n <= p.budget ? 0 : p.budget - p.sinks - p.recent;   // of the middle
-  const int wanted = want;
-  if (wanted > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      hist[tid] = 0;
-      __syncthreads();
-      for (int j = lo + tid; j < hi; j += 256) {
-        const uint32_t k = order_key(mass[j]);
-        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255u], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int b = 255, left = want;
-        while (b > 0 && hist[b] < left) left -= hist[b--];
-        prefix_s = prefix | ((uint32_t)b << shift); want_s = left;
-      }
-      __syncthreads();
-      prefix = prefix_s; want = want_s;
-      __syncthreads();
-    }
-  }
-  // now `want` of the keys equal to `prefix` are kept, and all above it
-  int base = 0, ties = 0;
-  for (int j0 = 0; j0 < n; j0 += 256) {
-    const int j = j0 + tid;
-    bool take = false, tie = false;
-    if (j < n) {
-      if (n <= p.budget || j < lo || j >= hi) take = true;
-      else if (wanted > 0) { const uint32_t k = order_key(mass[j]); take = k > prefix; tie = k == prefix; }
-    }
-    const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) warp_tie[warp] = __popc(tie_mask);
-    __syncthreads();
-    int before = ties, all = 0;
-    for (int w = 0; w < 8; ++w) { if (w < warp) before += warp_tie[w]; all += warp_tie[w]; }
-    ties += all;
-    if (tie) take = before + __popc(tie_mask & ((1u << lane) - 1u)) < want;
-    const uint32_t mask = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) warp_keep[warp] = __popc(mask);
-    __syncthreads();
-    int at = base; all = 0;
-    for (int w = 0; w < 8; ++w) { if (w < warp) at += warp_keep[w]; all += warp_keep[w]; }
-    base += all;
-    if (take) e.kept[head * p.budget + at + __popc(mask & ((1u << lane) - 1u))] = j;
-    __syncthreads();
-  }
-  for (int i = keep + tid; i < p.budget; i += 256) e.kept[head * p.budget + i] = -1;
-  if (hk == 0 && tid == 0) e.new_lens[r] = keep;
-  __syncthreads();
-  if (e.mass_out)   // mass_out is an array of its own: the indices were written by this CTA
-    for (int i = tid; i < p.budget; i += 256) e.mass_out[head * p.budget + i] = i < keep ? mass[e.kept[head * p.budget + i]] : 0.0f;
-}
-// A CTA per (32 channels, kv head, row x {key, value}): kept key i goes to slot i.  Slots are filled in ascending order, 256 at
-// a time, every read of a group before its writes: slot i <= kept[i], so in place a group writes only what it or earlier groups read.
-__global__ void __launch_bounds__(256) evict_move_kernel(Evict e) {
-  const gn_evict_params& p = e.p;
-  const int hk = blockIdx.y, r = blockIdx.z >> 1, c0 = blockIdx.x * 32, tid = threadIdx.x;
-  float* pages = (blockIdx.z & 1) ? p.value_pages : p.key_pages;
-  const int keep = min(evict_len(p, r), p.budget), lane = tid & 31, warp = tid >> 5;
-  const int32_t* kept = e.kept + ((int64_t)r * p.n_kv_head + hk) * p.budget;
-  const bool in = c0 + lane < p.head_dim;
-  auto slot = [&](const int32_t* table, int width, int j) -> int64_t {
-    const int page = table[(int64_t)r * width + j / p.page_size];
-    if ((unsigned)page >= (unsigned)p.pages) return -1;
-    return (((int64_t)page * p.n_kv_head + hk) * p.page_size + j % p.page_size) * p.head_dim;
-  };
-  for (int i0 = 0; i0 < keep; i0 += 256) {
-    float x[32];
-#pragma unroll
-    for (int u = 0; u < 32; ++u) {
-      const int i = i0 + warp * 32 + u;
-      x[u] = 0.0f;
-      if (i < keep && in) { const int64_t from = slot(p.page_table, p.table_width, kept[i]); if (from >= 0) x[u] = pages[from + c0 + lane]; }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 32; ++u) {
-      const int i = i0 + warp * 32 + u;
-      if (i < keep && in) { const int64_t to = slot(p.new_table, p.new_width, i); if (to >= 0) pages[to + c0 + lane] = x[u]; }
-    }
-    __syncthreads();
-  }
-}
-
 // ------------------------------------------------------------------ checks
 int on_this_device(const void* p, const char* what) {
   int device = 0;
@@ -355,15 +246,7 @@ int gn_cache_evict(const gn_evict_params* p, int32_t* kept, int32_t* new_lens, f
   GN_REQUIRE(mass_out == nullptr || mass_out != p->mass, "cache_evict: mass_out must not be mass");
   const void* ptrs[] = {p->context_lens, new_lens, kept, p->key_pages, p->value_pages, p->mass, p->page_table, p->new_table, mass_out};
   for (const void* x : ptrs) if (x) GN_TRY(on_this_device(x, "cache_evict"));
-  cudaStream_t st = (cudaStream_t)stream;
-  const Evict e{*p, kept, new_lens, mass_out};
-  evict_select_kernel<<<dim3(p->n_kv_head, p->rows), 256, 0, st>>>(e);
-  GN_LAUNCH_CHECK();
-  if (p->budget && p->max_context) {
-    evict_move_kernel<<<dim3(ceil_div(p->head_dim, 32), p->n_kv_head, 2 * p->rows), 256, 0, st>>>(e);
-    GN_LAUNCH_CHECK();
-  }
-  return GN_OK;
+  return stream_evict(*p, kept, new_lens, mass_out, (cudaStream_t)stream);
 }
 
 }  // extern "C"

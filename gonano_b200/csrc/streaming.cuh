@@ -24,6 +24,9 @@ int64_t stream_decode_bytes(const StreamRows& s, bool mass);
 int stream_decode(const StreamRows& s, const gn_view& nk, const gn_view& nv, const gn_view& out, float* lse, const float* mass, float* mass_out, void* workspace,
                   cudaStream_t st);
 
+// Eviction (streaming_evict.cu), arguments checked.
+int stream_evict(const gn_evict_params& p, int32_t* kept, int32_t* new_lens, float* mass_out, cudaStream_t st);
+
 #ifdef __CUDACC__
 struct RowSpan { int q_begin, q_len, ctx; };   // the row's first token, its new tokens, its keys
 
