@@ -46,6 +46,7 @@ __device__ __forceinline__ bool load_key(const StreamRows& s, bool value, bool v
   return true;
 }
 
+constexpr int kWholePlane = 160; // planes up to here are one CTA's
 constexpr int kPackRows = 128;   // keys of a CTA (256 threads, 16 half warps, 8 keys each)
 
 template <int CB, bool PAGED>
@@ -68,8 +69,9 @@ __global__ void __launch_bounds__(256) stream_amax_kernel(const __grid_constant_
   if ((threadIdx.x & 31) == 0 && top) atomicMax(pk.amax + ((int64_t)r * s.Hkv + hk) * 2 + value, top);   // a maximum does not depend on the order
 }
 
+// With whole = 1 a CTA takes a whole plane and finds its largest magnitude itself (short sequences: one launch instead of three).
 template <int CB, bool PAGED>
-__global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, uint32_t* norms, int vec) {
+__global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, uint32_t* norms, int vec, int whole) {
   const int hk = blockIdx.y, r = blockIdx.z >> 1, value = blockIdx.z & 1, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const RowSpan sp = row_span<PAGED>(s, r);
   const int begin = first_needed<PAGED>(s, sp), j0 = blockIdx.x * kPackRows;
@@ -77,13 +79,31 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
   const int last = min(dst.rows, (sp.ctx + 15) / 16 * 16 + 16);   // zero rows behind the sequence: a tile is copied in 16s
   if (j0 >= last) return;
   const int64_t plane = (int64_t)r * s.Hkv + hk;
+  __shared__ uint32_t most;
+  __shared__ int any_odd;
+  if (whole) {
+    if (threadIdx.x == 0) { most = 0; any_odd = 0; }
+    __syncthreads();
+    uint32_t top = 0;
+    for (int j = half; j < sp.ctx; j += 16) {
+      if (!is_needed<PAGED>(s, sp, begin, j)) continue;
+      float x[4 * CB];
+      load_key<CB, PAGED>(s, value, vec, r, hk, j, x);
+#pragma unroll
+      for (int e = 0; e < 4 * CB; ++e) if (finite_bits(x[e])) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    }
+    if (top) atomicMax(&most, top);
+    __syncthreads();
+    if (threadIdx.x == 0) pk.amax[plane * 2 + value] = most;
+  }
   uint8_t* base = dst.data + plane * dst.plane_bytes(CB);
   uint8_t* flags = (value ? pk.flags_v : pk.flags_k) + plane * dst.rows;
   float sc, inv;
-  plane_scale(pk.amax[plane * 2 + value], sc, inv);
+  plane_scale(whole ? most : pk.amax[plane * 2 + value], sc, inv);
   float top = 0.0f;
+  const int steps = whole ? (last + 15) / 16 : kPackRows / 16;
 #pragma unroll 2
-  for (int u = 0; u < kPackRows / 16; ++u) {
+  for (int u = 0; u < steps; ++u) {
     const int j = j0 + u * 16 + half;
     float x[4 * CB];
 #pragma unroll
@@ -116,12 +136,21 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
     }
     if (l16 == 0) {
       flags[j] = flag;
-      if (flag) pk.odd[plane] = 1;
+      if (flag) { if (whole) any_odd = 1; else pk.odd[plane * 2 + value] = 1; }
     }
+  }
+  if (whole) {
+    __syncthreads();
+    if (threadIdx.x == 0) { pk.odd[plane * 2 + value] = any_odd; most = 0; }
+    __syncthreads();
   }
   if (norms && value) {
     top = warp_max(top);
-    if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(norms + plane * 2, __float_as_uint(top));
+    if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &most : norms + plane * 2, __float_as_uint(top));
+    if (whole) {
+      __syncthreads();
+      if (threadIdx.x == 0) norms[plane * 2] = most;
+    }
   }
 }
 
@@ -436,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       // what the row sees, in virtual keys: [0, s_end) and [lo, hi]
       const int s_end = live ? max(0, min(s.sinks, pos + 1)) : 0;
       const int lo_key = live ? (s.window < 0 ? 0 : max(0, pos - s.window)) - it.runs.shift : 0, hi_key = live ? pos - it.runs.shift : -1;
-      const bool odd_plane = p.pk.odd[it.plane] != 0;
+      const bool odd_plane = (p.pk.odd[it.plane * 2] | p.pk.odd[it.plane * 2 + 1]) != 0;
       ok = ok && mbar_wait(q_ready, count & 1);
       const float c = rowc[(count & 3) * 128 + row];
       ++count;
@@ -557,7 +586,7 @@ int64_t carve_forward(const StreamRows& s, const Plan& pl, void* workspace, Forw
   Carve c{static_cast<uint8_t*>(workspace)};
   const int rows = packed_rows(pl.max_k);
   PackedKeys& pk = f->pk;
-  pk.amax = c.take<uint32_t>(pl.planes * 3);   // amax and odd in one piece: cleared together
+  pk.amax = c.take<uint32_t>(pl.planes * 4);   // amax and odd in one piece: cleared together
   pk.odd = reinterpret_cast<int*>(pk.amax + pl.planes * 2);
   pk.k.rows = pk.v.rows = rows;
   pk.k.data = c.take<uint8_t>(pl.planes * pk.k.plane_bytes(pl.DP / 64));
@@ -577,10 +606,14 @@ bool vec_keys(const StreamRows& s) {
 
 template <int CB, bool PAGED>
 int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t st) {
-  const int vec = vec_keys(s), keys = pk.k.rows;
-  stream_amax_kernel<CB, PAGED><<<dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, vec);
-  GN_LAUNCH_CHECK();
-  stream_pack_kernel<CB, PAGED><<<dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, norms, vec);
+  const int vec = vec_keys(s), keys = pk.k.rows, whole = keys <= kWholePlane;
+  if (!whole) {
+    GN_CUDA(cudaMemsetAsync(pk.amax, 0, (int64_t)s.rows * s.Hkv * 4 * sizeof(uint32_t), st));   // amax and odd
+    if (norms) GN_CUDA(cudaMemsetAsync(norms, 0, (int64_t)s.rows * s.Hkv * 2 * sizeof(uint32_t), st));
+    stream_amax_kernel<CB, PAGED><<<dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, vec);
+    GN_LAUNCH_CHECK();
+  }
+  stream_pack_kernel<CB, PAGED><<<dim3(whole ? 1 : ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, norms, vec, whole);
   GN_LAUNCH_CHECK();
   return GN_OK;
 }
@@ -588,7 +621,6 @@ int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStre
 template <int DP, bool PAGED>
 int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t st) {
   constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 1024;
-  GN_CUDA(cudaMemsetAsync(f.pk.amax, 0, pl.planes * 3 * sizeof(uint32_t), st));
   GN_TRY(stream_pack_keys(s, f.pk, nullptr, st));
   static PerDeviceOnce once;
   if (once.first()) {

@@ -31,7 +31,7 @@ static inline int packed_rows(int64_t n) { return (int)((n + 15) / 16 * 16 + 16)
 struct PackedKeys {
   Packed k, v;
   uint32_t* amax = nullptr;    // [plane][2]: bits of the largest finite |k|, |v|
-  int* odd = nullptr;          // [plane]: a key is non-finite or has no page
+  int* odd = nullptr;          // [plane][2]: a key, a value is not finite or has no page
   uint8_t* flags_k = nullptr;  // [plane][k.rows]: kOdd: a component is not finite (stored as 0), kAbsent: no such page
   uint8_t* flags_v = nullptr;
 };
@@ -54,7 +54,7 @@ int check_registers(const void* kernel, int threads, int shared_out);
 static inline bool vec_view(const gn_view& v, int D) {
   return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && D % 4 == 0 && v.batch_stride % 4 == 0 && v.head_stride % 4 == 0 && v.token_stride % 4 == 0;
 }
-// Packs keys and values (amax and odd cleared by the caller on the stream).  norms: null, or [plane][2]: [0] receives the bits of the
+// Packs keys and values; amax and the 2 * planes words of odd stand in one piece.  norms: null, or [plane][2]: [0] receives the bits of the
 // largest squared norm of a scaled value row.
 int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t stream);
 

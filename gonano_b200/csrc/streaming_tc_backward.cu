@@ -31,6 +31,7 @@ struct BackwardTc {
   float* part;                   // [plane][unit][dV, dK][128][DP] of key tiles in several parts
 };
 
+constexpr int kWholePlaneQ = 256;   // planes up to here are one CTA's
 constexpr int kPackRowsQ = 64;   // 256 threads, 16 half warps
 
 // Half a warp per query row f: channels 4 i .. of the 64-channel blocks.
@@ -80,19 +81,38 @@ __global__ void __launch_bounds__(256) stream_query_amax_kernel(const __grid_con
 
 // Packs q and dO and leaves each row's lse and delta in the form that the kernels use.
 template <int CB>
-__global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_constant__ BackwardTc p) {
+__global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_constant__ BackwardTc p, int whole) {
   const StreamRows& s = p.s;
   const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15, f0 = blockIdx.x * kPackRowsQ;
   const int nf = row_span<false>(s, r).q_len * s.G, last = min(p.q.rows, (nf + 15) / 16 * 16 + 16);
   if (f0 >= last) return;
   const int64_t plane = (int64_t)r * s.Hkv + hk;
+  __shared__ uint32_t most[2], norm;
+  if (whole) {   // the plane is this CTA's: its largest magnitudes first
+    if (threadIdx.x == 0) most[0] = most[1] = norm = 0;
+    __syncthreads();
+    uint32_t top[2] = {0, 0};
+    for (int f = half; f < nf; f += 16)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        float x[4 * CB];
+        load_query_row<CB>(s, w ? p.dout : s.q, p.vec_in, r, hk, f, x);
+#pragma unroll
+        for (int e = 0; e < 4 * CB; ++e) if (finite_bits(x[e])) top[w] = max(top[w], __float_as_uint(x[e]) & 0x7fffffffu);
+      }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) if (top[w]) atomicMax(&most[w], top[w]);
+    __syncthreads();
+    if (threadIdx.x < 2) p.qamax[plane * 2 + threadIdx.x] = most[threadIdx.x];
+  }
   float sc[2], inv, sv;
-  plane_scale(p.qamax[plane * 2], sc[0], inv);
-  plane_scale(p.qamax[plane * 2 + 1], sc[1], inv);
+  plane_scale(whole ? most[0] : p.qamax[plane * 2], sc[0], inv);
+  plane_scale(whole ? most[1] : p.qamax[plane * 2 + 1], sc[1], inv);
   plane_scale(p.pk.amax[plane * 2 + 1], sv, inv);
   float top = 0.0f;
+  const int steps = whole ? (last + 15) / 16 : kPackRowsQ / 16;
 #pragma unroll 1
-  for (int u = 0; u < kPackRowsQ / 16; ++u) {
+  for (int u = 0; u < steps; ++u) {
     const int f = f0 + u * 16 + half;
     float x[2][4 * CB], delta = 0.0f, sq = 0.0f;
     bool odd = false;
@@ -140,7 +160,11 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
     }
   }
   top = warp_max(top);
-  if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(p.norms + plane * 2 + 1, __float_as_uint(top));
+  if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &norm : p.norms + plane * 2 + 1, __float_as_uint(top));
+  if (whole) {
+    __syncthreads();
+    if (threadIdx.x == 0) p.norms[plane * 2 + 1] = norm;
+  }
 }
 
 // Factors of a plane: scores to log2 units, dO.V - delta (scaled) into f16's range with the weights' 2^15 taken out, and the
@@ -701,10 +725,10 @@ int64_t carve_backward(const StreamRows& s, void* workspace, BackwardTc* b) {
   b->units = b->sink_tiles * b->parts_sink + (b->key_tiles - b->sink_tiles) * b->parts;
   Carve c{static_cast<uint8_t*>(workspace)};
   PackedKeys& pk = b->pk;
-  pk.amax = c.take<uint32_t>(planes * 7);   // cleared together: the largest magnitudes of k, v; odd; of q, dO; norms
+  pk.amax = c.take<uint32_t>(planes * 4);
   pk.odd = reinterpret_cast<int*>(pk.amax + planes * 2);
-  b->qamax = pk.amax + planes * 3;
-  b->norms = pk.amax + planes * 5;
+  b->qamax = c.take<uint32_t>(planes * 2);
+  b->norms = c.take<uint32_t>(planes * 2);
   pk.k.rows = pk.v.rows = packed_rows(s.seq);
   b->q.rows = b->g.rows = packed_rows((int64_t)s.seq * s.G);
   pk.k.data = c.take<uint8_t>(planes * pk.k.plane_bytes(CB));
@@ -731,12 +755,16 @@ int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
     GN_CUDA(cudaFuncSetAttribute(stream_tc_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemQ));
   }
   const int64_t planes = (int64_t)s.rows * s.Hkv;
-  GN_CUDA(cudaMemsetAsync(b.pk.amax, 0, planes * 7 * sizeof(uint32_t), st));
   GN_TRY(stream_pack_keys(s, b.pk, b.norms, st));
-  const dim3 rows(ceil_div(b.q.rows, kPackRowsQ), s.Hkv, s.rows);
-  stream_query_amax_kernel<CB><<<rows, 256, 0, st>>>(b);
-  GN_LAUNCH_CHECK();
-  stream_query_pack_kernel<CB><<<rows, 256, 0, st>>>(b);
+  const int whole = b.q.rows <= kWholePlaneQ;
+  if (!whole) {
+    const dim3 rows(ceil_div(b.q.rows, kPackRowsQ), s.Hkv, s.rows);
+    GN_CUDA(cudaMemsetAsync(b.qamax, 0, planes * 2 * sizeof(uint32_t), st));
+    GN_CUDA(cudaMemset2DAsync(b.norms + 1, 2 * sizeof(uint32_t), 0, sizeof(uint32_t), planes, st));
+    stream_query_amax_kernel<CB><<<rows, 256, 0, st>>>(b);
+    GN_LAUNCH_CHECK();
+  }
+  stream_query_pack_kernel<CB><<<dim3(whole ? 1 : ceil_div(b.q.rows, kPackRowsQ), s.Hkv, s.rows), 256, 0, st>>>(b, whole);
   GN_LAUNCH_CHECK();
   stream_tc_dkv_kernel<DP><<<dim3(b.units, s.Hkv, s.rows), kThreadsB, kSmemKv, st>>>(b);
   GN_LAUNCH_CHECK();

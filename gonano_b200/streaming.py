@@ -10,6 +10,7 @@ Tensors are float32 (lengths and tables int32) on one CUDA device; the channels 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -18,40 +19,63 @@ from . import _lib
 from ._lib import GnEvictParams, GnPagedParams, GnSinkParams, GnView, GonanoError, check
 
 
-def _need(condition, message):
-    if not condition:
-        raise GonanoError(message)
+def _refuse(message):
+    raise GonanoError(message)
 
 
-def _same(name, tensor, dtype, device, shape):
-    _need(isinstance(tensor, torch.Tensor) and tensor.dtype == dtype and tensor.device == device and tuple(tensor.shape) == tuple(shape),
-          f"{name}: want a {dtype} tensor of shape {tuple(shape)} on {device}")
+def _want(name, dtype, shape, device):
+    _refuse(f"{name}: want a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
 
 
-def _packed(name, tensor, dtype, device, shape):
-    _same(name, tensor, dtype, device, shape)
-    _need(tensor.is_contiguous(), f"{name}: want a contiguous tensor")
+def _packed(name, t, dtype, device, shape):
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.device == device):
+        _want(name, dtype, shape, device)
+    return t.data_ptr()
 
 
 def _view4(name, t, device, shape):
     """[batch, heads, tokens, channels]"""
-    _same(name, t, torch.float32, device, shape)
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.shape == shape and t.device == device):
+        _refuse(f"{name}: want a torch.float32 tensor of shape {tuple(shape)} on {device}")
     sb, sh, st, sd = t.stride()
-    _need(sd == 1 or t.shape[3] == 1, f"{name}: the channels of a head must be contiguous")
+    if sd != 1 and shape[3] > 1:
+        _refuse(f"{name}: the channels of a head must be contiguous")
     return GnView(t.data_ptr(), sb, sh, st)
 
 
 def _view3(name, t, device, shape):
     """[tokens, heads, channels]"""
-    _same(name, t, torch.float32, device, shape)
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.shape == shape and t.device == device):
+        _refuse(f"{name}: want a torch.float32 tensor of shape {tuple(shape)} on {device}")
     st, sh, sd = t.stride()
-    _need(sd == 1 or t.shape[2] == 1, f"{name}: the channels of a head must be contiguous")
+    if sd != 1 and shape[2] > 1:
+        _refuse(f"{name}: the channels of a head must be contiguous")
     return GnView(t.data_ptr(), 0, sh, st)
 
 
+def _shaped(name, t, dims, what):
+    if not (isinstance(t, torch.Tensor) and t.dim() == dims):
+        _refuse(f"{name}: want {what}")
+    return t.shape
+
+
 def _cuda(name, t, dims):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 and t.dim() == dims, f"{name}: want a float32 CUDA tensor of {dims} dimensions")
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.float32 and t.dim() == dims):
+        _refuse(f"{name}: want a float32 CUDA tensor of {dims} dimensions")
     return t.device
+
+
+def _on(device):
+    """The library works on the current device: makes it the tensors' one where it is another."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
+_NONE = GnView()
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)   # torch.cuda.current_stream builds a Stream object, 2 us
 
 
 def _workspace(nbytes, device):
@@ -66,13 +90,12 @@ def _address(tensor):
 def _sink_params(q, k, v, sinks, window, scale, lengths):
     device = _cuda("q", q, 4)
     batch, heads, seq, dim = q.shape
-    _need(isinstance(k, torch.Tensor) and k.dim() == 4, "k: want a float32 CUDA tensor of 4 dimensions")
-    shape = (batch, k.shape[1], seq, dim)
-    p = GnSinkParams(_view4("q", q, device, q.shape), _view4("k", k, device, shape), _view4("v", v, device, shape), batch, heads, k.shape[1], seq, dim,
+    kv_heads = _shaped("k", k, 4, "[batch, kv_heads, seq, dim]")[1]
+    shape = (batch, kv_heads, seq, dim)
+    p = GnSinkParams(_view4("q", q, device, q.shape), _view4("k", k, device, shape), _view4("v", v, device, shape), batch, heads, kv_heads, seq, dim,
                      sinks, window, scale)
     if lengths is not None:
-        _packed("lengths", lengths, torch.int32, device, (batch,))
-        p.lengths = lengths.data_ptr()
+        p.lengths = _packed("lengths", lengths, torch.int32, device, (batch,))
     return p, device
 
 
@@ -82,14 +105,14 @@ def sink_attention_forward(q, k, v, sinks, window, scale=1.0, lengths=None, out=
     and their lse -inf.  ``window`` < 0: no window."""
     lib = _lib.load()
     p, device = _sink_params(q, k, v, sinks, window, scale, lengths)
-    with torch.cuda.device(device):
+    with _on(device):
         out = torch.empty(q.shape, dtype=torch.float32, device=device) if out is None else out
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if lse is None else lse
         _packed("lse", lse, torch.float32, device, q.shape[:3])
         view, nbytes = _view4("out", out, device, q.shape), C.c_int64()
         check(lib.gn_attention_sink_workspace(C.byref(p), 0, C.byref(nbytes)))
         space = _workspace(nbytes.value, device)
-        check(lib.gn_attention_sink_forward(C.byref(p), C.byref(view), lse.data_ptr(), _address(space), nbytes.value, torch.cuda.current_stream(device).cuda_stream))
+        check(lib.gn_attention_sink_forward(C.byref(p), C.byref(view), lse.data_ptr(), _address(space), nbytes.value, _stream(device)))
     return out, lse
 
 
@@ -99,8 +122,9 @@ def sink_attention_backward(q, k, v, out, dout, lse, sinks, window, scale=1.0, l
     lib = _lib.load()
     p, device = _sink_params(q, k, v, sinks, window, scale, lengths)
     given = [g is not None for g in (dq, dk, dv)]
-    _need(all(given) or not any(given), "sink_attention_backward: give dq, dk and dv or none of them")
-    with torch.cuda.device(device):
+    if any(given) and not all(given):
+        _refuse("sink_attention_backward: give dq, dk and dv or none of them")
+    with _on(device):
         if not given[0]:
             dq, dk, dv = (torch.empty(x.shape, dtype=torch.float32, device=device) for x in (q, k, v))
         _packed("lse", lse, torch.float32, device, q.shape[:3])
@@ -109,7 +133,7 @@ def sink_attention_backward(q, k, v, out, dout, lse, sinks, window, scale=1.0, l
         check(lib.gn_attention_sink_workspace(C.byref(p), 1, C.byref(nbytes)))
         space = _workspace(nbytes.value, device)
         check(lib.gn_attention_sink_backward(C.byref(p), C.byref(views[0]), C.byref(views[1]), lse.data_ptr(), C.byref(views[2]), C.byref(views[3]),
-                                             C.byref(views[4]), int(given[0]), _address(space), nbytes.value, torch.cuda.current_stream(device).cuda_stream))
+                                             C.byref(views[4]), int(given[0]), _address(space), nbytes.value, _stream(device)))
     return dq, dk, dv
 
 
@@ -130,39 +154,32 @@ def paged_attention(q, key_pages, value_pages, page_table, query_starts, context
     lib = _lib.load()
     device = _cuda("q", q, 3)
     tokens, heads, dim = q.shape
-    _need(isinstance(key_pages, torch.Tensor) and key_pages.dim() == 4, "key_pages: want [pages, kv_heads, page_size, dim]")
-    pages, kv_heads, page_size = key_pages.shape[:3]
-    for name, t in (("key_pages", key_pages), ("value_pages", value_pages)):
-        _packed(name, t, torch.float32, device, (pages, kv_heads, page_size, dim))
-    _need(isinstance(page_table, torch.Tensor) and page_table.dim() == 2, "page_table: want [rows, width]")
-    rows, width = page_table.shape
-    _packed("page_table", page_table, torch.int32, device, (rows, width))
-    _packed("query_starts", query_starts, torch.int32, device, (rows + 1,))
-    _packed("context_lens", context_lens, torch.int32, device, (rows,))
-    _need((new_key is None) == (new_value is None), "paged_attention: give new_key and new_value or neither")
-    p = GnPagedParams(query=_view3("q", q, device, q.shape), key_pages=key_pages.data_ptr(), value_pages=value_pages.data_ptr(),
-                      page_table=page_table.data_ptr(), query_starts=query_starts.data_ptr(), context_lens=context_lens.data_ptr(), rows=rows, tokens=tokens,
-                      max_query=max_query, max_context=width * page_size if max_context is None else max_context, n_head=heads, n_kv_head=kv_heads,
-                      head_dim=dim, page_size=page_size, pages=pages, table_width=width, sinks=sinks, window=window, scale=scale)
-    if new_key is not None:
-        p.new_key, p.new_value = (_view3(n, t, device, (tokens, kv_heads, dim)) for n, t in (("new_key", new_key), ("new_value", new_value)))
-    with torch.cuda.device(device):
+    pages, kv_heads, page_size, _ = _shaped("key_pages", key_pages, 4, "[pages, kv_heads, page_size, dim]")
+    rows, width = _shaped("page_table", page_table, 2, "[rows, width]")
+    if (new_key is None) != (new_value is None):
+        _refuse("paged_attention: give new_key and new_value or neither")
+    store, fresh = (pages, kv_heads, page_size, dim), (tokens, kv_heads, dim)
+    p = GnPagedParams(_view3("q", q, device, q.shape), _NONE if new_key is None else _view3("new_key", new_key, device, fresh),
+                      _NONE if new_value is None else _view3("new_value", new_value, device, fresh), _packed("key_pages", key_pages, torch.float32, device, store),
+                      _packed("value_pages", value_pages, torch.float32, device, store), _packed("page_table", page_table, torch.int32, device, (rows, width)),
+                      _packed("query_starts", query_starts, torch.int32, device, (rows + 1,)), _packed("context_lens", context_lens, torch.int32, device, (rows,)),
+                      None, None, rows, tokens, max_query, width * page_size if max_context is None else max_context, heads, kv_heads, dim, page_size, pages, width,
+                      sinks, window, scale)
+    with _on(device):
         if mass is not None or mass_out is not None:
             shape = (rows, kv_heads, width * page_size)
             if mass is not None:
-                _packed("mass", mass, torch.float32, device, shape)
-                p.mass = mass.data_ptr()
+                p.mass = _packed("mass", mass, torch.float32, device, shape)
             if mass_out is None:
                 mass_out = mass.clone()
-            _packed("mass_out", mass_out, torch.float32, device, shape)
-            p.mass_out = mass_out.data_ptr()
+            p.mass_out = _packed("mass_out", mass_out, torch.float32, device, shape)
         out = torch.zeros(q.shape, dtype=torch.float32, device=device) if out is None else out
         lse = torch.zeros((tokens, heads), dtype=torch.float32, device=device) if lse is None else lse
         _packed("lse", lse, torch.float32, device, (tokens, heads))
         view, nbytes = _view3("out", out, device, q.shape), C.c_int64()
         check(lib.gn_attention_paged_workspace(C.byref(p), C.byref(nbytes)))
         space = _workspace(nbytes.value, device)
-        check(lib.gn_attention_paged(C.byref(p), C.byref(view), lse.data_ptr(), _address(space), nbytes.value, torch.cuda.current_stream(device).cuda_stream))
+        check(lib.gn_attention_paged(C.byref(p), C.byref(view), lse.data_ptr(), _address(space), nbytes.value, _stream(device)))
     return (out, lse) if mass_out is None else (out, lse, mass_out)
 
 
@@ -176,25 +193,21 @@ def evict_pages(key_pages, value_pages, mass, page_table, context_lens, budget, 
     kept keys' mass [rows, kv_heads, budget]."""
     lib = _lib.load()
     device = _cuda("key_pages", key_pages, 4)
-    pages, kv_heads, page_size, dim = key_pages.shape
-    for name, t in (("key_pages", key_pages), ("value_pages", value_pages)):
-        _packed(name, t, torch.float32, device, key_pages.shape)
-    _need(isinstance(page_table, torch.Tensor) and page_table.dim() == 2, "page_table: want [rows, width]")
-    rows, width = page_table.shape
+    pages, kv_heads, page_size, dim = store = key_pages.shape
+    rows, width = _shaped("page_table", page_table, 2, "[rows, width]")
     new_table = page_table if new_table is None else new_table
-    _need(isinstance(new_table, torch.Tensor) and new_table.dim() == 2, "new_table: want [rows, width]")
-    _packed("page_table", page_table, torch.int32, device, (rows, width))
-    _packed("new_table", new_table, torch.int32, device, (rows, new_table.shape[1]))
-    _packed("context_lens", context_lens, torch.int32, device, (rows,))
-    _need(isinstance(mass, torch.Tensor) and mass.dim() == 3, "mass: want [rows, kv_heads, n]")
-    _packed("mass", mass, torch.float32, device, (rows, kv_heads, mass.shape[2]))
-    _need(budget >= 0, f"evict_pages: budget {budget} is negative")
-    p = GnEvictParams(key_pages.data_ptr(), value_pages.data_ptr(), mass.data_ptr(), page_table.data_ptr(), new_table.data_ptr(), context_lens.data_ptr(), rows,
-                      kv_heads, dim, page_size, pages, width, new_table.shape[1], mass.shape[2], width * page_size if max_context is None else max_context,
-                      budget, sinks, recent)
-    with torch.cuda.device(device):
+    new_width = _shaped("new_table", new_table, 2, "[rows, width]")[1]
+    n = _shaped("mass", mass, 3, "[rows, kv_heads, n]")[2]
+    if budget < 0:
+        _refuse(f"evict_pages: budget {budget} is negative")
+    p = GnEvictParams(_packed("key_pages", key_pages, torch.float32, device, store), _packed("value_pages", value_pages, torch.float32, device, store),
+                      _packed("mass", mass, torch.float32, device, (rows, kv_heads, n)), _packed("page_table", page_table, torch.int32, device, (rows, width)),
+                      _packed("new_table", new_table, torch.int32, device, (rows, new_width)),
+                      _packed("context_lens", context_lens, torch.int32, device, (rows,)), rows, kv_heads, dim, page_size, pages, width, new_width, n,
+                      width * page_size if max_context is None else max_context, budget, sinks, recent)
+    with _on(device):
         kept = torch.empty((rows, kv_heads, budget), dtype=torch.int32, device=device)
         lens = torch.empty((rows,), dtype=torch.int32, device=device)
         mass_out = torch.empty((rows, kv_heads, budget), dtype=torch.float32, device=device)
-        check(lib.gn_cache_evict(C.byref(p), kept.data_ptr(), lens.data_ptr(), mass_out.data_ptr(), torch.cuda.current_stream(device).cuda_stream))
+        check(lib.gn_cache_evict(C.byref(p), kept.data_ptr(), lens.data_ptr(), mass_out.data_ptr(), _stream(device)))
     return kept, lens, mass_out
