@@ -1,4 +1,4 @@
-// Streaming attention: C entry points and the float32 kernels (a warp per row of the result).
+// Streaming attention: the C entry points, their checks, and the copy of new tokens to their pages.
 #include <algorithm>
 
 #include "streaming_tc.cuh"
@@ -6,27 +6,6 @@
 namespace gn {
 
 namespace {
-
-constexpr int kE = 4;   // channels of a lane: head_dim <= 128
-
-template <bool PAGED>
-__device__ __forceinline__ void load_lane(const float* p, int D, float (&x)[kE]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int e = 0; e < kE; ++e) x[e] = (p && lane + 32 * e < D) ? p[lane + 32 * e] : 0.0f;
-}
-__device__ __forceinline__ float dot_lane(const float (&a)[kE], const float (&b)[kE]) {
-  float d = 0.0f;
-#pragma unroll
-  for (int e = 0; e < kE; ++e) d = fmaf(a[e], b[e], d);
-  return warp_sum(d);
-}
-template <bool PAGED>
-__device__ __forceinline__ const float* key_ptr(const StreamRows& s, bool value, int r, int hk, int j) {
-  const int64_t off = key_offset<PAGED>(s, value ? s.v : s.k, r, hk, j);
-  if (off < 0 && PAGED) return nullptr;
-  return (PAGED ? (value ? s.pages_v : s.pages_k) : (value ? s.v.data : s.k.data)) + off;
-}
 
 // A warp per (row, new token, kv head): the new token's key and value go to its slot.
 __global__ void __launch_bounds__(128) stream_append_kernel(StreamRows s, gn_view nk, gn_view nv) {
@@ -41,33 +20,6 @@ __global__ void __launch_bounds__(128) stream_append_kernel(StreamRows s, gn_vie
   const float* a = nk.data + token_offset<true>(nk, r, hk, sp.q_begin + t); const float* b = nv.data + token_offset<true>(nv, r, hk, sp.q_begin + t);
   for (int c = lane; c < s.D; c += 32) { s.pages_k[to + c] = a[c]; s.pages_v[to + c] = b[c]; }
 }
-// A warp per (row, kv head, key): the weight that this call's queries gave the key.
-__global__ void __launch_bounds__(128) stream_mass_kernel(StreamRows s, const float* __restrict__ lse, const float* mass, float* mass_out) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int j = blockIdx.x * 4 + warp, hk = blockIdx.y, r = blockIdx.z;
-  const RowSpan sp = row_span<true>(s, r);
-  if (j >= sp.ctx) return;
-  const int first = sp.ctx - sp.q_len;
-  float sum = 0.0f;
-  const float* kp = key_ptr<true>(s, false, r, hk, j);
-  if (kp) {
-    float k[kE];
-    load_lane<true>(kp, s.D, k);
-    for (int t = max(0, j - first); t < sp.q_len; ++t) {
-      if (!sees(s, first + t, j)) continue;
-      for (int h = hk * s.G; h < (hk + 1) * s.G; ++h) {
-        float q[kE];
-        load_lane<true>(s.q.data + token_offset<true>(s.q, r, h, sp.q_begin + t), s.D, q);
-        sum += expf(dot_lane(q, k) * s.scale - lse[stat_offset<true>(s, r, h, sp.q_begin + t)]);
-      }
-    }
-  }
-  if (lane == 0) {
-    const int64_t at = ((int64_t)r * s.Hkv + hk) * s.width * s.page_size + j;
-    mass_out[at] = (mass && j < first ? mass[at] : 0.0f) + sum;
-  }
-}
-
 // ------------------------------------------------------------------ checks
 int on_this_device(const void* p, const char* what) {
   int device = 0;
@@ -128,7 +80,7 @@ int64_t sink_bytes(const StreamRows& s, int backward) { return backward ? stream
 // New tokens over a paged cache: up to 16 query rows a kv head run on the kernel that streams the cache once, more on the tensor
 // cores, which pack the keys first (3 times the cache's bytes) but take 128 rows for one reading.
 bool paged_on_tensor_cores(const StreamRows& s) { return (int64_t)s.max_query * s.G > 16; }
-int64_t paged_bytes(const StreamRows& s, bool mass) { return paged_on_tensor_cores(s) ? stream_tc_forward_bytes(s) : stream_decode_bytes(s, mass); }
+int64_t paged_bytes(const StreamRows& s, bool mass) { return !paged_on_tensor_cores(s) ? stream_decode_bytes(s, mass) : stream_tc_forward_bytes(s) + (mass ? stream_tc_mass_bytes(s) : 0); }
 
 int paged_rows(const gn_paged_params* p, StreamRows* s) {
   GN_REQUIRE(p, "attention_paged: null parameters");
@@ -222,12 +174,10 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
     stream_append_kernel<<<dim3(ceil_div(s.max_query, 4), s.Hkv, s.rows), 128, 0, st>>>(s, p->new_key, p->new_value);
     GN_LAUNCH_CHECK();
   }
-  GN_TRY(stream_tc_forward(s, *out, lse, workspace, st));
-  if (p->mass_out && s.max_context) {
-    stream_mass_kernel<<<dim3(ceil_div(s.max_context, 4), s.Hkv, s.rows), 128, 0, st>>>(s, lse, p->mass, p->mass_out);
-    GN_LAUNCH_CHECK();
-  }
-  return GN_OK;
+  PackedKeys packed;
+  GN_TRY(stream_tc_forward(s, *out, lse, workspace, st, &packed));
+  if (!p->mass_out || !s.max_context) return GN_OK;
+  return stream_tc_mass(s, packed, lse, p->mass, p->mass_out, static_cast<uint8_t*>(workspace) + stream_tc_forward_bytes(s), st);
 }
 
 int gn_cache_evict(const gn_evict_params* p, int32_t* kept, int32_t* new_lens, float* mass_out, void* stream) {

@@ -658,11 +658,12 @@ int64_t stream_tc_forward_bytes(const StreamRows& s) {
   ForwardTc f{};
   return carve_forward(s, plan_forward(s), nullptr, &f);
 }
-int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t st) {
+int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t st, PackedKeys* packed) {
   const Plan pl = plan_forward(s);
   ForwardTc f{};
   f.s = s; f.out = out; f.lse = lse; f.tiles = pl.tiles; f.splits = pl.splits;
   carve_forward(s, pl, workspace, &f);
+  if (packed) *packed = f.pk;
   f.vec_q = vec_view(s.q, s.D); f.vec_out = pl.splits > 1 || vec_view(out, s.D);
   if (pl.DP == 64) return s.paged() ? forward_go<64, true>(s, pl, f, st) : forward_go<64, false>(s, pl, f, st);
   return s.paged() ? forward_go<128, true>(s, pl, f, st) : forward_go<128, false>(s, pl, f, st);

@@ -60,7 +60,10 @@ int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms,
 
 // tcgen05 forward of a call (streaming_tc.cu): the workspace it wants, and the launches.
 int64_t stream_tc_forward_bytes(const StreamRows& s);
-int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t stream);
+int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t stream, PackedKeys* packed = nullptr);
+// The weights of a paged call's keys (streaming_tc_mass.cu), from the forward's packed keys and its log-sum-exps.
+int64_t stream_tc_mass_bytes(const StreamRows& s);
+int stream_tc_mass(const StreamRows& s, const PackedKeys& pk, const float* lse, const float* mass, float* mass_out, void* workspace, cudaStream_t stream);
 // tcgen05 backward (streaming_tc_backward.cu), padded batches.
 int64_t stream_tc_backward_bytes(const StreamRows& s);
 int stream_tc_backward(const StreamRows& s, const gn_view& out, const gn_view& dout, const float* lse, const gn_view& dq, const gn_view& dk, const gn_view& dv,
