@@ -187,49 +187,69 @@ __device__ __forceinline__ PlaneFactors plane_factors(const BackwardTc& p, int64
   return f;
 }
 
-constexpr int kThreadsB = 384;        // two warpgroups of softmax threads, one for the issuing and the copying warp
-constexpr int kRegsSoftmax = 224, kRegsOther = 56;
-constexpr int kFlush = 2;             // steps whose sums are left to the tensor core before they are rounded into registers
-// Adds 32 * N columns of an accumulator to registers.
+constexpr int kThreadsB = 640;        // four warpgroups of softmax threads, one for the issuing and the copying warps
+constexpr int kRegsSoftmax = 104, kRegsOther = 64;   // shares of the launch's 5 x 96
+constexpr int kFlush = 2;             // steps whose sums are left to the tensor core before they are rounded into registers: the error of
+                                      // dk and dv grows with it (1: 6.9e-7 of the largest norm, 2: 8.4e-7, 4: 1.2e-6, 8: 2.0e-6)
+
+// Adds N (32 or 16) columns of an accumulator to registers.
 template <int N>
-__device__ __forceinline__ void add_columns(uint32_t taddr, float* acc) {
+__device__ __forceinline__ void add_columns(uint32_t taddr, float (&acc)[N]) {
+  uint32_t y[N];
+  if constexpr (N == 32) tmem_ld32(taddr, y);
+  else tmem_ld16(taddr, y);
+  tmem_ld_wait();
 #pragma unroll
-  for (int h = 0; h < N; ++h) {
-    uint32_t y[32];
-    tmem_ld32(taddr + h * 32, y);
-    tmem_ld_wait();
-#pragma unroll
-    for (int e = 0; e < 32; ++e) acc[h * 32 + e] += __uint_as_float(y[e]);
-  }
+  for (int e = 0; e < N; ++e) acc[e] += __uint_as_float(y[e]);
 }
-// 32 values of a row to f16 pairs in tensor memory: 16 columns of hi, 16 of lo.
-__device__ __forceinline__ void store_pairs(uint32_t taddr, const float (&x)[32]) {
-  uint32_t y[32];
+// 16 values of a row to f16 pairs in tensor memory: 8 columns of hi, 8 of lo.
+__device__ __forceinline__ void store_pairs(uint32_t taddr, const float (&x)[16]) {
+  uint32_t y[16];
 #pragma unroll
-  for (int e = 0; e < 32; e += 2) split_f16(x[e], x[e + 1], y[e >> 1], y[16 + (e >> 1)]);
-  tmem_st32(taddr, y);
+  for (int e = 0; e < 16; e += 2) split_f16(x[e], x[e + 1], y[e >> 1], y[8 + (e >> 1)]);
+  tmem_st16(taddr, y);
   tmem_st_wait();
 }
-// Row `row` of a packed plane's hi half (channels 64 * block ..), unswizzled, to 32 columns of tensor memory.
-__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint8_t* src, int row, bool live) {
-  uint32_t y[32];
+// A quarter of a packed plane's hi row (half a 64-channel block, unswizzled) to 16 columns of tensor memory.
+__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint8_t* block, int row, int half, bool live) {
+  uint32_t y[16];
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
+  for (int c = 0; c < 4; ++c) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (live) v = *reinterpret_cast<const uint4*>(src + (int64_t)row * 128 + ((c ^ (row & 7)) << 4));
+    if (live) v = *reinterpret_cast<const uint4*>(block + (int64_t)row * 128 + (((half * 4 + c) ^ (row & 7)) << 4));
     y[4 * c] = v.x; y[4 * c + 1] = v.y; y[4 * c + 2] = v.z; y[4 * c + 3] = v.w;
   }
-  tmem_st32(taddr, y);
+  tmem_st16(taddr, y);
+}
+// A thread's QC channels of a gradient row.
+template <int QC>
+__device__ __forceinline__ void write_row(float* dst, int ch, int D, const float (&acc)[QC], float z, bool accumulate, bool vec) {
+#pragma unroll
+  for (int e = 0; e < QC; e += 4) {
+    if (vec) {
+      if (ch + e < D) {
+        float4 v = make_float4(acc[e] * z, acc[e + 1] * z, acc[e + 2] * z, acc[e + 3] * z);
+        if (accumulate) { const float4 o = *reinterpret_cast<const float4*>(dst + ch + e); v.x = __fadd_rn(o.x, v.x); v.y = __fadd_rn(o.y, v.y); v.z = __fadd_rn(o.z, v.z); v.w = __fadd_rn(o.w, v.w); }
+        *reinterpret_cast<float4*>(dst + ch + e) = v;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (ch + e + u < D) dst[ch + e + u] = accumulate ? __fadd_rn(dst[ch + e + u], __fmul_rn(acc[e + u], z)) : acc[e + u] * z;
+    }
+  }
 }
 
 // dK and dV.  One CTA per (128 keys or a part of their query rows, kv head, sequence): S^T = K Q^T and dP^T = V dO^T of 64 query rows a
-// step, a softmax thread per (key, 32 query rows) turns them into P^T and dS^T in place, and dV += P^T dO, dK += dS^T Q take them
-// from tensor memory.  The hi half of K lives in tensor memory too, which leaves room for two stages of Q and dO.
+// step, a softmax thread per (key, 16 query rows) turns them into P^T and dS^T in place, and dV += P^T dO, dK += dS^T Q take them
+// from tensor memory.  The hi half of K lives in tensor memory too, which leaves room for two stages of Q and dO.  Two warps issue,
+// one the scores and one the sums, so that neither's waits hold up the other's instructions.
 // Tensor memory: S^T 2 x 64 columns, dP^T 64, K hi 64, dV 128, dK 128.  Shared memory: V 64 KB, K lo 32 KB, 2 x (Q 32 KB + dO 32 KB).
-// Every kFlush steps dV and dK are added to float32 registers (64 + 64 a thread).  Bound: tensor pipe.
+// Every kFlush steps dV and dK are added to float32 registers (32 + 32 a thread), one step later, between that step's weights and
+// its dS, while the products that end the chunk run.  Bound: tensor pipe, 48 instructions of 46 cycles and 24 of 64 a step.
 template <int DP>
 __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __grid_constant__ BackwardTc p) {
-  constexpr int CB = DP / 64, HC = DP / 2;
+  constexpr int CB = DP / 64, QC = DP / 4;
   constexpr uint32_t SLOT = CB * 16384u, OFF_KL = CB * 32768u, OFF_Q = OFF_KL + CB * 16384u, OFF_G = OFF_Q + 2 * SLOT, STATS = OFF_G + 2 * SLOT, BARS = STATS + 1024;
   constexpr uint32_t COL_S = 0, COL_DP = 128, COL_KH = 192, COL_DV = 256, COL_DK = 384;
   extern __shared__ uint8_t smem_raw[];
@@ -237,160 +257,161 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   const int hk = blockIdx.y, r = blockIdx.z, x0 = blockIdx.x;
   const bool sink = x0 < p.sink_tiles * p.parts_sink;
   const int parts = sink ? p.parts_sink : p.parts, y0 = sink ? x0 : x0 - p.sink_tiles * p.parts_sink;
-  const int kt = (sink ? 0 : p.sink_tiles) + y0 / parts, part = y0 % parts, k0 = kt * 128;
+  const int kt = (sink ? 0 : p.sink_tiles) + y0 / parts, part_i = y0 % parts, k0 = kt * 128;
   const int len = row_span<false>(s, r).ctx;
   if (k0 >= len && parts > 1) return;   // the summing kernel does not look at padding
   const int nf = len * s.G;
   const int64_t t_end = (s.window < 0 || k0 < s.sinks) ? len : min((int64_t)len, (int64_t)k0 + 128 + s.window);
   const int f_begin = (k0 * s.G) & ~7, f_end = (int)t_end * s.G;
   const int steps = k0 < len ? (f_end - f_begin + 63) / 64 : 0, per = (steps + parts - 1) / parts;
-  const int i0 = part * per, n = max(0, min(steps, i0 + per) - i0);
+  const int i0 = part_i * per, n = max(0, min(steps, i0 + per) - i0);
   const int64_t plane = (int64_t)r * s.Hkv + hk;
 
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bars = base + BARS;
-  const uint32_t v_full = bars, kh_ready = bars + 8, dp_full = bars + 16, ds_full = bars + 24, acc_full = bars + 32, acc_empty = bars + 40, tmem_slot = bars + 128;
+  const uint32_t v_full = bars, kh_ready = bars + 8, dp_full = bars + 16, ds_full = bars + 24, acc_full = bars + 32, acc_empty = bars + 40, dp_free = bars + 152, tmem_slot = bars + 176;
   auto q_full = [&](int i) { return bars + 48u + 8u * i; };
   auto g_full = [&](int i) { return bars + 64u + 8u * i; };
   auto q_empty = [&](int i) { return bars + 80u + 8u * i; };
   auto g_empty = [&](int i) { return bars + 96u + 8u * i; };
   auto s_full = [&](int i) { return bars + 112u + 8u * i; };
-  auto p_full = [&](int i) { return bars + 136u + 8u * i; };
+  auto p_full = [&](int i) { return bars + 128u + 8u * i; };
+  auto s_free = [&](int i) { return bars + 160u + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(v_full, 1); mbar_init(kh_ready, 256); mbar_init(dp_full, 1); mbar_init(ds_full, 256); mbar_init(acc_full, 1); mbar_init(acc_empty, 256);
+    mbar_init(v_full, 1); mbar_init(kh_ready, 512); mbar_init(dp_full, 1); mbar_init(ds_full, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512); mbar_init(dp_free, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full(i), 1); mbar_init(g_full(i), 1); mbar_init(q_empty(i), 1); mbar_init(g_empty(i), 1); mbar_init(s_full(i), 1); mbar_init(p_full(i), 256);
+      mbar_init(q_full(i), 1); mbar_init(g_full(i), 1); mbar_init(q_empty(i), 1); mbar_init(g_empty(i), 2); mbar_init(s_full(i), 1); mbar_init(p_full(i), 512);
+      mbar_init(s_free(i), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 16) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 128);
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 176);
   auto row0 = [&](int i) { return f_begin + (i0 + i) * 64; };
   auto rows16 = [&](int i) { return min(64, (f_end - row0(i) + 15) & ~15); };
 
-  if (warp >= 8) {
+  if (warp >= 16) {
     regs_dec<kRegsOther>();
-    if (warp == 9 && lane == 0 && n > 0) {
+    if (warp == 17 && lane == 0 && n > 0) {
       // ----------------------------------------------------------- copies
       const int keys = min(128, (len - k0 + 15) & ~15);
       mbar_expect_tx(v_full, (uint32_t)CB * 3u * keys * 128u);
       const uint8_t* vp = p.pk.v.data + plane * p.pk.v.plane_bytes(CB); const uint8_t* kp = p.pk.k.data + plane * p.pk.k.plane_bytes(CB);
+#pragma unroll 1
       for (int b = 0; b < CB * 2; ++b) bulk_load(base + b * 16384, vp + ((int64_t)b * p.pk.v.rows + k0) * 128, keys * 128, v_full);
+#pragma unroll 1
       for (int b = 0; b < CB; ++b) bulk_load(base + OFF_KL + b * 16384, kp + ((int64_t)(2 * b + 1) * p.pk.k.rows + k0) * 128, keys * 128, v_full);
       const uint8_t* qp = p.q.data + plane * p.q.plane_bytes(CB); const uint8_t* gp = p.g.data + plane * p.g.plane_bytes(CB);
       bool ok = true;
-      int jq = 0, jg = 0;
-      for (uint32_t idle = 0; jg < n && ok;) {
-        bool did = false;
-        if (jq < n && (jq < 2 || mbar_test(q_empty(jq & 1), ((jq >> 1) - 1) & 1))) {
-          const int rows = rows16(jq);
-          const uint32_t bar = q_full(jq & 1), dst = base + OFF_Q + (jq & 1) * SLOT, st = base + STATS + (jq & 1) * 512;
-          mbar_expect_tx(bar, (uint32_t)CB * 2u * rows * 128u + 2u * rows * 4u);
-          for (int b = 0; b < CB * 2; ++b) bulk_load(dst + b * 8192, qp + ((int64_t)b * p.q.rows + row0(jq)) * 128, rows * 128, bar);
-          bulk_load(st, p.off + plane * p.q.rows + row0(jq), rows * 4, bar);
-          bulk_load(st + 256, p.delta + plane * p.q.rows + row0(jq), rows * 4, bar);
-          ++jq; did = true;
-        }
-        if (jg < jq && (jg < 2 || mbar_test(g_empty(jg & 1), ((jg >> 1) - 1) & 1))) {
-          const int rows = rows16(jg);
-          const uint32_t bar = g_full(jg & 1), dst = base + OFF_G + (jg & 1) * SLOT;
-          mbar_expect_tx(bar, (uint32_t)CB * 2u * rows * 128u);
-          for (int b = 0; b < CB * 2; ++b) bulk_load(dst + b * 8192, gp + ((int64_t)b * p.g.rows + row0(jg)) * 128, rows * 128, bar);
-          ++jg; did = true;
-        }
-        if (did) idle = 0;
-        else if (++idle > kSpinLimit) ok = false;
-        else if (idle > 4096) __nanosleep(64);
+      for (int i = 0; i < n && ok; ++i) {
+        const int rows = rows16(i), f = row0(i), b2 = i & 1;
+        if (i >= 2) ok = mbar_wait(q_empty(b2), ((i >> 1) - 1) & 1);
+        if (!ok) break;
+        mbar_expect_tx(q_full(b2), (uint32_t)CB * 2u * rows * 128u + 2u * rows * 4u);
+#pragma unroll 1
+        for (int b = 0; b < CB * 2; ++b) bulk_load(base + OFF_Q + b2 * SLOT + b * 8192, qp + ((int64_t)b * p.q.rows + f) * 128, rows * 128, q_full(b2));
+        bulk_load(base + STATS + b2 * 512, p.off + plane * p.q.rows + f, rows * 4, q_full(b2));
+        bulk_load(base + STATS + b2 * 512 + 256, p.delta + plane * p.q.rows + f, rows * 4, q_full(b2));
+        if (i >= 2) ok = mbar_wait(g_empty(b2), ((i >> 1) - 1) & 1);
+        if (!ok) break;
+        mbar_expect_tx(g_full(b2), (uint32_t)CB * 2u * rows * 128u);
+#pragma unroll 1
+        for (int b = 0; b < CB * 2; ++b) bulk_load(base + OFF_G + b2 * SLOT + b * 8192, gp + ((int64_t)b * p.g.rows + f) * 128, rows * 128, g_full(b2));
       }
       if (!ok)   // copies in flight land before the CTA goes
         for (int i = 0; i < 2; ++i)
           for (int ph = 0; ph < 2; ++ph) { mbar_wait(q_full(i), ph); mbar_wait(g_full(i), ph); }
       mbar_wait(v_full, 0);
     }
-    if (warp == 8 && n > 0) {
+    if (warp == 16 && n > 0) {
+      // ----------------------------------------------------------- scores: S^T(0), dP^T(0), S^T(1), dP^T(1), ...
       const uint32_t el = elect_lane();
-      // ----------------------------------------------------------- instructions: whichever product has its operands
-      int is = 0, ip = 0, iv = 0, ik = 0, chunk = 0;   // next S, dP, dV, dK; the accumulation chunk that may be written
       bool ok = mbar_wait(v_full, 0) && mbar_wait(kh_ready, 0);
       tc_fence_after();
-      const uint32_t kl = base + OFF_KL;
-      auto in_chunk = [&](int i) {
-        if (i / kFlush > chunk && mbar_test(acc_empty, chunk & 1)) ++chunk;
-        return i / kFlush <= chunk;
-      };
-      // rows of a query tile as the MN-major operand of dV, dK
-      auto accumulate = [&](uint32_t d, uint32_t a, uint32_t slot, int i) {
-        const uint32_t id = instr_desc_f16(128, DP, 1);
-        const int slices = rows16(i) >> 4;
-        const uint32_t fresh = i % kFlush == 0 ? 0u : 1u;
-        auto one = [&](int ks, int al, int bl, uint32_t acc) {
-          umma_f16_ts(el, d, a + (ks >> 1) * 32 + al * 16 + (ks & 1) * 8, smem_desc_mn(slot + bl * 8192 + ks * 2048, 16384), id, acc);
-        };
-        for (int ks = 0; ks < slices; ++ks) { one(ks, 1, 0, ks > 0 ? 1u : fresh); one(ks, 0, 1, 1); }
-        for (int ks = 0; ks < slices; ++ks) one(ks, 0, 0, 1);
-      };
-      auto end_chunk = [&]() { if (iv == ik && (iv % kFlush == 0 || iv == n)) commit_by(el, acc_full); };
-      for (uint32_t idle = 0; (ik < n || iv < n) && ok;) {
-        bool did = false;
-        if (ik < ip && in_chunk(ik) && mbar_test(ds_full, ik & 1)) {
-          tc_fence_after();
-          accumulate(tmem + COL_DK, tmem + COL_DP, base + OFF_Q + (ik & 1) * SLOT, ik);
-          commit_by(el, q_empty(ik & 1));
-          ++ik; did = true;
-          end_chunk();
-        }
-        if (ip < n && ip <= ik && mbar_test(g_full(ip & 1), (ip >> 1) & 1)) {
-          tc_fence_after();
-          const uint32_t id = instr_desc_f16(128, rows16(ip), 0), g = base + OFF_G + (ip & 1) * SLOT;
-          auto one = [&](int ks, int vl, int gl, uint32_t acc) {
-            umma_f16(el, tmem + COL_DP, smem_desc_sw128(base + (ks >> 2) * 32768 + vl * 16384) + 2u * (ks & 3),
-                     smem_desc_sw128(g + (ks >> 2) * 16384 + gl * 8192) + 2u * (ks & 3), id, acc);
-          };
-#pragma unroll
-          for (int ks = 0; ks < CB * 4; ++ks) { one(ks, 1, 0, ks > 0); one(ks, 0, 1, 1); }
-#pragma unroll
-          for (int ks = 0; ks < CB * 4; ++ks) one(ks, 0, 0, 1);
-          commit_by(el, dp_full);
-          ++ip; did = true;
-        }
-        if (iv < is && iv < ip && in_chunk(iv) && mbar_test(p_full(iv & 1), (iv >> 1) & 1)) {
-          tc_fence_after();
-          accumulate(tmem + COL_DV, tmem + COL_S + (iv & 1) * 64, base + OFF_G + (iv & 1) * SLOT, iv);
-          commit_by(el, g_empty(iv & 1));
-          ++iv; did = true;
-          end_chunk();
-        }
-        if (is < n && is < iv + 2 && mbar_test(q_full(is & 1), (is >> 1) & 1)) {
-          tc_fence_after();
-          const uint32_t d = tmem + COL_S + (is & 1) * 64, id = instr_desc_f16(128, rows16(is), 0), q = base + OFF_Q + (is & 1) * SLOT;
-          auto b_of = [&](int ks, int ql) { return smem_desc_sw128(q + (ks >> 2) * 16384 + ql * 8192) + 2u * (ks & 3); };
-#pragma unroll
-          for (int ks = 0; ks < CB * 4; ++ks) {
-            umma_f16(el, d, smem_desc_sw128(kl + (ks >> 2) * 16384) + 2u * (ks & 3), b_of(ks, 0), id, ks > 0);
-            umma_f16_ts(el, d, tmem + COL_KH + ks * 8, b_of(ks, 1), id, 1);
+      const uint64_t kl = smem_desc_sw128(base + OFF_KL), vd = smem_desc_sw128(base);
+      for (int i = 0; i < n && ok; ++i) {
+        const int b2 = i & 1;
+        const uint32_t id = instr_desc_f16(128, rows16(i), 0);
+        ok = mbar_wait(q_full(b2), (i >> 1) & 1) && (i < 2 || mbar_wait(s_free(b2), ((i >> 1) - 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        {
+          const uint32_t d = tmem + COL_S + b2 * 64;
+          const uint64_t q = smem_desc_sw128(base + OFF_Q + b2 * SLOT);
+#pragma unroll 2
+          for (int ks = 0; ks < CB * 4; ++ks) {   // a 64-channel block is 16 KB of 128 rows, 2 x 8 KB of 64
+            const uint32_t in = (ks & 3) * 2;
+            umma_f16(el, d, kl + (ks >> 2) * 1024 + in, q + (ks >> 2) * 1024 + in, id, ks > 0);
+            umma_f16_ts(el, d, tmem + COL_KH + ks * 8, q + (ks >> 2) * 1024 + 512 + in, id, 1);
           }
-#pragma unroll
-          for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, tmem + COL_KH + ks * 8, b_of(ks, 0), id, 1);
-          commit_by(el, s_full(is & 1));
-          ++is; did = true;
+#pragma unroll 2
+          for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, tmem + COL_KH + ks * 8, q + (ks >> 2) * 1024 + (ks & 3) * 2, id, 1);
+          commit_by(el, s_full(b2));
         }
-        if (did) idle = 0;
-        else if (++idle > kSpinLimit) ok = false;
-        else if (idle > 4096) __nanosleep(64);
+        ok = mbar_wait(g_full(b2), (i >> 1) & 1) && (i < 1 || mbar_wait(dp_free, (i - 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        {
+          const uint32_t d = tmem + COL_DP;
+          const uint64_t g = smem_desc_sw128(base + OFF_G + b2 * SLOT);
+#pragma unroll 2
+          for (int ks = 0; ks < CB * 4; ++ks) {
+            const uint64_t a = vd + (ks >> 2) * 2048 + (ks & 3) * 2, bb = g + (ks >> 2) * 1024 + (ks & 3) * 2;
+            umma_f16(el, d, a + 1024, bb, id, ks > 0);
+            umma_f16(el, d, a, bb + 512, id, 1);
+          }
+#pragma unroll 2
+          for (int ks = 0; ks < CB * 4; ++ks) umma_f16(el, d, vd + (ks >> 2) * 2048 + (ks & 3) * 2, g + (ks >> 2) * 1024 + (ks & 3) * 2, id, 1);
+          commit_by(el, dp_full);
+          commit_by(el, g_empty(b2));
+        }
+      }
+    }
+    if (warp == 18 && n > 0) {
+      // ----------------------------------------------------------- sums: dV(0), dK(0), dV(1), ...
+      const uint32_t el = elect_lane(), id = instr_desc_f16(128, DP, 1);
+      bool ok = true;
+      auto accumulate = [&](uint32_t d, uint32_t a, uint32_t slot, int slices, uint32_t fresh) {
+        const uint64_t b = smem_desc_mn(slot, 16384);
+#pragma unroll 1
+        for (int ks = 0; ks < slices; ++ks) {
+          umma_f16_ts(el, d, a + ks * 16 + 8, b + ks * 128, id, ks > 0 ? 1u : fresh);
+          umma_f16_ts(el, d, a + ks * 16, b + ks * 128 + 512, id, 1);
+        }
+#pragma unroll 1
+        for (int ks = 0; ks < slices; ++ks) umma_f16_ts(el, d, a + ks * 16, b + ks * 128, id, 1);
+      };
+      for (int i = 0; i < n && ok; ++i) {
+        const int b2 = i & 1, slices = rows16(i) >> 4;
+        const uint32_t fresh = i % kFlush == 0 ? 0u : 1u;
+        ok = mbar_wait(p_full(b2), (i >> 1) & 1) && mbar_wait(g_full(b2), (i >> 1) & 1) && (fresh || i == 0 || mbar_wait(acc_empty, (i / kFlush - 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        accumulate(tmem + COL_DV, tmem + COL_S + b2 * 64, base + OFF_G + b2 * SLOT, slices, fresh);
+        commit_by(el, g_empty(b2));
+        commit_by(el, s_free(b2));
+        ok = mbar_wait(ds_full, i & 1);
+        if (!ok) break;
+        tc_fence_after();
+        accumulate(tmem + COL_DK, tmem + COL_DP, base + OFF_Q + b2 * SLOT, slices, fresh);
+        commit_by(el, q_empty(b2));
+        commit_by(el, dp_free);
+        if ((i + 1) % kFlush == 0 || i + 1 == n) commit_by(el, acc_full);
       }
     }
   } else {
     regs_inc<kRegsSoftmax>();
-    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane, key = k0 + row;
+    const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane, key = k0 + row;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const PlaneFactors fc = plane_factors(p, plane);
     if (n > 0) {
-      if (half < CB) row_to_tmem(lane_addr + COL_KH + half * 32, p.pk.k.data + plane * p.pk.k.plane_bytes(CB) + (int64_t)half * 2 * p.pk.k.rows * 128, key, key < len);
+      if (part < 2 * CB)
+        row_to_tmem(lane_addr + COL_KH + part * 16, p.pk.k.data + plane * p.pk.k.plane_bytes(CB) + (int64_t)(part >> 1) * 2 * p.pk.k.rows * 128, key, part & 1, key < len);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(kh_ready);
@@ -398,121 +419,114 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     // the query rows that see the key
     const int f_lo = key < len ? key * s.G : 0;
     const int f_hi = key >= len ? 0 : (s.window < 0 || key < s.sinks) ? nf : (int)min((int64_t)nf, ((int64_t)key + s.window + 1) * s.G);
-    float dv[HC], dk[HC];
+    float dv[QC], dk[QC];
 #pragma unroll
-    for (int e = 0; e < HC; ++e) dv[e] = dk[e] = 0.0f;
+    for (int e = 0; e < QC; ++e) dv[e] = dk[e] = 0.0f;
     bool ok = true;
-    // a chunk's sums are fetched one step later, between that step's weights and its dS: the products that end the chunk run meanwhile
     auto flush = [&](int chunk) {
       ok = ok && mbar_wait(acc_full, chunk & 1);
       tc_fence_after();
-      add_columns<HC / 32>(lane_addr + COL_DV + half * HC, dv);
-      add_columns<HC / 32>(lane_addr + COL_DK + half * HC, dk);
+      add_columns<QC>(lane_addr + COL_DV + part * QC, dv);
+      add_columns<QC>(lane_addr + COL_DK + part * QC, dk);
       tc_fence_before();
       mbar_arrive(acc_empty);
     };
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      const int f0 = row0(i) + half * 32;
+      const int f0 = row0(i) + part * 16;
       const uint32_t see = (uint32_t)(bits_below(f_hi - f0) & ~bits_below(f_lo - f0));
-      const float* off = reinterpret_cast<const float*>(gen + STATS + (i & 1) * 512) + half * 32;
-      float w[32];
+      const float4* off = reinterpret_cast<const float4*>(gen + STATS + (i & 1) * 512 + part * 64);
+      float w[16];
       ok = ok && mbar_wait(q_full(i & 1), (i >> 1) & 1) && mbar_wait(s_full(i & 1), (i >> 1) & 1);
       tc_fence_after();
       {
-        uint32_t y[32];
-        tmem_ld32(lane_addr + COL_S + (i & 1) * 64 + half * 32, y);
+        uint32_t y[16];
+        tmem_ld16(lane_addr + COL_S + (i & 1) * 64 + part * 16, y);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) w[e] = ((see >> e) & 1u) ? exp2_fast(fmaf(__uint_as_float(y[e]), fc.score, off[e])) : 0.0f;
+        for (int e = 0; e < 16; e += 4) {
+          const float4 c = off[e >> 2];
+          w[e] = exp2_fast(fmaf(__uint_as_float(y[e]), fc.score, c.x)); w[e + 1] = exp2_fast(fmaf(__uint_as_float(y[e + 1]), fc.score, c.y));
+          w[e + 2] = exp2_fast(fmaf(__uint_as_float(y[e + 2]), fc.score, c.z)); w[e + 3] = exp2_fast(fmaf(__uint_as_float(y[e + 3]), fc.score, c.w));
+        }
       }
-      store_pairs(lane_addr + COL_S + (i & 1) * 64 + half * 32, w);
+      const bool whole = __all_sync(0xffffffffu, (see & 0xffffu) == 0xffffu);
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) if (!((see >> e) & 1u)) w[e] = 0.0f;
+      }
+      store_pairs(lane_addr + COL_S + (i & 1) * 64 + part * 16, w);
       tc_fence_before();
       mbar_arrive(p_full(i & 1));
       if (i > 0 && i % kFlush == 0) flush(i / kFlush - 1);
       ok = ok && mbar_wait(dp_full, i & 1);
       tc_fence_after();
       {
-        uint32_t y[32];
-        tmem_ld32(lane_addr + COL_DP + half * 32, y);
+        uint32_t y[16];
+        tmem_ld16(lane_addr + COL_DP + part * 16, y);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) w[e] = ((see >> e) & 1u) ? w[e] * ((__uint_as_float(y[e]) - off[64 + e]) * fc.grad) : 0.0f;
+        for (int e = 0; e < 16; e += 4) {
+          const float4 c = off[16 + (e >> 2)];
+          w[e] *= (__uint_as_float(y[e]) - c.x) * fc.grad; w[e + 1] *= (__uint_as_float(y[e + 1]) - c.y) * fc.grad;
+          w[e + 2] *= (__uint_as_float(y[e + 2]) - c.z) * fc.grad; w[e + 3] *= (__uint_as_float(y[e + 3]) - c.w) * fc.grad;
+        }
       }
-      store_pairs(lane_addr + COL_DP + half * 32, w);
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) if (!((see >> e) & 1u)) w[e] = 0.0f;   // what stands in a masked place may not be a number
+      }
+      store_pairs(lane_addr + COL_DP + part * 16, w);
       tc_fence_before();
       mbar_arrive(ds_full);
     }
     if (n > 0) flush((n - 1) / kFlush);
     const float zk = ok ? fc.dk : NAN, zv = ok ? fc.dv : NAN;
     if (parts > 1) {
-      float* at = p.part + (((plane * p.units + x0) * 2) * 128 + row) * DP + half * HC;
-#pragma unroll
-      for (int e = 0; e < HC; e += 4) {
-        *reinterpret_cast<float4*>(at + e) = make_float4(dv[e] * zv, dv[e + 1] * zv, dv[e + 2] * zv, dv[e + 3] * zv);
-        *reinterpret_cast<float4*>(at + 128 * DP + e) = make_float4(dk[e] * zk, dk[e + 1] * zk, dk[e + 2] * zk, dk[e + 3] * zk);
-      }
+      float* at = p.part + (((plane * p.units + x0) * 2) * 128 + row) * DP;
+      write_row<QC>(at, part * QC, DP, dv, zv, false, true);
+      write_row<QC>(at + 128 * DP, part * QC, DP, dk, zk, false, true);
     } else if (key < s.seq) {
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const gn_view& view = which ? p.dk : p.dv;
-        const float* acc = which ? dk : dv;
-        const float z = which ? zk : zv;
-        float* dst = view.data + token_offset<false>(view, r, hk, key);
-#pragma unroll
-        for (int e = 0; e < HC; e += 4) {
-          const int ch = half * HC + e;
-          if (p.vec_dkv) {
-            if (ch < s.D) {
-              float4 v = make_float4(acc[e] * z, acc[e + 1] * z, acc[e + 2] * z, acc[e + 3] * z);
-              if (p.accumulate) { const float4 o = *reinterpret_cast<const float4*>(dst + ch); v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; }
-              *reinterpret_cast<float4*>(dst + ch) = v;
-            }
-          } else {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) if (ch + u < s.D) dst[ch + u] = __fadd_rn(p.accumulate ? dst[ch + u] : 0.0f, acc[e + u] * z);
-          }
-        }
-      }
+      write_row<QC>(p.dv.data + token_offset<false>(p.dv, r, hk, key), part * QC, s.D, dv, zv, p.accumulate, p.vec_dkv);
+      write_row<QC>(p.dk.data + token_offset<false>(p.dk, r, hk, key), part * QC, s.D, dk, zk, p.accumulate, p.vec_dkv);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
-// Sums the parts of key tiles that were divided, in their order: a warp per key row and tensor.
+// Sums the parts of key tiles that were divided, in their order: DP / 4 threads per key row and tensor.
 template <int DP>
 __global__ void __launch_bounds__(256) stream_tc_dkv_sum_kernel(const __grid_constant__ BackwardTc p) {
+  constexpr int LANES = DP / 4;
   const StreamRows& s = p.s;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y, r = blockIdx.z >> 1, which = blockIdx.z & 1, key = blockIdx.x * 8 + warp;
+  const int hk = blockIdx.y, r = blockIdx.z >> 1, which = blockIdx.z & 1, key = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, ch = threadIdx.x % LANES * 4;
   if (key >= s.seq) return;
   const int kt = key / 128;
   const bool sink = kt < p.sink_tiles;
   const int parts = sink ? p.parts_sink : p.parts, unit = sink ? kt * parts : p.sink_tiles * p.parts_sink + (kt - p.sink_tiles) * parts;
   if (parts == 1) return;
   const int64_t plane = (int64_t)r * s.Hkv + hk;
-  float x[DP / 32];
-#pragma unroll
-  for (int e = 0; e < DP / 32; ++e) x[e] = 0.0f;
-  if (key < row_span<false>(s, r).ctx)
+  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (key < row_span<false>(s, r).ctx) {
+    const float* at = p.part + (((plane * p.units + unit) * 2 + which) * 128 + key % 128) * DP + ch;
+#pragma unroll 8
     for (int i = 0; i < parts; ++i) {
-      const float* at = p.part + (((plane * p.units + unit + i) * 2 + which) * 128 + key % 128) * DP;
-#pragma unroll
-      for (int e = 0; e < DP / 32; ++e) x[e] += at[lane + 32 * e];
+      const float4 v = *reinterpret_cast<const float4*>(at + (int64_t)i * 2 * 128 * DP);
+      x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
     }
+  }
   const gn_view& view = which ? p.dk : p.dv;
-  float* dst = view.data + token_offset<false>(view, r, hk, key);
-#pragma unroll
-  for (int e = 0; e < DP / 32; ++e)
-    if (lane + 32 * e < s.D) dst[lane + 32 * e] = p.accumulate ? dst[lane + 32 * e] + x[e] : x[e];
+  write_row<4>(view.data + token_offset<false>(view, r, hk, key), ch, s.D, x, 1.0f, p.accumulate, p.vec_dkv);
 }
 
 // dQ.  One CTA per (128 query rows, kv head, sequence): S = Q K^T and dP = dO V^T of 64 keys a step, dS in place of dP, dQ += dS K with
-// dS from tensor memory and the same K tile read the other way.
+// dS from tensor memory and the same K tile read the other way.  Threads, issuing warps and the rounding of sums as above.
 // Tensor memory: Q hi 64 columns, dO hi 64, S 2 x 64, dP 2 x 64, dQ 128.  Shared memory: Q lo, dO lo 32 KB each, 3 K and 2 V tiles of 32 KB.
 template <int DP>
 __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid_constant__ BackwardTc p) {
-  constexpr int CB = DP / 64, HC = DP / 2;
+  constexpr int CB = DP / 64, QC = DP / 4;
   constexpr uint32_t SLOT = CB * 16384u, OFF_GL = CB * 16384u, OFF_K = 2 * CB * 16384u, OFF_V = OFF_K + 3 * SLOT, BARS = OFF_V + 2 * SLOT;
   constexpr uint32_t COL_Q = 0, COL_G = 64, COL_S = 128, COL_DP = 256, COL_DQ = 384;
   extern __shared__ uint8_t smem_raw[];
@@ -527,30 +541,31 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bars = base + BARS;
-  const uint32_t lo_full = bars, hi_ready = bars + 8, acc_full = bars + 16, acc_empty = bars + 24, tmem_slot = bars + 136;
+  const uint32_t lo_full = bars, hi_ready = bars + 8, acc_full = bars + 16, acc_empty = bars + 24, tmem_slot = bars + 176;
   auto k_full = [&](int i) { return bars + 32u + 8u * i; };
   auto k_empty = [&](int i) { return bars + 56u + 8u * i; };
   auto v_full = [&](int i) { return bars + 80u + 8u * i; };
   auto v_empty = [&](int i) { return bars + 96u + 8u * i; };
   auto sp_full = [&](int i) { return bars + 112u + 8u * i; };
-  auto ds_full = [&](int i) { return bars + 144u + 8u * i; };
+  auto ds_full = [&](int i) { return bars + 128u + 8u * i; };
+  auto ds_free = [&](int i) { return bars + 144u + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(lo_full, 1); mbar_init(hi_ready, 256); mbar_init(acc_full, 1); mbar_init(acc_empty, 256);
+    mbar_init(lo_full, 1); mbar_init(hi_ready, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512);
     for (int i = 0; i < 3; ++i) { mbar_init(k_full(i), 1); mbar_init(k_empty(i), 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(v_full(i), 1); mbar_init(v_empty(i), 1); mbar_init(sp_full(i), 1); mbar_init(ds_full(i), 256); }
+    for (int i = 0; i < 2; ++i) { mbar_init(v_full(i), 1); mbar_init(v_empty(i), 1); mbar_init(sp_full(i), 1); mbar_init(ds_full(i), 512); mbar_init(ds_free(i), 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 16) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 136);
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 176);
   auto rows16 = [&](int j) { return min(64, (runs.total - j * 64 + 15) & ~15); };
 
-  if (warp >= 8) {
+  if (warp >= 16) {
     regs_dec<kRegsOther>();
-    if (warp == 9 && lane == 0 && n > 0) {
+    if (warp == 17 && lane == 0 && n > 0) {
       const int rows = min(128, (nf - f0 + 15) & ~15);
       mbar_expect_tx(lo_full, (uint32_t)CB * 2u * rows * 128u);
       for (int w = 0; w < 2; ++w) {
@@ -560,22 +575,23 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       }
       auto copy_tile = [&](const Packed& src, uint32_t dst, uint32_t bar, int j) {
         const int c0 = j * 64, m = rows16(j), na = min(max(runs.a_len - c0, 0), m), nb = m - na;
-        const uint8_t* from = src.data + plane * src.plane_bytes(CB);
+        const uint8_t* from = src.data + plane * src.plane_bytes(CB) + (int64_t)c0 * 128;
         mbar_expect_tx(bar, (uint32_t)CB * 2u * m * 128u);
+#pragma unroll 1
         for (int b = 0; b < CB * 2; ++b) {
-          if (na) bulk_load(dst + b * 8192, from + ((int64_t)b * src.rows + c0) * 128, na * 128, bar);
-          if (nb) bulk_load(dst + b * 8192 + na * 128, from + ((int64_t)b * src.rows + c0 + na + runs.shift) * 128, nb * 128, bar);
+          if (na) bulk_load(dst, from, na * 128, bar);
+          if (nb) bulk_load(dst + na * 128, from + (int64_t)(na + runs.shift) * 128, nb * 128, bar);
+          dst += 8192; from += (int64_t)src.rows * 128;
         }
       };
       bool ok = true;
-      int jk = 0, jv = 0;
-      for (uint32_t idle = 0; (jv < n || jk < n) && ok;) {
-        bool did = false;
-        if (jk < n && (jk < 3 || mbar_test(k_empty(jk % 3), (jk / 3 - 1) & 1))) { copy_tile(p.pk.k, base + OFF_K + (jk % 3) * SLOT, k_full(jk % 3), jk); ++jk; did = true; }
-        if (jv < jk && (jv < 2 || mbar_test(v_empty(jv & 1), ((jv >> 1) - 1) & 1))) { copy_tile(p.pk.v, base + OFF_V + (jv & 1) * SLOT, v_full(jv & 1), jv); ++jv; did = true; }
-        if (did) idle = 0;
-        else if (++idle > kSpinLimit) ok = false;
-        else if (idle > 4096) __nanosleep(64);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j >= 3) ok = mbar_wait(k_empty(j % 3), (j / 3 - 1) & 1);
+        if (!ok) break;
+        copy_tile(p.pk.k, base + OFF_K + (j % 3) * SLOT, k_full(j % 3), j);
+        if (j >= 2) ok = mbar_wait(v_empty(j & 1), ((j >> 1) - 1) & 1);
+        if (!ok) break;
+        copy_tile(p.pk.v, base + OFF_V + (j & 1) * SLOT, v_full(j & 1), j);
       }
       if (!ok)
         for (int ph = 0; ph < 2; ++ph) {
@@ -584,52 +600,60 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
         }
       mbar_wait(lo_full, 0);
     }
-    if (warp == 8 && n > 0) {
+    if (warp == 16 && n > 0) {
+      // ----------------------------------------------------------- scores
       const uint32_t el = elect_lane();
       bool ok = mbar_wait(lo_full, 0) && mbar_wait(hi_ready, 0);
       tc_fence_after();
-      auto scores = [&](int j) {
+      for (int j = 0; j < n && ok; ++j) {
         const uint32_t id = instr_desc_f16(128, rows16(j), 0);
         for (int w = 0; w < 2 && ok; ++w) {
-          ok = ok && (w ? mbar_wait(v_full(j & 1), (j >> 1) & 1) : mbar_wait(k_full(j % 3), (j / 3) & 1));
+          ok = w ? mbar_wait(v_full(j & 1), (j >> 1) & 1) : mbar_wait(k_full(j % 3), (j / 3) & 1) && (j < 2 || mbar_wait(ds_free(j & 1), ((j >> 1) - 1) & 1));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t d = tmem + (w ? COL_DP : COL_S) + (j & 1) * 64, hi = tmem + (w ? COL_G : COL_Q), lo = base + w * OFF_GL;
-          const uint32_t slot = w ? base + OFF_V + (j & 1) * SLOT : base + OFF_K + (j % 3) * SLOT;
-          auto b_of = [&](int ks, int l) { return smem_desc_sw128(slot + (ks >> 2) * 16384 + l * 8192) + 2u * (ks & 3); };
-#pragma unroll
+          const uint32_t d = tmem + (w ? COL_DP : COL_S) + (j & 1) * 64, hi = tmem + (w ? COL_G : COL_Q);
+          const uint64_t lo = smem_desc_sw128(base + w * OFF_GL), slot = smem_desc_sw128(w ? base + OFF_V + (j & 1) * SLOT : base + OFF_K + (j % 3) * SLOT);
+#pragma unroll 2
           for (int ks = 0; ks < CB * 4; ++ks) {
-            umma_f16(el, d, smem_desc_sw128(lo + (ks >> 2) * 16384) + 2u * (ks & 3), b_of(ks, 0), id, ks > 0);
-            umma_f16_ts(el, d, hi + ks * 8, b_of(ks, 1), id, 1);
+            const uint32_t in = (ks >> 2) * 1024 + (ks & 3) * 2;
+            umma_f16(el, d, lo + in, slot + in, id, ks > 0);
+            umma_f16_ts(el, d, hi + ks * 8, slot + in + 512, id, 1);
           }
-#pragma unroll
-          for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, hi + ks * 8, b_of(ks, 0), id, 1);
+#pragma unroll 2
+          for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, hi + ks * 8, slot + (ks >> 2) * 1024 + (ks & 3) * 2, id, 1);
         }
-        if (!ok) return;
+        if (!ok) break;
         commit_by(el, v_empty(j & 1));
         commit_by(el, sp_full(j & 1));
-      };
-      if (ok) scores(0);
+      }
+    }
+    if (warp == 18 && n > 0) {
+      // ----------------------------------------------------------- sums
+      const uint32_t el = elect_lane(), id = instr_desc_f16(128, DP, 1);
+      bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) scores(j + 1);
-        ok = ok && mbar_wait(ds_full(j & 1), (j >> 1) & 1) && (j < kFlush || j % kFlush || mbar_wait(acc_empty, (j / kFlush - 1) & 1));
+        const uint32_t fresh = j % kFlush == 0 ? 0u : 1u;
+        ok = mbar_wait(ds_full(j & 1), (j >> 1) & 1) && mbar_wait(k_full(j % 3), (j / 3) & 1) && (fresh || j == 0 || mbar_wait(acc_empty, (j / kFlush - 1) & 1));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t id = instr_desc_f16(128, DP, 1), a = tmem + COL_DP + (j & 1) * 64, slot = base + OFF_K + (j % 3) * SLOT;
+        const uint32_t a = tmem + COL_DP + (j & 1) * 64;
+        const uint64_t b = smem_desc_mn(base + OFF_K + (j % 3) * SLOT, 16384);
         const int slices = rows16(j) >> 4;
-        const uint32_t fresh = j % kFlush == 0 ? 0u : 1u;
-        auto one = [&](int ks, int al, int bl, uint32_t acc) {
-          umma_f16_ts(el, tmem + COL_DQ, a + (ks >> 1) * 32 + al * 16 + (ks & 1) * 8, smem_desc_mn(slot + bl * 8192 + ks * 2048, 16384), id, acc);
-        };
-        for (int ks = 0; ks < slices; ++ks) { one(ks, 1, 0, ks > 0 ? 1u : fresh); one(ks, 0, 1, 1); }
-        for (int ks = 0; ks < slices; ++ks) one(ks, 0, 0, 1);
+#pragma unroll 1
+        for (int ks = 0; ks < slices; ++ks) {
+          umma_f16_ts(el, tmem + COL_DQ, a + ks * 16 + 8, b + ks * 128, id, ks > 0 ? 1u : fresh);
+          umma_f16_ts(el, tmem + COL_DQ, a + ks * 16, b + ks * 128 + 512, id, 1);
+        }
+#pragma unroll 1
+        for (int ks = 0; ks < slices; ++ks) umma_f16_ts(el, tmem + COL_DQ, a + ks * 16, b + ks * 128, id, 1);
         commit_by(el, k_empty(j % 3));
+        commit_by(el, ds_free(j & 1));
         if ((j + 1) % kFlush == 0 || j + 1 == n) commit_by(el, acc_full);
       }
     }
   } else {
     regs_inc<kRegsSoftmax>();
-    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane, f = f0 + row;
+    const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane, f = f0 + row;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const bool live = f < nf;
     const int t = f / s.G, h = hk * s.G + f - t * s.G;
@@ -639,7 +663,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const Packed& src = w ? p.g : p.q;
-        if (half < CB) row_to_tmem(lane_addr + (w ? COL_G : COL_Q) + half * 32, src.data + plane * src.plane_bytes(CB) + (int64_t)half * 2 * src.rows * 128, f, live);
+        if (part < 2 * CB)
+          row_to_tmem(lane_addr + (w ? COL_G : COL_Q) + part * 16, src.data + plane * src.plane_bytes(CB) + (int64_t)(part >> 1) * 2 * src.rows * 128, f, part & 1, live);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -648,62 +673,47 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     }
     const int s_end = live ? min(s.sinks, t + 1) : 0;
     const int lo_key = live ? (s.window < 0 ? 0 : max(0, t - s.window)) - runs.shift : 0, hi_key = live ? t - runs.shift : -1;
-    float acc[HC];
+    float acc[QC];
 #pragma unroll
-    for (int e = 0; e < HC; ++e) acc[e] = 0.0f;
+    for (int e = 0; e < QC; ++e) acc[e] = 0.0f;
     bool ok = true;
     auto flush = [&](int chunk) {   // one step later, as above
       ok = ok && mbar_wait(acc_full, chunk & 1);
       tc_fence_after();
-      add_columns<HC / 32>(lane_addr + COL_DQ + half * HC, acc);
+      add_columns<QC>(lane_addr + COL_DQ + part * QC, acc);
       tc_fence_before();
       mbar_arrive(acc_empty);
     };
+#pragma unroll 1
     for (int j = 0; j < n; ++j) {
-      const int c0 = j * 64 + half * 32;
+      const int c0 = j * 64 + part * 16;
       const uint32_t see = (uint32_t)(bits_below(s_end - c0) | (bits_below(hi_key + 1 - c0) & ~bits_below(lo_key - c0)));
       ok = ok && mbar_wait(sp_full(j & 1), (j >> 1) & 1);
       tc_fence_after();
-      float w[32];
+      float w[16];
       {
-        uint32_t y[32];
-        tmem_ld32(lane_addr + COL_S + (j & 1) * 64 + half * 32, y);
+        uint32_t y[16], z[16];
+        tmem_ld16(lane_addr + COL_S + (j & 1) * 64 + part * 16, y);
+        tmem_ld16(lane_addr + COL_DP + (j & 1) * 64 + part * 16, z);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) w[e] = exp2_fast(fmaf(__uint_as_float(y[e]), fc.score, off));
-        tmem_ld32(lane_addr + COL_DP + (j & 1) * 64 + half * 32, y);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) w[e] = ((see >> e) & 1u) ? w[e] * ((__uint_as_float(y[e]) - delta) * fc.grad) : 0.0f;
+        for (int e = 0; e < 16; ++e) w[e] = exp2_fast(fmaf(__uint_as_float(y[e]), fc.score, off)) * ((__uint_as_float(z[e]) - delta) * fc.grad);
       }
-      store_pairs(lane_addr + COL_DP + (j & 1) * 64 + half * 32, w);
+      if (!__all_sync(0xffffffffu, (see & 0xffffu) == 0xffffu)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) if (!((see >> e) & 1u)) w[e] = 0.0f;
+      }
+      store_pairs(lane_addr + COL_DP + (j & 1) * 64 + part * 16, w);
       tc_fence_before();
       mbar_arrive(ds_full(j & 1));
       if (j > 0 && j % kFlush == 0) flush(j / kFlush - 1);
     }
     if (n > 0) flush((n - 1) / kFlush);
-    if (f < s.seq * s.G) {
-      const float z = ok ? fc.dq : NAN;
-      float* dst = p.dq.data + token_offset<false>(p.dq, r, h, t);
-#pragma unroll
-      for (int e = 0; e < HC; e += 4) {
-        const int ch = half * HC + e;
-        if (p.vec_dq) {
-          if (ch < s.D) {
-            float4 v = make_float4(acc[e] * z, acc[e + 1] * z, acc[e + 2] * z, acc[e + 3] * z);
-            if (p.accumulate) { const float4 o = *reinterpret_cast<const float4*>(dst + ch); v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; }
-            *reinterpret_cast<float4*>(dst + ch) = v;
-          }
-        } else {
-#pragma unroll
-          for (int u = 0; u < 4; ++u) if (ch + u < s.D) dst[ch + u] = __fadd_rn(p.accumulate ? dst[ch + u] : 0.0f, acc[e + u] * z);
-        }
-      }
-    }
+    if (f < s.seq * s.G) write_row<QC>(p.dq.data + token_offset<false>(p.dq, r, h, t), part * QC, s.D, acc, ok ? fc.dq : NAN, p.accumulate, p.vec_dq);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 // ------------------------------------------------------------------ host
@@ -713,15 +723,20 @@ int64_t carve_backward(const StreamRows& s, void* workspace, BackwardTc* b) {
   b->q_tiles = ceil_div((int64_t)s.seq * s.G, 128);
   b->key_tiles = ceil_div(s.seq, 128);
   // Key tiles whose steps (64 query rows each) would make a long tail are divided.  A tile of sinks is seen by every later
-  // query and gets as many parts as make them about as long as the others'; and when there are fewer than four waves
-  // of CTAs all tiles are divided, while a part keeps 16 steps (writing and summing a part costs about one step).
+  // query and gets as many parts as make them about as long as the others'.
   const bool windowed = s.window >= 0 && s.sinks > 0 && (int64_t)s.window + 128 < s.seq;
   b->sink_tiles = windowed ? std::min(b->key_tiles, ceil_div(s.sinks, 128)) : 0;
   const int64_t reach = s.window >= 0 ? std::min<int64_t>(s.seq, (int64_t)s.window + 128) : s.seq;
   const int64_t steps = ceil_div(reach * s.G, 64), steps_sink = ceil_div((int64_t)s.seq * s.G, 64);
-  const int64_t ctas = planes * b->key_tiles;
-  b->parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(4 * 148, ctas), steps / 16));
-  b->parts_sink = b->sink_tiles ? (int)std::max<int64_t>(1, ceil_div(steps_sink * b->parts, steps)) : 1;
+  // Parts: the fewest rounds of 148 CTAs, counted in steps with 5 for a CTA's start and end, and the partial results' way to memory
+  // and back (0.02 of a step a CTA).
+  double best = 0.0;
+  for (int parts = 1; parts <= 16 && (parts == 1 || steps / parts >= 8); ++parts) {
+    const int64_t sink_parts = b->sink_tiles ? std::max<int64_t>(1, ceil_div(steps_sink * parts, steps)) : 1;
+    const int64_t units = planes * (b->sink_tiles * sink_parts + (int64_t)(b->key_tiles - b->sink_tiles) * parts);
+    const double cost = (double)ceil_div(units, 148) * (ceil_div(steps, parts) + 5) + (parts > 1 ? 0.02 * (double)units : 0.0);
+    if (parts == 1 || cost < best) { best = cost; b->parts = parts; b->parts_sink = (int)sink_parts; }
+  }
   b->units = b->sink_tiles * b->parts_sink + (b->key_tiles - b->sink_tiles) * b->parts;
   Carve c{static_cast<uint8_t*>(workspace)};
   PackedKeys& pk = b->pk;
@@ -749,8 +764,8 @@ int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
   constexpr int kSmemKv = CB * (32768 + 16384 + 4 * 16384) + 1024 + 256 + 1024, kSmemQ = CB * (2 * 16384 + 5 * 16384) + 256 + 1024;
   static PerDeviceOnce once;
   if (once.first()) {
-    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_dkv_kernel<DP>), kThreadsB, 256 * kRegsSoftmax + 128 * kRegsOther));
-    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_dq_kernel<DP>), kThreadsB, 256 * kRegsSoftmax + 128 * kRegsOther));
+    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_dkv_kernel<DP>), kThreadsB, 512 * kRegsSoftmax + 128 * kRegsOther));
+    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_dq_kernel<DP>), kThreadsB, 512 * kRegsSoftmax + 128 * kRegsOther));
     GN_CUDA(cudaFuncSetAttribute(stream_tc_dkv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemKv));
     GN_CUDA(cudaFuncSetAttribute(stream_tc_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemQ));
   }
@@ -769,7 +784,7 @@ int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
   stream_tc_dkv_kernel<DP><<<dim3(b.units, s.Hkv, s.rows), kThreadsB, kSmemKv, st>>>(b);
   GN_LAUNCH_CHECK();
   if (b.parts > 1 || b.parts_sink > 1) {
-    stream_tc_dkv_sum_kernel<DP><<<dim3(ceil_div(s.seq, 8), s.Hkv, 2 * s.rows), 256, 0, st>>>(b);
+    stream_tc_dkv_sum_kernel<DP><<<dim3(ceil_div(s.seq, 1024 / DP), s.Hkv, 2 * s.rows), 256, 0, st>>>(b);
     GN_LAUNCH_CHECK();
   }
   stream_tc_dq_kernel<DP><<<dim3(b.q_tiles, s.Hkv, s.rows), kThreadsB, kSmemQ, st>>>(b);
