@@ -210,33 +210,36 @@ __device__ __forceinline__ void store_pairs(uint32_t taddr, const float (&x)[16]
   tmem_st16(taddr, y);
   tmem_st_wait();
 }
-// A quarter of a packed plane's hi row (half a 64-channel block, unswizzled) to 16 columns of tensor memory.
-__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint8_t* block, int row, int half, bool live) {
+// A quarter of a packed hi row that a bulk copy left in shared memory (half a 64-channel block, unswizzled) to 16 columns of tensor memory.
+__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint8_t* block, int row, int half) {
   uint32_t y[16];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (live) v = *reinterpret_cast<const uint4*>(block + (int64_t)row * 128 + (((half * 4 + c) ^ (row & 7)) << 4));
+    const uint4 v = *reinterpret_cast<const uint4*>(block + row * 128 + (((half * 4 + c) ^ (row & 7)) << 4));
     y[4 * c] = v.x; y[4 * c + 1] = v.y; y[4 * c + 2] = v.z; y[4 * c + 3] = v.w;
   }
   tmem_st16(taddr, y);
 }
-// A thread's QC channels of a gradient row.
+// A thread's QC channels, from ch on, of a gradient row (dst null: no row); a warp's 32 threads hold as many rows.
 template <int QC>
-__device__ __forceinline__ void write_row(float* dst, int ch, int D, const float (&acc)[QC], float z, bool accumulate, bool vec) {
+__device__ __forceinline__ void write_row(float* dst, int ch, int D, float (&acc)[QC], float z, bool accumulate, bool vec) {
 #pragma unroll
-  for (int e = 0; e < QC; e += 4) {
-    if (vec) {
-      if (ch + e < D) {
-        float4 v = make_float4(acc[e] * z, acc[e + 1] * z, acc[e + 2] * z, acc[e + 3] * z);
-        if (accumulate) { const float4 o = *reinterpret_cast<const float4*>(dst + ch + e); v.x = __fadd_rn(o.x, v.x); v.y = __fadd_rn(o.y, v.y); v.z = __fadd_rn(o.z, v.z); v.w = __fadd_rn(o.w, v.w); }
-        *reinterpret_cast<float4*>(dst + ch + e) = v;
-      }
-    } else {
+  for (int e = 0; e < QC; ++e) acc[e] *= z;
+  if (vec) {
+    constexpr int N = QC / 4;
+    const int lane = threadIdx.x & 31, c = ch + (lane & (N - 1)) * 4;
+    transpose_blocks<N>(acc);
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (ch + e + u < D) dst[ch + e + u] = accumulate ? __fadd_rn(dst[ch + e + u], __fmul_rn(acc[e + u], z)) : acc[e + u] * z;
+    for (int k = 0; k < N; ++k) {
+      float* at = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & ~(N - 1)) + k));
+      if (!at || c >= D) continue;
+      float4 v = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
+      if (accumulate) { const float4 o = *reinterpret_cast<const float4*>(at + c); v.x = __fadd_rn(o.x, v.x); v.y = __fadd_rn(o.y, v.y); v.z = __fadd_rn(o.z, v.z); v.w = __fadd_rn(o.w, v.w); }
+      *reinterpret_cast<float4*>(at + c) = v;
     }
+  } else if (dst) {
+#pragma unroll
+    for (int e = 0; e < QC; ++e) if (ch + e < D) dst[ch + e] = accumulate ? __fadd_rn(dst[ch + e], acc[e]) : acc[e];
   }
 }
 
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bars = base + BARS;
-  const uint32_t v_full = bars, kh_ready = bars + 8, dp_full = bars + 16, ds_full = bars + 24, acc_full = bars + 32, acc_empty = bars + 40, dp_free = bars + 152, tmem_slot = bars + 176;
+  const uint32_t v_full = bars, kh_ready = bars + 8, dp_full = bars + 16, ds_full = bars + 24, acc_full = bars + 32, acc_empty = bars + 40, dp_free = bars + 152, kh_full = bars + 144, tmem_slot = bars + 176;
   auto q_full = [&](int i) { return bars + 48u + 8u * i; };
   auto g_full = [&](int i) { return bars + 64u + 8u * i; };
   auto q_empty = [&](int i) { return bars + 80u + 8u * i; };
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   auto s_free = [&](int i) { return bars + 160u + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(v_full, 1); mbar_init(kh_ready, 512); mbar_init(dp_full, 1); mbar_init(ds_full, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512); mbar_init(dp_free, 1);
+    mbar_init(v_full, 1); mbar_init(kh_full, 1); mbar_init(kh_ready, 512); mbar_init(dp_full, 1); mbar_init(ds_full, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512); mbar_init(dp_free, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full(i), 1); mbar_init(g_full(i), 1); mbar_init(q_empty(i), 1); mbar_init(g_empty(i), 2); mbar_init(s_full(i), 1); mbar_init(p_full(i), 512);
       mbar_init(s_free(i), 1);
@@ -306,6 +309,10 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       for (int b = 0; b < CB * 2; ++b) bulk_load(base + b * 16384, vp + ((int64_t)b * p.pk.v.rows + k0) * 128, keys * 128, v_full);
 #pragma unroll 1
       for (int b = 0; b < CB; ++b) bulk_load(base + OFF_KL + b * 16384, kp + ((int64_t)(2 * b + 1) * p.pk.k.rows + k0) * 128, keys * 128, v_full);
+      // K hi passes through the second dO stage on its way to tensor memory
+      mbar_expect_tx(kh_full, (uint32_t)CB * keys * 128u);
+#pragma unroll 1
+      for (int b = 0; b < CB; ++b) bulk_load(base + OFF_G + SLOT + b * 16384, kp + ((int64_t)(2 * b) * p.pk.k.rows + k0) * 128, keys * 128, kh_full);
       const uint8_t* qp = p.q.data + plane * p.q.plane_bytes(CB); const uint8_t* gp = p.g.data + plane * p.g.plane_bytes(CB);
       bool ok = true;
       for (int i = 0; i < n && ok; ++i) {
@@ -317,6 +324,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         for (int b = 0; b < CB * 2; ++b) bulk_load(base + OFF_Q + b2 * SLOT + b * 8192, qp + ((int64_t)b * p.q.rows + f) * 128, rows * 128, q_full(b2));
         bulk_load(base + STATS + b2 * 512, p.off + plane * p.q.rows + f, rows * 4, q_full(b2));
         bulk_load(base + STATS + b2 * 512 + 256, p.delta + plane * p.q.rows + f, rows * 4, q_full(b2));
+        if (i == 1) ok = mbar_wait(kh_ready, 0);
         if (i >= 2) ok = mbar_wait(g_empty(b2), ((i >> 1) - 1) & 1);
         if (!ok) break;
         mbar_expect_tx(g_full(b2), (uint32_t)CB * 2u * rows * 128u);
@@ -327,6 +335,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         for (int i = 0; i < 2; ++i)
           for (int ph = 0; ph < 2; ++ph) { mbar_wait(q_full(i), ph); mbar_wait(g_full(i), ph); }
       mbar_wait(v_full, 0);
+      mbar_wait(kh_full, 0);
     }
     if (warp == 16 && n > 0) {
       // ----------------------------------------------------------- scores: S^T(0), dP^T(0), S^T(1), dP^T(1), ...
@@ -409,9 +418,10 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane, key = k0 + row;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const PlaneFactors fc = plane_factors(p, plane);
+    bool ok = true;
     if (n > 0) {
-      if (part < 2 * CB)
-        row_to_tmem(lane_addr + COL_KH + part * 16, p.pk.k.data + plane * p.pk.k.plane_bytes(CB) + (int64_t)(part >> 1) * 2 * p.pk.k.rows * 128, key, part & 1, key < len);
+      ok = mbar_wait(kh_full, 0);
+      if (part < 2 * CB) row_to_tmem(lane_addr + COL_KH + part * 16, gen + OFF_G + SLOT + (part >> 1) * 16384, row, part & 1);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(kh_ready);
@@ -422,7 +432,6 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     float dv[QC], dk[QC];
 #pragma unroll
     for (int e = 0; e < QC; ++e) dv[e] = dk[e] = 0.0f;
-    bool ok = true;
     auto flush = [&](int chunk) {
       ok = ok && mbar_wait(acc_full, chunk & 1);
       tc_fence_after();
@@ -486,9 +495,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       float* at = p.part + (((plane * p.units + x0) * 2) * 128 + row) * DP;
       write_row<QC>(at, part * QC, DP, dv, zv, false, true);
       write_row<QC>(at + 128 * DP, part * QC, DP, dk, zk, false, true);
-    } else if (key < s.seq) {
-      write_row<QC>(p.dv.data + token_offset<false>(p.dv, r, hk, key), part * QC, s.D, dv, zv, p.accumulate, p.vec_dkv);
-      write_row<QC>(p.dk.data + token_offset<false>(p.dk, r, hk, key), part * QC, s.D, dk, zk, p.accumulate, p.vec_dkv);
+    } else {
+      write_row<QC>(key < s.seq ? p.dv.data + token_offset<false>(p.dv, r, hk, key) : nullptr, part * QC, s.D, dv, zv, p.accumulate, p.vec_dkv);
+      write_row<QC>(key < s.seq ? p.dk.data + token_offset<false>(p.dk, r, hk, key) : nullptr, part * QC, s.D, dk, zk, p.accumulate, p.vec_dkv);
     }
   }
   tc_fence_before();
@@ -518,7 +527,16 @@ __global__ void __launch_bounds__(256) stream_tc_dkv_sum_kernel(const __grid_con
     }
   }
   const gn_view& view = which ? p.dk : p.dv;
-  write_row<4>(view.data + token_offset<false>(view, r, hk, key), ch, s.D, x, 1.0f, p.accumulate, p.vec_dkv);
+  float* dst = view.data + token_offset<false>(view, r, hk, key) + ch;
+  if (p.vec_dkv) {
+    if (ch >= s.D) return;
+    float4 v = make_float4(x[0], x[1], x[2], x[3]);
+    if (p.accumulate) { const float4 o = *reinterpret_cast<const float4*>(dst); v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; }
+    *reinterpret_cast<float4*>(dst) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (ch + e < s.D) dst[e] = p.accumulate ? dst[e] + x[e] : x[e];
+  }
 }
 
 // dQ.  One CTA per (128 query rows, kv head, sequence): S = Q K^T and dP = dO V^T of 64 keys a step, dS in place of dP, dQ += dS K with
@@ -541,7 +559,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bars = base + BARS;
-  const uint32_t lo_full = bars, hi_ready = bars + 8, acc_full = bars + 16, acc_empty = bars + 24, tmem_slot = bars + 176;
+  const uint32_t lo_full = bars, hi_ready = bars + 8, acc_full = bars + 16, acc_empty = bars + 24, hi_full = bars + 160, tmem_slot = bars + 176;
   auto k_full = [&](int i) { return bars + 32u + 8u * i; };
   auto k_empty = [&](int i) { return bars + 56u + 8u * i; };
   auto v_full = [&](int i) { return bars + 80u + 8u * i; };
@@ -551,7 +569,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
   auto ds_free = [&](int i) { return bars + 144u + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(lo_full, 1); mbar_init(hi_ready, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512);
+    mbar_init(lo_full, 1); mbar_init(hi_full, 1); mbar_init(hi_ready, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512);
     for (int i = 0; i < 3; ++i) { mbar_init(k_full(i), 1); mbar_init(k_empty(i), 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(v_full(i), 1); mbar_init(v_empty(i), 1); mbar_init(sp_full(i), 1); mbar_init(ds_full(i), 512); mbar_init(ds_free(i), 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -573,6 +591,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
         for (int b = 0; b < CB; ++b)
           bulk_load(base + w * OFF_GL + b * 16384, src.data + plane * src.plane_bytes(CB) + ((int64_t)(2 * b + 1) * src.rows + f0) * 128, rows * 128, lo_full);
       }
+      // the hi halves pass through the last K and V tiles' places on their way to tensor memory
+      mbar_expect_tx(hi_full, (uint32_t)CB * 2u * rows * 128u);
+      for (int w = 0; w < 2; ++w) {
+        const Packed& src = w ? p.g : p.q;
+        for (int b = 0; b < CB; ++b)
+          bulk_load(base + (w ? OFF_V + SLOT : OFF_K + 2 * SLOT) + b * 16384, src.data + plane * src.plane_bytes(CB) + ((int64_t)(2 * b) * src.rows + f0) * 128, rows * 128, hi_full);
+      }
       auto copy_tile = [&](const Packed& src, uint32_t dst, uint32_t bar, int j) {
         const int c0 = j * 64, m = rows16(j), na = min(max(runs.a_len - c0, 0), m), nb = m - na;
         const uint8_t* from = src.data + plane * src.plane_bytes(CB) + (int64_t)c0 * 128;
@@ -586,9 +611,11 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       };
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
+        if (j == 2) ok = mbar_wait(hi_ready, 0);
         if (j >= 3) ok = mbar_wait(k_empty(j % 3), (j / 3 - 1) & 1);
         if (!ok) break;
         copy_tile(p.pk.k, base + OFF_K + (j % 3) * SLOT, k_full(j % 3), j);
+        if (j == 1) ok = mbar_wait(hi_ready, 0);
         if (j >= 2) ok = mbar_wait(v_empty(j & 1), ((j >> 1) - 1) & 1);
         if (!ok) break;
         copy_tile(p.pk.v, base + OFF_V + (j & 1) * SLOT, v_full(j & 1), j);
@@ -599,6 +626,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
           for (int i = 0; i < 2; ++i) mbar_wait(v_full(i), ph);
         }
       mbar_wait(lo_full, 0);
+      mbar_wait(hi_full, 0);
     }
     if (warp == 16 && n > 0) {
       // ----------------------------------------------------------- scores
@@ -659,13 +687,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     const int t = f / s.G, h = hk * s.G + f - t * s.G;
     const PlaneFactors fc = plane_factors(p, plane);
     float off = 0.0f, delta = 0.0f;
+    bool ok = true;
     if (n > 0) {
+      ok = mbar_wait(hi_full, 0);
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const Packed& src = w ? p.g : p.q;
+      for (int w = 0; w < 2; ++w)
         if (part < 2 * CB)
-          row_to_tmem(lane_addr + (w ? COL_G : COL_Q) + part * 16, src.data + plane * src.plane_bytes(CB) + (int64_t)(part >> 1) * 2 * src.rows * 128, f, part & 1, live);
-      }
+          row_to_tmem(lane_addr + (w ? COL_G : COL_Q) + part * 16, gen + (w ? OFF_V + SLOT : OFF_K + 2 * SLOT) + (part >> 1) * 16384, row, part & 1);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(hi_ready);
@@ -676,7 +704,6 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     float acc[QC];
 #pragma unroll
     for (int e = 0; e < QC; ++e) acc[e] = 0.0f;
-    bool ok = true;
     auto flush = [&](int chunk) {   // one step later, as above
       ok = ok && mbar_wait(acc_full, chunk & 1);
       tc_fence_after();
@@ -709,7 +736,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       if (j > 0 && j % kFlush == 0) flush(j / kFlush - 1);
     }
     if (n > 0) flush((n - 1) / kFlush);
-    if (f < s.seq * s.G) write_row<QC>(p.dq.data + token_offset<false>(p.dq, r, h, t), part * QC, s.D, acc, ok ? fc.dq : NAN, p.accumulate, p.vec_dq);
+    write_row<QC>(f < s.seq * s.G ? p.dq.data + token_offset<false>(p.dq, r, h, t) : nullptr, part * QC, s.D, acc, ok ? fc.dq : NAN, p.accumulate, p.vec_dq);
   }
   tc_fence_before();
   __syncthreads();
