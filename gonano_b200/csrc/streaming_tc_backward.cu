@@ -244,10 +244,11 @@ __device__ __forceinline__ void write_row(float* dst, int ch, int D, float (&acc
 }
 
 // dK and dV.  One CTA per (128 keys or a part of their query rows, kv head, sequence): S^T = K Q^T and dP^T = V dO^T of 64 query rows a
-// step, a softmax thread per (key, 16 query rows) turns them into P^T and dS^T in place, and dV += P^T dO, dK += dS^T Q take them
-// from tensor memory.  The hi half of K lives in tensor memory too, which leaves room for two stages of Q and dO.  Two warps issue,
+// step, a softmax thread per (key, 16 query rows) writes P^T over the scores and, once dV += P^T dO has read it, dS^T over P^T, from where
+// dK += dS^T Q takes it: dP^T is free for the next step as soon as it is read (with dS^T in its place the chain dP, dS, dK, next dP
+// took 4500 cycles a step).  The hi half of K lives in tensor memory too, which leaves room for two stages of Q and dO.  Two warps issue,
 // one the scores and one the sums, so that neither's waits hold up the other's instructions.
-// Tensor memory: S^T 2 x 64 columns, dP^T 64, K hi 64, dV 128, dK 128.  Shared memory: V 64 KB, K lo 32 KB, 2 x (Q 32 KB + dO 32 KB).
+// Tensor memory: S^T / P^T / dS^T 2 x 64 columns, dP^T 64, K hi 64, dV 128, dK 128.  Shared memory: V 64 KB, K lo 32 KB, 2 x (Q 32 KB + dO 32 KB).
 // Every kFlush steps dV and dK are added to float32 registers (32 + 32 a thread), one step later, between that step's weights and
 // its dS, while the products that end the chunk run.  Bound: tensor pipe, 48 instructions of 46 cycles and 24 of 64 a step.
 template <int DP>
@@ -281,12 +282,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   auto s_full = [&](int i) { return bars + 112u + 8u * i; };
   auto p_full = [&](int i) { return bars + 128u + 8u * i; };
   auto s_free = [&](int i) { return bars + 160u + 8u * i; };
+  auto v_done = [&](int i) { return bars + 184u + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(v_full, 1); mbar_init(kh_full, 1); mbar_init(kh_ready, 512); mbar_init(dp_full, 1); mbar_init(ds_full, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512); mbar_init(dp_free, 1);
+    mbar_init(v_full, 1); mbar_init(kh_full, 1); mbar_init(kh_ready, 512); mbar_init(dp_full, 1); mbar_init(ds_full, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512); mbar_init(dp_free, 512);
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full(i), 1); mbar_init(g_full(i), 1); mbar_init(q_empty(i), 1); mbar_init(g_empty(i), 2); mbar_init(s_full(i), 1); mbar_init(p_full(i), 512);
-      mbar_init(s_free(i), 1);
+      mbar_init(s_free(i), 1); mbar_init(v_done(i), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -402,14 +404,14 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         if (!ok) break;
         tc_fence_after();
         accumulate(tmem + COL_DV, tmem + COL_S + b2 * 64, base + OFF_G + b2 * SLOT, slices, fresh);
+        commit_by(el, v_done(b2));
         commit_by(el, g_empty(b2));
-        commit_by(el, s_free(b2));
         ok = mbar_wait(ds_full, i & 1);
         if (!ok) break;
         tc_fence_after();
-        accumulate(tmem + COL_DK, tmem + COL_DP, base + OFF_Q + b2 * SLOT, slices, fresh);
+        accumulate(tmem + COL_DK, tmem + COL_S + b2 * 64, base + OFF_Q + b2 * SLOT, slices, fresh);
         commit_by(el, q_empty(b2));
-        commit_by(el, dp_free);
+        commit_by(el, s_free(b2));
         if ((i + 1) % kFlush == 0 || i + 1 == n) commit_by(el, acc_full);
       }
     }
@@ -474,6 +476,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         uint32_t y[16];
         tmem_ld16(lane_addr + COL_DP + part * 16, y);
         tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive(dp_free);
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 c = off[16 + (e >> 2)];
@@ -485,7 +489,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
 #pragma unroll
         for (int e = 0; e < 16; ++e) if (!((see >> e) & 1u)) w[e] = 0.0f;   // what stands in a masked place may not be a number
       }
-      store_pairs(lane_addr + COL_DP + part * 16, w);
+      ok = ok && mbar_wait(v_done(i & 1), (i >> 1) & 1);
+      tc_fence_after();
+      store_pairs(lane_addr + COL_S + (i & 1) * 64 + part * 16, w);
       tc_fence_before();
       mbar_arrive(ds_full);
     }
