@@ -59,7 +59,7 @@ int sink_rows(const gn_sink_params* p, StreamRows* s) {
   GN_REQUIRE(p->sinks >= 0 && p->scale == p->scale, "attention_sink: bad sinks or scale");
   GN_REQUIRE(strides_ok(p->query) && strides_ok(p->key) && strides_ok(p->value), "attention_sink: negative stride");
   GN_REQUIRE((int64_t)p->seq * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_sink: seq x heads of a group exceeds 2^30");
-  s->rows = p->batch; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->D = p->head_dim;
+  s->rows = p->batch; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->by_G = FastDiv(s->G); s->D = p->head_dim;
   s->window = p->window; s->sinks = p->sinks; s->scale = p->scale; s->q = p->query; s->k = p->key; s->v = p->value; s->seq = p->seq; s->lengths = p->lengths;
   return GN_OK;
 }
@@ -96,7 +96,7 @@ int paged_rows(const gn_paged_params* p, StreamRows* s) {
   GN_REQUIRE((int64_t)p->max_query * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_paged: max_query x heads of a group exceeds 2^30");
   GN_REQUIRE(p->sinks >= 0 && p->scale == p->scale, "attention_paged: bad sinks or scale");
   GN_REQUIRE(strides_ok(p->query) && strides_ok(p->new_key) && strides_ok(p->new_value), "attention_paged: negative stride");
-  s->rows = p->rows; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->D = p->head_dim;
+  s->rows = p->rows; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->by_G = FastDiv(s->G); s->D = p->head_dim;
   s->window = p->window; s->sinks = p->sinks; s->scale = p->scale; s->q = p->query;
   s->pages_k = p->key_pages; s->pages_v = p->value_pages; s->table = p->page_table; s->starts = p->query_starts; s->lens = p->context_lens;
   s->tokens = p->tokens; s->max_query = std::min(p->max_query, p->tokens); s->max_context = p->max_context; s->page_size = p->page_size; s->pages = p->pages;

@@ -4,9 +4,24 @@
 
 namespace gn {
 
+// Division of 0 <= n < 2^31 by a number that a launch fixes: the high half of n m, m = floor(2^(31 + s) / d) + 1, 2^(s - 1) < d <= 2^s.
+// (The error of m, below 2^-31 of it, moves n m / 2^(31 + s) by less than 1 / d, so the floor is exact.)
+struct FastDiv {
+  uint32_t d = 1, m = 0; int s = 0;
+  FastDiv() = default;
+  explicit FastDiv(int64_t by) : d((uint32_t)by) {
+    while ((1ll << s) < by) ++s;
+    m = s == 0 ? 0u : (uint32_t)((1ull << (31 + s)) / d + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int of(int n) const { return s == 0 ? n : (int)(__umulhi((uint32_t)n, m) >> (s - 1)); }
+#endif
+};
+
 // The rows (sequences) of a call, padded batch or paged cache, as the kernels see them.
 struct StreamRows {
   int rows = 0, Hq = 0, Hkv = 0, G = 0, D = 0, window = -1, sinks = 0;
+  FastDiv by_G;
   float scale = 1.0f;
   gn_view q{}, k{}, v{};            // k, v: padded batch
   // padded batch: `seq` tokens a row, lengths nullable

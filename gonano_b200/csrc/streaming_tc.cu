@@ -161,12 +161,14 @@ struct ForwardTc {
   gn_view out;
   float* lse;
   int vec_q, vec_out, tiles, splits;
+  int planes;
+  FastDiv by_planes, by_splits, by_Hkv;
   float* part_o; float* part_l;   // splits > 1: [plane][tile][split][128] rows of DP channels, and their log2-sum-exps
 };
 
 constexpr int kRowsT = 128;      // query rows of an item = keys of a tile = UMMA M and N
 constexpr int kThreads = 768;    // four softmax warpgroups, one that fetches Q, one with the issuing and the copying warp
-constexpr int kRegsSoftmax = 88, kRegsFetch = 72, kRegsOther = 56;   // shares of the launch's 6 x 80
+constexpr int kRegsSoftmax = 88, kRegsFetch = 80, kRegsOther = 48;   // shares of the launch's 6 x 80 (the fetching one keeps its)
 
 // What a CTA works on next: 128 query rows of a plane against a range of their key tiles.
 struct Item {
@@ -177,19 +179,19 @@ struct Item {
   __device__ __forceinline__ int rows16(int j) const { return min(kRowsT, (runs.total - (j0 + j) * kRowsT + 15) & ~15); }   // keys of tile j, in 16s
 };
 template <bool PAGED>
-__device__ __forceinline__ Item get_item(const ForwardTc& p, int64_t w) {
+__device__ __forceinline__ Item get_item(const ForwardTc& p, int w) {
   const StreamRows& s = p.s;
   Item it;
-  const int64_t planes = (int64_t)s.rows * s.Hkv, level = w / planes;   // the last tiles first: under a causal mask they are the longest
-  it.plane = w - level * planes;
-  it.split = (int)(level % p.splits); it.tile = p.tiles - 1 - (int)(level / p.splits);
-  it.r = (int)(it.plane / s.Hkv); it.hk = (int)(it.plane - (int64_t)it.r * s.Hkv);
+  const int level = p.by_planes.of(w), plane = w - level * p.planes, last = p.by_splits.of(level);   // the last tiles first: under a causal mask they are the longest
+  it.plane = plane;
+  it.split = level - last * p.splits; it.tile = p.tiles - 1 - last;
+  it.r = p.by_Hkv.of(plane); it.hk = plane - it.r * s.Hkv;
   const RowSpan sp = row_span<PAGED>(s, it.r);
   it.f0 = it.tile * kRowsT; it.nf = sp.q_len * s.G; it.first = sp.ctx - sp.q_len; it.q_begin = sp.q_begin;
   it.inside = it.f0 < (PAGED ? it.nf : s.seq * s.G);
   it.runs = KeyRuns{0, 0, 0};
-  if (it.f0 < it.nf) it.runs = key_runs(s, it.first + it.f0 / s.G, it.first + min(it.f0 + kRowsT - 1, it.nf - 1) / s.G);
-  const int all = (it.runs.total + kRowsT - 1) / kRowsT, per = (all + p.splits - 1) / p.splits;
+  if (it.f0 < it.nf) it.runs = key_runs(s, it.first + s.by_G.of(it.f0), it.first + s.by_G.of(min(it.f0 + kRowsT - 1, it.nf - 1)));
+  const int all = (it.runs.total + kRowsT - 1) / kRowsT, per = p.by_splits.of(all + p.splits - 1);
   it.j0 = it.split * per; it.n = max(0, min(all, it.j0 + per) - it.j0);
   return it;
 }
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 160);
-  const int64_t items = (int64_t)s.rows * s.Hkv * p.tiles * p.splits;
+  const int items = p.planes * p.tiles * p.splits;
 
   if (warp >= 20) {
     regs_dec<kRegsOther>();
@@ -244,12 +246,12 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       // ------------------------------------------------------------- copies: K_0, K_1, V_0, K_2, V_1, ... as they are used
       bool ok = true;
       int slot = 0; uint32_t turn = 0;
-      for (int64_t w = blockIdx.x; w < items && ok; w += gridDim.x) {
+      for (int w = blockIdx.x; w < items && ok; w += gridDim.x) {
         const Item it = get_item<PAGED>(p, w);
         for (int m = 0; m < 2 * it.n && ok; ++m) {
           const bool value = m == 2 * it.n - 1 || (m > 0 && (m & 1) == 0);
           const int j = value ? (m == 2 * it.n - 1 ? it.n - 1 : (m >> 1) - 1) : (m + 1) >> 1;
-          if (turn > 0) ok = mbar_wait(empty(slot), (turn - 1) & 1);
+          if (turn > 0) ok = hold(empty(slot), (turn - 1) & 1);
           if (!ok) break;
           const Packed& src = value ? p.pk.v : p.pk.k;
           const int c0 = (it.j0 + j) * kRowsT, rows = it.rows16(j), na = min(max(it.runs.a_len - c0, 0), rows), nb = rows - na;
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         }
       }
       if (!ok)   // copies in flight land before the CTA goes
-        for (int i = 0; i < RING; ++i) { mbar_wait(full(i), 0); mbar_wait(full(i), 1); }
+        for (int i = 0; i < RING; ++i) { hold(full(i), 0); hold(full(i), 1); }
     }
     if (warp == 20 || warp == 22) {
       // ------------------------------------------------------------- instructions
@@ -275,18 +277,18 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       bool ok = true;
       uint32_t tile = 0, count = 0, ring = 0;   // tiles, items and copies so far
       Item it = get_item<PAGED>(p, blockIdx.x);   // the grid is no larger than the number of items
-      for (int64_t w = blockIdx.x; w < items && ok;) {
+      for (int w = blockIdx.x; w < items && ok;) {
         const int n = it.n, last16 = n > 0 ? it.rows16(n - 1) : 0;
         w += gridDim.x;
         if (w < items) it = get_item<PAGED>(p, w);   // the next item's geometry is on its way while this one runs
         if (n == 0) continue;
-        if (!products) ok = mbar_wait(q_ready, count & 1);
+        if (!products) ok = hold(q_ready, count & 1);
         for (int j = 0; j < n && ok; ++j, ++tile) {
           const int rows = j + 1 == n ? last16 : kRowsT, b = tile & 1;
           const uint32_t m = ring + (products ? min(2 * j + 2, 2 * n - 1) : j == 0 ? 0 : 2 * j - 1), slot = m % RING;
-          ok = mbar_wait(full(slot), (m / RING) & 1);
-          if (products) ok = ok && mbar_wait(p_full(b), (tile >> 1) & 1) && (tile == 0 || mbar_wait(o_empty, (tile - 1) & 1));
-          else ok = ok && (tile < 2 || mbar_wait(s_free(b), ((tile >> 1) - 1) & 1));
+          ok = hold(full(slot), (m / RING) & 1);
+          if (products) ok = ok && hold(p_full(b), (tile >> 1) & 1) && (tile == 0 || hold(o_empty, (tile - 1) & 1));
+          else ok = ok && (tile < 2 || hold(s_free(b), ((tile >> 1) - 1) & 1));
           if (!ok) break;
           tc_fence_after();
           if (products) {
@@ -325,60 +327,83 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     }
   } else if (warp >= 16) {
     // --------------------------------------------------------------- Q rows to tensor memory
-    regs_dec<kRegsFetch>();
     const int row = (warp & 3) * 32 + lane;
     const uint32_t q_addr = tmem + COL_Q + ((uint32_t)((warp & 3) * 32) << 16);
     float* rowc = reinterpret_cast<float*>(gen + ROWC);
     bool ok = true;
     uint32_t count = 0;
-    for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
+    for (int w = blockIdx.x; w < items; w += gridDim.x) {
       const Item it = get_item<PAGED>(p, w);
       if (it.n == 0) continue;
-      const int f = it.f0 + row, t = f / s.G, g = f - t * s.G;
+      const int f = it.f0 + row, t = s.by_G.of(f), g = f - t * s.G;
       const bool live = f < it.nf;
       const float* src = live ? s.q.data + token_offset<PAGED>(s.q, it.r, it.hk * s.G + g, it.q_begin + t) : nullptr;
       // 32 channels of the row from ch on: with float4 accesses the lanes of eight rows read one row after the other
       auto load = [&](int ch, float (&x)[32]) {
-        if (p.vec_q) {
-          const int mine = ch + (lane & 7) * 4;
+        if (p.vec_q) {   // every load unconditional (a row that is not there reads the first one), so that all eight are in flight at once
+          const int mine = ch + (lane & 7) * 4, at = min(mine, s.D - 4);
+          uint32_t there = 0;
+          float4 v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float* at = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), (lane & 24) + k));
-            float4 v = make_float4(0, 0, 0, 0);
-            if (at && mine < s.D) v = *reinterpret_cast<const float4*>(at + mine);
-            x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+            const float* row = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), (lane & 24) + k));
+            if (row && mine < s.D) there |= 1u << k;
+            v[k] = *reinterpret_cast<const float4*>((row ? row : s.q.data) + at);
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const bool in = (there >> k) & 1u;
+            x[4 * k] = in ? v[k].x : 0.0f; x[4 * k + 1] = in ? v[k].y : 0.0f; x[4 * k + 2] = in ? v[k].z : 0.0f; x[4 * k + 3] = in ? v[k].w : 0.0f;
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = src && ch + e < s.D ? src[ch + e] : 0.0f;
         }
       };
+      // One pass: the scale comes from the first 32 channels, with 2^6 to spare for the others; a warp with a row that needs
+      // more (or whose first channels are zeros) goes over its rows again.
       uint32_t top = 0;
-#pragma unroll 1
-      for (int h = 0; h < DP / 32; ++h) {
-        float x[32];
-        load(h * 32, x);
+      float sq = 1.0f, iq = 1.0f, x[32], next[32];
+      auto fetch = [&](int h, float (&to)[32]) { load(h * 32, to); };
+      auto emit = [&](int h) {
         if (p.vec_q) transpose_blocks<8>(x);
+        if (top == 0xffffffffu) {   // the second pass: scales stand
+        } else {
+          uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) if (finite_bits(x[e])) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-      }
-      float sq, iq, sk, ik;
-      plane_scale(top, sq, iq);
-      plane_scale(p.pk.amax[it.plane * 2], sk, ik);
-      // a negative scale goes into Q, so that larger products are larger scores; a vanishing one stays a positive number
-      const float c = fmaxf(fabsf(s.scale) * kLog2e * iq * ik, 1e-30f);
-      if (s.scale < 0.0f) sq = -sq;
-#pragma unroll 1
-      for (int h = 0; h < DP / 32; ++h) {
-        float x[32];
-        load(h * 32, x);
-        if (p.vec_q) transpose_blocks<8>(x);
+          for (int e = 0; e < 32; ++e) if (finite_bits(x[e])) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+          if (h == 0) {
+            plane_scale(most, sq, iq);
+            sq *= 0x1p-6f; iq *= 0x1p6f;
+          }
+          top = max(top, most);
+        }
+        const float by = s.scale < 0.0f ? -sq : sq;   // a negative scale goes into Q, so that larger products are larger scores
         uint32_t y[32];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) split_f16(x[e] * sq, x[e + 1] * sq, y[e >> 1], y[16 + (e >> 1)]);
-        if (h == 0 && count > 0) { ok = ok && mbar_wait(q_free, (count - 1) & 1); tc_fence_after(); }
+        for (int e = 0; e < 32; e += 2) split_f16(x[e] * by, x[e + 1] * by, y[e >> 1], y[16 + (e >> 1)]);
+        if (h == 0 && count > 0) { ok = ok && hold(q_free, (count - 1) & 1); tc_fence_after(); }
         tmem_st32(q_addr + h * 32, y);
+      };
+      fetch(0, x);
+#pragma unroll 1
+      for (int h = 0; h < DP / 32; ++h) {
+        if (h + 1 < DP / 32) fetch(h + 1, next);
+        emit(h);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = next[e];
       }
+      const float largest = __uint_as_float(top) * sq;
+      const bool again = top != 0 && !(largest >= 0x1p7f && largest < 0x1p15f);
+      if (__any_sync(0xffffffffu, again)) {
+        if (again) plane_scale(top, sq, iq);
+        top = 0xffffffffu;
+#pragma unroll 1
+        for (int h = 0; h < DP / 32; ++h) { fetch(h, x); emit(h); }
+      }
+      float sk, ik;
+      plane_scale(p.pk.amax[it.plane * 2], sk, ik);
+      const float c = fmaxf(fabsf(s.scale) * kLog2e * iq * ik, 1e-30f);   // a vanishing scale stays a positive number
       rowc[(count & 3) * 128 + row] = c;   // four: the fetcher can be three items ahead of the softmax threads
       tmem_st_wait();
       tc_fence_before();
@@ -403,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     struct Target { float* out; float* lse; float iv; } to{nullptr, nullptr, 1.0f};
 
     auto gather = [&]() {   // O of the last tile, against the maximum that it used
-      ok = ok && mbar_wait(o_full, (tiles - 1) & 1);
+      ok = ok && hold(o_full, (tiles - 1) & 1);
       tc_fence_after();
       uint32_t y[QC];
       if constexpr (QC == 32) tmem_ld32(lane_addr + COL_O + part * QC, y);
@@ -440,10 +465,10 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       }
     };
 
-    for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
+    for (int w = blockIdx.x; w < items; w += gridDim.x) {
       const Item it = get_item<PAGED>(p, w);
       if (!it.inside) continue;
-      const int f = it.f0 + row, t = f / s.G, g = f - t * s.G, token = it.q_begin + t, pos = it.first + t;
+      const int f = it.f0 + row, t = s.by_G.of(f), g = f - t * s.G, token = it.q_begin + t, pos = it.first + t;
       const bool live = f < it.nf;
       Target here;
       if (p.splits > 1) {
@@ -466,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       const int s_end = live ? max(0, min(s.sinks, pos + 1)) : 0;
       const int lo_key = live ? (s.window < 0 ? 0 : max(0, pos - s.window)) - it.runs.shift : 0, hi_key = live ? pos - it.runs.shift : -1;
       const bool odd_plane = (p.pk.odd[it.plane * 2] | p.pk.odd[it.plane * 2 + 1]) != 0;
-      ok = ok && mbar_wait(q_ready, count & 1);
+      ok = ok && hold(q_ready, count & 1);
       const float c = rowc[(count & 3) * 128 + row];
       ++count;
       float m_here = -INFINITY, l_here = 0.0f;
@@ -484,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
               else if (flag & kOdd) l_here = NAN;
             }
         }
-        ok = ok && mbar_wait(s_full(tiles & 1), (tiles >> 1) & 1);
+        ok = ok && hold(s_full(tiles & 1), (tiles >> 1) & 1);
         tc_fence_after();
         uint32_t y[32];
         tmem_ld32(buf, y);
@@ -628,6 +653,7 @@ int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t s
     GN_CUDA(cudaFuncSetAttribute(stream_tc_forward_kernel<DP, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   }
   const int64_t items = pl.planes * pl.tiles * pl.splits;
+  GN_REQUIRE(items < (1ll << 31) - 1024, "attention: %lld tiles of query rows", (long long)items);
   stream_tc_forward_kernel<DP, PAGED><<<(unsigned)std::min<int64_t>(items, num_sms()), kThreads, kSmem, st>>>(f);
   GN_LAUNCH_CHECK();
   if (pl.splits > 1) {
@@ -661,7 +687,8 @@ int64_t stream_tc_forward_bytes(const StreamRows& s) {
 int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t st, PackedKeys* packed) {
   const Plan pl = plan_forward(s);
   ForwardTc f{};
-  f.s = s; f.out = out; f.lse = lse; f.tiles = pl.tiles; f.splits = pl.splits;
+  f.s = s; f.out = out; f.lse = lse; f.tiles = pl.tiles; f.splits = pl.splits; f.planes = (int)pl.planes;
+  f.by_planes = FastDiv(pl.planes); f.by_splits = FastDiv(pl.splits); f.by_Hkv = FastDiv(s.Hkv);
   carve_forward(s, pl, workspace, &f);
   if (packed) *packed = f.pk;
   f.vec_q = vec_view(s.q, s.D); f.vec_out = pl.splits > 1 || vec_view(out, s.D);

@@ -72,6 +72,17 @@ int stream_tc_backward(const StreamRows& s, const gn_view& out, const gn_view& d
 #ifdef __CUDACC__
 namespace {
 
+// Bounded wait in which the hardware holds the thread back (up to 2 us a try): sixteen warps that poll instead take the issue slots and the
+// shared memory from the others, which made the fetching of Q four times slower.  False when the bound (about a second) ran out.
+__device__ __forceinline__ bool hold(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 19); ++i) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(2000u) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }

@@ -37,7 +37,7 @@ constexpr int kPackRowsQ = 64;   // 256 threads, 16 half warps
 // Half a warp per query row f: channels 4 i .. of the 64-channel blocks.
 template <int CB>
 __device__ __forceinline__ void load_query_row(const StreamRows& s, const gn_view& v, int vec, int r, int hk, int f, float (&x)[4 * CB]) {
-  const int l16 = threadIdx.x & 15, t = f / s.G, h = hk * s.G + f - t * s.G;
+  const int l16 = threadIdx.x & 15, t = s.by_G.of(f), h = hk * s.G + f - t * s.G;
   const float* p = v.data + token_offset<false>(v, r, h, t);
 #pragma unroll
   for (int b = 0; b < CB; ++b) {
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
     }
     if (l16 == 0) {
       float off = 0.0f;
-      if (f < nf) { const int t = f / s.G; off = odd ? NAN : kWeightShift - p.lse[stat_offset<false>(s, r, hk * s.G + f - t * s.G, t)] * kLog2e; }
+      if (f < nf) { const int t = s.by_G.of(f); off = odd ? NAN : kWeightShift - p.lse[stat_offset<false>(s, r, hk * s.G + f - t * s.G, t)] * kLog2e; }
       p.off[plane * p.q.rows + f] = off;
       p.delta[plane * p.q.rows + f] = delta * sc[1] * sv;
     }
@@ -319,15 +319,15 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       bool ok = true;
       for (int i = 0; i < n && ok; ++i) {
         const int rows = rows16(i), f = row0(i), b2 = i & 1;
-        if (i >= 2) ok = mbar_wait(q_empty(b2), ((i >> 1) - 1) & 1);
+        if (i >= 2) ok = hold(q_empty(b2), ((i >> 1) - 1) & 1);
         if (!ok) break;
         mbar_expect_tx(q_full(b2), (uint32_t)CB * 2u * rows * 128u + 2u * rows * 4u);
 #pragma unroll 1
         for (int b = 0; b < CB * 2; ++b) bulk_load(base + OFF_Q + b2 * SLOT + b * 8192, qp + ((int64_t)b * p.q.rows + f) * 128, rows * 128, q_full(b2));
         bulk_load(base + STATS + b2 * 512, p.off + plane * p.q.rows + f, rows * 4, q_full(b2));
         bulk_load(base + STATS + b2 * 512 + 256, p.delta + plane * p.q.rows + f, rows * 4, q_full(b2));
-        if (i == 1) ok = mbar_wait(kh_ready, 0);
-        if (i >= 2) ok = mbar_wait(g_empty(b2), ((i >> 1) - 1) & 1);
+        if (i == 1) ok = hold(kh_ready, 0);
+        if (i >= 2) ok = hold(g_empty(b2), ((i >> 1) - 1) & 1);
         if (!ok) break;
         mbar_expect_tx(g_full(b2), (uint32_t)CB * 2u * rows * 128u);
 #pragma unroll 1
@@ -335,20 +335,20 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       }
       if (!ok)   // copies in flight land before the CTA goes
         for (int i = 0; i < 2; ++i)
-          for (int ph = 0; ph < 2; ++ph) { mbar_wait(q_full(i), ph); mbar_wait(g_full(i), ph); }
-      mbar_wait(v_full, 0);
-      mbar_wait(kh_full, 0);
+          for (int ph = 0; ph < 2; ++ph) { hold(q_full(i), ph); hold(g_full(i), ph); }
+      hold(v_full, 0);
+      hold(kh_full, 0);
     }
     if (warp == 16 && n > 0) {
       // ----------------------------------------------------------- scores: S^T(0), dP^T(0), S^T(1), dP^T(1), ...
       const uint32_t el = elect_lane();
-      bool ok = mbar_wait(v_full, 0) && mbar_wait(kh_ready, 0);
+      bool ok = hold(v_full, 0) && hold(kh_ready, 0);
       tc_fence_after();
       const uint64_t kl = smem_desc_sw128(base + OFF_KL), vd = smem_desc_sw128(base);
       for (int i = 0; i < n && ok; ++i) {
         const int b2 = i & 1;
         const uint32_t id = instr_desc_f16(128, rows16(i), 0);
-        ok = mbar_wait(q_full(b2), (i >> 1) & 1) && (i < 2 || mbar_wait(s_free(b2), ((i >> 1) - 1) & 1));
+        ok = hold(q_full(b2), (i >> 1) & 1) && (i < 2 || hold(s_free(b2), ((i >> 1) - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         {
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
           for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, tmem + COL_KH + ks * 8, q + (ks >> 2) * 1024 + (ks & 3) * 2, id, 1);
           commit_by(el, s_full(b2));
         }
-        ok = mbar_wait(g_full(b2), (i >> 1) & 1) && (i < 1 || mbar_wait(dp_free, (i - 1) & 1));
+        ok = hold(g_full(b2), (i >> 1) & 1) && (i < 1 || hold(dp_free, (i - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         {
@@ -400,13 +400,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       for (int i = 0; i < n && ok; ++i) {
         const int b2 = i & 1, slices = rows16(i) >> 4;
         const uint32_t fresh = i % kFlush == 0 ? 0u : 1u;
-        ok = mbar_wait(p_full(b2), (i >> 1) & 1) && mbar_wait(g_full(b2), (i >> 1) & 1) && (fresh || i == 0 || mbar_wait(acc_empty, (i / kFlush - 1) & 1));
+        ok = hold(p_full(b2), (i >> 1) & 1) && hold(g_full(b2), (i >> 1) & 1) && (fresh || i == 0 || hold(acc_empty, (i / kFlush - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         accumulate(tmem + COL_DV, tmem + COL_S + b2 * 64, base + OFF_G + b2 * SLOT, slices, fresh);
         commit_by(el, v_done(b2));
         commit_by(el, g_empty(b2));
-        ok = mbar_wait(ds_full, i & 1);
+        ok = hold(ds_full, i & 1);
         if (!ok) break;
         tc_fence_after();
         accumulate(tmem + COL_DK, tmem + COL_S + b2 * 64, base + OFF_Q + b2 * SLOT, slices, fresh);
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     const PlaneFactors fc = plane_factors(p, plane);
     bool ok = true;
     if (n > 0) {
-      ok = mbar_wait(kh_full, 0);
+      ok = hold(kh_full, 0);
       if (part < 2 * CB) row_to_tmem(lane_addr + COL_KH + part * 16, gen + OFF_G + SLOT + (part >> 1) * 16384, row, part & 1);
       tmem_st_wait();
       tc_fence_before();
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
 #pragma unroll
     for (int e = 0; e < QC; ++e) dv[e] = dk[e] = 0.0f;
     auto flush = [&](int chunk) {
-      ok = ok && mbar_wait(acc_full, chunk & 1);
+      ok = ok && hold(acc_full, chunk & 1);
       tc_fence_after();
       add_columns<QC>(lane_addr + COL_DV + part * QC, dv);
       add_columns<QC>(lane_addr + COL_DK + part * QC, dk);
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       const uint32_t see = (uint32_t)(bits_below(f_hi - f0) & ~bits_below(f_lo - f0));
       const float4* off = reinterpret_cast<const float4*>(gen + STATS + (i & 1) * 512 + part * 64);
       float w[16];
-      ok = ok && mbar_wait(q_full(i & 1), (i >> 1) & 1) && mbar_wait(s_full(i & 1), (i >> 1) & 1);
+      ok = ok && hold(q_full(i & 1), (i >> 1) & 1) && hold(s_full(i & 1), (i >> 1) & 1);
       tc_fence_after();
       {
         uint32_t y[16];
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       tc_fence_before();
       mbar_arrive(p_full(i & 1));
       if (i > 0 && i % kFlush == 0) flush(i / kFlush - 1);
-      ok = ok && mbar_wait(dp_full, i & 1);
+      ok = ok && hold(dp_full, i & 1);
       tc_fence_after();
       {
         uint32_t y[16];
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
 #pragma unroll
         for (int e = 0; e < 16; ++e) if (!((see >> e) & 1u)) w[e] = 0.0f;   // what stands in a masked place may not be a number
       }
-      ok = ok && mbar_wait(v_done(i & 1), (i >> 1) & 1);
+      ok = ok && hold(v_done(i & 1), (i >> 1) & 1);
       tc_fence_after();
       store_pairs(lane_addr + COL_S + (i & 1) * 64 + part * 16, w);
       tc_fence_before();
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
   const int hk = blockIdx.y, r = blockIdx.z, tile = p.q_tiles - 1 - (int)blockIdx.x, f0 = tile * 128;
   const int len = row_span<false>(s, r).ctx, nf = len * s.G;
   KeyRuns runs{0, 0, 0};
-  if (f0 < nf) runs = key_runs(s, f0 / s.G, min(f0 + 127, nf - 1) / s.G);
+  if (f0 < nf) runs = key_runs(s, s.by_G.of(f0), s.by_G.of(min(f0 + 127, nf - 1)));
   const int n = (runs.total + 63) / 64;
   const int64_t plane = (int64_t)r * s.Hkv + hk;
 
@@ -617,32 +617,32 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       };
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
-        if (j == 2) ok = mbar_wait(hi_ready, 0);
-        if (j >= 3) ok = mbar_wait(k_empty(j % 3), (j / 3 - 1) & 1);
+        if (j == 2) ok = hold(hi_ready, 0);
+        if (j >= 3) ok = hold(k_empty(j % 3), (j / 3 - 1) & 1);
         if (!ok) break;
         copy_tile(p.pk.k, base + OFF_K + (j % 3) * SLOT, k_full(j % 3), j);
-        if (j == 1) ok = mbar_wait(hi_ready, 0);
-        if (j >= 2) ok = mbar_wait(v_empty(j & 1), ((j >> 1) - 1) & 1);
+        if (j == 1) ok = hold(hi_ready, 0);
+        if (j >= 2) ok = hold(v_empty(j & 1), ((j >> 1) - 1) & 1);
         if (!ok) break;
         copy_tile(p.pk.v, base + OFF_V + (j & 1) * SLOT, v_full(j & 1), j);
       }
       if (!ok)
         for (int ph = 0; ph < 2; ++ph) {
-          for (int i = 0; i < 3; ++i) mbar_wait(k_full(i), ph);
-          for (int i = 0; i < 2; ++i) mbar_wait(v_full(i), ph);
+          for (int i = 0; i < 3; ++i) hold(k_full(i), ph);
+          for (int i = 0; i < 2; ++i) hold(v_full(i), ph);
         }
-      mbar_wait(lo_full, 0);
-      mbar_wait(hi_full, 0);
+      hold(lo_full, 0);
+      hold(hi_full, 0);
     }
     if (warp == 16 && n > 0) {
       // ----------------------------------------------------------- scores
       const uint32_t el = elect_lane();
-      bool ok = mbar_wait(lo_full, 0) && mbar_wait(hi_ready, 0);
+      bool ok = hold(lo_full, 0) && hold(hi_ready, 0);
       tc_fence_after();
       for (int j = 0; j < n && ok; ++j) {
         const uint32_t id = instr_desc_f16(128, rows16(j), 0);
         for (int w = 0; w < 2 && ok; ++w) {
-          ok = w ? mbar_wait(v_full(j & 1), (j >> 1) & 1) : mbar_wait(k_full(j % 3), (j / 3) & 1) && (j < 2 || mbar_wait(ds_free(j & 1), ((j >> 1) - 1) & 1));
+          ok = w ? hold(v_full(j & 1), (j >> 1) & 1) : hold(k_full(j % 3), (j / 3) & 1) && (j < 2 || hold(ds_free(j & 1), ((j >> 1) - 1) & 1));
           if (!ok) break;
           tc_fence_after();
           const uint32_t d = tmem + (w ? COL_DP : COL_S) + (j & 1) * 64, hi = tmem + (w ? COL_G : COL_Q);
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
         const uint32_t fresh = j % kFlush == 0 ? 0u : 1u;
-        ok = mbar_wait(ds_full(j & 1), (j >> 1) & 1) && mbar_wait(k_full(j % 3), (j / 3) & 1) && (fresh || j == 0 || mbar_wait(acc_empty, (j / kFlush - 1) & 1));
+        ok = hold(ds_full(j & 1), (j >> 1) & 1) && hold(k_full(j % 3), (j / 3) & 1) && (fresh || j == 0 || hold(acc_empty, (j / kFlush - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         const uint32_t a = tmem + COL_DP + (j & 1) * 64;
@@ -690,12 +690,12 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane, f = f0 + row;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const bool live = f < nf;
-    const int t = f / s.G, h = hk * s.G + f - t * s.G;
+    const int t = s.by_G.of(f), h = hk * s.G + f - t * s.G;
     const PlaneFactors fc = plane_factors(p, plane);
     float off = 0.0f, delta = 0.0f;
     bool ok = true;
     if (n > 0) {
-      ok = mbar_wait(hi_full, 0);
+      ok = hold(hi_full, 0);
 #pragma unroll
       for (int w = 0; w < 2; ++w)
         if (part < 2 * CB)
@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
 #pragma unroll
     for (int e = 0; e < QC; ++e) acc[e] = 0.0f;
     auto flush = [&](int chunk) {   // one step later, as above
-      ok = ok && mbar_wait(acc_full, chunk & 1);
+      ok = ok && hold(acc_full, chunk & 1);
       tc_fence_after();
       add_columns<QC>(lane_addr + COL_DQ + part * QC, acc);
       tc_fence_before();
@@ -721,7 +721,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     for (int j = 0; j < n; ++j) {
       const int c0 = j * 64 + part * 16;
       const uint32_t see = (uint32_t)(bits_below(s_end - c0) | (bits_below(hi_key + 1 - c0) & ~bits_below(lo_key - c0)));
-      ok = ok && mbar_wait(sp_full(j & 1), (j >> 1) & 1);
+      ok = ok && hold(sp_full(j & 1), (j >> 1) & 1);
       tc_fence_after();
       float w[16];
       {

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(256) stream_mass_pack_kernel(const __grid_cons
   uint8_t* base = p.q.data + plane * p.q.plane_bytes(CB);
 #pragma unroll 1
   for (int f = blockIdx.x * 64 + half; f < min(last, (int)blockIdx.x * 64 + 64); f += 16) {   // whole 16s: the warp's halves go together
-    const int t = f / s.G, h = hk * s.G + f - t * s.G;
+    const int t = s.by_G.of(f), h = hk * s.G + f - t * s.G;
     float x[4 * CB];
     const float* src = s.q.data + (f < nf ? token_offset<true>(s.q, r, h, sp.q_begin + t) : 0);
     uint32_t top = 0;
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
       bool ok = true;
       for (int i = 0; i < n && ok; ++i) {
         // the tile has been multiplied, and its factors read
-        if (i >= 2) ok = mbar_wait(q_empty(i & 1), ((i >> 1) - 1) & 1) && mbar_wait(s_empty(i & 1), ((i >> 1) - 1) & 1);
+        if (i >= 2) ok = hold(q_empty(i & 1), ((i >> 1) - 1) & 1) && hold(s_empty(i & 1), ((i >> 1) - 1) & 1);
         if (!ok) break;
         const int rows = rows16(i), f = f_begin + i * 128;
         const uint32_t bar = q_full(i & 1), st = base + STATS + (i & 1) * 1024;
@@ -136,16 +136,16 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
         bulk_load(st + 512, p.off + plane * p.q.rows + f, rows * 4, bar);
       }
       if (!ok)   // copies in flight land before the CTA goes
-        for (int i = 0; i < 2; ++i) { mbar_wait(q_full(i), 0); mbar_wait(q_full(i), 1); }
-      mbar_wait(k_full, 0);
+        for (int i = 0; i < 2; ++i) { hold(q_full(i), 0); hold(q_full(i), 1); }
+      hold(k_full, 0);
     }
   } else if (warp == 16) {
     if (n > 0) {
       const uint32_t el = elect_lane();
-      bool ok = mbar_wait(k_full, 0);
+      bool ok = hold(k_full, 0);
       const uint64_t a = smem_desc_sw128(base);
       for (int i = 0; i < n && ok; ++i) {
-        ok = mbar_wait(q_full(i & 1), (i >> 1) & 1) && (i < 2 || mbar_wait(s_empty(i & 1), ((i >> 1) - 1) & 1));
+        ok = hold(q_full(i & 1), (i >> 1) & 1) && (i < 2 || hold(s_empty(i & 1), ((i >> 1) - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + (i & 1) * 128, id = instr_desc_f16(128, rows16(i), 0);
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
       const int f0 = f_begin + i * 128 + part * 32;
       const uint32_t see = (uint32_t)(bits_below(f_hi - f0) & ~bits_below(f_lo - f0));
       const float* st = reinterpret_cast<const float*>(gen + STATS + (i & 1) * 1024) + part * 32;
-      ok = ok && mbar_wait(q_full(i & 1), (i >> 1) & 1) && mbar_wait(s_full(i & 1), (i >> 1) & 1);
+      ok = ok && hold(q_full(i & 1), (i >> 1) & 1) && hold(s_full(i & 1), (i >> 1) & 1);
       tc_fence_after();
       uint32_t y[32];
       tmem_ld32(lane_addr + (i & 1) * 128 + part * 32, y);
