@@ -338,21 +338,16 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       const int f = it.f0 + row, t = s.by_G.of(f), g = f - t * s.G;
       const bool live = f < it.nf;
       const float* src = live ? s.q.data + token_offset<PAGED>(s.q, it.r, it.hk * s.G + g, it.q_begin + t) : nullptr;
-      // 32 channels of the row from ch on: with float4 accesses the lanes of eight rows read one row after the other
+      // 32 channels of the row from ch on, all loads in flight at once (a row that is not there reads the tensor's first)
       auto load = [&](int ch, float (&x)[32]) {
-        if (p.vec_q) {   // every load unconditional (a row that is not there reads the first one), so that all eight are in flight at once
-          const int mine = ch + (lane & 7) * 4, at = min(mine, s.D - 4);
-          uint32_t there = 0;
+        if (p.vec_q) {
+          const float* row = src ? src : s.q.data;
           float4 v[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float* row = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), (lane & 24) + k));
-            if (row && mine < s.D) there |= 1u << k;
-            v[k] = *reinterpret_cast<const float4*>((row ? row : s.q.data) + at);
-          }
+          for (int k = 0; k < 8; ++k) v[k] = __ldg(reinterpret_cast<const float4*>(row + min(ch + 4 * k, s.D - 4)));
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const bool in = (there >> k) & 1u;
+            const bool in = src && ch + 4 * k < s.D;
             x[4 * k] = in ? v[k].x : 0.0f; x[4 * k + 1] = in ? v[k].y : 0.0f; x[4 * k + 2] = in ? v[k].z : 0.0f; x[4 * k + 3] = in ? v[k].w : 0.0f;
           }
         } else {
@@ -366,7 +361,6 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       float sq = 1.0f, iq = 1.0f, x[32], next[32];
       auto fetch = [&](int h, float (&to)[32]) { load(h * 32, to); };
       auto emit = [&](int h) {
-        if (p.vec_q) transpose_blocks<8>(x);
         if (top == 0xffffffffu) {   // the second pass: scales stand
         } else {
           uint32_t most = 0;
