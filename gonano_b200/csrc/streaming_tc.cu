@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
     if (threadIdx.x == 0) { most = 0; any_odd = 0; }
     __syncthreads();
     uint32_t top = 0;
+#pragma unroll 4
     for (int j = half; j < sp.ctx; j += 16) {
       if (!is_needed<PAGED>(s, sp, begin, j)) continue;
       float x[4 * CB];
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
   plane_scale(whole ? most : pk.amax[plane * 2 + value], sc, inv);
   float top = 0.0f;
   const int steps = whole ? (last + 15) / 16 : kPackRows / 16;
-#pragma unroll 2
+#pragma unroll 4
   for (int u = 0; u < steps; ++u) {
     const int j = j0 + u * 16 + half;
     float x[4 * CB];

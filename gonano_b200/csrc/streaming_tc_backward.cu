@@ -32,6 +32,7 @@ struct BackwardTc {
 };
 
 constexpr int kWholePlaneQ = 256;   // planes up to here are one CTA's
+constexpr int kAmaxRowsQ = 256;
 constexpr int kPackRowsQ = 64;   // 256 threads, 16 half warps
 
 // Half a warp per query row f: channels 4 i .. of the 64-channel blocks.
@@ -56,12 +57,12 @@ __device__ __forceinline__ void load_query_row(const StreamRows& s, const gn_vie
 template <int CB>
 __global__ void __launch_bounds__(256) stream_query_amax_kernel(const __grid_constant__ BackwardTc p) {
   const StreamRows& s = p.s;
-  const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, f0 = blockIdx.x * kPackRowsQ;
+  const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, f0 = blockIdx.x * kAmaxRowsQ;
   const int nf = row_span<false>(s, r).q_len * s.G;
   if (f0 >= nf) return;
   uint32_t top[2] = {0, 0};
-#pragma unroll
-  for (int u = 0; u < kPackRowsQ / 16; ++u) {
+#pragma unroll 4
+  for (int u = 0; u < kAmaxRowsQ / 16; ++u) {
     const int f = f0 + u * 16 + half;
     if (f >= nf) continue;
 #pragma unroll
@@ -92,6 +93,7 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
     if (threadIdx.x == 0) most[0] = most[1] = norm = 0;
     __syncthreads();
     uint32_t top[2] = {0, 0};
+#pragma unroll 4
     for (int f = half; f < nf; f += 16)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
@@ -806,10 +808,9 @@ int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
   GN_TRY(stream_pack_keys(s, b.pk, b.norms, st));
   const int whole = b.q.rows <= kWholePlaneQ;
   if (!whole) {
-    const dim3 rows(ceil_div(b.q.rows, kPackRowsQ), s.Hkv, s.rows);
     GN_CUDA(cudaMemsetAsync(b.qamax, 0, planes * 2 * sizeof(uint32_t), st));
     GN_CUDA(cudaMemset2DAsync(b.norms + 1, 2 * sizeof(uint32_t), 0, sizeof(uint32_t), planes, st));
-    stream_query_amax_kernel<CB><<<rows, 256, 0, st>>>(b);
+    stream_query_amax_kernel<CB><<<dim3(ceil_div(b.q.rows, kAmaxRowsQ), s.Hkv, s.rows), 256, 0, st>>>(b);
     GN_LAUNCH_CHECK();
   }
   stream_query_pack_kernel<CB><<<dim3(whole ? 1 : ceil_div(b.q.rows, kPackRowsQ), s.Hkv, s.rows), 256, 0, st>>>(b, whole);
