@@ -55,7 +55,7 @@ __device__ __forceinline__ void mma(float (&c)[4], float a0, float a1, float a2,
 // R = 8 NT query rows.  Lane = (g, t) = (lane / 4, lane % 4), as the instruction's fragments are laid out: rows g and g + 8, contraction
 // indices t and t + 4, columns g of the second operand and 2 t, 2 t + 1 of the result.
 template <int NT, int DP, bool MULTI>
-__global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __grid_constant__ Decode p) {
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) stream_decode_kernel(const __grid_constant__ Decode p) {
   constexpr int R = 8 * NT, PAIRS = DP / 16, EACH = DP / 8;   // float4s of a K row in a lane; channels of a V row in a lane
   __shared__ __align__(16) float room[kWarps * R * DP];
   float (&q_s)[NT][PAIRS][2][32][4] = *reinterpret_cast<float (*)[NT][PAIRS][2][32][4]>(room);   // queries as fragments, hi and lo
@@ -71,13 +71,19 @@ __global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __g
   const Range rg = seen_range(s, sp);
   const int per = ((rg.total + p.splits - 1) / p.splits + kTile - 1) / kTile * kTile, c0 = split * per, c1 = min(rg.total, c0 + per);
   const int64_t plane = (int64_t)r * s.Hkv + hk;
-  for (int i = threadIdx.x; i < R * DP; i += 32 * kWarps) {
-    const int qi = i / DP, ch = i % DP;
-    const float x = qi < nq && ch < s.D ? s.q.data[token_offset<true>(s.q, r, hk * s.G + qi % s.G, sp.q_begin + qi / s.G) + ch] * (s.scale * kLog2e) : 0.0f;
-    const int to = (qi & 7) * 4 + ((ch & 15) >> 2);
-    const float hi = nearest(x);
-    q_s[qi >> 3][ch >> 4][0][to][ch & 3] = hi;
-    q_s[qi >> 3][ch >> 4][1][to][ch & 3] = x - hi;
+#pragma unroll
+  for (int i = threadIdx.x; i < R * DP / 4; i += 32 * kWarps) {   // four channels a thread; rows behind the last query are zeros
+    const int qi = i / (DP / 4), ch = i % (DP / 4) * 4, qt = s.by_G.of(qi);
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (qi < nq) {
+      const float* src = s.q.data + token_offset<true>(s.q, r, hk * s.G + qi - qt * s.G, sp.q_begin + qt) + ch;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (ch + e < s.D) x[e] = src[e] * (s.scale * kLog2e);
+    }
+    float* to = &q_s[qi >> 3][ch >> 4][0][(qi & 7) * 4 + ((ch & 15) >> 2)][0];
+    const float4 hi = make_float4(nearest(x[0]), nearest(x[1]), nearest(x[2]), nearest(x[3]));
+    *reinterpret_cast<float4*>(to) = hi;
+    *reinterpret_cast<float4*>(to + 128) = make_float4(x[0] - hi.x, x[1] - hi.y, x[2] - hi.z, x[3] - hi.w);
   }
   __syncthreads();
 
@@ -94,14 +100,15 @@ __global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __g
     if (slot >= 0) return pages + (int64_t)slot * s.D;
     return slot == -1 ? nullptr : fresh.data + token_offset<true>(fresh, r, hk, sp.q_begin - 2 - slot);
   };
-  auto load4 = [&](const float* row, int ch, float* x) {
-    x[0] = x[1] = x[2] = x[3] = 0.0f;
-    if (!row) return;
+  // four channels from ch on.  With 16-byte accesses without a condition, so that all of a tile's loads are in flight at once: channels
+  // behind the last read the last ones (the queries are 0 there, and such outputs are not stored), a key that is not there the first slot
+  auto load4 = [&](const float* row, const float* any, int ch, float* x) {
     if (p.vec) {
-      if (ch < s.D) { const float4 v = *reinterpret_cast<const float4*>(row + ch); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+      const float4 v = __ldg(reinterpret_cast<const float4*>((row ? row : any) + min(ch, s.D - 4)));
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) if (ch + e < s.D) x[e] = row[ch + e];
+      for (int e = 0; e < 4; ++e) x[e] = row && ch + e < s.D ? row[ch + e] : 0.0f;
     }
   };
   float kr[2][PAIRS * 4];   // rows g and g + 8 of the tile, channels 16 i + 4 t ..
@@ -110,7 +117,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __g
     for (int u = 0; u < 2; ++u) {
       const float* row = row_of(__shfl_sync(0xffffffffu, slots, g + 8 * u), s.pages_k, p.nk);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) load4(row, 16 * i + 4 * t, &kr[u][4 * i]);
+      for (int i = 0; i < PAIRS; ++i) load4(row, s.pages_k, 16 * i + 4 * t, &kr[u][4 * i]);
     }
   };
   float m[2 * NT], l[2 * NT], o[NT][PAIRS][4];
@@ -124,16 +131,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __g
   constexpr int kStride = kTile * kWarps;
   int c = c0 + warp * kTile;
   int slots = locate(c), next = locate(c + kStride);   // the table is read two tiles ahead
-  load_k(slots);
   for (; c < c1; c += kStride) {
     const int after = locate(c + 2 * kStride);
-    float vr[4][EACH];   // V rows t, t + 4, t + 8, t + 12, channels EACH g ..
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float* row = row_of(__shfl_sync(0xffffffffu, slots, t + 4 * u), s.pages_v, p.nv);
-#pragma unroll
-      for (int e = 0; e < EACH; e += 4) load4(row, EACH * g + e, &vr[u][e]);
-    }
+    load_k(slots);
     // the instruction cuts its sums off: the small terms have sums of their own, and the large ones four that are then added rounded
     float x[NT][4], big[NT][4][4], small[NT][2][4];
 #pragma unroll
@@ -160,7 +160,21 @@ __global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __g
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[nt][e] = ((big[nt][0][e] + big[nt][1][e]) + (big[nt][2][e] + big[nt][3][e])) + (small[nt][0][e] + small[nt][1][e]);
-    load_k(next);   // the next tile's keys are on their way from here on
+    float vr[4][EACH];   // V rows t, t + 4, t + 8, t + 12, channels EACH g ..
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* row = row_of(__shfl_sync(0xffffffffu, slots, t + 4 * u), s.pages_v, p.nv);
+#pragma unroll
+      for (int e = 0; e < EACH; e += 4) load4(row, s.pages_v, EACH * g + e, &vr[u][e]);
+    }
+    if (__any_sync(0xffffffffu, lane < kTile && slots == -1)) {   // keys of weight 0, whatever was read for them
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (__shfl_sync(0xffffffffu, slots, t + 4 * u) == -1) {
+#pragma unroll
+          for (int e = 0; e < EACH; ++e) vr[u][e] = 0.0f;
+        }
+    }
     bool odd[2] = {false, false};
     if (MULTI) {   // a value that is not finite must reach only the queries that see it
       uint32_t bad = 0;
@@ -185,7 +199,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __g
         float a = x[nt][h], b = x[nt][2 + h];
         bool see_a = slot_a != -1, see_b = slot_b != -1;
         if (MULTI) {
-          const int pos = first + q / s.G;
+          const int pos = first + s.by_G.of(q);
           see_a = see_a && q < nq && sees(s, pos, key_of(rg, c + g)); see_b = see_b && q < nq && sees(s, pos, key_of(rg, c + g + 8));
         }
         if (!see_a) a = -INFINITY;
@@ -281,7 +295,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) stream_decode_kernel(const __g
       p.part_o[at * DP + ch] = y;
       if (ch == 0) p.part_l[at] = L;
     } else {
-      const int h = hk * s.G + q % s.G, token = sp.q_begin + q / s.G;
+      const int qt = s.by_G.of(q), h = hk * s.G + q - qt * s.G, token = sp.q_begin + qt;
       if (ch < s.D) p.out.data[token_offset<true>(p.out, r, h, token) + ch] = y;
       if (ch == 0) p.lse[stat_offset<true>(s, r, h, token)] = L * kLn2;
     }
@@ -312,7 +326,7 @@ __global__ void __launch_bounds__(128) stream_decode_join_kernel(const __grid_co
 #pragma unroll
       for (int e = 0; e < DP / 32; ++e) o[e] = fmaf(w, p.part_o[(at + (int64_t)i * R) * DP + lane + 32 * e], o[e]);
     }
-  const int h = hk * s.G + q % s.G, token = sp.q_begin + q / s.G;
+  const int qt = s.by_G.of(q), h = hk * s.G + q - qt * s.G, token = sp.q_begin + qt;
   float* dst = p.out.data + token_offset<true>(p.out, r, h, token);
   const float z = bad ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
