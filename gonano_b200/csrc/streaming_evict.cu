@@ -28,12 +28,15 @@ __device__ __forceinline__ int64_t slot_of(const gn_evict_params& p, const int32
 }
 
 constexpr int kSelect = 1024, kWarpsS = kSelect / 32;
+constexpr int kCached = 49152;
 
 // A CTA per (row, kv head).  The threshold (the smallest kept order key among those that are neither sinks nor recent) by three radix
-// passes of 11, 11 and 10 bits: a warp adds each of its distinct digits once (weights are often alike: keys nobody looked at hold
-// 0).  Then every warp takes a run of keys, counts what it keeps, and writes the indices behind those of the warps before it: two
-// passes, no order left to chance.  Of the keys equal to the threshold the first ones are kept.
-__global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ Evict e) {
+// passes of 11, 11 and 10 bits; the digit of a warp's first key is added once for all that share it (weights are often alike: keys
+// nobody looked at hold 0).  Then every warp takes a run of keys, counts what it keeps, and writes the indices behind those of the warps before it: two
+// passes, no order left to chance.  Of the keys equal to the threshold the first ones are kept.  Up to kCached keys are read from memory
+// once and kept as order keys in shared memory.
+__global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ Evict e, int cached) {
+  extern __shared__ uint32_t cache[];
   const gn_evict_params& p = e.p;
   const int hk = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = evict_len(p, r), keep = min(n, p.budget), lo = p.sinks, hi = n - p.recent;
@@ -47,6 +50,12 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   const int wanted = n <= p.budget ? 0 : p.budget - p.sinks - p.recent;   // of the middle
   uint32_t prefix = 0;
   int want = wanted;
+  if (wanted > 0 && cached) {
+#pragma unroll 4
+    for (int j = lo + tid; j < hi; j += kSelect) cache[j] = order_key(mass[j]);
+    __syncthreads();
+  }
+  auto key_at = [&](int j) { return cached ? cache[j] : order_key(mass[j]); };   // of the middle
   if (wanted > 0) {
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
@@ -55,11 +64,12 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
       __syncthreads();
       for (int j0 = lo; j0 < hi; j0 += kSelect) {
         const int j = j0 + tid;
-        const uint32_t k = j < hi ? order_key(mass[j]) : 0u;
+        const uint32_t k = j < hi ? key_at(j) : 0u;
         const bool in = j < hi && (pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix);
         const uint32_t digit = in ? (k >> shift) & (uint32_t)(bins - 1) : 0xffffffffu;
-        const uint32_t same = __match_any_sync(0xffffffffu, digit);
-        if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+        const uint32_t most = __shfl_sync(0xffffffffu, digit, 0), same = __ballot_sync(0xffffffffu, in && digit == most);
+        if (in && digit != most) atomicAdd(&hist[digit], 1);
+        else if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
       }
       __syncthreads();
       // the digit at which the count from above reaches `want`: thread t holds bins 2t' and 2t' + 1 counted from the top
@@ -85,7 +95,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
     take = tie = false;
     if (j >= j1) return;
     if (n <= p.budget || j < lo || j >= hi) take = true;
-    else if (wanted > 0) { const uint32_t k = order_key(mass[j]); take = k > prefix; tie = k == prefix; }
+    else if (wanted > 0) { const uint32_t k = key_at(j); take = k > prefix; tie = k == prefix; }
   };
   int sure = 0, equal = 0;
   for (int j = j0; j < j1; j += 32) {
@@ -207,7 +217,10 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
 int stream_evict(const gn_evict_params& p, int32_t* kept, int32_t* new_lens, float* mass_out, cudaStream_t st) {
   Evict e{p, kept, new_lens, mass_out, 0};
   e.vec = p.head_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.key_pages) | reinterpret_cast<uintptr_t>(p.value_pages)) & 15) == 0;
-  evict_select_kernel<<<dim3(p.n_kv_head, p.rows), kSelect, 0, st>>>(e);
+  const int cached = p.max_context <= kCached;
+  static PerDeviceOnce once;
+  if (once.first()) GN_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * (int)sizeof(uint32_t)));
+  evict_select_kernel<<<dim3(p.n_kv_head, p.rows), kSelect, cached ? p.max_context * sizeof(uint32_t) : 0, st>>>(e, cached);
   GN_LAUNCH_CHECK();
   const int most = std::min(p.budget, p.max_context);
   if (most == 0) return GN_OK;

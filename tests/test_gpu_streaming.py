@@ -475,6 +475,11 @@ def test_evict(case, in_place, kind):
 
 
 @pytest.mark.gpu
+def test_evict_more_keys_than_are_cached():
+    check_evict([60000, 49153], 1, 4, 256, 5000, 4, 100, lambda m: (m * 1000).floor(), False)
+
+
+@pytest.mark.gpu
 def test_evict_bad_pages():
     """Pages that do not exist are neither read nor written: a key from one leaves zeros."""
     cache = Cache(1, 1, 32, 8, 8)
