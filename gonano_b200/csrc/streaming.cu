@@ -1,5 +1,6 @@
 // Streaming attention: the C entry points, their checks, and the copy of new tokens to their pages.
 #include <algorithm>
+#include <cmath>
 
 #include "streaming_tc.cuh"
 
@@ -50,17 +51,19 @@ bool apart(const gn_view& v, int64_t batch, int64_t heads, int64_t tokens, int64
 }
 bool strides_ok(const gn_view& v) { return v.batch_stride >= 0 && v.head_stride >= 0 && v.token_stride >= 0; }
 
+constexpr int kFar = 1 << 30;   // no sequence is longer: wider windows and more sinks are cut to it, so that sums with positions stay in 32 bits
+
 int sink_rows(const gn_sink_params* p, StreamRows* s) {
   GN_REQUIRE(p, "attention_sink: null parameters");
   GN_REQUIRE(p->batch >= 0 && p->seq >= 0 && p->n_kv_head > 0 && p->n_head > 0 && p->n_head % p->n_kv_head == 0,
              "attention_sink: batch %d, seq %d, %d heads on %d kv heads", p->batch, p->seq, p->n_head, p->n_kv_head);
   GN_REQUIRE(p->head_dim > 0 && p->head_dim <= 128, "attention_sink: head_dim %d outside [1, 128]", p->head_dim);
   GN_REQUIRE(p->batch <= 32767 && p->n_head <= 65535, "attention_sink: more than 32767 sequences or 65535 heads");
-  GN_REQUIRE(p->sinks >= 0 && p->scale == p->scale, "attention_sink: bad sinks or scale");
+  GN_REQUIRE(p->sinks >= 0 && std::isfinite(p->scale), "attention_sink: bad sinks or scale");
   GN_REQUIRE(strides_ok(p->query) && strides_ok(p->key) && strides_ok(p->value), "attention_sink: negative stride");
   GN_REQUIRE((int64_t)p->seq * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_sink: seq x heads of a group exceeds 2^30");
   s->rows = p->batch; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->by_G = FastDiv(s->G); s->D = p->head_dim;
-  s->window = p->window; s->sinks = p->sinks; s->scale = p->scale; s->q = p->query; s->k = p->key; s->v = p->value; s->seq = p->seq; s->lengths = p->lengths;
+  s->window = std::min(p->window, kFar); s->sinks = std::min(p->sinks, kFar); s->scale = p->scale; s->q = p->query; s->k = p->key; s->v = p->value; s->seq = p->seq; s->lengths = p->lengths;
   return GN_OK;
 }
 int sink_pointers(const gn_sink_params* p) {
@@ -88,16 +91,16 @@ int paged_rows(const gn_paged_params* p, StreamRows* s) {
              "attention_paged: rows %d, tokens %d, max_query %d, %d heads on %d kv heads", p->rows, p->tokens, p->max_query, p->n_head, p->n_kv_head);
   GN_REQUIRE(p->head_dim > 0 && p->head_dim <= 128, "attention_paged: head_dim %d outside [1, 128]", p->head_dim);
   GN_REQUIRE(p->rows <= 32767 && p->n_head <= 65535, "attention_paged: more than 32767 rows or 65535 heads");
-  GN_REQUIRE(p->page_size > 0 && p->pages >= 0 && p->table_width >= 0 && (int64_t)p->table_width * p->page_size < (1ll << 31),
+  GN_REQUIRE(p->page_size > 0 && p->pages >= 0 && p->table_width >= 0 && (int64_t)p->table_width * p->page_size <= kFar,
              "attention_paged: pages %d of %d keys, table of %d", p->pages, p->page_size, p->table_width);
   GN_REQUIRE((int64_t)p->pages * p->n_kv_head < (1ll << 31) / p->page_size, "attention_paged: more than 2^31 slots of keys");
   GN_REQUIRE(p->max_context >= 0 && (int64_t)p->max_context <= (int64_t)p->table_width * p->page_size, "attention_paged: max_context %d, but a row of the table holds %lld keys",
              p->max_context, (long long)p->table_width * p->page_size);
   GN_REQUIRE((int64_t)p->max_query * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_paged: max_query x heads of a group exceeds 2^30");
-  GN_REQUIRE(p->sinks >= 0 && p->scale == p->scale, "attention_paged: bad sinks or scale");
+  GN_REQUIRE(p->sinks >= 0 && std::isfinite(p->scale), "attention_paged: bad sinks or scale");
   GN_REQUIRE(strides_ok(p->query) && strides_ok(p->new_key) && strides_ok(p->new_value), "attention_paged: negative stride");
   s->rows = p->rows; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->by_G = FastDiv(s->G); s->D = p->head_dim;
-  s->window = p->window; s->sinks = p->sinks; s->scale = p->scale; s->q = p->query;
+  s->window = std::min(p->window, kFar); s->sinks = std::min(p->sinks, kFar); s->scale = p->scale; s->q = p->query;
   s->pages_k = p->key_pages; s->pages_v = p->value_pages; s->table = p->page_table; s->starts = p->query_starts; s->lens = p->context_lens;
   s->tokens = p->tokens; s->max_query = std::min(p->max_query, p->tokens); s->max_context = p->max_context; s->page_size = p->page_size; s->pages = p->pages;
   s->width = p->table_width;

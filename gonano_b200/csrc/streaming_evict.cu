@@ -3,7 +3,7 @@
 // Bound: HBM, the kept rows read and written once (16 D bytes a key) and 4 bytes of weight a key.
 #include <algorithm>
 
-#include "streaming.cuh"
+#include "streaming_tc.cuh"
 
 namespace gn {
 
@@ -218,8 +218,8 @@ int stream_evict(const gn_evict_params& p, int32_t* kept, int32_t* new_lens, flo
   Evict e{p, kept, new_lens, mass_out, 0};
   e.vec = p.head_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.key_pages) | reinterpret_cast<uintptr_t>(p.value_pages)) & 15) == 0;
   const int cached = p.max_context <= kCached;
-  static PerDeviceOnce once;
-  if (once.first()) GN_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * (int)sizeof(uint32_t)));
+  static std::atomic<uint64_t> ready{0};
+  GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(evict_select_kernel), kCached * (int)sizeof(uint32_t), kSelect, 0));
   evict_select_kernel<<<dim3(p.n_kv_head, p.rows), kSelect, cached ? p.max_context * sizeof(uint32_t) : 0, st>>>(e, cached);
   GN_LAUNCH_CHECK();
   const int most = std::min(p.budget, p.max_context);

@@ -642,11 +642,8 @@ template <int DP, bool PAGED>
 int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t st) {
   constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 1024;
   GN_TRY(stream_pack_keys(s, f.pk, nullptr, st));
-  static PerDeviceOnce once;
-  if (once.first()) {
-    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_forward_kernel<DP, PAGED>), kThreads, 512 * kRegsSoftmax + 128 * (kRegsFetch + kRegsOther)));
-    GN_CUDA(cudaFuncSetAttribute(stream_tc_forward_kernel<DP, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  }
+  static std::atomic<uint64_t> ready{0};
+  GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(stream_tc_forward_kernel<DP, PAGED>), kSmem, kThreads, 512 * kRegsSoftmax + 128 * (kRegsFetch + kRegsOther)));
   const int64_t items = pl.planes * pl.tiles * pl.splits;
   GN_REQUIRE(items < (1ll << 31) - 1024, "attention: %lld tiles of query rows", (long long)items);
   stream_tc_forward_kernel<DP, PAGED><<<(unsigned)std::min<int64_t>(items, num_sms()), kThreads, kSmem, st>>>(f);
@@ -660,13 +657,19 @@ int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t s
 
 }  // namespace
 
-int check_registers(const void* kernel, int threads, int shared_out) {
+int prepare_kernel(std::atomic<uint64_t>& ready, const void* kernel, int smem, int threads, int shared_out) {
+  int device = 0;
+  GN_CUDA(cudaGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (ready.load(std::memory_order_acquire) & bit)) return GN_OK;
   cudaFuncAttributes a{};
   GN_CUDA(cudaFuncGetAttributes(&a, kernel));
   if (a.numRegs * threads < shared_out) {
     set_error("streaming attention: built with %d registers a thread, too few for the kernel's split", a.numRegs);
     return GN_ERR_UNSUPPORTED;
   }
+  GN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (device < 64) ready.fetch_or(bit, std::memory_order_release);   // only now: a call that failed leaves the next one to try again
   return GN_OK;
 }
 

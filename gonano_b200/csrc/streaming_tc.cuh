@@ -48,8 +48,9 @@ struct Carve {   // workspace layout; with a null base it only counts
     return at;
   }
 };
-// A register split needs the launch to hold what its warpgroups share out, or the wait for registers would not end.
-int check_registers(const void* kernel, int threads, int shared_out);
+// Allows a kernel its dynamic shared memory, once per device (`ready` holds a bit for each), and refuses one that was built with fewer
+// registers than its warpgroups share out: the wait for registers would not end.
+int prepare_kernel(std::atomic<uint64_t>& ready, const void* kernel, int smem, int threads, int shared_out);
 // Whether float4 accesses fit a view of head_dim D.
 static inline bool vec_view(const gn_view& v, int D) {
   return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && D % 4 == 0 && v.batch_stride % 4 == 0 && v.head_stride % 4 == 0 && v.token_stride % 4 == 0;
@@ -169,7 +170,7 @@ __device__ __forceinline__ void plane_scale(uint32_t amax, float& s, float& inve
   inverse = amax == 0 ? 1.0f : __uint_as_float((uint32_t)(e - 14 + 127) << 23);
 }
 
-// Registers move between warpgroups inside what the launch holds (check_registers).
+// Registers move between warpgroups inside what the launch holds (prepare_kernel).
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 

@@ -797,13 +797,10 @@ template <int DP>
 int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
   constexpr int CB = DP / 64;
   constexpr int kSmemKv = CB * (32768 + 16384 + 4 * 16384) + 1024 + 256 + 1024, kSmemQ = CB * (2 * 16384 + 5 * 16384) + 256 + 1024;
-  static PerDeviceOnce once;
-  if (once.first()) {
-    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_dkv_kernel<DP>), kThreadsB, 512 * kRegsSoftmax + 128 * kRegsOther));
-    GN_TRY(check_registers(reinterpret_cast<const void*>(stream_tc_dq_kernel<DP>), kThreadsB, 512 * kRegsSoftmax + 128 * kRegsOther));
-    GN_CUDA(cudaFuncSetAttribute(stream_tc_dkv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemKv));
-    GN_CUDA(cudaFuncSetAttribute(stream_tc_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemQ));
-  }
+  static std::atomic<uint64_t> ready_kv{0}, ready_q{0};
+  constexpr int kShared = 512 * kRegsSoftmax + 128 * kRegsOther;
+  GN_TRY(prepare_kernel(ready_kv, reinterpret_cast<const void*>(stream_tc_dkv_kernel<DP>), kSmemKv, kThreadsB, kShared));
+  GN_TRY(prepare_kernel(ready_q, reinterpret_cast<const void*>(stream_tc_dq_kernel<DP>), kSmemQ, kThreadsB, kShared));
   const int64_t planes = (int64_t)s.rows * s.Hkv;
   GN_TRY(stream_pack_keys(s, b.pk, b.norms, st));
   const int whole = b.q.rows <= kWholePlaneQ;

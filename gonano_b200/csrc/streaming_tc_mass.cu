@@ -221,8 +221,8 @@ template <int DP>
 int go(const MassTc& m, cudaStream_t st) {
   constexpr int kSmem = DP / 64 * 3 * 32768 + 2048 + 128 + 2048 + 1024;
   const StreamRows& s = m.s;
-  static PerDeviceOnce once;
-  if (once.first()) GN_CUDA(cudaFuncSetAttribute(stream_tc_mass_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  static std::atomic<uint64_t> ready{0};
+  GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(stream_tc_mass_kernel<DP>), kSmem, kThreadsM, 0));
   stream_mass_pack_kernel<DP / 64><<<dim3(ceil_div(m.q.rows, 64), s.Hkv, s.rows), 256, 0, st>>>(m);
   GN_LAUNCH_CHECK();
   stream_tc_mass_kernel<DP><<<dim3(ceil_div(s.max_context, 128), s.Hkv, s.rows), kThreadsM, kSmem, st>>>(m);

@@ -171,6 +171,34 @@ def test_strides(D):
 
 
 @pytest.mark.gpu
+def test_broadcast_inputs():
+    """Keys and values shared by the sequences of a batch through a stride of 0: the gradients are those of the expanded tensors."""
+    q, k, v, dout = tensors(3, 4, 2, 140, 64, seed=14)
+    k, v = k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)
+    check_window(q, k, v, dout, None, 30, 2, 0.125)
+    with pytest.raises(GonanoError):
+        out, lse = streaming.sink_attention_forward(q, k, v, 2, 30)
+        streaming.sink_attention_backward(q, k, v, out, dout, lse, 2, 30, dq=torch.zeros_like(q), dk=torch.zeros(1, 2, 140, 64, device=DEVICE).expand(3, -1, -1, -1),
+                                          dv=torch.zeros(3, 2, 140, 64, device=DEVICE))
+
+
+@pytest.mark.gpu
+def test_windows_and_sinks_beyond_every_length():
+    big = 2 ** 31 - 1
+    q, k, v, dout = tensors(1, 4, 2, 200, 64, seed=15)
+    for window, sinks in ((big, 0), (5, big), (big, big)):
+        check_window(q, k, v, dout, None, window, sinks, 0.125)
+    for counts in ([1, 1], [40, 7]):
+        check_paged(counts, [90, 8], 4, 2, 64, 16, big, big)
+    cache = Cache(1, 1, 64, 16, 2)   # tokens that stand before the cache, with the widest window
+    cache.fill([20])
+    x = torch.randn(30, 2, 64, device=DEVICE)
+    starts, lens = torch.tensor([0, 30], dtype=torch.int32, device=DEVICE), torch.tensor([20], dtype=torch.int32, device=DEVICE)
+    got = [streaming.paged_attention(x, cache.k, cache.v, cache.table, starts, lens, 30, scale=0.125, window=w) for w in (-1, big)]
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.gpu
 def test_misaligned_views():
     """Tensors that start 4 bytes behind a 16-byte boundary."""
     def shift(x):
@@ -378,6 +406,38 @@ def test_more_tokens_than_keys():
     starts, lens = torch.tensor([0, 30], dtype=torch.int32, device=DEVICE), torch.tensor([20], dtype=torch.int32, device=DEVICE)
     out, lse = streaming.paged_attention(q, cache.k, cache.v, cache.table, starts, lens, 30, scale=0.125)
     assert bool((out[:10] == 0).all()) and bool((lse[:10] == -math.inf).all()) and bool(out.isfinite().all()) and bool(lse[10:].isfinite().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 40])
+def test_pages_beyond_32_bits(count):
+    """Pages whose elements lie past 2^31 and 2^32: attention, the new tokens' slots and eviction."""
+    pages, page, dim, n = 600_000, 64, 128, 300
+    k = torch.zeros(pages, 1, page, dim, device=DEVICE)   # 19.7 GB
+    v = torch.zeros(pages, 1, page, dim, device=DEVICE)
+    gen = torch.Generator(device=DEVICE).manual_seed(16)
+    ids = [pages - 1, 270_000, 3, 530_000, pages - 2]
+    flat = torch.randn(2, n, dim, generator=gen, device=DEVICE)
+    for i, p in enumerate(ids):
+        m = min(page, n - count - i * page)
+        if m > 0:
+            k[p, 0, :m], v[p, 0, :m] = flat[0, i * page:i * page + m], flat[1, i * page:i * page + m]
+    table = torch.tensor([ids], dtype=torch.int32, device=DEVICE)
+    q = torch.randn(count, 4, dim, generator=gen, device=DEVICE)
+    starts, lens = torch.tensor([0, count], dtype=torch.int32, device=DEVICE), torch.tensor([n], dtype=torch.int32, device=DEVICE)
+    out, lse, mass = streaming.paged_attention(q, k, v, table, starts, lens, count, new_key=flat[0, n - count:, None], new_value=flat[1, n - count:, None], scale=0.09,
+                                               mass_out=torch.zeros(1, 1, 5 * page, device=DEVICE))
+    see = visible(torch.arange(n - count, n, device=DEVICE), torch.arange(n, device=DEVICE), -1, 0)
+    o, l, w = attend64(q.double().transpose(0, 1), flat[0].double(), flat[1].double(), see, 0.09)
+    e = 2 * score_bound(q, flat[0], 0.09) + PRODUCT
+    close(out.transpose(0, 1), o, e * torch.einsum("gnm,md->gnd", w, flat[1].double().abs()) + FLOOR * (n + 2) * float(flat[1].abs().max()), "out")
+    for i, p in enumerate(ids):
+        m = min(page, n - i * page)
+        assert torch.equal(k[p, 0, :m], flat[0, i * page:i * page + m]) and torch.equal(v[p, 0, :m], flat[1, i * page:i * page + m])
+    fresh = torch.tensor([[pages - 3, 400_000]], dtype=torch.int32, device=DEVICE)
+    kept, _, _ = streaming.evict_pages(k, v, mass, table, lens, 100, 4, 10, new_table=fresh)
+    got = k[fresh[0].long(), 0].reshape(-1, dim)[:100]
+    assert torch.equal(got, flat[0, kept[0, 0].long()])
 
 
 @pytest.mark.gpu
@@ -658,7 +718,7 @@ def lib():
 
 
 @pytest.mark.parametrize("over", [dict(head_dim=0), dict(head_dim=129), dict(n_kv_head=3), dict(n_kv_head=0), dict(n_head=0), dict(batch=-1), dict(seq=-1), dict(sinks=-1),
-                                  dict(scale=math.nan), dict(batch=70000), dict(query=_lib.GnView(None, -1, 1, 1)), dict(seq=2 ** 30)])
+                                  dict(scale=math.nan), dict(scale=math.inf), dict(batch=70000), dict(query=_lib.GnView(None, -1, 1, 1)), dict(seq=2 ** 30)])
 def test_sink_refusals(lib, over):
     import ctypes as C
     n = C.c_int64()
