@@ -214,7 +214,7 @@ __device__ __forceinline__ Item get_item(const ForwardTc& p, int w) {
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __grid_constant__ ForwardTc p) {
   constexpr int CB = DP / 64, QC = DP / 4, RING = DP == 64 ? 6 : 3;
-  constexpr uint32_t TILE = CB * 32768u, BARS = RING * TILE, ROWC = BARS + 256, XCH = ROWC + 2048;
+  constexpr uint32_t TILE = CB * 32768u, BARS = RING * TILE, ROWC = BARS + 256, XCH = ROWC + 2048, STASH = XCH + 6144;
   constexpr uint32_t COL_O = 256, COL_Q = 384;
   extern __shared__ uint8_t smem_raw[];
   const StreamRows& s = p.s;
@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     const int row = (warp & 3) * 32 + lane;
     const uint32_t q_addr = tmem + COL_Q + ((uint32_t)((warp & 3) * 32) << 16);
     float* rowc = reinterpret_cast<float*>(gen + ROWC);
+    uint4* stash = reinterpret_cast<uint4*>(gen + STASH);   // each thread its own column
     bool ok = true;
     uint32_t count = 0;
     for (int w = blockIdx.x; w < items; w += gridDim.x) {
@@ -357,44 +358,54 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         }
       };
       // One pass: the scale comes from the first 32 channels, with 2^6 to spare for the others; a warp with a row that needs
-      // more (or whose first channels are zeros) goes over its rows again.
-      uint32_t top = 0;
-      float sq = 1.0f, iq = 1.0f, x[32], next[32];
-      auto fetch = [&](int h, float (&to)[32]) { load(h * 32, to); };
-      auto emit = [&](int h) {
-        if (top == 0xffffffffu) {   // the second pass: scales stand
-        } else {
-          uint32_t most = 0;
+      // more (or whose first channels are zeros) goes over its rows again.  While the last item's scores still read Q, the first
+      // 32 channels wait in shared memory, the next in registers, and the third are being loaded: what is left to do once Q is free
+      // took 9600 cycles when only the first were ready.
+      uint32_t top = 0, y[32];
+      float sq, iq, x[32];
+      auto largest_of = [&](const float (&x)[32]) {
+        uint32_t most = 0;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) if (finite_bits(x[e])) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
-          if (h == 0) {
-            plane_scale(most, sq, iq);
-            sq *= 0x1p-6f; iq *= 0x1p6f;
-          }
-          top = max(top, most);
-        }
+        for (int e = 0; e < 32; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);   // a row that is not finite has no result whatever its scale
+        return most;
+      };
+      auto split = [&](const float (&x)[32]) {
         const float by = s.scale < 0.0f ? -sq : sq;   // a negative scale goes into Q, so that larger products are larger scores
-        uint32_t y[32];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) split_f16(x[e] * by, x[e + 1] * by, y[e >> 1], y[16 + (e >> 1)]);
-        if (h == 0 && count > 0) { ok = ok && hold(q_free, (count - 1) & 1); tc_fence_after(); }
-        tmem_st32(q_addr + h * 32, y);
       };
-      fetch(0, x);
-#pragma unroll 1
-      for (int h = 0; h < DP / 32; ++h) {
-        if (h + 1 < DP / 32) fetch(h + 1, next);
-        emit(h);
+      load(0, x);
+      top = largest_of(x);
+      plane_scale(top, sq, iq);
+      sq *= 0x1p-6f; iq *= 0x1p6f;
+      split(x);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = next[e];
+      for (int e = 0; e < 8; ++e) stash[e * 128 + row] = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+      load(32, x);
+      top = max(top, largest_of(x));
+      split(x);
+      if (DP > 64) load(64, x);
+      if (count > 0) { ok = ok && hold(q_free, (count - 1) & 1); tc_fence_after(); }
+      tmem_st32(q_addr + 32, y);
+      float next[32];
+      if (DP > 64) load(96, next);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { const uint4 v = stash[e * 128 + row]; y[4 * e] = v.x; y[4 * e + 1] = v.y; y[4 * e + 2] = v.z; y[4 * e + 3] = v.w; }
+      tmem_st32(q_addr, y);
+      if (DP > 64) {
+        top = max(top, largest_of(x));
+        split(x);
+        tmem_st32(q_addr + 64, y);
+        top = max(top, largest_of(next));
+        split(next);
+        tmem_st32(q_addr + 96, y);
       }
       const float largest = __uint_as_float(top) * sq;
       const bool again = top != 0 && !(largest >= 0x1p7f && largest < 0x1p15f);
       if (__any_sync(0xffffffffu, again)) {
         if (again) plane_scale(top, sq, iq);
-        top = 0xffffffffu;
 #pragma unroll 1
-        for (int h = 0; h < DP / 32; ++h) { fetch(h, x); emit(h); }
+        for (int h = 0; h < DP / 32; ++h) { load(h * 32, x); split(x); tmem_st32(q_addr + h * 32, y); }
       }
       float sk, ik;
       plane_scale(p.pk.amax[it.plane * 2], sk, ik);
@@ -640,7 +651,7 @@ int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStre
 
 template <int DP, bool PAGED>
 int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t st) {
-  constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 1024;
+  constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 16384 + 1024;
   GN_TRY(stream_pack_keys(s, f.pk, nullptr, st));
   static std::atomic<uint64_t> ready{0};
   GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(stream_tc_forward_kernel<DP, PAGED>), kSmem, kThreads, 512 * kRegsSoftmax + 128 * (kRegsFetch + kRegsOther)));
