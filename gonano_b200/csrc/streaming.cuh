@@ -21,7 +21,7 @@ struct FastDiv {
 // The rows (sequences) of a call, padded batch or paged cache, as the kernels see them.
 struct StreamRows {
   int rows = 0, Hq = 0, Hkv = 0, G = 0, D = 0, window = -1, sinks = 0;
-  FastDiv by_G;
+  FastDiv by_G, by_page;
   float scale = 1.0f;
   gn_view q{}, k{}, v{};            // k, v: padded batch
   // padded batch: `seq` tokens a row, lengths nullable
@@ -59,9 +59,9 @@ __device__ __forceinline__ RowSpan row_span(const StreamRows& s, int r) {
 template <bool PAGED>
 __device__ __forceinline__ int64_t key_offset(const StreamRows& s, const gn_view& view, int r, int hk, int j) {
   if (!PAGED) return (int64_t)r * view.batch_stride + (int64_t)hk * view.head_stride + (int64_t)j * view.token_stride;
-  const int page = s.table[(int64_t)r * s.width + j / s.page_size];
+  const int at = s.by_page.of(j), page = s.table[(int64_t)r * s.width + at];
   if ((unsigned)page >= (unsigned)s.pages) return -1;
-  return (((int64_t)page * s.Hkv + hk) * s.page_size + j % s.page_size) * s.D;
+  return (((int64_t)page * s.Hkv + hk) * s.page_size + j - at * s.page_size) * s.D;
 }
 template <bool PAGED>
 __device__ __forceinline__ int64_t token_offset(const gn_view& view, int r, int h, int token) {

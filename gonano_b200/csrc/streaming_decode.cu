@@ -91,10 +91,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) stream_decode_ke
   auto locate = [&](int c) {
     if (lane >= kTile || c + lane >= c1) return -1;
     const int key = key_of(rg, c + lane);
-    const int page = s.table[(int64_t)r * s.width + key / s.page_size];
+    const int at = s.by_page.of(key), page = s.table[(int64_t)r * s.width + at];
     if ((unsigned)page >= (unsigned)s.pages) return -1;
     if (p.nk.data && key >= first) return -2 - (key - first);
-    return (page * s.Hkv + hk) * s.page_size + key % s.page_size;
+    return (page * s.Hkv + hk) * s.page_size + key - at * s.page_size;
   };
   auto row_of = [&](int slot, const float* pages, const gn_view& fresh) -> const float* {
     if (slot >= 0) return pages + (int64_t)slot * s.D;

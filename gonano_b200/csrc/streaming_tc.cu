@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) stream_amax_kernel(const __grid_constant_
   const int hk = blockIdx.y, r = blockIdx.z >> 1, value = blockIdx.z & 1, half = threadIdx.x >> 4;
   const RowSpan sp = row_span<PAGED>(s, r);
   const int begin = first_needed<PAGED>(s, sp), j0 = blockIdx.x * kPackRows;
-  if (j0 >= sp.ctx) return;
+  if (j0 >= sp.ctx || (j0 + kPackRows <= begin && j0 >= s.sinks)) return;
   uint32_t top = 0;
 #pragma unroll 4
   for (int u = 0; u < kPackRows / 16; ++u) {
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
   const int begin = first_needed<PAGED>(s, sp), j0 = blockIdx.x * kPackRows;
   const Packed& dst = value ? pk.v : pk.k;
   const int last = min(dst.rows, (sp.ctx + 15) / 16 * 16 + 16);   // zero rows behind the sequence: a tile is copied in 16s
-  if (j0 >= last) return;
+  if (j0 >= last || (!whole && j0 + kPackRows <= begin && j0 >= s.sinks)) return;   // nothing that anyone sees
   const int64_t plane = (int64_t)r * s.Hkv + hk;
   __shared__ uint32_t most;
   __shared__ int any_odd;
@@ -183,7 +183,11 @@ template <bool PAGED>
 __device__ __forceinline__ Item get_item(const ForwardTc& p, int w) {
   const StreamRows& s = p.s;
   Item it;
-  const int level = p.by_planes.of(w), plane = w - level * p.planes, last = p.by_splits.of(level);   // the last tiles first: under a causal mask they are the longest
+  // the last tiles first: under a causal mask they are the longest.  Planes are turned by one from level to level, or a number of them
+  // that divides the grid's would leave each to the same few CTAs
+  const int level = p.by_planes.of(w), last = p.by_splits.of(level);
+  int plane = w - level * p.planes + level - p.by_planes.of(level) * p.planes;
+  if (plane >= p.planes) plane -= p.planes;
   it.plane = plane;
   it.split = level - last * p.splits; it.tile = p.tiles - 1 - last;
   it.r = p.by_Hkv.of(plane); it.hk = plane - it.r * s.Hkv;
@@ -605,12 +609,14 @@ Plan plan_forward(const StreamRows& s) {
   pl.max_q = s.paged() ? s.max_query : s.seq;
   pl.max_k = s.paged() ? s.max_context : s.seq;
   pl.tiles = ceil_div(pl.max_q * s.G, kRowsT);
-  // Splitting the keys of a tile: only while there are fewer CTAs than SMs, and no finer than four key tiles a CTA (a split
-  // repeats the conversion of Q and adds a pass over the partial results).
+  // Splitting the keys of a tile.  With fewer CTAs than SMs down to four key tiles a part (a part converts Q anew and adds a pass over
+  // the partial results); long key ranges also until there are four parts an SM, so that rows of unequal chunks even out
+  // (4 chunks of 512, 0, ... tokens over 8704 keys: 184 us in one part, DESIGN's table has what it is now), down to eight tiles.
   int64_t seen = pl.max_k;
   if (s.window >= 0) seen = std::min<int64_t>(seen, (int64_t)s.window + s.sinks + kRowsT / s.G + 1);
-  const int64_t ctas = pl.planes * pl.tiles;
-  pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({148 / std::max<int64_t>(ctas, 1), ceil_div(seen, 4 * kRowsT), 64}));
+  const int64_t ctas = std::max<int64_t>(1, pl.planes * pl.tiles);
+  const int64_t few = std::min<int64_t>(148 / ctas, ceil_div(seen, 4 * kRowsT)), even = std::min<int64_t>(ceil_div(4 * 148, ctas), seen / (8 * kRowsT));
+  pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(few, even), 64));
   return pl;
 }
 int64_t carve_forward(const StreamRows& s, const Plan& pl, void* workspace, ForwardTc* f) {
