@@ -213,7 +213,7 @@ __device__ __forceinline__ Item get_item(const ForwardTc& p, int w) {
 //   warp 21     copies K and V tiles (bulk copies of packed rows) through a ring of tile buffers.
 // Tensor memory: two score / weight buffers of 128 columns, O 128, Q hi and lo 128.  Code is kept short: warps that run through
 // long unrolled code once a tile wait for instructions most of the time.  Sixteen warps, because eight took 3360 cycles a tile
-// (read 530, meet 250, weights 1650, O 850) against the 3072 = 48 x 64 of the tensor pipe, which is the bound.  Every wait is
+// (read 530, meet 250, weights 1650, O 850) against the 48 instructions of 64 cycles of the tensor pipe, which is the bound of a tile.  Every wait is
 // bounded; a kernel whose wait ran out writes NaN.
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __grid_constant__ ForwardTc p) {
@@ -229,13 +229,17 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
   auto empty = [&](int i) { return bars + 48u + 8u * i; };
   auto s_full = [&](int i) { return bars + 96u + 8u * i; };
   auto p_full = [&](int i) { return bars + 112u + 8u * i; };
-  const uint32_t o_full = bars + 128, o_empty = bars + 136, q_ready = bars + 144, q_free = bars + 152, tmem_slot = bars + 160;
+  const uint32_t o_full = bars + 128, o_empty = bars + 136, q_free = bars + 152, tmem_slot = bars + 160;
   auto s_free = [&](int i) { return bars + 168u + 8u * i; };
+  // Items' Q by turns on four barriers: with items of one key tile the fetcher gets two items ahead of a softmax thread that still stores
+  // an earlier result, and a barrier that is two phases on looks like one that has not moved
+  auto q_ready = [&](uint32_t item) { return bars + 184u + 8u * (item & 3); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(s_full(i), 1); mbar_init(p_full(i), 512); mbar_init(s_free(i), 1); }
-    mbar_init(o_full, 1); mbar_init(o_empty, 512); mbar_init(q_ready, 128); mbar_init(q_free, 1);
+    mbar_init(o_full, 1); mbar_init(o_empty, 512); mbar_init(q_free, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(q_ready(i), 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 20) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         w += gridDim.x;
         if (w < items) it = get_item<PAGED>(p, w);   // the next item's geometry is on its way while this one runs
         if (n == 0) continue;
-        if (!products) ok = hold(q_ready, count & 1);
+        if (!products) ok = hold(q_ready(count), (count >> 2) & 1);
         for (int j = 0; j < n && ok; ++j, ++tile) {
           const int rows = j + 1 == n ? last16 : kRowsT, b = tile & 1;
           const uint32_t m = ring + (products ? min(2 * j + 2, 2 * n - 1) : j == 0 ? 0 : 2 * j - 1), slot = m % RING;
@@ -414,10 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       float sk, ik;
       plane_scale(p.pk.amax[it.plane * 2], sk, ik);
       const float c = fmaxf(fabsf(s.scale) * kLog2e * iq * ik, 1e-30f);   // a vanishing scale stays a positive number
-      rowc[(count & 3) * 128 + row] = c;   // four: the fetcher can be three items ahead of the softmax threads
+      rowc[(count & 3) * 128 + row] = c;   // four, as the barriers
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(q_ready);
+      mbar_arrive(q_ready(count));
       ++count;
     }
   } else {
@@ -501,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       const int s_end = live ? max(0, min(s.sinks, pos + 1)) : 0;
       const int lo_key = live ? (s.window < 0 ? 0 : max(0, pos - s.window)) - it.runs.shift : 0, hi_key = live ? pos - it.runs.shift : -1;
       const bool odd_plane = (p.pk.odd[it.plane * 2] | p.pk.odd[it.plane * 2 + 1]) != 0;
-      ok = ok && hold(q_ready, count & 1);
+      ok = ok && hold(q_ready(count), (count >> 2) & 1);
       const float c = rowc[(count & 3) * 128 + row];
       ++count;
       float m_here = -INFINITY, l_here = 0.0f;
@@ -611,7 +615,7 @@ Plan plan_forward(const StreamRows& s) {
   pl.tiles = ceil_div(pl.max_q * s.G, kRowsT);
   // Splitting the keys of a tile.  With fewer CTAs than SMs down to four key tiles a part (a part converts Q anew and adds a pass over
   // the partial results); long key ranges also until there are four parts an SM, so that rows of unequal chunks even out
-  // (4 chunks of 512, 0, ... tokens over 8704 keys: 184 us in one part, DESIGN's table has what it is now), down to eight tiles.
+  // (4 chunks of 512, 0, ... tokens over 8704 keys: 184 us in one part each, 168 in up to five), down to eight tiles.
   int64_t seen = pl.max_k;
   if (s.window >= 0) seen = std::min<int64_t>(seen, (int64_t)s.window + s.sinks + kRowsT / s.G + 1);
   const int64_t ctas = std::max<int64_t>(1, pl.planes * pl.tiles);

@@ -221,6 +221,34 @@ def test_extreme_magnitudes():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("B", [37, 77, 113])
+def test_many_short_sequences_with_slow_stores(B, D):
+    """Two to six pieces of one key tile for every SM, whose queries are at hand long before the last results are stored (a word at a time)."""
+    H, Hkv, T = 8, 2, 106
+    q, k, v, _ = tensors(B, H, Hkv, T, D)
+    store = torch.empty(B, H, T, D + 1, device=DEVICE)
+    got = [torch.zeros(1, device=DEVICE)]
+    for window, sinks in [(0, 0), (20, 1)]:
+        out, lse = streaming.sink_attention_forward(q, k, v, sinks, window, 0.25, out=store[..., :D])
+        at = torch.arange(T, device=DEVICE)
+        see = visible(at, at, window, sinks)
+        for b in (0, B // 2, B - 1):
+            for h in range(Hkv):
+                mine = slice(h * 4, h * 4 + 4)
+                qq, kk, vv = (x.double() for x in (q[b, mine], k[b, h], v[b, h]))
+                want, wlse, w = attend64(qq, kk, vv, see, 0.25)
+                e = 2 * score_bound(qq, kk, 0.25)
+                close(out[b, mine], want, (e + PRODUCT) * torch.einsum("gnm,md->gnd", w, vv.abs()) + FLOOR * (see.double() @ vv.abs() + 2 * float(vv.abs().max())), "out")
+                close(lse[b, mine], wlse, (e + PRODUCT) * (1 + wlse.abs()), "lse")
+        first = out.clone()
+        for _ in range(50):
+            streaming.sink_attention_forward(q, k, v, sinks, window, 0.25, out=store[..., :D])
+            got.append((out != first).sum())
+    assert int(torch.stack([x.reshape(()).float() for x in got]).sum()) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 @pytest.mark.parametrize("which", ["k", "v"])
 def test_non_finite_key_reaches_only_its_queries(value, which):
