@@ -46,11 +46,12 @@ __device__ __forceinline__ bool load_key(const StreamRows& s, bool value, bool v
   return true;
 }
 
-constexpr int kWholePlane = 160; // planes up to here are one CTA's
 constexpr int kPackRows = 128;   // keys of a CTA (256 threads, 16 half warps, 8 keys each)
 
 template <int CB, bool PAGED>
 __global__ void __launch_bounds__(256) stream_amax_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, int vec) {
+  pdl_trigger();
+  pdl_wait();
   const int hk = blockIdx.y, r = blockIdx.z >> 1, value = blockIdx.z & 1, half = threadIdx.x >> 4;
   const RowSpan sp = row_span<PAGED>(s, r);
   const int begin = first_needed<PAGED>(s, sp), j0 = blockIdx.x * kPackRows;
@@ -69,43 +70,48 @@ __global__ void __launch_bounds__(256) stream_amax_kernel(const __grid_constant_
   if ((threadIdx.x & 31) == 0 && top) atomicMax(pk.amax + ((int64_t)r * s.Hkv + hk) * 2 + value, top);   // a maximum does not depend on the order
 }
 
-// With whole = 1 a CTA takes a whole plane and finds its largest magnitude itself (short sequences: one launch instead of three).
+// With whole = 1 a plane is a cluster's (its CTAs take 16 keys in turn), which finds the largest magnitude itself.
 template <int CB, bool PAGED>
 __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, uint32_t* norms, int vec, int whole) {
+  pdl_trigger();
+  pdl_wait();
   const int hk = blockIdx.y, r = blockIdx.z >> 1, value = blockIdx.z & 1, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const RowSpan sp = row_span<PAGED>(s, r);
-  const int begin = first_needed<PAGED>(s, sp), j0 = blockIdx.x * kPackRows;
+  const int ctas = gridDim.x, step = whole ? 16 * ctas : 16;
+  const int begin = first_needed<PAGED>(s, sp), j0 = blockIdx.x * (whole ? 16 : kPackRows);
   const Packed& dst = value ? pk.v : pk.k;
   const int last = min(dst.rows, (sp.ctx + 15) / 16 * 16 + 16);   // zero rows behind the sequence: a tile is copied in 16s
-  if (j0 >= last || (!whole && j0 + kPackRows <= begin && j0 >= s.sinks)) return;   // nothing that anyone sees
+  if (!whole && (j0 >= last || (j0 + kPackRows <= begin && j0 >= s.sinks))) return;   // nothing that anyone sees
   const int64_t plane = (int64_t)r * s.Hkv + hk;
-  __shared__ uint32_t most;
-  __shared__ int any_odd;
+  __shared__ uint32_t found[3];   // of this CTA's rows: largest magnitude, whether one is odd, largest norm
+  uint32_t largest;
   if (whole) {
-    if (threadIdx.x == 0) { most = 0; any_odd = 0; }
+    if (threadIdx.x < 3) found[threadIdx.x] = 0;
     __syncthreads();
     uint32_t top = 0;
 #pragma unroll 4
-    for (int j = half; j < sp.ctx; j += 16) {
+    for (int j = j0 + half; j < sp.ctx; j += step) {
       if (!is_needed<PAGED>(s, sp, begin, j)) continue;
       float x[4 * CB];
       load_key<CB, PAGED>(s, value, vec, r, hk, j, x);
 #pragma unroll
       for (int e = 0; e < 4 * CB; ++e) if (finite_bits(x[e])) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
     }
-    if (top) atomicMax(&most, top);
-    __syncthreads();
-    if (threadIdx.x == 0) pk.amax[plane * 2 + value] = most;
+    if (top) atomicMax(&found[0], top);
+    cluster_meet();
+    largest = cluster_largest(&found[0], ctas);
+  } else {
+    largest = pk.amax[plane * 2 + value];
   }
   uint8_t* base = dst.data + plane * dst.plane_bytes(CB);
   uint8_t* flags = (value ? pk.flags_v : pk.flags_k) + plane * dst.rows;
   float sc, inv;
-  plane_scale(whole ? most : pk.amax[plane * 2 + value], sc, inv);
+  plane_scale(largest, sc, inv);
   float top = 0.0f;
-  const int steps = whole ? (last + 15) / 16 : kPackRows / 16;
+  const int end = whole ? last : min(last, j0 + kPackRows);
 #pragma unroll 4
-  for (int u = 0; u < steps; ++u) {
-    const int j = j0 + u * 16 + half;
+  for (int j16 = j0; j16 < end; j16 += step) {
+    const int j = j16 + half;
     float x[4 * CB];
 #pragma unroll
     for (int e = 0; e < 4 * CB; ++e) x[e] = 0.0f;
@@ -125,7 +131,7 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
       for (int d = 8; d > 0; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
       top = fmaxf(top, sq);
     }
-    if (j >= last || (!needed && j < sp.ctx)) continue;
+    if (!needed && j < sp.ctx) continue;
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
       uint2 hi, lo;
@@ -137,21 +143,23 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
     }
     if (l16 == 0) {
       flags[j] = flag;
-      if (flag) { if (whole) any_odd = 1; else pk.odd[plane * 2 + value] = 1; }
+      if (flag) { if (whole) found[1] = 1; else pk.odd[plane * 2 + value] = 1; }
     }
-  }
-  if (whole) {
-    __syncthreads();
-    if (threadIdx.x == 0) { pk.odd[plane * 2 + value] = any_odd; most = 0; }
-    __syncthreads();
   }
   if (norms && value) {
     top = warp_max(top);
-    if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &most : norms + plane * 2, __float_as_uint(top));
-    if (whole) {
-      __syncthreads();
-      if (threadIdx.x == 0) norms[plane * 2] = most;
+    if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &found[2] : norms + plane * 2, __float_as_uint(top));
+  }
+  if (whole) {
+    cluster_meet();
+    if (blockIdx.x == 0 && threadIdx.x < 32) {
+      const uint32_t odd = cluster_largest(&found[1], ctas), norm = cluster_largest(&found[2], ctas);
+      if (threadIdx.x == 0) {
+        pk.amax[plane * 2 + value] = largest; pk.odd[plane * 2 + value] = odd;
+        if (norms && value) norms[plane * 2] = norm;
+      }
     }
+    cluster_meet();   // no CTA goes while its words are read
   }
 }
 
@@ -243,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 20) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  pdl_trigger();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -255,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       // ------------------------------------------------------------- copies: K_0, K_1, V_0, K_2, V_1, ... as they are used
       bool ok = true;
       int slot = 0; uint32_t turn = 0;
+      pdl_wait();   // for the packed planes; the fetching warps wait later, for they read the caller's queries first
       for (int w = blockIdx.x; w < items && ok; w += gridDim.x) {
         const Item it = get_item<PAGED>(p, w);
         for (int m = 0; m < 2 * it.n && ok; ++m) {
@@ -416,6 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         for (int h = 0; h < DP / 32; ++h) { load(h * 32, x); split(x); tmem_st32(q_addr + h * 32, y); }
       }
       float sk, ik;
+      if (count == 0) pdl_wait();
       plane_scale(p.pk.amax[it.plane * 2], sk, ik);
       const float c = fmaxf(fabsf(s.scale) * kLog2e * iq * ik, 1e-30f);   // a vanishing scale stays a positive number
       rowc[(count & 3) * 128 + row] = c;   // four, as the barriers
@@ -427,6 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
   } else {
     // --------------------------------------------------------------- softmax threads
     regs_inc<kRegsSoftmax>();
+    pdl_wait();
     const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;   // a warp reaches the tensor-memory lanes [32 * (warp % 4), +32)
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     float* xch = reinterpret_cast<float*>(gen + XCH);   // [2][4 parts][128] maxima, then [4 parts][128] sums
@@ -578,6 +590,8 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
 // Joins the key splits of a row: a warp per query row.
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(256) stream_tc_combine_kernel(const __grid_constant__ ForwardTc p) {
+  pdl_trigger();
+  pdl_wait();
   const StreamRows& s = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y, r = blockIdx.z, f = blockIdx.x * 8 + warp;
   const RowSpan sp = row_span<PAGED>(s, r);
@@ -646,33 +660,30 @@ bool vec_keys(const StreamRows& s) {
 }
 
 template <int CB, bool PAGED>
-int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t st) {
-  const int vec = vec_keys(s), keys = pk.k.rows, whole = keys <= kWholePlane;
-  if (!whole) {
+int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dependent, cudaStream_t st) {
+  const int vec = vec_keys(s), keys = pk.k.rows, ctas = pack_cluster(keys, 2ll * s.rows * s.Hkv);
+  if (ctas) {
+    GN_CUDA(launch_cluster(stream_pack_kernel<CB, PAGED>, dim3(ctas, s.Hkv, 2 * s.rows), 256, ctas, dependent, st, s, pk, norms, vec, 1));
+  } else {
     GN_CUDA(cudaMemsetAsync(pk.amax, 0, (int64_t)s.rows * s.Hkv * 4 * sizeof(uint32_t), st));   // amax and odd
     if (norms) GN_CUDA(cudaMemsetAsync(norms, 0, (int64_t)s.rows * s.Hkv * 2 * sizeof(uint32_t), st));
     stream_amax_kernel<CB, PAGED><<<dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, vec);
     GN_LAUNCH_CHECK();
+    GN_CUDA(launch_pdl(stream_pack_kernel<CB, PAGED>, dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), dim3(256), 0, st, s, pk, norms, vec, 0));
   }
-  stream_pack_kernel<CB, PAGED><<<dim3(whole ? 1 : ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, norms, vec, whole);
-  GN_LAUNCH_CHECK();
   return GN_OK;
 }
 
 template <int DP, bool PAGED>
-int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t st) {
+int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, bool dependent, cudaStream_t st) {
   constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 16384 + 1024;
-  GN_TRY(stream_pack_keys(s, f.pk, nullptr, st));
+  GN_TRY(stream_pack_keys(s, f.pk, nullptr, dependent, st));
   static std::atomic<uint64_t> ready{0};
   GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(stream_tc_forward_kernel<DP, PAGED>), kSmem, kThreads, 512 * kRegsSoftmax + 128 * (kRegsFetch + kRegsOther)));
   const int64_t items = pl.planes * pl.tiles * pl.splits;
   GN_REQUIRE(items < (1ll << 31) - 1024, "attention: %lld tiles of query rows", (long long)items);
-  stream_tc_forward_kernel<DP, PAGED><<<(unsigned)std::min<int64_t>(items, num_sms()), kThreads, kSmem, st>>>(f);
-  GN_LAUNCH_CHECK();
-  if (pl.splits > 1) {
-    stream_tc_combine_kernel<DP, PAGED><<<dim3(ceil_div(pl.max_q * s.G, 8), s.Hkv, s.rows), 256, 0, st>>>(f);
-    GN_LAUNCH_CHECK();
-  }
+  GN_CUDA(launch_pdl(stream_tc_forward_kernel<DP, PAGED>, dim3((unsigned)std::min<int64_t>(items, num_sms())), dim3(kThreads), kSmem, st, f));
+  if (pl.splits > 1) GN_CUDA(launch_pdl(stream_tc_combine_kernel<DP, PAGED>, dim3(ceil_div(pl.max_q * s.G, 8), s.Hkv, s.rows), dim3(256), 0, st, f));
   return GN_OK;
 }
 
@@ -694,16 +705,16 @@ int prepare_kernel(std::atomic<uint64_t>& ready, const void* kernel, int smem, i
   return GN_OK;
 }
 
-int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t st) {
-  if (s.D <= 64) return s.paged() ? pack_go<1, true>(s, pk, norms, st) : pack_go<1, false>(s, pk, norms, st);
-  return s.paged() ? pack_go<2, true>(s, pk, norms, st) : pack_go<2, false>(s, pk, norms, st);
+int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dependent, cudaStream_t st) {
+  if (s.D <= 64) return s.paged() ? pack_go<1, true>(s, pk, norms, dependent, st) : pack_go<1, false>(s, pk, norms, dependent, st);
+  return s.paged() ? pack_go<2, true>(s, pk, norms, dependent, st) : pack_go<2, false>(s, pk, norms, dependent, st);
 }
 
 int64_t stream_tc_forward_bytes(const StreamRows& s) {
   ForwardTc f{};
   return carve_forward(s, plan_forward(s), nullptr, &f);
 }
-int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t st, PackedKeys* packed) {
+int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, bool dependent, cudaStream_t st, PackedKeys* packed) {
   const Plan pl = plan_forward(s);
   ForwardTc f{};
   f.s = s; f.out = out; f.lse = lse; f.tiles = pl.tiles; f.splits = pl.splits; f.planes = (int)pl.planes;
@@ -711,8 +722,8 @@ int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void*
   carve_forward(s, pl, workspace, &f);
   if (packed) *packed = f.pk;
   f.vec_q = vec_view(s.q, s.D); f.vec_out = pl.splits > 1 || vec_view(out, s.D);
-  if (pl.DP == 64) return s.paged() ? forward_go<64, true>(s, pl, f, st) : forward_go<64, false>(s, pl, f, st);
-  return s.paged() ? forward_go<128, true>(s, pl, f, st) : forward_go<128, false>(s, pl, f, st);
+  if (pl.DP == 64) return s.paged() ? forward_go<64, true>(s, pl, f, dependent, st) : forward_go<64, false>(s, pl, f, dependent, st);
+  return s.paged() ? forward_go<128, true>(s, pl, f, dependent, st) : forward_go<128, false>(s, pl, f, dependent, st);
 }
 
 }  // namespace gn

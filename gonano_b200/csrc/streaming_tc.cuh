@@ -57,11 +57,34 @@ static inline bool vec_view(const gn_view& v, int D) {
 }
 // Packs keys and values; amax and the 2 * planes words of odd stand in one piece.  norms: null, or [plane][2]: [0] receives the bits of the
 // largest squared norm of a scaled value row.
-int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t stream);
+// CTAs of a cluster that packs a plane of `rows` rows and finds its largest magnitude on the way (0: a launch of its own finds it).
+// A CTA has 64 rows or more, and the second reading of a row comes from a cache.  Long planes of which there are few leave SMs idle that way.
+static inline int pack_cluster(int64_t rows, int64_t planes) {
+  int ctas = 1;
+  while (ctas < 8 && rows >= 128 * ctas) ctas *= 2;
+  return rows <= 1280 || planes * ctas >= 296 ? ctas : 0;
+}
+// `dependent`: as launch_pdl.  Every kernel of a call but its first is launched so: it sets up while the one before runs, and each of its
+// CTAs waits for that one to be complete before it ends (and before it reads what that one writes), so that complete means complete
+// with all before it.  A call's first kernel waits for the stream as usual; what the caller passed in is there from then on.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, int ctas, bool dependent, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = dependent ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+// `dependent`: a kernel of the same call stands before it.
+int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dependent, cudaStream_t stream);
 
 // tcgen05 forward of a call (streaming_tc.cu): the workspace it wants, and the launches.
 int64_t stream_tc_forward_bytes(const StreamRows& s);
-int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t stream, PackedKeys* packed = nullptr);
+int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, bool dependent, cudaStream_t stream, PackedKeys* packed = nullptr);
 // The weights of a paged call's keys (streaming_tc_mass.cu), from the forward's packed keys and its log-sum-exps.
 int64_t stream_tc_mass_bytes(const StreamRows& s);
 int stream_tc_mass(const StreamRows& s, const PackedKeys& pk, const float* lse, const float* mass, float* mass_out, void* workspace, cudaStream_t stream);
@@ -151,6 +174,18 @@ __device__ __forceinline__ void transpose_blocks(float (&x)[4 * N]) {
       }
     }
   }
+}
+// All threads of the cluster's CTAs meet; what each wrote to shared memory before is seen by the others after.
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The largest of the words that the cluster's CTAs hold where this one holds `mine` (shared memory; all of a warp's threads call).
+__device__ __forceinline__ uint32_t cluster_largest(const uint32_t* mine, int ctas) {
+  uint32_t x = 0;
+  const int lane = threadIdx.x & 31;
+  if (lane < ctas)
+    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %1, %2;\n\tld.shared::cluster.u32 %0, [at];\n\t}" : "=r"(x) : "r"(smem_u32(mine)), "r"(lane) : "memory");
+  return __reduce_max_sync(0xffffffffu, x);
 }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u; }

@@ -31,7 +31,6 @@ struct BackwardTc {
   float* part;                   // [plane][unit][dV, dK][128][DP] of key tiles in several parts
 };
 
-constexpr int kWholePlaneQ = 256;   // planes up to here are one CTA's
 constexpr int kAmaxRowsQ = 256;
 constexpr int kPackRowsQ = 64;   // 256 threads, 16 half warps
 
@@ -56,6 +55,8 @@ __device__ __forceinline__ void load_query_row(const StreamRows& s, const gn_vie
 
 template <int CB>
 __global__ void __launch_bounds__(256) stream_query_amax_kernel(const __grid_constant__ BackwardTc p) {
+  pdl_trigger();
+  pdl_wait();
   const StreamRows& s = p.s;
   const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, f0 = blockIdx.x * kAmaxRowsQ;
   const int nf = row_span<false>(s, r).q_len * s.G;
@@ -83,18 +84,22 @@ __global__ void __launch_bounds__(256) stream_query_amax_kernel(const __grid_con
 // Packs q and dO and leaves each row's lse and delta in the form that the kernels use.
 template <int CB>
 __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_constant__ BackwardTc p, int whole) {
+  pdl_trigger();
+  if (!whole) pdl_wait();
   const StreamRows& s = p.s;
-  const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15, f0 = blockIdx.x * kPackRowsQ;
+  const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+  const int ctas = gridDim.x, step = whole ? 16 * ctas : 16, f0 = blockIdx.x * (whole ? 16 : kPackRowsQ);
   const int nf = row_span<false>(s, r).q_len * s.G, last = min(p.q.rows, (nf + 15) / 16 * 16 + 16);
-  if (f0 >= last) return;
+  if (!whole && f0 >= last) return;
   const int64_t plane = (int64_t)r * s.Hkv + hk;
-  __shared__ uint32_t most[2], norm;
-  if (whole) {   // the plane is this CTA's: its largest magnitudes first
-    if (threadIdx.x == 0) most[0] = most[1] = norm = 0;
+  __shared__ uint32_t found[3];   // of this CTA's rows: largest magnitudes of q and dO, largest norm
+  uint32_t largest[2];
+  if (whole) {   // the plane is this cluster's: its largest magnitudes first
+    if (threadIdx.x < 3) found[threadIdx.x] = 0;
     __syncthreads();
     uint32_t top[2] = {0, 0};
 #pragma unroll 4
-    for (int f = half; f < nf; f += 16)
+    for (int f = f0 + half; f < nf; f += step)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         float x[4 * CB];
@@ -103,19 +108,22 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
         for (int e = 0; e < 4 * CB; ++e) if (finite_bits(x[e])) top[w] = max(top[w], __float_as_uint(x[e]) & 0x7fffffffu);
       }
 #pragma unroll
-    for (int w = 0; w < 2; ++w) if (top[w]) atomicMax(&most[w], top[w]);
-    __syncthreads();
-    if (threadIdx.x < 2) p.qamax[plane * 2 + threadIdx.x] = most[threadIdx.x];
+    for (int w = 0; w < 2; ++w) if (top[w]) atomicMax(&found[w], top[w]);
+    cluster_meet();
+    for (int w = 0; w < 2; ++w) largest[w] = cluster_largest(&found[w], ctas);
+    pdl_wait();   // for V's scale; what was read so far is the caller's
+  } else {
+    for (int w = 0; w < 2; ++w) largest[w] = p.qamax[plane * 2 + w];
   }
   float sc[2], inv, sv;
-  plane_scale(whole ? most[0] : p.qamax[plane * 2], sc[0], inv);
-  plane_scale(whole ? most[1] : p.qamax[plane * 2 + 1], sc[1], inv);
+  plane_scale(largest[0], sc[0], inv);
+  plane_scale(largest[1], sc[1], inv);
   plane_scale(p.pk.amax[plane * 2 + 1], sv, inv);
   float top = 0.0f;
-  const int steps = whole ? (last + 15) / 16 : kPackRowsQ / 16;
+  const int end = whole ? last : min(last, f0 + kPackRowsQ);
 #pragma unroll 1
-  for (int u = 0; u < steps; ++u) {
-    const int f = f0 + u * 16 + half;
+  for (int f16 = f0; f16 < end; f16 += step) {
+    const int f = f16 + half;
     float x[2][4 * CB], delta = 0.0f, sq = 0.0f;
     bool odd = false;
 #pragma unroll
@@ -140,7 +148,6 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
     for (int d = 8; d > 0; d >>= 1) { delta += __shfl_xor_sync(0xffffffffu, delta, d); sq += __shfl_xor_sync(0xffffffffu, sq, d); }
     top = fmaxf(top, sq);
     odd = ((__ballot_sync(0xffffffffu, odd) >> (threadIdx.x & 16)) & 0xffffu) != 0;
-    if (f >= last) continue;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const Packed& dst = w ? p.g : p.q;
@@ -162,10 +169,14 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
     }
   }
   top = warp_max(top);
-  if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &norm : p.norms + plane * 2 + 1, __float_as_uint(top));
+  if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &found[2] : p.norms + plane * 2 + 1, __float_as_uint(top));
   if (whole) {
-    __syncthreads();
-    if (threadIdx.x == 0) p.norms[plane * 2 + 1] = norm;
+    cluster_meet();
+    if (blockIdx.x == 0 && threadIdx.x < 32) {
+      const uint32_t norm = cluster_largest(&found[2], ctas);
+      if (threadIdx.x == 0) { p.qamax[plane * 2] = largest[0]; p.qamax[plane * 2 + 1] = largest[1]; p.norms[plane * 2 + 1] = norm; }
+    }
+    cluster_meet();   // no CTA goes while its words are read
   }
 }
 
@@ -265,7 +276,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   const int parts = sink ? p.parts_sink : p.parts, y0 = sink ? x0 : x0 - p.sink_tiles * p.parts_sink;
   const int kt = (sink ? 0 : p.sink_tiles) + y0 / parts, part_i = y0 % parts, k0 = kt * 128;
   const int len = row_span<false>(s, r).ctx;
-  if (k0 >= len && parts > 1) return;   // the summing kernel does not look at padding
+  if (k0 >= len && parts > 1) { pdl_wait(); return; }   // the summing kernel does not look at padding
   const int nf = len * s.G;
   const int64_t t_end = (s.window < 0 || k0 < s.sinks) ? len : min((int64_t)len, (int64_t)k0 + 128 + s.window);
   const int f_begin = (k0 * s.G) & ~7, f_end = (int)t_end * s.G;
@@ -299,6 +310,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 176);
+  pdl_wait();
+  pdl_trigger();   // not before: the dQ kernel starts without a wait
   auto row0 = [&](int i) { return f_begin + (i0 + i) * 64; };
   auto rows16 = [&](int i) { return min(64, (f_end - row0(i) + 15) & ~15); };
 
@@ -516,6 +529,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
 // Sums the parts of key tiles that were divided, in their order: DP / 4 threads per key row and tensor.
 template <int DP>
 __global__ void __launch_bounds__(256) stream_tc_dkv_sum_kernel(const __grid_constant__ BackwardTc p) {
+  pdl_wait();
   constexpr int LANES = DP / 4;
   const StreamRows& s = p.s;
   const int hk = blockIdx.y, r = blockIdx.z >> 1, which = blockIdx.z & 1, key = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, ch = threadIdx.x % LANES * 4;
@@ -549,6 +563,8 @@ __global__ void __launch_bounds__(256) stream_tc_dkv_sum_kernel(const __grid_con
 
 // dQ.  One CTA per (128 query rows, kv head, sequence): S = Q K^T and dP = dO V^T of 64 keys a step, dS in place of dP, dQ += dS K with
 // dS from tensor memory and the same K tile read the other way.  Threads, issuing warps and the rounding of sums as above.
+// It needs nothing from the dK and dV kernel, which stands before it on the stream: its CTAs fill the SMs that that one's last CTAs leave
+// free.  (They start once every CTA there has seen the packing kernels complete, and end after it has ended.)
 // Tensor memory: Q hi 64 columns, dO hi 64, S 2 x 64, dP 2 x 64, dQ 128.  Shared memory: Q lo, dO lo 32 KB each, 3 K and 2 V tiles of 32 KB.
 template <int DP>
 __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid_constant__ BackwardTc p) {
@@ -582,6 +598,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     for (int i = 0; i < 2; ++i) { mbar_init(v_full(i), 1); mbar_init(v_empty(i), 1); mbar_init(sp_full(i), 1); mbar_init(ds_full(i), 512); mbar_init(ds_free(i), 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  pdl_trigger();
   if (warp == 16) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
@@ -749,6 +766,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   if (warp == 16) tmem_dealloc(tmem, 512);
+  pdl_wait();
 }
 
 // ------------------------------------------------------------------ host
@@ -802,24 +820,21 @@ int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
   GN_TRY(prepare_kernel(ready_kv, reinterpret_cast<const void*>(stream_tc_dkv_kernel<DP>), kSmemKv, kThreadsB, kShared));
   GN_TRY(prepare_kernel(ready_q, reinterpret_cast<const void*>(stream_tc_dq_kernel<DP>), kSmemQ, kThreadsB, kShared));
   const int64_t planes = (int64_t)s.rows * s.Hkv;
-  GN_TRY(stream_pack_keys(s, b.pk, b.norms, st));
-  const int whole = b.q.rows <= kWholePlaneQ;
-  if (!whole) {
+  GN_TRY(stream_pack_keys(s, b.pk, b.norms, false, st));
+  const int ctas = pack_cluster(b.q.rows, planes);
+  if (ctas) {
+    GN_CUDA(launch_cluster(stream_query_pack_kernel<CB>, dim3(ctas, s.Hkv, s.rows), 256, ctas, true, st, b, 1));
+  } else {
     GN_CUDA(cudaMemsetAsync(b.qamax, 0, planes * 2 * sizeof(uint32_t), st));
     GN_CUDA(cudaMemset2DAsync(b.norms + 1, 2 * sizeof(uint32_t), 0, sizeof(uint32_t), planes, st));
     stream_query_amax_kernel<CB><<<dim3(ceil_div(b.q.rows, kAmaxRowsQ), s.Hkv, s.rows), 256, 0, st>>>(b);
     GN_LAUNCH_CHECK();
+    GN_CUDA(launch_pdl(stream_query_pack_kernel<CB>, dim3(ceil_div(b.q.rows, kPackRowsQ), s.Hkv, s.rows), dim3(256), 0, st, b, 0));
   }
-  stream_query_pack_kernel<CB><<<dim3(whole ? 1 : ceil_div(b.q.rows, kPackRowsQ), s.Hkv, s.rows), 256, 0, st>>>(b, whole);
-  GN_LAUNCH_CHECK();
-  stream_tc_dkv_kernel<DP><<<dim3(b.units, s.Hkv, s.rows), kThreadsB, kSmemKv, st>>>(b);
-  GN_LAUNCH_CHECK();
-  if (b.parts > 1 || b.parts_sink > 1) {
-    stream_tc_dkv_sum_kernel<DP><<<dim3(ceil_div(s.seq, 1024 / DP), s.Hkv, 2 * s.rows), 256, 0, st>>>(b);
-    GN_LAUNCH_CHECK();
-  }
-  stream_tc_dq_kernel<DP><<<dim3(b.q_tiles, s.Hkv, s.rows), kThreadsB, kSmemQ, st>>>(b);
-  GN_LAUNCH_CHECK();
+  GN_CUDA(launch_pdl(stream_tc_dkv_kernel<DP>, dim3(b.units, s.Hkv, s.rows), dim3(kThreadsB), kSmemKv, st, b));
+  GN_CUDA(launch_pdl(stream_tc_dq_kernel<DP>, dim3(b.q_tiles, s.Hkv, s.rows), dim3(kThreadsB), kSmemQ, st, b));
+  if (b.parts > 1 || b.parts_sink > 1)
+    GN_CUDA(launch_pdl(stream_tc_dkv_sum_kernel<DP>, dim3(ceil_div(s.seq, 1024 / DP), s.Hkv, 2 * s.rows), dim3(256), 0, st, b));
   return GN_OK;
 }
 
