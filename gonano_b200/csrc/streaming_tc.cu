@@ -170,12 +170,13 @@ struct ForwardTc {
   gn_view out;
   float* lse;
   int vec_q, vec_out, tiles, splits;
-  int planes;
+  int planes, listed;   // listed: items are counted over the tiles that exist
   FastDiv by_planes, by_splits, by_Hkv;
   float* part_o; float* part_l;   // splits > 1: [plane][tile][split][128] rows of DP channels, and their log2-sum-exps
 };
 
 constexpr int kRowsT = 128;      // query rows of an item = keys of a tile = UMMA M and N
+constexpr int kRowsListed = 511;
 constexpr int kThreads = 768;    // four softmax warpgroups, one that fetches Q, one with the issuing and the copying warp
 constexpr int kRegsSoftmax = 88, kRegsFetch = 80, kRegsOther = 48;   // shares of the launch's 6 x 80 (the fetching one keeps its)
 
@@ -187,18 +188,32 @@ struct Item {
   KeyRuns runs;
   __device__ __forceinline__ int rows16(int j) const { return min(kRowsT, (runs.total - (j0 + j) * kRowsT + 15) & ~15); }   // keys of tile j, in 16s
 };
+// `before`: of a paged call with few enough rows, how many tiles of new tokens stand before each row's (shared memory).  Its items are
+// counted over these, so that every CTA gets as many that exist.  (Two parts of chunks of 512, 0, 180 and 332 tokens, 8 x 8704 keys: the 128
+// items that exist went to 94 of 148 CTAs when the 256 that could exist were dealt out.)
 template <bool PAGED>
-__device__ __forceinline__ Item get_item(const ForwardTc& p, int w) {
+__device__ __forceinline__ Item get_item(const ForwardTc& p, const int* before, int w) {
   const StreamRows& s = p.s;
   Item it;
-  // the last tiles first: under a causal mask they are the longest.  Planes are turned by one from level to level, or a number of them
-  // that divides the grid's would leave each to the same few CTAs
-  const int level = p.by_planes.of(w), last = p.by_splits.of(level);
-  int plane = w - level * p.planes + level - p.by_planes.of(level) * p.planes;
-  if (plane >= p.planes) plane -= p.planes;
-  it.plane = plane;
-  it.split = level - last * p.splits; it.tile = p.tiles - 1 - last;
-  it.r = p.by_Hkv.of(plane); it.hk = plane - it.r * s.Hkv;
+  if (PAGED && p.listed) {
+    const int c = p.by_splits.of(w), t = p.by_Hkv.of(c);
+    int low = 0, high = s.rows - 1;   // the last row with before[row] <= t
+    while (low < high) {
+      const int mid = (low + high + 1) >> 1;
+      if (before[mid] <= t) low = mid; else high = mid - 1;
+    }
+    it.split = w - c * p.splits; it.hk = c - t * s.Hkv; it.r = low; it.tile = t - before[low];
+    it.plane = (int64_t)low * s.Hkv + it.hk;
+  } else {
+    // the last tiles first: under a causal mask they are the longest.  Planes are turned by one from level to level, or a number of them
+    // that divides the grid's would leave each to the same few CTAs
+    const int level = p.by_planes.of(w), last = p.by_splits.of(level);
+    int plane = w - level * p.planes + level - p.by_planes.of(level) * p.planes;
+    if (plane >= p.planes) plane -= p.planes;
+    it.plane = plane;
+    it.split = level - last * p.splits; it.tile = p.tiles - 1 - last;
+    it.r = p.by_Hkv.of(plane); it.hk = plane - it.r * s.Hkv;
+  }
   const RowSpan sp = row_span<PAGED>(s, it.r);
   it.f0 = it.tile * kRowsT; it.nf = sp.q_len * s.G; it.first = sp.ctx - sp.q_len; it.q_begin = sp.q_begin;
   it.inside = it.f0 < (PAGED ? it.nf : s.seq * s.G);
@@ -226,7 +241,7 @@ __device__ __forceinline__ Item get_item(const ForwardTc& p, int w) {
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __grid_constant__ ForwardTc p) {
   constexpr int CB = DP / 64, QC = DP / 4, RING = DP == 64 ? 6 : 3;
-  constexpr uint32_t TILE = CB * 32768u, BARS = RING * TILE, ROWC = BARS + 256, XCH = ROWC + 2048, STASH = XCH + 6144;
+  constexpr uint32_t TILE = CB * 32768u, BARS = RING * TILE, ROWC = BARS + 256, XCH = ROWC + 2048, STASH = XCH + 6144, BEFORE = STASH + 16384;
   constexpr uint32_t COL_O = 256, COL_Q = 384;
   extern __shared__ uint8_t smem_raw[];
   const StreamRows& s = p.s;
@@ -252,11 +267,28 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
   }
   if (warp == 20) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   pdl_trigger();
+  int* before = reinterpret_cast<int*>(gen + BEFORE);
+  if (PAGED && p.listed) {
+    for (int r = threadIdx.x; r < s.rows; r += kThreads) before[r] = (row_span<PAGED>(s, r).q_len * s.G + kRowsT - 1) / kRowsT;
+    __syncthreads();
+    if (warp == 0) {
+      int sum = 0;
+      for (int r = lane; r - lane < s.rows; r += 32) {
+        const int x = r < s.rows ? before[r] : 0;
+        int y = x;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) { const int z = __shfl_up_sync(0xffffffffu, y, d); if (lane >= d) y += z; }
+        if (r < s.rows) before[r] = sum + y - x;
+        sum += __shfl_sync(0xffffffffu, y, 31);
+      }
+      if (lane == 0) before[s.rows] = sum;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 160);
-  const int items = p.planes * p.tiles * p.splits;
+  const int items = PAGED && p.listed ? before[s.rows] * s.Hkv * p.splits : p.planes * p.tiles * p.splits;
 
   if (warp >= 20) {
     regs_dec<kRegsOther>();
@@ -266,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       int slot = 0; uint32_t turn = 0;
       pdl_wait();   // for the packed planes; the fetching warps wait later, for they read the caller's queries first
       for (int w = blockIdx.x; w < items && ok; w += gridDim.x) {
-        const Item it = get_item<PAGED>(p, w);
+        const Item it = get_item<PAGED>(p, before, w);
         for (int m = 0; m < 2 * it.n && ok; ++m) {
           const bool value = m == 2 * it.n - 1 || (m > 0 && (m & 1) == 0);
           const int j = value ? (m == 2 * it.n - 1 ? it.n - 1 : (m >> 1) - 1) : (m + 1) >> 1;
@@ -295,11 +327,11 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       const bool products = warp == 22;   // O = P V; the other warp S = Q K^T
       bool ok = true;
       uint32_t tile = 0, count = 0, ring = 0;   // tiles, items and copies so far
-      Item it = get_item<PAGED>(p, blockIdx.x);   // the grid is no larger than the number of items
+      Item it = get_item<PAGED>(p, before, blockIdx.x);   // may not exist
       for (int w = blockIdx.x; w < items && ok;) {
         const int n = it.n, last16 = n > 0 ? it.rows16(n - 1) : 0;
         w += gridDim.x;
-        if (w < items) it = get_item<PAGED>(p, w);   // the next item's geometry is on its way while this one runs
+        if (w < items) it = get_item<PAGED>(p, before, w);   // the next item's geometry is on its way while this one runs
         if (n == 0) continue;
         if (!products) ok = hold(q_ready(count), (count >> 2) & 1);
         for (int j = 0; j < n && ok; ++j, ++tile) {
@@ -353,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     bool ok = true;
     uint32_t count = 0;
     for (int w = blockIdx.x; w < items; w += gridDim.x) {
-      const Item it = get_item<PAGED>(p, w);
+      const Item it = get_item<PAGED>(p, before, w);
       if (it.n == 0) continue;
       const int f = it.f0 + row, t = s.by_G.of(f), g = f - t * s.G;
       const bool live = f < it.nf;
@@ -492,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     };
 
     for (int w = blockIdx.x; w < items; w += gridDim.x) {
-      const Item it = get_item<PAGED>(p, w);
+      const Item it = get_item<PAGED>(p, before, w);
       if (!it.inside) continue;
       const int f = it.f0 + row, t = s.by_G.of(f), g = f - t * s.G, token = it.q_begin + t, pos = it.first + t;
       const bool live = f < it.nf;
@@ -627,14 +659,19 @@ Plan plan_forward(const StreamRows& s) {
   pl.max_q = s.paged() ? s.max_query : s.seq;
   pl.max_k = s.paged() ? s.max_context : s.seq;
   pl.tiles = ceil_div(pl.max_q * s.G, kRowsT);
-  // Splitting the keys of a tile.  With fewer CTAs than SMs down to four key tiles a part (a part converts Q anew and adds a pass over
-  // the partial results); long key ranges also until there are four parts an SM, so that rows of unequal chunks even out
-  // (4 chunks of 512, 0, ... tokens over 8704 keys: 184 us in one part each, 168 in up to five), down to eight tiles.
-  int64_t seen = pl.max_k;
+  int64_t seen = pl.max_k, ctas = std::max<int64_t>(1, pl.planes * pl.tiles);
   if (s.window >= 0) seen = std::min<int64_t>(seen, (int64_t)s.window + s.sinks + kRowsT / s.G + 1);
-  const int64_t ctas = std::max<int64_t>(1, pl.planes * pl.tiles);
-  const int64_t few = std::min<int64_t>(148 / ctas, ceil_div(seen, 4 * kRowsT)), even = std::min<int64_t>(ceil_div(4 * 148, ctas), seen / (8 * kRowsT));
-  pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(few, even), 64));
+  if (s.paged()) ctas = std::min(ctas, s.Hkv * (ceil_div((int64_t)s.tokens * s.G, kRowsT) + (int64_t)s.rows));   // no more tiles exist
+  // Parts of a tile's keys: the fewest rounds of 148 items, counted in key tiles with 3.5 for an item's start and end, 2 for the pass that
+  // joins the parts and the partial results' way to memory and back (0.012 a part); no part below four tiles.  In one part and in two:
+  // 12 planes x 49 tiles of 2049 keys 134 and 173 us, 1 x 128 of 2048 58 and 65, 2 x 32 of 1024 40 and 41, 16 x up to 4 of 4000 125 and 106.
+  const double keys = (double)seen / kRowsT;
+  double best = 0.0;
+  pl.splits = 1;
+  for (int parts = 1; parts <= 64 && (parts == 1 || keys / parts >= 4.0); ++parts) {
+    const double cost = (double)((ctas * parts + 147) / 148) * (keys / parts + 3.5) + (parts > 1 ? 2.0 + 0.012 * (double)(ctas * parts) : 0.0);
+    if (parts == 1 || cost < best) { best = cost; pl.splits = parts; }
+  }
   return pl;
 }
 int64_t carve_forward(const StreamRows& s, const Plan& pl, void* workspace, ForwardTc* f) {
@@ -676,7 +713,7 @@ int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dep
 
 template <int DP, bool PAGED>
 int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, bool dependent, cudaStream_t st) {
-  constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 16384 + 1024;
+  constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 16384 + (kRowsListed + 1) * 4 + 1024;
   GN_TRY(stream_pack_keys(s, f.pk, nullptr, dependent, st));
   static std::atomic<uint64_t> ready{0};
   GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(stream_tc_forward_kernel<DP, PAGED>), kSmem, kThreads, 512 * kRegsSoftmax + 128 * (kRegsFetch + kRegsOther)));
@@ -718,6 +755,7 @@ int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void*
   const Plan pl = plan_forward(s);
   ForwardTc f{};
   f.s = s; f.out = out; f.lse = lse; f.tiles = pl.tiles; f.splits = pl.splits; f.planes = (int)pl.planes;
+  f.listed = s.paged() && s.rows <= kRowsListed;
   f.by_planes = FastDiv(pl.planes); f.by_splits = FastDiv(pl.splits); f.by_Hkv = FastDiv(s.Hkv);
   carve_forward(s, pl, workspace, &f);
   if (packed) *packed = f.pk;

@@ -83,6 +83,11 @@ def _workspace(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _like(tensor):
+    # contiguous; half the time of torch.empty with a type and a device
+    return torch.empty_like(tensor, memory_format=torch.contiguous_format)
+
+
 def _address(tensor):
     return tensor.data_ptr() if tensor is not None else None
 
@@ -106,8 +111,8 @@ def sink_attention_forward(q, k, v, sinks, window, scale=1.0, lengths=None, out=
     lib = _lib.load()
     p, device = _sink_params(q, k, v, sinks, window, scale, lengths)
     with _on(device):
-        out = torch.empty(q.shape, dtype=torch.float32, device=device) if out is None else out
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if lse is None else lse
+        out = _like(q) if out is None else out
+        lse = q.new_empty(q.shape[:3]) if lse is None else lse
         _packed("lse", lse, torch.float32, device, q.shape[:3])
         view, nbytes = _view4("out", out, device, q.shape), C.c_int64()
         check(lib.gn_attention_sink_workspace(C.byref(p), 0, C.byref(nbytes)))
@@ -126,7 +131,7 @@ def sink_attention_backward(q, k, v, out, dout, lse, sinks, window, scale=1.0, l
         _refuse("sink_attention_backward: give dq, dk and dv or none of them")
     with _on(device):
         if not given[0]:
-            dq, dk, dv = (torch.empty(x.shape, dtype=torch.float32, device=device) for x in (q, k, v))
+            dq, dk, dv = _like(q), _like(k), _like(v)
         _packed("lse", lse, torch.float32, device, q.shape[:3])
         views = [_view4(n, t, device, like.shape) for n, t, like in (("out", out, q), ("dout", dout, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v))]
         nbytes = C.c_int64()
