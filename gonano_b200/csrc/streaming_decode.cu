@@ -58,6 +58,7 @@ template <int NT, int DP, bool MULTI>
 __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) stream_decode_kernel(const __grid_constant__ Decode p) {
   constexpr int R = 8 * NT, PAIRS = DP / 16, EACH = DP / 8;   // float4s of a K row in a lane; channels of a V row in a lane
   __shared__ __align__(16) float room[kWarps * R * DP];
+  pdl_trigger();
   float (&q_s)[NT][PAIRS][2][32][4] = *reinterpret_cast<float (*)[NT][PAIRS][2][32][4]>(room);   // queries as fragments, hi and lo
   float (&o_s)[kWarps][R][DP] = *reinterpret_cast<float (*)[kWarps][R][DP]>(room);               // at the end, the warps' results
   __shared__ __align__(16) float p_s[kWarps][kTile * R];
@@ -305,6 +306,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) stream_decode_ke
 // A warp per query of a (row, kv head): joins the ranges.
 template <int R, int DP>
 __global__ void __launch_bounds__(128) stream_decode_join_kernel(const __grid_constant__ Decode p) {
+  pdl_trigger();
+  pdl_wait();
   const StreamRows& s = p.s;
   const int q = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, hk = blockIdx.y, r = blockIdx.z;
   const RowSpan sp = row_span<true>(s, r);
@@ -337,6 +340,7 @@ __global__ void __launch_bounds__(128) stream_decode_join_kernel(const __grid_co
 // A thread per key: the weights that this call's queries gave it, from the kept scores and the final log-sum-exps.
 template <int R>
 __global__ void __launch_bounds__(256) stream_decode_mass_kernel(const __grid_constant__ Decode p) {
+  pdl_wait();
   const StreamRows& s = p.s;
   __shared__ float L[R];
   const int key = blockIdx.x * 256 + threadIdx.x, hk = blockIdx.y, r = blockIdx.z;
@@ -389,14 +393,8 @@ int go(const Decode& d, cudaStream_t st) {
   const StreamRows& s = d.s;
   stream_decode_kernel<NT, DP, MULTI><<<dim3(d.splits, s.Hkv, s.rows), 32 * kWarps, 0, st>>>(d);
   GN_LAUNCH_CHECK();
-  if (d.splits > 1) {
-    stream_decode_join_kernel<R, DP><<<dim3(ceil_div(s.max_query * s.G, 4), s.Hkv, s.rows), 128, 0, st>>>(d);
-    GN_LAUNCH_CHECK();
-  }
-  if (d.mass_out && s.max_context) {
-    stream_decode_mass_kernel<R><<<dim3(ceil_div(s.max_context, 256), s.Hkv, s.rows), 256, 0, st>>>(d);
-    GN_LAUNCH_CHECK();
-  }
+  if (d.splits > 1) GN_CUDA(launch_pdl(stream_decode_join_kernel<R, DP>, dim3(ceil_div(s.max_query * s.G, 4), s.Hkv, s.rows), dim3(128), 0, st, d));
+  if (d.mass_out && s.max_context) GN_CUDA(launch_pdl(stream_decode_mass_kernel<R>, dim3(ceil_div(s.max_context, 256), s.Hkv, s.rows), dim3(256), 0, st, d));
   return GN_OK;
 }
 template <int NT>

@@ -37,6 +37,7 @@ constexpr int kCached = 49152;
 // once and kept as order keys in shared memory.
 __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ Evict e, int cached) {
   extern __shared__ uint32_t cache[];
+  pdl_trigger();
   const gn_evict_params& p = e.p;
   const int hk = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = evict_len(p, r), keep = min(n, p.budget), lo = p.sinks, hi = n - p.recent;
@@ -62,6 +63,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
       hist[tid] = 0; hist[tid + 1024] = 0;
       __syncthreads();
+#pragma unroll 4
       for (int j0 = lo; j0 < hi; j0 += kSelect) {
         const int j = j0 + tid;
         const uint32_t k = j < hi ? key_at(j) : 0u;
@@ -79,8 +81,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
       for (int d = 1; d < 32; d <<= 1) { const int y = __shfl_up_sync(0xffffffffu, before, d); if (lane >= d) before += y; }
       if (lane == 31) sums[warp] = before;
       __syncthreads();
-      int base = 0;
-      for (int w = 0; w < warp; ++w) base += sums[w];
+      const int base = __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0);
       const int above1 = base + before - h1 - h0, above0 = above1 + h1;   // keys of larger digits
       if (above1 < want && want <= above1 + h1) { prefix_s = (pass == 0 ? 0u : prefix << (pass == 1 ? 11 : 10)) | (uint32_t)b1; want_s = want - above1; }
       if (above0 < want && want <= above0 + h0) { prefix_s = (pass == 0 ? 0u : prefix << (pass == 1 ? 11 : 10)) | (uint32_t)b0; want_s = want - above0; }
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
     else if (wanted > 0) { const uint32_t k = key_at(j); take = k > prefix; tie = k == prefix; }
   };
   int sure = 0, equal = 0;
+#pragma unroll 4
   for (int j = j0; j < j1; j += 32) {
     bool take, tie;
     look(j + lane, take, tie);
@@ -106,8 +108,9 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   }
   if (lane == 0) { sums[warp] = sure; ties_s[warp] = equal; }
   __syncthreads();
-  int at = 0, ties = 0;   // kept and equal keys before this warp's
-  for (int w = 0; w < warp; ++w) { at += sums[w] + min(ties_s[w], max(0, want - ties)); ties += ties_s[w]; }
+  // kept and equal keys before this warp's
+  int ties = __reduce_add_sync(0xffffffffu, lane < warp ? ties_s[lane] : 0);
+  int at = __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0) + min(ties, want);
   for (int j = j0; j < j1; j += 32) {
     bool take, tie;
     look(j + lane, take, tie);
@@ -129,6 +132,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
 // To pages of their own: every kept key on its own.  A CTA per (64 kept keys, kv head, row x {key, value}); with 16-byte accesses
 // `lanes` threads carry a row, all reads of a thread before its writes.
 __global__ void __launch_bounds__(256) evict_copy_kernel(const __grid_constant__ Evict e, int lanes) {
+  pdl_wait();
   const gn_evict_params& p = e.p;
   const int hk = blockIdx.y, r = blockIdx.z >> 1, i0 = blockIdx.x * 64;
   const int keep = min(evict_len(p, r), p.budget);
@@ -170,6 +174,7 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(const __grid_constant__
 // In place: a CTA per (32 channels, kv head, row x {key, value}) fills the slots in ascending order, 256 at a time, every read of a
 // group before its writes: slot i <= kept[i], so a group writes only what it or earlier groups have read.
 __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ Evict e) {
+  pdl_wait();
   const gn_evict_params& p = e.p;
   const int hk = blockIdx.y, r = blockIdx.z >> 1, c0 = blockIdx.x * 32, tid = threadIdx.x;
   float* pages = (blockIdx.z & 1) ? p.value_pages : p.key_pages;
@@ -224,13 +229,12 @@ int stream_evict(const gn_evict_params& p, int32_t* kept, int32_t* new_lens, flo
   GN_LAUNCH_CHECK();
   const int most = std::min(p.budget, p.max_context);
   if (most == 0) return GN_OK;
-  if (p.new_table == p.page_table) evict_move_kernel<<<dim3(ceil_div(p.head_dim, 32), p.n_kv_head, 2 * p.rows), 256, 0, st>>>(e);
+  if (p.new_table == p.page_table) GN_CUDA(launch_pdl(evict_move_kernel, dim3(ceil_div(p.head_dim, 32), p.n_kv_head, 2 * p.rows), dim3(256), 0, st, e));
   else {
     int lanes = 1;
     while (lanes < 32 && lanes * 4 < p.head_dim) lanes *= 2;
-    evict_copy_kernel<<<dim3(ceil_div(most, 64), p.n_kv_head, 2 * p.rows), 256, 0, st>>>(e, lanes);
+    GN_CUDA(launch_pdl(evict_copy_kernel, dim3(ceil_div(most, 64), p.n_kv_head, 2 * p.rows), dim3(256), 0, st, e, lanes));
   }
-  GN_LAUNCH_CHECK();
   return GN_OK;
 }
 

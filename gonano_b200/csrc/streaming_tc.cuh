@@ -58,10 +58,12 @@ static inline bool vec_view(const gn_view& v, int D) {
 // Packs keys and values; amax and the 2 * planes words of odd stand in one piece.  norms: null, or [plane][2]: [0] receives the bits of the
 // largest squared norm of a scaled value row.
 // CTAs of a cluster that packs a plane of `rows` rows and finds its largest magnitude on the way (0: a launch of its own finds it).
-// A CTA has 64 rows or more, and the second reading of a row comes from a cache.  Long planes of which there are few leave SMs idle that way.
+// CTAs until the machine has four each, then until their rows (128 or fewer) still stand in a cache when they are read again.  Long planes of which
+// there are few leave SMs idle that way.  In one launch and in two: 128 planes of 383 keys and 1149 query rows 433 and 450 us (forward and
+// backward), 48 of 2000 keys 74 and 79, 8 of 63 keys and 126 rows 49 and 72; 4 of 8704 keys and 69632 rows 2095 and 830.
 static inline int pack_cluster(int64_t rows, int64_t planes) {
   int ctas = 1;
-  while (ctas < 8 && rows >= 128 * ctas) ctas *= 2;
+  while (ctas < 8 && (rows >= 128 * ctas || (rows > 16 * ctas && planes * ctas < 592))) ctas *= 2;
   return rows <= 1280 || planes * ctas >= 296 ? ctas : 0;
 }
 // `dependent`: as launch_pdl.  Every kernel of a call but its first is launched so: it sets up while the one before runs, and each of its
