@@ -109,8 +109,9 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
   plane_scale(largest, sc, inv);
   float top = 0.0f;
   const int end = whole ? last : min(last, j0 + kPackRows);
+  // backwards: what was read last is in a cache
 #pragma unroll 4
-  for (int j16 = j0; j16 < end; j16 += step) {
+  for (int j16 = j0 + (end - j0 + step - 1) / step * step - step; j16 >= j0; j16 -= step) {
     const int j = j16 + half;
     float x[4 * CB];
 #pragma unroll

@@ -87,8 +87,8 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
   pdl_trigger();
   if (!whole) pdl_wait();
   const StreamRows& s = p.s;
-  const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-  const int ctas = gridDim.x, step = whole ? 16 * ctas : 16, f0 = blockIdx.x * (whole ? 16 : kPackRowsQ);
+  const int hk = blockIdx.y, r = whole ? blockIdx.z : gridDim.z - 1 - blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+  const int ctas = gridDim.x, step = whole ? 16 * ctas : 16, f0 = whole ? blockIdx.x * 16 : (gridDim.x - 1 - blockIdx.x) * kPackRowsQ;
   const int nf = row_span<false>(s, r).q_len * s.G, last = min(p.q.rows, (nf + 15) / 16 * 16 + 16);
   if (!whole && f0 >= last) return;
   const int64_t plane = (int64_t)r * s.Hkv + hk;
@@ -121,8 +121,9 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
   plane_scale(p.pk.amax[plane * 2 + 1], sv, inv);
   float top = 0.0f;
   const int end = whole ? last : min(last, f0 + kPackRowsQ);
+  // backwards: what was read last is in a cache
 #pragma unroll 1
-  for (int f16 = f0; f16 < end; f16 += step) {
+  for (int f16 = f0 + (end - f0 + step - 1) / step * step - step; f16 >= f0; f16 -= step) {
     const int f = f16 + half;
     float x[2][4 * CB], delta = 0.0f, sq = 0.0f;
     bool odd = false;
