@@ -34,7 +34,7 @@ constexpr int kCached = 49152;
 // passes of 11, 11 and 10 bits; the digit of a warp's first key is added once for all that share it (weights are often alike: keys
 // nobody looked at hold 0).  Then every warp takes a run of keys, counts what it keeps, and writes the indices behind those of the warps before it: two
 // passes, no order left to chance.  Of the keys equal to the threshold the first ones are kept.  Up to kCached keys are read from memory
-// once and kept as order keys in shared memory.
+// once and kept as order keys in shared memory.  Bound: the latency of its passes; 22 us for 32 rows of 8704 keys.
 __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ Evict e, int cached) {
   extern __shared__ uint32_t cache[];
   pdl_trigger();
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
 }
 
 // To pages of their own: every kept key on its own.  A CTA per (64 kept keys, kv head, row x {key, value}); with 16-byte accesses
-// `lanes` threads carry a row, all reads of a thread before its writes.
+// `lanes` threads carry a row, all reads of a thread before its writes.  Bound: HBM; 24 us for 32 rows of 2048 keys (67 MB read and written, 5.6 TB/s).
 __global__ void __launch_bounds__(256) evict_copy_kernel(const __grid_constant__ Evict e, int lanes) {
   pdl_wait();
   const gn_evict_params& p = e.p;

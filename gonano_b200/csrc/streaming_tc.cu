@@ -48,6 +48,7 @@ __device__ __forceinline__ bool load_key(const StreamRows& s, bool value, bool v
 
 constexpr int kPackRows = 128;   // keys of a CTA (256 threads, 16 half warps, 8 keys each)
 
+// Largest finite magnitude of every plane.  Bound: HBM; 9.7 us for 2 planes of 8704 keys (18 MB, too few CTAs in flight to reach it).
 template <int CB, bool PAGED>
 __global__ void __launch_bounds__(256) stream_amax_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, int vec) {
   pdl_trigger();
@@ -70,7 +71,10 @@ __global__ void __launch_bounds__(256) stream_amax_kernel(const __grid_constant_
   if ((threadIdx.x & 31) == 0 && top) atomicMax(pk.amax + ((int64_t)r * s.Hkv + hk) * 2 + value, top);   // a maximum does not depend on the order
 }
 
-// With whole = 1 a plane is a cluster's (its CTAs take 16 keys in turn), which finds the largest magnitude itself.
+// Keys and values times a power of two that brings the plane's largest to [2^14, 2^15), as f16 pairs in the layout that the tiles are copied in.
+// With whole = 1 a plane is a cluster's (its CTAs take 16 keys in turn), which finds the largest magnitude itself.  Half a warp per row:
+// 16-byte loads and whole 128-byte lines of stores.  Bound: HBM, 4 D bytes a row in and out; 28 us for 2 x 128 planes of up to 383 keys
+// (37 MB read, 37 written; the meeting of the cluster and two readings in a row are its latency).
 template <int CB, bool PAGED>
 __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, uint32_t* norms, int vec, int whole) {
   pdl_trigger();
@@ -239,6 +243,8 @@ __device__ __forceinline__ Item get_item(const ForwardTc& p, const int* before, 
 // long unrolled code once a tile wait for instructions most of the time.  Sixteen warps, because eight took 3360 cycles a tile
 // (read 530, meet 250, weights 1650, O 850) against the 48 instructions of 64 cycles of the tensor pipe, which is the bound of a tile.  Every wait is
 // bounded; a kernel whose wait ran out writes NaN.
+// 4 x 8192 tokens, 8 heads on one, window 512 and 64 sinks: 275 us, tensor pipe busy 42 %; a tile takes about 3400 cycles, and an item's start
+// (Q, once the last scores have read theirs) about as long as two.  Chunks over 8704 keys: 53 %.
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __grid_constant__ ForwardTc p) {
   constexpr int CB = DP / 64, QC = DP / 4, RING = DP == 64 ? 6 : 3;
@@ -620,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
   if (warp == 20) tmem_dealloc(tmem, 512);
 }
 
-// Joins the key splits of a row: a warp per query row.
+// Joins the parts of a row's keys by their log-sum-exps: a warp per query row.  Bound: reading them; 8.5 us for 8192 rows in two parts.
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(256) stream_tc_combine_kernel(const __grid_constant__ ForwardTc p) {
   pdl_trigger();

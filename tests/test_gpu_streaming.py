@@ -413,6 +413,16 @@ def test_paged(case, mass):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [33, 511, 512])
+def test_many_ragged_chunks(rows):
+    """Most rows without new tokens, the first and the last ones among them, some with one tile of them and one with several."""
+    counts = [0 if r < 2 or r > rows - 3 or r % 7 else r % 5 for r in range(rows)]
+    counts[14], counts[rows // 2] = 70, 33
+    lens = [max(c, (r * 37) % 90) for r, c in enumerate(counts)]
+    check_paged(counts, lens, 8, 2, 32, 16, -1, 0, mass=False)
+
+
+@pytest.mark.gpu
 def test_paged_without_append_and_with_unit_scale():
     check_paged([1, 1], [77, 300], 6, 2, 128, 16, -1, 0, append=False, scale=1.0)
     check_paged([40, 70], [77, 300], 6, 2, 128, 16, -1, 0, append=False, scale=1.0)
