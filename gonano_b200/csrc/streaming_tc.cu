@@ -234,7 +234,8 @@ __device__ __forceinline__ Item get_item(const ForwardTc& p, const int* before, 
 //               running maximum, and write 2^15 p as f16 pairs over the scores they came from: P is the A operand of O = P V
 //               straight from tensor memory.  Each tile's O starts from zero and is added to float32 registers one tile later, where the
 //               rescaling by the grown maximum costs nothing extra: sums over many keys are rounded, not cut off.  An item's
-//               result is stored in the shadow of the next item's first products;
+//               result is stored while the next one's Q is fetched and its first products run (behind the next item's first weights, where it
+//               was before, it held up everything: 31 400 cycles an item of five tiles);
 //   warps 16-19 fetch the next item's Q rows (raw float32), scale, split and leave them in tensor memory (A operand of S = Q K^T);
 //   warps 20, 22  issue the instructions, 24 of 128 x 128 x 16 for a tile's S and 24 for its O: each a queue of its own, so that the
 //               waits of one pass while the other's instructions run;
@@ -416,53 +417,44 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       };
       // One pass: the scale comes from the first 32 channels, with 2^6 to spare for the others; a warp with a row that needs
       // more (or whose first channels are zeros) goes over its rows again.  While the last item's scores still read Q, the first
-      // 32 channels wait in shared memory, the next in registers, and the third are being loaded: what is left to do once Q is free
-      // took 9600 cycles when only the first were ready.
-      uint32_t top = 0, y[32];
-      float sq, iq, x[32];
-      auto largest_of = [&](const float (&x)[32]) {
-        uint32_t most = 0;
+      // 32 channels wait in shared memory, the next in registers, and the others are on their way to L2.  One copy of the code serves all of
+      // them: unrolled it was 7400 cycles from the last scores to Q, most of them spent waiting for instructions, its own and the other warps'.
+      uint32_t top = 0;
+      float sq = 1.0f, iq = 1.0f;
+      if (p.vec_q && src)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);   // a row that is not finite has no result whatever its scale
-        return most;
-      };
-      auto split = [&](const float (&x)[32]) {
-        const float by = s.scale < 0.0f ? -sq : sq;   // a negative scale goes into Q, so that larger products are larger scores
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) split_f16(x[e] * by, x[e + 1] * by, y[e >> 1], y[16 + (e >> 1)]);
-      };
-      load(0, x);
-      top = largest_of(x);
-      plane_scale(top, sq, iq);
-      sq *= 0x1p-6f; iq *= 0x1p6f;
-      split(x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) stash[e * 128 + row] = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
-      load(32, x);
-      top = max(top, largest_of(x));
-      split(x);
-      if (DP > 64) load(64, x);
-      if (count > 0) { ok = ok && hold(q_free, (count - 1) & 1); tc_fence_after(); }
-      tmem_st32(q_addr + 32, y);
-      float next[32];
-      if (DP > 64) load(96, next);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { const uint4 v = stash[e * 128 + row]; y[4 * e] = v.x; y[4 * e + 1] = v.y; y[4 * e + 2] = v.z; y[4 * e + 3] = v.w; }
-      tmem_st32(q_addr, y);
-      if (DP > 64) {
-        top = max(top, largest_of(x));
-        split(x);
-        tmem_st32(q_addr + 64, y);
-        top = max(top, largest_of(next));
-        split(next);
-        tmem_st32(q_addr + 96, y);
-      }
-      const float largest = __uint_as_float(top) * sq;
-      const bool again = top != 0 && !(largest >= 0x1p7f && largest < 0x1p15f);
-      if (__any_sync(0xffffffffu, again)) {
-        if (again) plane_scale(top, sq, iq);
+        for (int ch = 64; ch < DP; ch += 32) if (ch < s.D) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + ch));
 #pragma unroll 1
-        for (int h = 0; h < DP / 32; ++h) { load(h * 32, x); split(x); tmem_st32(q_addr + h * 32, y); }
+      for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+        for (int h = 0; h < DP / 32; ++h) {
+          float x[32];
+          uint32_t y[32];
+          load(h * 32, x);
+          if (pass == 0) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);   // a row that is not finite has no result whatever its scale
+            if (h == 0) { plane_scale(top, sq, iq); sq *= 0x1p-6f; iq *= 0x1p6f; }
+          }
+          const float by = s.scale < 0.0f ? -sq : sq;   // a negative scale goes into Q, so that larger products are larger scores
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) split_f16(x[e] * by, x[e + 1] * by, y[e >> 1], y[16 + (e >> 1)]);
+          if (h == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) stash[e * 128 + row] = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+          } else {
+            if (h == 1 && pass == 0 && count > 0) { ok = ok && hold(q_free, (count - 1) & 1); tc_fence_after(); }
+            tmem_st32(q_addr + h * 32, y);
+          }
+        }
+        uint32_t y[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { const uint4 v = stash[e * 128 + row]; y[4 * e] = v.x; y[4 * e + 1] = v.y; y[4 * e + 2] = v.z; y[4 * e + 3] = v.w; }
+        tmem_st32(q_addr, y);
+        const float largest = __uint_as_float(top) * sq;
+        const bool again = top != 0 && !(largest >= 0x1p7f && largest < 0x1p15f);
+        if (pass == 1 || !__any_sync(0xffffffffu, again)) break;
+        if (again) plane_scale(top, sq, iq);
       }
       float sk, ik;
       if (count == 0) pdl_wait();
@@ -487,8 +479,6 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     uint32_t tiles = 0, count = 0;
     float m = -INFINITY, l = 0.0f, alpha = 0.0f;   // l of a poisoned row is not a number
     float o[QC];
-#pragma unroll
-    for (int e = 0; e < QC; ++e) o[e] = 0.0f;
     // where the row's result goes: out from this thread's channels on (null: nowhere), lse null in all but one of the row's threads
     struct Target { float* out; float* lse; float iv; } to{nullptr, nullptr, 1.0f};
 
@@ -535,23 +525,23 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       if (!it.inside) continue;
       const int f = it.f0 + row, t = s.by_G.of(f), g = f - t * s.G, token = it.q_begin + t, pos = it.first + t;
       const bool live = f < it.nf;
-      Target here;
+      to = Target{nullptr, nullptr, 1.0f};
       if (p.splits > 1) {
         const int64_t at = ((it.plane * p.tiles + it.tile) * p.splits + it.split) * kRowsT + row;
-        here.out = p.part_o + at * DP + part * QC;
-        here.lse = p.part_l + at;
+        to.out = p.part_o + at * DP + part * QC;
+        to.lse = p.part_l + at;
       } else {
-        here.out = f < (PAGED ? it.nf : s.seq * s.G) ? p.out.data + token_offset<PAGED>(p.out, it.r, it.hk * s.G + g, token) + part * QC : nullptr;
-        here.lse = p.lse + stat_offset<PAGED>(s, it.r, it.hk * s.G + g, token);
+        to.out = f < (PAGED ? it.nf : s.seq * s.G) ? p.out.data + token_offset<PAGED>(p.out, it.r, it.hk * s.G + g, token) + part * QC : nullptr;
+        to.lse = p.lse + stat_offset<PAGED>(s, it.r, it.hk * s.G + g, token);
       }
-      if (!here.out || part != 0) here.lse = nullptr;
+      if (!to.out || part != 0) to.lse = nullptr;
       if (it.n == 0) {   // rows that see nothing: padding, or tokens before the cache
-        if (here.lse) *here.lse = -INFINITY;
-        if (here.out) for (int e = 0; e < min(QC, p.splits > 1 ? QC : s.D - part * QC); ++e) here.out[e] = 0.0f;
+        if (to.lse) *to.lse = -INFINITY;
+        if (to.out) for (int e = 0; e < min(QC, p.splits > 1 ? QC : s.D - part * QC); ++e) to.out[e] = 0.0f;
         continue;
       }
       float sv;
-      plane_scale(p.pk.amax[it.plane * 2 + 1], sv, here.iv);
+      plane_scale(p.pk.amax[it.plane * 2 + 1], sv, to.iv);
       // what the row sees, in virtual keys: [0, s_end) and [lo, hi]
       const int s_end = live ? max(0, min(s.sinks, pos + 1)) : 0;
       const int lo_key = live ? (s.window < 0 ? 0 : max(0, pos - s.window)) - it.runs.shift : 0, hi_key = live ? pos - it.runs.shift : -1;
@@ -559,19 +549,22 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       ok = ok && hold(q_ready(count), (count >> 2) & 1);
       const float c = rowc[(count & 3) * 128 + row];
       ++count;
-      float m_here = -INFINITY, l_here = 0.0f;
+      m = -INFINITY; l = 0.0f;
+#pragma unroll
+      for (int e = 0; e < QC; ++e) o[e] = 0.0f;
 #pragma unroll 1
       for (int j = 0; j < it.n; ++j) {
         const uint32_t buf = lane_addr + (tiles & 1) * 128 + part * 32;
         const int c0 = (it.j0 + j) * kRowsT + part * 32;
         uint32_t see = (uint32_t)(bits_below(s_end - c0) | (bits_below(hi_key + 1 - c0) & ~bits_below(lo_key - c0)));
         if (odd_plane) {
+#pragma unroll 1
           for (int e = 0; e < 32; ++e)
             if ((see >> e) & 1u) {
               const int key = c0 + e < it.runs.a_len ? c0 + e : c0 + e + it.runs.shift;
               const uint8_t flag = p.pk.flags_k[it.plane * p.pk.k.rows + key] | p.pk.flags_v[it.plane * p.pk.v.rows + key];
               if (flag & kAbsent) see &= ~(1u << e);
-              else if (flag & kOdd) l_here = NAN;
+              else if (flag & kOdd) l = NAN;
             }
         }
         ok = ok && hold(s_full(tiles & 1), (tiles >> 1) & 1);
@@ -590,9 +583,9 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         mine[part * 128] = top;
         meet();
         top = fmaxf(fmaxf(mine[0], mine[128]), fmaxf(mine[256], mine[384]));
-        const float m_new = fmaxf(m_here, top == -INFINITY ? -INFINITY : top * c), m_use = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha_here = exp2_fast(m_here - m_use), off = kWeightShift - m_use;
-        m_here = m_new;
+        const float m_new = fmaxf(m, top == -INFINITY ? -INFINITY : top * c), m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha_here = exp2_fast(m - m_use), off = kWeightShift - m_use;
+        m = m_new;
         float sum = 0.0f;
         uint32_t z[32];
 #pragma unroll
@@ -605,21 +598,14 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(p_full(tiles & 1));
-        l_here = fmaf(l_here, alpha_here, sum);
-        if (tiles > 0) {
-          gather();
-          if (j == 0) {
-            store();
-#pragma unroll
-            for (int e = 0; e < QC; ++e) o[e] = 0.0f;
-          }
-        }
+        l = fmaf(l, alpha_here, sum);
+        if (j > 0) gather();
         alpha = alpha_here;
         ++tiles;
       }
-      to = here; m = m_here; l = l_here;
+      gather();
+      store();
     }
-    if (tiles > 0) { gather(); store(); }
   }
   tc_fence_before();
   __syncthreads();
