@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(256) stream_amax_kernel(const __grid_constant_
 
 // Keys and values times a power of two that brings the plane's largest to [2^14, 2^15), as f16 pairs in the layout that the tiles are copied in.
 // With whole = 1 a plane is a cluster's (its CTAs take 16 keys in turn), which finds the largest magnitude itself.  Half a warp per row:
-// 16-byte loads and whole 128-byte lines of stores.  Bound: HBM, 4 D bytes a row in and out; 28 us for 2 x 128 planes of up to 383 keys
+// 16-byte loads and whole 128-byte lines of stores.  Bound: HBM, 4 D bytes a row in and out; 25 us for 2 x 128 planes of up to 383 keys
 // (37 MB read, 37 written; the meeting of the cluster and two readings in a row are its latency).
 template <int CB, bool PAGED>
 __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant__ StreamRows s, PackedKeys pk, uint32_t* norms, int vec, int whole) {
@@ -244,8 +244,8 @@ __device__ __forceinline__ Item get_item(const ForwardTc& p, const int* before, 
 // long unrolled code once a tile wait for instructions most of the time.  Sixteen warps, because eight took 3360 cycles a tile
 // (read 530, meet 250, weights 1650, O 850) against the 48 instructions of 64 cycles of the tensor pipe, which is the bound of a tile.  Every wait is
 // bounded; a kernel whose wait ran out writes NaN.
-// 4 x 8192 tokens, 8 heads on one, window 512 and 64 sinks: 275 us, tensor pipe busy 42 %; a tile takes about 3400 cycles, and an item's start
-// (Q, once the last scores have read theirs) about as long as two.  Chunks over 8704 keys: 53 %.
+// 4 x 8192 tokens, 8 heads on one, window 512 and 64 sinks: 249 us, tensor pipe busy 47 %; a tile takes about 3400 cycles, and between two
+// items (O to memory in 6700, the next rows' bounds 2000) there are about three tiles' time.  Chunks over 8704 keys: 57 %.
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __grid_constant__ ForwardTc p) {
   constexpr int CB = DP / 64, QC = DP / 4, RING = DP == 64 ? 6 : 3;

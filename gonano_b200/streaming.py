@@ -211,8 +211,8 @@ def evict_pages(key_pages, value_pages, mass, page_table, context_lens, budget, 
                       _packed("context_lens", context_lens, torch.int32, device, (rows,)), rows, kv_heads, dim, page_size, pages, width, new_width, n,
                       width * page_size if max_context is None else max_context, budget, sinks, recent)
     with _on(device):
-        kept = torch.empty((rows, kv_heads, budget), dtype=torch.int32, device=device)
-        lens = torch.empty((rows,), dtype=torch.int32, device=device)
-        mass_out = torch.empty((rows, kv_heads, budget), dtype=torch.float32, device=device)
+        kept = page_table.new_empty((rows, kv_heads, budget))
+        lens = torch.empty_like(context_lens)
+        mass_out = mass.new_empty((rows, kv_heads, budget))
         check(lib.gn_cache_evict(C.byref(p), kept.data_ptr(), lens.data_ptr(), mass_out.data_ptr(), _stream(device)))
     return kept, lens, mass_out
