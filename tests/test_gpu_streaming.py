@@ -681,6 +681,64 @@ def test_runs_on_the_current_stream():
     side.synchronize()
 
 
+TRAINING = [  # B, H, Hkv, T, D, window, sinks, ragged: planes of a cluster, of two launches, key tiles in parts, tiny ones
+    (5, 6, 2, 150, 128, 40, 3, True),
+    (1, 8, 1, 2100, 128, 256, 5, False),
+    (1, 2, 1, 1500, 64, -1, 0, True),
+    (9, 2, 1, 20, 40, 5, 1, True),
+]
+
+
+def training_pass(case, seed):
+    B, H, Hkv, T, D, window, sinks, ragged = case
+    q, k, v, dout = tensors(B, H, Hkv, T, D, seed=seed)
+    lengths = torch.tensor([(T * (b + 1)) // B for b in range(B)], dtype=torch.int32, device=DEVICE) if ragged else None
+    mask = dict(sinks=sinks, window=window, scale=0.1, lengths=lengths)
+
+    def run():
+        out, lse = streaming.sink_attention_forward(q, k, v, **mask)
+        grads = streaming.sink_attention_backward(q, k, v, out, dout, lse, **mask)
+        return [x * 1.0 for x in (out, lse, *grads)]   # what a following kernel reads
+    return (q, k, v, dout), run
+
+
+@pytest.mark.gpu
+def test_training_passes_behind_one_another():
+    """Nothing waits on the host between calls, which take over one another's memory."""
+    passes = [training_pass(case, seed)[1] for seed, case in enumerate(TRAINING)]
+    alone = []
+    for run in passes:
+        alone.append(run())
+        torch.cuda.synchronize()
+    for _ in range(10):
+        got = [run() for run in passes]
+        for want, have in zip(alone, got):
+            for x, y in zip(want, have):
+                assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", TRAINING)
+def test_captured_training_pass(case):
+    inputs, run = training_pass(case, 3)
+    run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        captured = run()
+    for step in range(3):
+        for x in inputs:
+            x.mul_(1.0 + 0.25 * step)
+        graph.replay()
+        replayed = [x.clone() for x in captured]
+        for x, y in zip(replayed, run()):
+            assert torch.equal(x, y)
+
+
 @pytest.mark.gpu
 def test_two_graphs_at_once():
     """Two captured calls replayed on two streams at once give what eager calls give, on the inputs that stand there at replay."""
