@@ -55,8 +55,6 @@ int prepare_kernel(std::atomic<uint64_t>& ready, const void* kernel, int smem, i
 static inline bool vec_view(const gn_view& v, int D) {
   return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && D % 4 == 0 && v.batch_stride % 4 == 0 && v.head_stride % 4 == 0 && v.token_stride % 4 == 0;
 }
-// Packs keys and values; amax and the 2 * planes words of odd stand in one piece.  norms: null, or [plane][2]: [0] receives the bits of the
-// largest squared norm of a scaled value row.
 // CTAs of a cluster that packs a plane of `rows` rows and finds its largest magnitude on the way (0: a launch of its own finds it).
 // CTAs until the machine has four each, then until their rows (128 or fewer) still stand in a cache when they are read again.  Long planes of which
 // there are few leave SMs idle that way.  In one launch and in two: 128 planes of 383 keys and 1149 query rows 433 and 450 us (forward and
@@ -66,7 +64,7 @@ static inline int pack_cluster(int64_t rows, int64_t planes) {
   while (ctas < 8 && (rows >= 128 * ctas || (rows > 16 * ctas && planes * ctas < 592))) ctas *= 2;
   return rows <= 1280 || planes * ctas >= 296 ? ctas : 0;
 }
-// `dependent`: as launch_pdl.  Every kernel of a call but its first is launched so: it sets up while the one before runs, and each of its
+// `dependent`: as launch_pdl.  A kernel that stands behind another of the same call is launched so: it sets up while that one runs, and each of its
 // CTAs waits for that one to be complete before it ends (and before it reads what that one writes), so that complete means complete
 // with all before it.  A call's first kernel waits for the stream as usual; what the caller passed in is there from then on.
 template <typename... KArgs, typename... Args>
@@ -81,7 +79,8 @@ inline cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int threa
   cfg.attrs = attr; cfg.numAttrs = dependent ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
-// `dependent`: a kernel of the same call stands before it.
+// Packs keys and values; amax and the 2 * planes words of odd stand in one piece.  norms: null, or [plane][2]: [0] receives the bits of the
+// largest squared norm of a scaled value row.  `dependent`: a kernel of the same call stands before it.
 int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dependent, cudaStream_t stream);
 
 // tcgen05 forward of a call (streaming_tc.cu): the workspace it wants, and the launches.
