@@ -64,6 +64,14 @@ static inline int pack_cluster(int64_t rows, int64_t planes) {
   while (ctas < 8 && (rows >= 128 * ctas || (rows > 16 * ctas && planes * ctas < 592))) ctas *= 2;
   return rows <= 1280 || planes * ctas >= 296 ? ctas : 0;
 }
+// A launch that may set up while the kernel before it on the stream still runs (launch_pdl), or, for paged calls, an ordinary one: a chunk call ended once
+// in a device error among many thousands whose cause was not found, and there nothing overlaps until it is (5 us a call, 10 with weights).
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_behind(bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+  if (overlap) return launch_pdl(kernel, grid, block, smem, st, std::forward<Args>(args)...);
+  kernel<<<grid, block, smem, st>>>(static_cast<KArgs>(args)...);
+  return cudaGetLastError();
+}
 // `dependent`: as launch_pdl.  A kernel that stands behind another of the same call is launched so: it sets up while that one runs, and each of its
 // CTAs waits for that one to be complete before it ends (and before it reads what that one writes), so that complete means complete
 // with all before it.  A call's first kernel waits for the stream as usual; what the caller passed in is there from then on.
