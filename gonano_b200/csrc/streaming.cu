@@ -10,7 +10,6 @@ namespace {
 
 // A warp per (row, new token, kv head): the new token's key and value go to its slot.
 __global__ void __launch_bounds__(128) stream_append_kernel(StreamRows s, gn_view nk, gn_view nv) {
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * 4 + warp, hk = blockIdx.y, r = blockIdx.z;
   const RowSpan sp = row_span<true>(s, r);
@@ -132,7 +131,7 @@ int gn_attention_sink_forward(const gn_sink_params* p, const gn_view* out, float
   GN_REQUIRE(strides_ok(*out) && apart(*out, s.rows, s.Hq, s.seq, s.D), "attention_sink_forward: elements of out share memory");
   GN_TRY(on_this_device(out->data, "attention_sink_forward: out")); GN_TRY(on_this_device(lse, "attention_sink_forward: lse"));
   GN_TRY(workspace_ok(workspace, workspace_bytes, sink_bytes(s, 0), "attention_sink_forward"));
-  return stream_tc_forward(s, *out, lse, workspace, false, (cudaStream_t)stream);
+  return stream_tc_forward(s, *out, lse, workspace, (cudaStream_t)stream);
 }
 
 int gn_attention_sink_backward(const gn_sink_params* p, const gn_view* out, const gn_view* out_grad, const float* lse, const gn_view* dq, const gn_view* dk,
@@ -174,13 +173,12 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
   GN_TRY(workspace_ok(workspace, workspace_bytes, paged_bytes(s, p->mass_out != nullptr), "attention_paged"));
   cudaStream_t st = (cudaStream_t)stream;
   if (!paged_on_tensor_cores(s)) return stream_decode(s, p->new_key, p->new_value, *out, lse, p->mass, p->mass_out, workspace, st);
-  const bool append = p->new_key.data && s.max_context;
-  if (append) {
+  if (p->new_key.data && s.max_context) {
     stream_append_kernel<<<dim3(ceil_div(s.max_query, 4), s.Hkv, s.rows), 128, 0, st>>>(s, p->new_key, p->new_value);
     GN_LAUNCH_CHECK();
   }
   PackedKeys packed;
-  GN_TRY(stream_tc_forward(s, *out, lse, workspace, append, st, &packed));
+  GN_TRY(stream_tc_forward(s, *out, lse, workspace, st, &packed));
   if (!p->mass_out || !s.max_context) return GN_OK;
   return stream_tc_mass(s, packed, lse, p->mass, p->mass_out, static_cast<uint8_t*>(workspace) + stream_tc_forward_bytes(s), st);
 }

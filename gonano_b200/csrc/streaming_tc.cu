@@ -690,10 +690,10 @@ bool vec_keys(const StreamRows& s) {
 }
 
 template <int CB, bool PAGED>
-int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dependent, cudaStream_t st) {
+int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t st) {
   const int vec = vec_keys(s), keys = pk.k.rows, ctas = pack_cluster(keys, 2ll * s.rows * s.Hkv);
   if (ctas) {
-    GN_CUDA(launch_cluster(stream_pack_kernel<CB, PAGED>, dim3(ctas, s.Hkv, 2 * s.rows), 256, ctas, dependent && !PAGED, st, s, pk, norms, vec, 1));
+    GN_CUDA(launch_cluster(stream_pack_kernel<CB, PAGED>, dim3(ctas, s.Hkv, 2 * s.rows), 256, ctas, st, s, pk, norms, vec, 1));
   } else {
     GN_CUDA(cudaMemsetAsync(pk.amax, 0, (int64_t)s.rows * s.Hkv * 4 * sizeof(uint32_t), st));   // amax and odd
     if (norms) GN_CUDA(cudaMemsetAsync(norms, 0, (int64_t)s.rows * s.Hkv * 2 * sizeof(uint32_t), st));
@@ -705,9 +705,9 @@ int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dep
 }
 
 template <int DP, bool PAGED>
-int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, bool dependent, cudaStream_t st) {
+int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t st) {
   constexpr int kSmem = 6 * 32768 + 256 + 2048 + 6144 + 16384 + (kRowsListed + 1) * 4 + 1024;
-  GN_TRY(stream_pack_keys(s, f.pk, nullptr, dependent, st));
+  GN_TRY(stream_pack_keys(s, f.pk, nullptr, st));
   static std::atomic<uint64_t> ready{0};
   GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(stream_tc_forward_kernel<DP, PAGED>), kSmem, kThreads, 512 * kRegsSoftmax + 128 * (kRegsFetch + kRegsOther)));
   const int64_t items = pl.planes * pl.tiles * pl.splits;
@@ -735,16 +735,16 @@ int prepare_kernel(std::atomic<uint64_t>& ready, const void* kernel, int smem, i
   return GN_OK;
 }
 
-int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dependent, cudaStream_t st) {
-  if (s.D <= 64) return s.paged() ? pack_go<1, true>(s, pk, norms, dependent, st) : pack_go<1, false>(s, pk, norms, dependent, st);
-  return s.paged() ? pack_go<2, true>(s, pk, norms, dependent, st) : pack_go<2, false>(s, pk, norms, dependent, st);
+int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t st) {
+  if (s.D <= 64) return s.paged() ? pack_go<1, true>(s, pk, norms, st) : pack_go<1, false>(s, pk, norms, st);
+  return s.paged() ? pack_go<2, true>(s, pk, norms, st) : pack_go<2, false>(s, pk, norms, st);
 }
 
 int64_t stream_tc_forward_bytes(const StreamRows& s) {
   ForwardTc f{};
   return carve_forward(s, plan_forward(s), nullptr, &f);
 }
-int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, bool dependent, cudaStream_t st, PackedKeys* packed) {
+int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t st, PackedKeys* packed) {
   const Plan pl = plan_forward(s);
   ForwardTc f{};
   f.s = s; f.out = out; f.lse = lse; f.tiles = pl.tiles; f.splits = pl.splits; f.planes = (int)pl.planes;
@@ -753,8 +753,8 @@ int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void*
   carve_forward(s, pl, workspace, &f);
   if (packed) *packed = f.pk;
   f.vec_q = vec_view(s.q, s.D); f.vec_out = pl.splits > 1 || vec_view(out, s.D);
-  if (pl.DP == 64) return s.paged() ? forward_go<64, true>(s, pl, f, dependent, st) : forward_go<64, false>(s, pl, f, dependent, st);
-  return s.paged() ? forward_go<128, true>(s, pl, f, dependent, st) : forward_go<128, false>(s, pl, f, dependent, st);
+  if (pl.DP == 64) return s.paged() ? forward_go<64, true>(s, pl, f, st) : forward_go<64, false>(s, pl, f, st);
+  return s.paged() ? forward_go<128, true>(s, pl, f, st) : forward_go<128, false>(s, pl, f, st);
 }
 
 }  // namespace gn

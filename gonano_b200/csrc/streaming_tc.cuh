@@ -66,34 +66,32 @@ static inline int pack_cluster(int64_t rows, int64_t planes) {
 }
 // A launch that may set up while the kernel before it on the stream still runs (launch_pdl), or, for paged calls, an ordinary one: a chunk call ended once
 // in a device error among many thousands whose cause was not found, and there nothing overlaps until it is (5 us a call, 10 with weights).
+// Each CTA of a kernel that may overlap waits for the one before to be complete before it ends (and before it reads what that one writes), so that
+// complete means complete with all before it.  A call's first kernel waits for the stream as usual; what the caller passed in is there from then on.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_behind(bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
   if (overlap) return launch_pdl(kernel, grid, block, smem, st, std::forward<Args>(args)...);
   kernel<<<grid, block, smem, st>>>(static_cast<KArgs>(args)...);
   return cudaGetLastError();
 }
-// `dependent`: as launch_pdl.  A kernel that stands behind another of the same call is launched so: it sets up while that one runs, and each of its
-// CTAs waits for that one to be complete before it ends (and before it reads what that one writes), so that complete means complete
-// with all before it.  A call's first kernel waits for the stream as usual; what the caller passed in is there from then on.
+// Clusters are launched in the ordinary way for the same reason.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, int ctas, bool dependent, cudaStream_t st, Args&&... args) {
+inline cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, int ctas, cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.stream = st;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr; cfg.numAttrs = dependent ? 2 : 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 // Packs keys and values; amax and the 2 * planes words of odd stand in one piece.  norms: null, or [plane][2]: [0] receives the bits of the
-// largest squared norm of a scaled value row.  `dependent`: a kernel of the same call stands before it.
-int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, bool dependent, cudaStream_t stream);
+// largest squared norm of a scaled value row.
+int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t stream);
 
 // tcgen05 forward of a call (streaming_tc.cu): the workspace it wants, and the launches.
 int64_t stream_tc_forward_bytes(const StreamRows& s);
-int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, bool dependent, cudaStream_t stream, PackedKeys* packed = nullptr);
+int stream_tc_forward(const StreamRows& s, const gn_view& out, float* lse, void* workspace, cudaStream_t stream, PackedKeys* packed = nullptr);
 // The weights of a paged call's keys (streaming_tc_mass.cu), from the forward's packed keys and its log-sum-exps.
 int64_t stream_tc_mass_bytes(const StreamRows& s);
 int stream_tc_mass(const StreamRows& s, const PackedKeys& pk, const float* lse, const float* mass, float* mass_out, void* workspace, cudaStream_t stream);

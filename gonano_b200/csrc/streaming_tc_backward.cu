@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) stream_query_amax_kernel(const __grid_con
 template <int CB>
 __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_constant__ BackwardTc p, int whole) {
   pdl_trigger();
-  if (!whole) pdl_wait();
+  pdl_wait();
   const StreamRows& s = p.s;
   const int hk = blockIdx.y, r = whole ? blockIdx.z : gridDim.z - 1 - blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const int ctas = gridDim.x, step = whole ? 16 * ctas : 16, f0 = whole ? blockIdx.x * 16 : (gridDim.x - 1 - blockIdx.x) * kPackRowsQ;
@@ -113,7 +113,6 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
     for (int w = 0; w < 2; ++w) if (top[w]) atomicMax(&found[w], top[w]);
     cluster_meet();
     for (int w = 0; w < 2; ++w) largest[w] = cluster_largest(&found[w], ctas);
-    pdl_wait();   // for V's scale; what was read so far is the caller's
   } else {
     for (int w = 0; w < 2; ++w) largest[w] = p.qamax[plane * 2 + w];
   }
@@ -825,10 +824,10 @@ int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
   GN_TRY(prepare_kernel(ready_kv, reinterpret_cast<const void*>(stream_tc_dkv_kernel<DP>), kSmemKv, kThreadsB, kShared));
   GN_TRY(prepare_kernel(ready_q, reinterpret_cast<const void*>(stream_tc_dq_kernel<DP>), kSmemQ, kThreadsB, kShared));
   const int64_t planes = (int64_t)s.rows * s.Hkv;
-  GN_TRY(stream_pack_keys(s, b.pk, b.norms, false, st));
+  GN_TRY(stream_pack_keys(s, b.pk, b.norms, st));
   const int ctas = pack_cluster(b.q.rows, planes);
   if (ctas) {
-    GN_CUDA(launch_cluster(stream_query_pack_kernel<CB>, dim3(ctas, s.Hkv, s.rows), 256, ctas, true, st, b, 1));
+    GN_CUDA(launch_cluster(stream_query_pack_kernel<CB>, dim3(ctas, s.Hkv, s.rows), 256, ctas, st, b, 1));
   } else {
     GN_CUDA(cudaMemsetAsync(b.qamax, 0, planes * 2 * sizeof(uint32_t), st));
     GN_CUDA(cudaMemset2DAsync(b.norms + 1, 2 * sizeof(uint32_t), 0, sizeof(uint32_t), planes, st));
