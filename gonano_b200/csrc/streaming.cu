@@ -101,7 +101,7 @@ int paged_rows(const gn_paged_params* p, StreamRows* s) {
   GN_REQUIRE(strides_ok(p->query) && strides_ok(p->new_key) && strides_ok(p->new_value), "attention_paged: negative stride");
   s->rows = p->rows; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->by_G = FastDiv(s->G); s->D = p->head_dim;
   s->window = std::min(p->window, kFar); s->sinks = std::min(p->sinks, kFar); s->scale = p->scale; s->q = p->query;
-  s->pages_k = p->key_pages; s->pages_v = p->value_pages; s->table = p->page_table; s->starts = p->query_starts; s->lens = p->context_lens;
+  s->is_paged = true; s->pages_k = p->key_pages; s->pages_v = p->value_pages; s->table = p->page_table; s->starts = p->query_starts; s->lens = p->context_lens;
   s->tokens = p->tokens; s->max_query = std::min(p->max_query, p->tokens); s->max_context = p->max_context; s->page_size = p->page_size; s->by_page = FastDiv(p->page_size); s->pages = p->pages;
   s->width = p->table_width;
   return GN_OK;

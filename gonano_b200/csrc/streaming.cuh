@@ -27,11 +27,12 @@ struct StreamRows {
   // padded batch: `seq` tokens a row, lengths nullable
   int seq = 0;
   const int32_t* lengths = nullptr;
-  // paged cache (pages_k != null)
+  // paged cache
+  bool is_paged = false;
   float* pages_k = nullptr; float* pages_v = nullptr;
   const int32_t* table = nullptr; const int32_t* starts = nullptr; const int32_t* lens = nullptr;
   int tokens = 0, max_query = 0, max_context = 0, page_size = 1, pages = 0, width = 0;
-  bool paged() const { return pages_k != nullptr; }
+  bool paged() const { return is_paged; }   // not by the pages' address: a workspace may be asked for before there are pages, and an empty pool has none
 };
 
 // Few new tokens a row over a paged cache (streaming_decode.cu): max_query * G <= 16.  Appends, attends and gathers the mass.

@@ -1,0 +1,52 @@
+"""Streaming attention (gonano_b200/streaming.py) at the calls that its documentation allows and a rollout rarely makes: empty pools
+and steps, tables that name their own pages, values that are not finite, gradients of very different sizes.  The float64 statements
+and the bounds are those of test_gpu_streaming.py.
+"""
+import ctypes as C
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from gonano_b200 import _lib, streaming  # noqa: E402
+from test_gpu_streaming import DEVICE, paged_params  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from gonano_b200 import build
+    build.build()
+    return _lib.load()
+
+
+def ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device=DEVICE)
+
+
+# ---------------------------------------------------------------- pools without pages
+
+@pytest.mark.parametrize("shape", [dict(rows=4, tokens=4, max_query=1), dict(rows=4, tokens=1024, max_query=512), dict(rows=4, tokens=64, max_query=16, mass_out=256)])
+def test_workspace_does_not_go_by_the_pages_address(lib, shape):
+    """Asked for before the pages are there, it is what the call wants."""
+    sizes = []
+    for address in (None, 256):
+        p = paged_params(n_head=8, n_kv_head=1, head_dim=128, page_size=64, pages=600, table_width=136, max_context=8704, key_pages=address, value_pages=address, **shape)
+        n = C.c_int64()
+        assert lib.gn_attention_paged_workspace(C.byref(p), C.byref(n)) == 0
+        sizes.append(n.value)
+    assert sizes[0] == sizes[1]
+    # the packed keys and values of a chunk: 4 bytes an element of 4 x 8704 keys and as many values
+    assert sizes[0] > (2 * 4 * 8704 * 128 * 4 if shape["max_query"] > 2 else 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 3, 40])
+def test_a_pool_without_pages(count):
+    """No key is there: zeros and -inf, by every kernel."""
+    q = torch.randn(2 * count, 8, 64, device=DEVICE)
+    pages = torch.zeros(0, 2, 16, 64, device=DEVICE)
+    new = torch.randn(2 * count, 2, 64, device=DEVICE)
+    out, lse = streaming.paged_attention(q, pages, pages.clone(), torch.zeros(2, 0, dtype=torch.int32, device=DEVICE), ints(0, count, 2 * count), ints(0, 0), count,
+                                         new_key=new, new_value=new, out=torch.full_like(q, 3.0))
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
