@@ -341,13 +341,13 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         w += gridDim.x;
         if (w < items) it = get_item<PAGED>(p, before, w);   // the next item's geometry is on its way while this one runs
         if (n == 0) continue;
-        if (!products) ok = hold(q_ready(count), (count >> 2) & 1);
+        if (!products) ok = hold_warp(q_ready(count), (count >> 2) & 1);
         for (int j = 0; j < n && ok; ++j, ++tile) {
           const int rows = j + 1 == n ? last16 : kRowsT, b = tile & 1;
           const uint32_t m = ring + (products ? min(2 * j + 2, 2 * n - 1) : j == 0 ? 0 : 2 * j - 1), slot = m % RING;
-          ok = hold(full(slot), (m / RING) & 1);
-          if (products) ok = ok && hold(p_full(b), (tile >> 1) & 1) && (tile == 0 || hold(o_empty, (tile - 1) & 1));
-          else ok = ok && (tile < 2 || hold(s_free(b), ((tile >> 1) - 1) & 1));
+          ok = hold_warp(full(slot), (m / RING) & 1);
+          if (products) ok = ok && hold_warp(p_full(b), (tile >> 1) & 1) && (tile == 0 || hold_warp(o_empty, (tile - 1) & 1));
+          else ok = ok && (tile < 2 || hold_warp(s_free(b), ((tile >> 1) - 1) & 1));
           if (!ok) break;
           tc_fence_after();
           if (products) {
@@ -443,13 +443,15 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
 #pragma unroll
             for (int e = 0; e < 8; ++e) stash[e * 128 + row] = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
           } else {
-            if (h == 1 && pass == 0 && count > 0) { ok = ok && hold(q_free, (count - 1) & 1); tc_fence_after(); }
+            if (h == 1 && pass == 0 && count > 0) { ok = ok && hold_warp(q_free, (count - 1) & 1); tc_fence_after(); }
+            __syncwarp();
             tmem_st32(q_addr + h * 32, y);
           }
         }
         uint32_t y[32];
 #pragma unroll
         for (int e = 0; e < 8; ++e) { const uint4 v = stash[e * 128 + row]; y[4 * e] = v.x; y[4 * e + 1] = v.y; y[4 * e + 2] = v.z; y[4 * e + 3] = v.w; }
+        __syncwarp();
         tmem_st32(q_addr, y);
         const float largest = __uint_as_float(top) * sq;
         const bool again = top != 0 && !(largest >= 0x1p7f && largest < 0x1p15f);
@@ -474,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     float* xch = reinterpret_cast<float*>(gen + XCH);   // [2][4 parts][128] maxima, then [4 parts][128] sums
     const float* rowc = reinterpret_cast<const float*>(gen + ROWC);
-    auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory"); };   // the four warps of these 32 rows
+    auto meet = [&]() { __syncwarp(); asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory"); };   // the four warps of these 32 rows
     bool ok = true;
     uint32_t tiles = 0, count = 0;
     float m = -INFINITY, l = 0.0f, alpha = 0.0f;   // l of a poisoned row is not a number
@@ -483,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
     struct Target { float* out; float* lse; float iv; } to{nullptr, nullptr, 1.0f};
 
     auto gather = [&]() {   // O of the last tile, against the maximum that it used
-      ok = ok && hold(o_full, (tiles - 1) & 1);
+      ok = ok && hold_warp(o_full, (tiles - 1) & 1);
       tc_fence_after();
       uint32_t y[QC];
       if constexpr (QC == 32) tmem_ld32(lane_addr + COL_O + part * QC, y);
@@ -546,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       const int s_end = live ? max(0, min(s.sinks, pos + 1)) : 0;
       const int lo_key = live ? (s.window < 0 ? 0 : max(0, pos - s.window)) - it.runs.shift : 0, hi_key = live ? pos - it.runs.shift : -1;
       const bool odd_plane = (p.pk.odd[it.plane * 2] | p.pk.odd[it.plane * 2 + 1]) != 0;
-      ok = ok && hold(q_ready(count), (count >> 2) & 1);
+      ok = ok && hold_warp(q_ready(count), (count >> 2) & 1);
       const float c = rowc[(count & 3) * 128 + row];
       ++count;
       m = -INFINITY; l = 0.0f;
@@ -567,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
               else if (flag & kOdd) l = NAN;
             }
         }
-        ok = ok && hold(s_full(tiles & 1), (tiles >> 1) & 1);
+        ok = ok && hold_warp(s_full(tiles & 1), (tiles >> 1) & 1);
         tc_fence_after();
         uint32_t y[32];
         tmem_ld32(buf, y);
@@ -607,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
       store();
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 20) tmem_dealloc(tmem, 512);

@@ -103,8 +103,8 @@ int stream_tc_backward(const StreamRows& s, const gn_view& out, const gn_view& d
 #ifdef __CUDACC__
 namespace {
 
-// Bounded wait in which the hardware holds the thread back (up to 2 us a try): sixteen warps that poll instead take the issue slots and the
-// shared memory from the others, which made the fetching of Q four times slower.  False when the bound (about a second) ran out.
+// Bounded wait of one thread in which the hardware holds it back (up to 2 us a try): sixteen warps that poll instead take the issue slots and the
+// shared memory from the others, which made the fetching of Q four times slower.  False when the tries (up to about a second) ran out.
 __device__ __forceinline__ bool hold(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < (1u << 19); ++i) {
     uint32_t ok;
@@ -113,6 +113,13 @@ __device__ __forceinline__ bool hold(uint32_t bar, uint32_t parity) {
     if (ok) return true;
   }
   return false;
+}
+// The same for a whole warp, whose lanes may leave the loop on different tries: they meet before they go on, because warp-aligned instructions
+// (tensor memory, named barriers) follow, and all of them take the same answer.
+__device__ __forceinline__ bool hold_warp(uint32_t bar, uint32_t parity) {
+  const bool ok = __all_sync(0xffffffffu, hold(bar, parity));
+  __syncwarp();
+  return ok;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");

@@ -222,6 +222,7 @@ __device__ __forceinline__ void store_pairs(uint32_t taddr, const float (&x)[16]
   uint32_t y[16];
 #pragma unroll
   for (int e = 0; e < 16; e += 2) split_f16(x[e], x[e + 1], y[e >> 1], y[8 + (e >> 1)]);
+  __syncwarp();
   tmem_st16(taddr, y);
   tmem_st_wait();
 }
@@ -233,6 +234,7 @@ __device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint8_t* block
     const uint4 v = *reinterpret_cast<const uint4*>(block + row * 128 + (((half * 4 + c) ^ (row & 7)) << 4));
     y[4 * c] = v.x; y[4 * c + 1] = v.y; y[4 * c + 2] = v.z; y[4 * c + 3] = v.w;
   }
+  __syncwarp();
   tmem_st16(taddr, y);
 }
 // A thread's QC channels, from ch on, of a gradient row (dst null: no row); a warp's 32 threads hold as many rows.
@@ -360,13 +362,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     if (warp == 16 && n > 0) {
       // ----------------------------------------------------------- scores: S^T(0), dP^T(0), S^T(1), dP^T(1), ...
       const uint32_t el = elect_lane();
-      bool ok = hold(v_full, 0) && hold(kh_ready, 0);
+      bool ok = hold_warp(v_full, 0) && hold_warp(kh_ready, 0);
       tc_fence_after();
       const uint64_t kl = smem_desc_sw128(base + OFF_KL), vd = smem_desc_sw128(base);
       for (int i = 0; i < n && ok; ++i) {
         const int b2 = i & 1;
         const uint32_t id = instr_desc_f16(128, rows16(i), 0);
-        ok = hold(q_full(b2), (i >> 1) & 1) && (i < 2 || hold(s_free(b2), ((i >> 1) - 1) & 1));
+        ok = hold_warp(q_full(b2), (i >> 1) & 1) && (i < 2 || hold_warp(s_free(b2), ((i >> 1) - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         {
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
           for (int ks = 0; ks < CB * 4; ++ks) umma_f16_ts(el, d, tmem + COL_KH + ks * 8, q + (ks >> 2) * 1024 + (ks & 3) * 2, id, 1);
           commit_by(el, s_full(b2));
         }
-        ok = hold(g_full(b2), (i >> 1) & 1) && (i < 1 || hold(dp_free, (i - 1) & 1));
+        ok = hold_warp(g_full(b2), (i >> 1) & 1) && (i < 1 || hold_warp(dp_free, (i - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         {
@@ -418,13 +420,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       for (int i = 0; i < n && ok; ++i) {
         const int b2 = i & 1, slices = rows16(i) >> 4;
         const uint32_t fresh = i % kFlush == 0 ? 0u : 1u;
-        ok = hold(p_full(b2), (i >> 1) & 1) && hold(g_full(b2), (i >> 1) & 1) && (fresh || i == 0 || hold(acc_empty, (i / kFlush - 1) & 1));
+        ok = hold_warp(p_full(b2), (i >> 1) & 1) && hold_warp(g_full(b2), (i >> 1) & 1) && (fresh || i == 0 || hold_warp(acc_empty, (i / kFlush - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         accumulate(tmem + COL_DV, tmem + COL_S + b2 * 64, base + OFF_G + b2 * SLOT, slices, fresh);
         commit_by(el, v_done(b2));
         commit_by(el, g_empty(b2));
-        ok = hold(ds_full, i & 1);
+        ok = hold_warp(ds_full, i & 1);
         if (!ok) break;
         tc_fence_after();
         accumulate(tmem + COL_DK, tmem + COL_S + b2 * 64, base + OFF_Q + b2 * SLOT, slices, fresh);
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     const PlaneFactors fc = plane_factors(p, plane);
     bool ok = true;
     if (n > 0) {
-      ok = hold(kh_full, 0);
+      ok = hold_warp(kh_full, 0);
       if (part < 2 * CB) row_to_tmem(lane_addr + COL_KH + part * 16, gen + OFF_G + SLOT + (part >> 1) * 16384, row, part & 1);
       tmem_st_wait();
       tc_fence_before();
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
 #pragma unroll
     for (int e = 0; e < QC; ++e) dv[e] = dk[e] = 0.0f;
     auto flush = [&](int chunk) {
-      ok = ok && hold(acc_full, chunk & 1);
+      ok = ok && hold_warp(acc_full, chunk & 1);
       tc_fence_after();
       add_columns<QC>(lane_addr + COL_DV + part * QC, dv);
       add_columns<QC>(lane_addr + COL_DK + part * QC, dk);
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       const uint32_t see = (uint32_t)(bits_below(f_hi - f0) & ~bits_below(f_lo - f0));
       const float4* off = reinterpret_cast<const float4*>(gen + STATS + (i & 1) * 512 + part * 64);
       float w[16];
-      ok = ok && hold(q_full(i & 1), (i >> 1) & 1) && hold(s_full(i & 1), (i >> 1) & 1);
+      ok = ok && hold_warp(q_full(i & 1), (i >> 1) & 1) && hold_warp(s_full(i & 1), (i >> 1) & 1);
       tc_fence_after();
       {
         uint32_t y[16];
@@ -488,7 +490,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       tc_fence_before();
       mbar_arrive(p_full(i & 1));
       if (i > 0 && i % kFlush == 0) flush(i / kFlush - 1);
-      ok = ok && hold(dp_full, i & 1);
+      ok = ok && hold_warp(dp_full, i & 1);
       tc_fence_after();
       {
         uint32_t y[16];
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
 #pragma unroll
         for (int e = 0; e < 16; ++e) if (!((see >> e) & 1u)) w[e] = 0.0f;   // what stands in a masked place may not be a number
       }
-      ok = ok && hold(v_done(i & 1), (i >> 1) & 1);
+      ok = ok && hold_warp(v_done(i & 1), (i >> 1) & 1);
       tc_fence_after();
       store_pairs(lane_addr + COL_S + (i & 1) * 64 + part * 16, w);
       tc_fence_before();
@@ -524,6 +526,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       write_row<QC>(key < s.seq ? p.dk.data + token_offset<false>(p.dk, r, hk, key) : nullptr, part * QC, s.D, dk, zk, p.accumulate, p.vec_dkv);
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 16) tmem_dealloc(tmem, 512);
@@ -660,12 +663,12 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     if (warp == 16 && n > 0) {
       // ----------------------------------------------------------- scores
       const uint32_t el = elect_lane();
-      bool ok = hold(lo_full, 0) && hold(hi_ready, 0);
+      bool ok = hold_warp(lo_full, 0) && hold_warp(hi_ready, 0);
       tc_fence_after();
       for (int j = 0; j < n && ok; ++j) {
         const uint32_t id = instr_desc_f16(128, rows16(j), 0);
         for (int w = 0; w < 2 && ok; ++w) {
-          ok = w ? hold(v_full(j & 1), (j >> 1) & 1) : hold(k_full(j % 3), (j / 3) & 1) && (j < 2 || hold(ds_free(j & 1), ((j >> 1) - 1) & 1));
+          ok = w ? hold_warp(v_full(j & 1), (j >> 1) & 1) : hold_warp(k_full(j % 3), (j / 3) & 1) && (j < 2 || hold_warp(ds_free(j & 1), ((j >> 1) - 1) & 1));
           if (!ok) break;
           tc_fence_after();
           const uint32_t d = tmem + (w ? COL_DP : COL_S) + (j & 1) * 64, hi = tmem + (w ? COL_G : COL_Q);
@@ -690,7 +693,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
         const uint32_t fresh = j % kFlush == 0 ? 0u : 1u;
-        ok = hold(ds_full(j & 1), (j >> 1) & 1) && hold(k_full(j % 3), (j / 3) & 1) && (fresh || j == 0 || hold(acc_empty, (j / kFlush - 1) & 1));
+        ok = hold_warp(ds_full(j & 1), (j >> 1) & 1) && hold_warp(k_full(j % 3), (j / 3) & 1) && (fresh || j == 0 || hold_warp(acc_empty, (j / kFlush - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         const uint32_t a = tmem + COL_DP + (j & 1) * 64;
@@ -718,7 +721,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     float off = 0.0f, delta = 0.0f;
     bool ok = true;
     if (n > 0) {
-      ok = hold(hi_full, 0);
+      ok = hold_warp(hi_full, 0);
 #pragma unroll
       for (int w = 0; w < 2; ++w)
         if (part < 2 * CB)
@@ -734,7 +737,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
 #pragma unroll
     for (int e = 0; e < QC; ++e) acc[e] = 0.0f;
     auto flush = [&](int chunk) {   // one step later, as above
-      ok = ok && hold(acc_full, chunk & 1);
+      ok = ok && hold_warp(acc_full, chunk & 1);
       tc_fence_after();
       add_columns<QC>(lane_addr + COL_DQ + part * QC, acc);
       tc_fence_before();
@@ -744,7 +747,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     for (int j = 0; j < n; ++j) {
       const int c0 = j * 64 + part * 16;
       const uint32_t see = (uint32_t)(bits_below(s_end - c0) | (bits_below(hi_key + 1 - c0) & ~bits_below(lo_key - c0)));
-      ok = ok && hold(sp_full(j & 1), (j >> 1) & 1);
+      ok = ok && hold_warp(sp_full(j & 1), (j >> 1) & 1);
       tc_fence_after();
       float w[16];
       {
@@ -767,6 +770,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     if (n > 0) flush((n - 1) / kFlush);
     write_row<QC>(f < s.seq * s.G ? p.dq.data + token_offset<false>(p.dq, r, h, t) : nullptr, part * QC, s.D, acc, ok ? fc.dq : NAN, p.accumulate, p.vec_dq);
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 16) tmem_dealloc(tmem, 512);

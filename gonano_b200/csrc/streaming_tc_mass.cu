@@ -143,10 +143,10 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
   } else if (warp == 16) {
     if (n > 0) {
       const uint32_t el = elect_lane();
-      bool ok = hold(k_full, 0);
+      bool ok = hold_warp(k_full, 0);
       const uint64_t a = smem_desc_sw128(base);
       for (int i = 0; i < n && ok; ++i) {
-        ok = hold(q_full(i & 1), (i >> 1) & 1) && (i < 2 || hold(s_empty(i & 1), ((i >> 1) - 1) & 1));
+        ok = hold_warp(q_full(i & 1), (i >> 1) & 1) && (i < 2 || hold_warp(s_empty(i & 1), ((i >> 1) - 1) & 1));
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + (i & 1) * 128, id = instr_desc_f16(128, rows16(i), 0);
@@ -178,7 +178,8 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
       const int f0 = f_begin + i * 128 + part * 32;
       const uint32_t see = (uint32_t)(bits_below(f_hi - f0) & ~bits_below(f_lo - f0));
       const float* st = reinterpret_cast<const float*>(gen + STATS + (i & 1) * 1024) + part * 32;
-      ok = ok && hold(q_full(i & 1), (i >> 1) & 1) && hold(s_full(i & 1), (i >> 1) & 1);
+      ok = ok && hold_warp(q_full(i & 1), (i >> 1) & 1) && hold_warp(s_full(i & 1), (i >> 1) & 1);
+      __syncwarp();
       tc_fence_after();
       uint32_t y[32];
       tmem_ld32(lane_addr + (i & 1) * 128 + part * 32, y);
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
     }
     float* sums = reinterpret_cast<float*>(gen + SUMS);
     sums[part * 128 + row] = ok ? sum : NAN;
+    __syncwarp();
     asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
     if (part == 0 && key < sp.ctx) {
       const float total = (sums[row] + sums[128 + row]) + (sums[256 + row] + sums[384 + row]);
@@ -202,6 +204,7 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
       p.mass_out[at] = (p.mass && key < first ? p.mass[at] : 0.0f) + total;
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 16) tmem_dealloc(tmem, 256);
