@@ -383,6 +383,13 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         ++count;
         ring += 2 * n;
       }
+      // What the instructions still signal, nobody else waits for: it has arrived before this CTA's shared memory goes to another
+      if (products) {
+        for (uint32_t t = tile < 2 ? 0 : tile - 2; t < tile && ok; ++t) ok = hold_warp(s_free(t & 1), (t >> 1) & 1);
+      } else {
+        for (uint32_t m = ring < RING ? 0 : ring - RING; m < ring && ok; ++m) ok = hold_warp(empty(m % RING), (m / RING) & 1);
+        if (count > 0 && ok) hold_warp(q_free, (count - 1) & 1);
+      }
     }
   } else if (warp >= 16) {
     // --------------------------------------------------------------- Q rows to tensor memory

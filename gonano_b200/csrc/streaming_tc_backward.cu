@@ -434,6 +434,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         commit_by(el, s_free(b2));
         if ((i + 1) % kFlush == 0 || i + 1 == n) commit_by(el, acc_full);
       }
+      // what the instructions still signal, nobody else waits for: it has arrived before this CTA's shared memory goes to another
+      for (int i = max(0, n - 2); i < n && ok; ++i)
+        ok = hold_warp(q_empty(i & 1), (i >> 1) & 1) && hold_warp(g_empty(i & 1), (i >> 1) & 1) && hold_warp(s_free(i & 1), (i >> 1) & 1);
     }
   } else {
     regs_inc<kRegsSoftmax>();
@@ -686,6 +689,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
         commit_by(el, v_empty(j & 1));
         commit_by(el, sp_full(j & 1));
       }
+      for (int j = max(0, n - 2); j < n && ok; ++j) ok = hold_warp(v_empty(j & 1), (j >> 1) & 1);   // the last signals, as above
     }
     if (warp == 18 && n > 0) {
       // ----------------------------------------------------------- sums
@@ -710,6 +714,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
         commit_by(el, ds_free(j & 1));
         if ((j + 1) % kFlush == 0 || j + 1 == n) commit_by(el, acc_full);
       }
+      for (int j = max(0, n - 3); j < n && ok; ++j)
+        ok = hold_warp(k_empty(j % 3), (j / 3) & 1) && (j + 2 < n || hold_warp(ds_free(j & 1), (j >> 1) & 1));
     }
   } else {
     regs_inc<kRegsSoftmax>();

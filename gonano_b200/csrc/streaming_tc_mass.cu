@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
         commit_by(el, s_full(i & 1));
         commit_by(el, q_empty(i & 1));
       }
+      for (int i = max(0, n - 2); i < n && ok; ++i) ok = hold_warp(q_empty(i & 1), (i >> 1) & 1);   // nobody else waits for the last ones
     }
   } else if (warp < 16) {
     const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane, key = k0 + row;
