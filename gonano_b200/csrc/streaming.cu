@@ -189,6 +189,8 @@ int gn_cache_evict(const gn_evict_params* p, int32_t* kept, int32_t* new_lens, f
              "cache_evict: bad shape");
   GN_REQUIRE(p->budget >= 0 && p->sinks >= 0 && p->recent >= 0 && (int64_t)p->sinks + p->recent <= p->budget, "cache_evict: sinks %d + recent %d exceed the budget %d",
              p->sinks, p->recent, p->budget);
+  GN_REQUIRE((int64_t)p->table_width * p->page_size <= kFar && p->budget <= kFar, "cache_evict: a table of %lld keys a row or a budget of %d exceeds 2^30",
+             (long long)p->table_width * p->page_size, p->budget);   // indices that step over them stay in 32 bits
   GN_REQUIRE(p->max_context >= 0 && (int64_t)p->max_context <= (int64_t)p->table_width * p->page_size && p->max_context <= p->mass_stride,
              "cache_evict: max_context %d, but a row holds %lld keys and %d masses", p->max_context, (long long)p->table_width * p->page_size, p->mass_stride);
   GN_REQUIRE((int64_t)p->new_width * p->page_size >= std::min(p->budget, p->max_context), "cache_evict: new_table holds %lld keys a row, %d are kept",

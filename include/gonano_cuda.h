@@ -295,7 +295,7 @@ typedef struct gn_evict_params {
   const int32_t* new_table;        /* [rows, new_width], new_width * page_size >= budget */
   const int32_t* context_lens;     /* [rows] */
   int32_t rows, n_kv_head, head_dim, page_size, pages, table_width, new_width, mass_stride;
-  int32_t max_context, budget, sinks, recent; /* sinks + recent <= budget; max_context as above */
+  int32_t max_context, budget, sinks, recent; /* sinks + recent <= budget; max_context as above; budget and table_width * page_size up to 2^30 */
 } gn_evict_params;
 
 /* kept [rows, n_kv_head, budget]: the indices that the kept keys had (-1 behind them); new_lens [rows]; mass_out [rows, n_kv_head,

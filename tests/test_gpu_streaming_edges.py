@@ -10,7 +10,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from gonano_b200 import _lib, streaming  # noqa: E402
-from test_gpu_streaming import DEVICE, paged_params  # noqa: E402
+from test_gpu_streaming import DEVICE, evict_params, paged_params  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -50,3 +50,15 @@ def test_a_pool_without_pages(count):
     out, lse = streaming.paged_attention(q, pages, pages.clone(), torch.zeros(2, 0, dtype=torch.int32, device=DEVICE), ints(0, count, 2 * count), ints(0, 0), count,
                                          new_key=new, new_value=new, out=torch.full_like(q, 3.0))
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+# ---------------------------------------------------------------- eviction
+
+@pytest.mark.parametrize("over", [dict(budget=2 ** 30 + 1, new_width=2 ** 27), dict(budget=2 ** 31 - 1, new_width=2 ** 28), dict(table_width=2 ** 27, max_context=32),
+                                  dict(table_width=2 ** 30 // 16 + 1, max_context=32)])
+def test_evict_refuses_more_keys_than_its_indices_count(lib, over):
+    """Steps of a block over 2^31 keys would leave 32 bits: refused, whatever the rows."""
+    for rows in (0, 2):
+        assert lib.gn_cache_evict(C.byref(evict_params(rows=rows, **over)), None, None, None, None) == 1
+        assert b"exceeds 2^30" in lib.gn_last_error()
+    assert lib.gn_cache_evict(C.byref(evict_params(rows=0, table_width=2 ** 26, new_width=2 ** 26, budget=2 ** 30, max_context=32)), None, None, None, None) == 0
