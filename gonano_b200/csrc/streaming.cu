@@ -49,6 +49,11 @@ bool apart(const gn_view& v, int64_t batch, int64_t heads, int64_t tokens, int64
   }
   return true;
 }
+// Whether two pieces of memory have a byte in common.
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
+}
 bool strides_ok(const gn_view& v) { return v.batch_stride >= 0 && v.head_stride >= 0 && v.token_stride >= 0; }
 
 constexpr int kFar = 1 << 30;   // no sequence is longer: wider windows and more sinks are cut to it, so that sums with positions stay in 32 bits
@@ -198,7 +203,16 @@ int gn_cache_evict(const gn_evict_params* p, int32_t* kept, int32_t* new_lens, f
   if (!p->rows) return GN_OK;
   GN_REQUIRE(p->context_lens && new_lens && (p->budget == 0 || kept), "cache_evict: null argument");
   GN_REQUIRE(p->max_context == 0 || (p->key_pages && p->value_pages && p->mass && p->page_table && (p->new_table || p->budget == 0)), "cache_evict: null argument");
-  GN_REQUIRE(mass_out == nullptr || mass_out != p->mass, "cache_evict: mass_out must not be mass");
+  // Blocks write the outputs while others still read the inputs (a row's length by the blocks of its other heads and by the move)
+  const int64_t planes = (int64_t)p->rows * p->n_kv_head, store = (int64_t)p->pages * p->n_kv_head * p->page_size * p->head_dim * 4;
+  const struct { const char* name; const void* at; int64_t bytes; } outs[] = {{"kept", kept, planes * p->budget * 4}, {"new_lens", new_lens, p->rows * 4ll},
+                                                                              {"mass_out", mass_out, planes * p->budget * 4}},
+      ins[] = {{"context_lens", p->context_lens, p->rows * 4ll}, {"mass", p->mass, planes * p->mass_stride * 4}, {"page_table", p->page_table, (int64_t)p->rows * p->table_width * 4},
+               {"new_table", p->new_table, (int64_t)p->rows * p->new_width * 4}, {"key_pages", p->key_pages, store}, {"value_pages", p->value_pages, store}};
+  for (int i = 0; i < 3; ++i) {
+    for (const auto& in : ins) GN_REQUIRE(!overlap(outs[i].at, outs[i].bytes, in.at, in.bytes), "cache_evict: %s shares memory with %s", outs[i].name, in.name);
+    for (int j = 0; j < i; ++j) GN_REQUIRE(!overlap(outs[i].at, outs[i].bytes, outs[j].at, outs[j].bytes), "cache_evict: %s shares memory with %s", outs[i].name, outs[j].name);
+  }
   const void* ptrs[] = {p->context_lens, new_lens, kept, p->key_pages, p->value_pages, p->mass, p->page_table, p->new_table, mass_out};
   for (const void* x : ptrs) if (x) GN_TRY(on_this_device(x, "cache_evict"));
   return stream_evict(*p, kept, new_lens, mass_out, (cudaStream_t)stream);

@@ -62,3 +62,32 @@ def test_evict_refuses_more_keys_than_its_indices_count(lib, over):
         assert lib.gn_cache_evict(C.byref(evict_params(rows=rows, **over)), None, None, None, None) == 1
         assert b"exceeds 2^30" in lib.gn_last_error()
     assert lib.gn_cache_evict(C.byref(evict_params(rows=0, table_width=2 ** 26, new_width=2 ** 26, budget=2 ** 30, max_context=32)), None, None, None, None) == 0
+
+
+EVICT_BUFFERS = dict(key_pages=2 ** 20, value_pages=2 ** 21, mass=2 ** 22, page_table=2 ** 23, new_table=2 ** 24, context_lens=2 ** 25)   # addresses that are never read
+EVICT_OUTPUTS = [2 ** 26, 2 ** 27, 2 ** 28]   # kept, new_lens, mass_out
+
+
+@pytest.mark.parametrize("which,at", [(1, 2 ** 25), (1, 2 ** 25 + 4), (2, 2 ** 22), (2, 2 ** 22 + 64), (0, 2 ** 23), (1, 2 ** 24 + 12), (0, 2 ** 27), (2, 2 ** 26 - 4), (0, 2 ** 20 + 40),
+                                      (2, 2 ** 21)])
+def test_evict_refuses_shared_memory(lib, which, at):
+    """Lengths written over the lengths that are read, weights over the weights, and so on: the answer would go by which block came first."""
+    outputs = list(EVICT_OUTPUTS)
+    outputs[which] = at
+    assert lib.gn_cache_evict(C.byref(evict_params(**EVICT_BUFFERS)), *outputs, None) == 1
+    assert b"shares memory" in lib.gn_last_error()
+
+
+@pytest.mark.gpu
+def test_evict_buffers_side_by_side(lib):
+    """Outputs directly behind one another and behind the lengths that are read are no shared memory."""
+    rows, heads, n, budget = 2, 2, 32, 16
+    pages = torch.randn(2, 4, heads, 16, 64, device=DEVICE)
+    mass = torch.rand(rows, heads, n, device=DEVICE)
+    table = ints(0, 1, 2, 3).view(rows, 2)
+    room = torch.cat([ints(32, 20), torch.full((rows + rows * heads * budget,), -9, dtype=torch.int32, device=DEVICE)])
+    want = streaming.evict_pages(pages[0].clone(), pages[1].clone(), mass, table, ints(32, 20), budget, 1, 2)
+    p = evict_params(key_pages=pages[0].data_ptr(), value_pages=pages[1].data_ptr(), mass=mass.data_ptr(), page_table=table.data_ptr(), new_table=table.data_ptr(),
+                     context_lens=room.data_ptr())
+    assert lib.gn_cache_evict(C.byref(p), room[2 * rows:].data_ptr(), room[rows:].data_ptr(), None, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(room[rows:2 * rows], want[1]) and torch.equal(room[2 * rows:].view_as(want[0]), want[0])
