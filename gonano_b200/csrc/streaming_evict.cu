@@ -129,7 +129,59 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   if (hk == 0 && tid == 0) e.new_lens[r] = keep;
 }
 
-// To pages of their own: every kept key on its own.  A CTA per (64 kept keys, kv head, row x {key, value}); with 16-byte accesses
+// A row's kept keys to slots that may be its own: the slots are filled in ascending order, KEYS at a time, every read of a group before its
+// writes: slot i <= kept[i], so a group writes only what it or earlier groups have read.  256 threads do a (row, kv head)'s channels c0 .. c0 + 31.
+template <int KEYS>
+__device__ __forceinline__ void move_row(const Evict& e, int hk, int r, float* pages, int c0, int64_t (&from)[KEYS], int64_t (&to)[KEYS]) {
+  const gn_evict_params& p = e.p;
+  const int tid = threadIdx.x, keep = min(evict_len(p, r), p.budget);
+  const int32_t* kept = e.kept + ((int64_t)r * p.n_kv_head + hk) * p.budget;
+  for (int i0 = 0; i0 < keep; i0 += KEYS) {
+    __syncthreads();
+    if (tid < KEYS) {
+      const int i = i0 + tid;
+      from[tid] = i < keep ? slot_of(p, p.page_table, p.table_width, r, hk, kept[i]) : -1;
+      to[tid] = i < keep ? slot_of(p, p.new_table, p.new_width, r, hk, i) : -1;
+    }
+    __syncthreads();
+    if (e.vec) {   // 8 threads carry a key's 32 channels
+      const int c = c0 + (tid & 7) * 4;
+      const bool in = c < p.head_dim;
+      float4 x[KEYS / 32];
+#pragma unroll
+      for (int u = 0; u < KEYS / 32; ++u) {
+        const int k = (tid >> 3) + u * 32;
+        x[u] = make_float4(0, 0, 0, 0);
+        if (in && from[k] >= 0) x[u] = *reinterpret_cast<const float4*>(pages + from[k] + c);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < KEYS / 32; ++u) {
+        const int k = (tid >> 3) + u * 32;
+        if (in && to[k] >= 0) *reinterpret_cast<float4*>(pages + to[k] + c) = x[u];
+      }
+    } else {
+      const int c = c0 + (tid & 31);
+      const bool in = c < p.head_dim;
+      float x[KEYS / 8];
+#pragma unroll
+      for (int u = 0; u < KEYS / 8; ++u) { const int k = (tid >> 5) + u * 8; x[u] = in && from[k] >= 0 ? pages[from[k] + c] : 0.0f; }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < KEYS / 8; ++u) { const int k = (tid >> 5) + u * 8; if (in && to[k] >= 0) pages[to[k] + c] = x[u]; }
+    }
+  }
+}
+
+// In place (new_table is page_table): a CTA per (32 channels, kv head, row x {key, value}).
+__global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ Evict e) {
+  pdl_wait();
+  __shared__ int64_t from[256], to[256];
+  const int r = blockIdx.z >> 1, n = evict_len(e.p, r);
+  if (n > e.p.budget) move_row(e, blockIdx.y, r, (blockIdx.z & 1) ? e.p.value_pages : e.p.key_pages, blockIdx.x * 32, from, to);   // else nothing moves
+}
+
+// To other pages: every kept key on its own.  A CTA per (64 kept keys, kv head, row x {key, value}); with 16-byte accesses
 // `lanes` threads carry a row, all reads of a thread before its writes.  Bound: HBM; 24 us for 32 rows of 2048 keys (67 MB read and written, 5.6 TB/s).
 __global__ void __launch_bounds__(256) evict_copy_kernel(const __grid_constant__ Evict e, int lanes) {
   pdl_wait();
@@ -140,6 +192,13 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(const __grid_constant__
   const int32_t* kept = e.kept + ((int64_t)r * p.n_kv_head + hk) * p.budget;
   float* pages = (blockIdx.z & 1) ? p.value_pages : p.key_pages;
   __shared__ int64_t from[64], to[64];
+  // A row that keeps a page of its own in its column (new_table may be a copy of page_table's first columns) goes in order, by the first blocks
+  int own = 0;
+  for (int c = threadIdx.x; (int64_t)c * p.page_size < keep; c += 256) own |= p.new_table[(int64_t)r * p.new_width + c] == p.page_table[(int64_t)r * p.table_width + c];
+  if (__syncthreads_or(own)) {
+    for (int c0 = blockIdx.x * 32; c0 < p.head_dim; c0 += (keep + 63) / 64 * 32) move_row(e, hk, r, pages, c0, from, to);
+    return;
+  }
   if (threadIdx.x < 64) {
     const int i = i0 + threadIdx.x;
     from[threadIdx.x] = i < keep ? slot_of(p, p.page_table, p.table_width, r, hk, kept[i]) : -1;
@@ -167,52 +226,6 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(const __grid_constant__
     for (int i = threadIdx.x; i < 64 * p.head_dim; i += 256) {
       const int k = i / p.head_dim, c = i % p.head_dim;
       if (to[k] >= 0) pages[to[k] + c] = from[k] >= 0 ? pages[from[k] + c] : 0.0f;
-    }
-  }
-}
-
-// In place: a CTA per (32 channels, kv head, row x {key, value}) fills the slots in ascending order, 256 at a time, every read of a
-// group before its writes: slot i <= kept[i], so a group writes only what it or earlier groups have read.
-__global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ Evict e) {
-  pdl_wait();
-  const gn_evict_params& p = e.p;
-  const int hk = blockIdx.y, r = blockIdx.z >> 1, c0 = blockIdx.x * 32, tid = threadIdx.x;
-  float* pages = (blockIdx.z & 1) ? p.value_pages : p.key_pages;
-  const int keep = min(evict_len(p, r), p.budget);
-  const int32_t* kept = e.kept + ((int64_t)r * p.n_kv_head + hk) * p.budget;
-  if (keep == 0 || keep == evict_len(p, r)) return;   // nothing to move
-  __shared__ int64_t from[256], to[256];
-  for (int i0 = 0; i0 < keep; i0 += 256) {
-    __syncthreads();
-    const int i = i0 + tid;
-    from[tid] = i < keep ? slot_of(p, p.page_table, p.table_width, r, hk, kept[i]) : -1;
-    to[tid] = i < keep ? slot_of(p, p.new_table, p.new_width, r, hk, i) : -1;
-    __syncthreads();
-    if (e.vec) {   // 8 threads carry a key's 32 channels
-      const int c = c0 + (tid & 7) * 4;
-      const bool in = c < p.head_dim;
-      float4 x[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int k = (tid >> 3) + u * 32;
-        x[u] = make_float4(0, 0, 0, 0);
-        if (in && from[k] >= 0) x[u] = *reinterpret_cast<const float4*>(pages + from[k] + c);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int k = (tid >> 3) + u * 32;
-        if (in && to[k] >= 0) *reinterpret_cast<float4*>(pages + to[k] + c) = x[u];
-      }
-    } else {
-      const int c = c0 + (tid & 31);
-      const bool in = c < p.head_dim;
-      float x[32];
-#pragma unroll
-      for (int u = 0; u < 32; ++u) { const int k = (tid >> 5) + u * 8; x[u] = in && from[k] >= 0 ? pages[from[k] + c] : 0.0f; }
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < 32; ++u) { const int k = (tid >> 5) + u * 8; if (in && to[k] >= 0) pages[to[k] + c] = x[u]; }
     }
   }
 }

@@ -191,8 +191,9 @@ def paged_attention(q, key_pages, value_pages, page_table, query_starts, context
 def evict_pages(key_pages, value_pages, mass, page_table, context_lens, budget, sinks=0, recent=0, new_table=None, max_context=None):
     """Keeps ``budget`` keys of every (row, kv head): the first ``sinks``, the last ``recent`` and of the others those of the largest
     ``mass`` ([rows, kv_heads, n], as ``paged_attention`` gathers it; ties to the lower index), in their order, moved to the front of
-    the row's pages in ``new_table`` (default: page_table itself, compaction in place - no page may then belong to two rows; else pages
-    that page_table does not name, which is how a prompt shared by several rows is left whole).  Rows of at most ``budget`` keys are kept whole.
+    the row's pages in ``new_table`` (default: page_table itself, compaction in place).  Every page there is the row's own page of the same
+    column - such a page may not belong to two rows - or one that page_table does not name, which is how a prompt shared by several rows is
+    left whole; ``page_table[:, :w].contiguous()`` compacts in place too.  Rows of at most ``budget`` keys are kept whole.
 
     Returns kept (int32 [rows, kv_heads, budget], the indices the keys had, -1 behind them), the new lengths (int32 [rows]) and the
     kept keys' mass [rows, kv_heads, budget]."""

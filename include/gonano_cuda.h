@@ -286,8 +286,9 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
 
 /* Keeps, for every row and kv head on its own, the first `sinks` keys, the last `recent` and of the others those of the largest
  * mass, `budget` in all (ties to the lower index, NaN below everything), in their order, and moves them to the front of the row's
- * pages in new_table.  A row of at most `budget` keys is kept whole.  new_table may be page_table itself (compaction in place; no
- * page may then belong to two rows) or name pages that page_table does not. */
+ * pages in new_table.  A row of at most `budget` keys is kept whole.  Every page of new_table is the row's own page of the
+ * same column (new_table is page_table or a copy of its first columns: compaction in place; such a page may not belong to two rows) or
+ * one that page_table does not name. */
 typedef struct gn_evict_params {
   float *key_pages, *value_pages;  /* [pages, n_kv_head, page_size, head_dim] */
   const float* mass;               /* [rows, n_kv_head, mass_stride] */

@@ -10,7 +10,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from gonano_b200 import _lib, streaming  # noqa: E402
-from test_gpu_streaming import DEVICE, evict_params, paged_params  # noqa: E402
+from test_gpu_streaming import DEVICE, Cache, evict64, evict_params, paged_params  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -91,3 +91,35 @@ def test_evict_buffers_side_by_side(lib):
                      context_lens=room.data_ptr())
     assert lib.gn_cache_evict(C.byref(p), room[2 * rows:].data_ptr(), room[rows:].data_ptr(), None, torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(room[rows:2 * rows], want[1]) and torch.equal(room[2 * rows:].view_as(want[0]), want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 16), (33, 1), (80, 7)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_evict_to_a_copy_of_the_own_pages(dim, page, mixed):
+    """new_table a narrower copy of page_table: in place, though it is another tensor.  Mixed: every second page is a fresh one."""
+    lens, heads, budget, sinks, recent = [1300, 900, 500, 20, 0], 2, 600, 3, 100
+    width, kept_pages = -(-1300 // page), -(-budget // page)
+    cache = Cache(len(lens), heads, dim, page, width + kept_pages, seed=30)
+    cache.fill(lens)
+    table, target = cache.table[:, :width].contiguous(), cache.table[:, :kept_pages].contiguous()
+    if mixed:
+        target[:, 1::2] = cache.table[:, width:width + kept_pages][:, 1::2]
+    mass = torch.rand(len(lens), heads, width * page, generator=cache.gen, device=DEVICE)
+    want = evict64(mass.cpu(), lens, budget, sinks, recent)
+    for _ in range(5):   # an order left to chance shows in some of the calls
+        k, v = cache.k.clone(), cache.v.clone()
+        kept, new_lens, _ = streaming.evict_pages(k, v, mass, table, ints(*lens), budget, sinks, recent, new_table=target)
+        assert new_lens.tolist() == [min(n, budget) for n in lens]
+        touched = torch.zeros(k.shape[:3], dtype=torch.bool, device=DEVICE)
+        for r in range(len(lens)):
+            for h in range(heads):
+                w = torch.tensor(want[r * heads + h], dtype=torch.long, device=DEVICE)
+                assert torch.equal(kept[r, h, :len(w)].long(), w)
+                slots = torch.arange(len(w), device=DEVICE)
+                src, dst = table[r].long()[w // page], target[r].long()[slots // page]
+                touched[dst, h, slots % page] = True
+                for now, then in ((k, cache.k), (v, cache.v)):
+                    assert torch.equal(now[dst, h, slots % page], then[src, h, w % page])
+        for now, then in ((k, cache.k), (v, cache.v)):
+            assert torch.equal(now[~touched].nan_to_num(9.0), then[~touched].nan_to_num(9.0))
