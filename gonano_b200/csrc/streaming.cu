@@ -21,6 +21,13 @@ __global__ void __launch_bounds__(128) stream_append_kernel(StreamRows s, gn_vie
   const float* a = nk.data + token_offset<true>(nk, r, hk, sp.q_begin + t); const float* b = nv.data + token_offset<true>(nv, r, hk, sp.q_begin + t);
   for (int c = lane; c < s.D; c += 32) { s.pages_k[to + c] = a[c]; s.pages_v[to + c] = b[c]; }
 }
+// A call without new tokens: every key keeps the weight that it has.
+__global__ void __launch_bounds__(256) stream_keep_mass_kernel(StreamRows s, const float* mass, float* mass_out) {
+  const int key = blockIdx.x * 256 + threadIdx.x, hk = blockIdx.y, r = blockIdx.z;
+  if (key >= min(s.lens[r], s.max_context)) return;
+  const int64_t at = ((int64_t)r * s.Hkv + hk) * s.width * s.page_size + key;
+  mass_out[at] = mass ? mass[at] : 0.0f;
+}
 // ------------------------------------------------------------------ checks
 int on_this_device(const void* p, const char* what) {
   int device = 0;
@@ -166,6 +173,12 @@ int gn_attention_paged_workspace(const gn_paged_params* p, int64_t* bytes) {
 int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   StreamRows s;
   GN_TRY(paged_rows(p, &s));
+  if (s.rows && !(s.tokens && s.max_query) && p->mass_out && p->mass_out != p->mass && s.max_context) {
+    GN_REQUIRE(p->context_lens, "attention_paged: null context_lens");
+    for (const void* x : {(const void*)p->context_lens, (const void*)p->mass, (const void*)p->mass_out}) if (x) GN_TRY(on_this_device(x, "attention_paged"));
+    stream_keep_mass_kernel<<<dim3(ceil_div(s.max_context, 256), s.Hkv, s.rows), 256, 0, (cudaStream_t)stream>>>(s, p->mass, p->mass_out);
+    GN_LAUNCH_CHECK();
+  }
   if (!s.rows || !s.tokens || !s.max_query) return GN_OK;
   GN_REQUIRE(p->query.data && p->query_starts && p->context_lens && out && out->data && lse, "attention_paged: null argument");
   GN_REQUIRE(p->max_context == 0 || (p->key_pages && p->value_pages && p->page_table), "attention_paged: null pages");

@@ -123,3 +123,30 @@ def test_evict_to_a_copy_of_the_own_pages(dim, page, mixed):
                     assert torch.equal(now[dst, h, slots % page], then[src, h, w % page])
         for now, then in ((k, cache.k), (v, cache.v)):
             assert torch.equal(now[~touched].nan_to_num(9.0), then[~touched].nan_to_num(9.0))
+
+
+# ---------------------------------------------------------------- weights
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,max_query", [(0, 4), (3, 0), (0, 0), (2, 1)])
+@pytest.mark.parametrize("start", ["mass", "nothing", "one buffer", "a copy"])
+def test_weights_of_a_step_without_tokens(tokens, max_query, start):
+    """No row has a new token: mass_out holds what mass holds (0 where there is none) up to every row's length, and is left as it is behind."""
+    lens, heads, page, width = [40, 0, 300, 512, 600], 2, 32, 16
+    cache = Cache(len(lens), heads, 64, page, width, seed=31)
+    mass = torch.rand(len(lens), heads, width * page, generator=cache.gen, device=DEVICE)
+    before, out = mass.clone(), torch.full_like(mass, 7.0)
+    q = torch.randn(tokens, 4, 64, device=DEVICE)
+    got = streaming.paged_attention(q, cache.k, cache.v, cache.table, ints(*[0] * (len(lens) + 1)), ints(*lens), max_query, scale=0.125,
+                                    mass=None if start == "nothing" else mass, mass_out={"one buffer": mass, "a copy": None}.get(start, out))[2]
+    assert torch.equal(mass, before)
+    for r, n in enumerate(lens):
+        assert torch.equal(got[r, :, :n], before[r, :, :n] * (0.0 if start == "nothing" else 1.0))
+        assert torch.equal(got[r, :, n:], (before if start in ("one buffer", "a copy") else torch.full_like(mass, 7.0))[r, :, n:])
+
+
+def test_weights_of_a_step_without_tokens_want_the_lengths(lib):
+    view = _lib.GnView(None, 64, 64, 64)
+    assert lib.gn_attention_paged(C.byref(paged_params(tokens=0, mass_out=2 ** 20)), C.byref(view), None, None, 0, None) == 1
+    assert b"context_lens" in lib.gn_last_error()
+    assert lib.gn_attention_paged(C.byref(paged_params(tokens=0, mass_out=2 ** 20, max_context=0)), C.byref(view), None, None, 0, None) == 0
