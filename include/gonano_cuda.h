@@ -272,7 +272,7 @@ typedef struct gn_paged_params {
   const int32_t* query_starts;     /* [rows + 1], ascending: row r's new tokens are query_starts[r] .. query_starts[r + 1] - 1 */
   const int32_t* context_lens;     /* [rows]: keys of the row, the new tokens' included; the new tokens stand at its end */
   const float* mass;               /* mass_out NULL: unused.  NULL, or [rows, n_kv_head, table_width * page_size]: the weight that each key has */
-  float* mass_out;                 /*   gathered so far (summed over queries and the heads of its group); mass_out (may be mass) gets it with this call's
+  float* mass_out;                 /*   gathered so far (summed over queries and the heads of its group); mass_out (mass itself, or apart from it) gets it with this call's
                                       added.  The new tokens' own keys start from 0; entries behind the row's length are left as they are. */
   int32_t rows, tokens, max_query; /* no row has more than max_query new tokens (further ones are left out) */
   int32_t max_context;             /* no row has more keys (further ones are left out) */
