@@ -111,9 +111,6 @@ int paged_rows(const gn_paged_params* p, StreamRows* s) {
   GN_REQUIRE((int64_t)p->max_query * (p->n_head / p->n_kv_head) < (1ll << 30), "attention_paged: max_query x heads of a group exceeds 2^30");
   GN_REQUIRE(p->sinks >= 0 && std::isfinite(p->scale), "attention_paged: bad sinks or scale");
   GN_REQUIRE(strides_ok(p->query) && strides_ok(p->new_key) && strides_ok(p->new_value), "attention_paged: negative stride");
-  // in one buffer a key's weight is read and written by one thread; in two that share a piece, another key's
-  const int64_t mass_bytes = (int64_t)p->rows * p->n_kv_head * p->table_width * p->page_size * 4;
-  GN_REQUIRE(p->mass == p->mass_out || !overlap(p->mass, mass_bytes, p->mass_out, mass_bytes), "attention_paged: mass and mass_out share a part of their memory");
   s->rows = p->rows; s->Hq = p->n_head; s->Hkv = p->n_kv_head; s->G = p->n_head / p->n_kv_head; s->by_G = FastDiv(s->G); s->D = p->head_dim;
   s->window = std::min(p->window, kFar); s->sinks = std::min(p->sinks, kFar); s->scale = p->scale; s->q = p->query;
   s->is_paged = true; s->pages_k = p->key_pages; s->pages_v = p->value_pages; s->table = p->page_table; s->starts = p->query_starts; s->lens = p->context_lens;
@@ -176,6 +173,9 @@ int gn_attention_paged_workspace(const gn_paged_params* p, int64_t* bytes) {
 int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   StreamRows s;
   GN_TRY(paged_rows(p, &s));
+  // in one buffer a key's weight is read and written by one thread; in two that share a piece, another key's
+  const int64_t mass_bytes = (int64_t)p->rows * p->n_kv_head * p->table_width * p->page_size * 4;
+  GN_REQUIRE(p->mass == p->mass_out || !overlap(p->mass, mass_bytes, p->mass_out, mass_bytes), "attention_paged: mass and mass_out share a part of their memory");
   if (s.rows && !(s.tokens && s.max_query) && p->mass_out && p->mass_out != p->mass && s.max_context) {
     GN_REQUIRE(p->context_lens, "attention_paged: null context_lens");
     for (const void* x : {(const void*)p->context_lens, (const void*)p->mass, (const void*)p->mass_out}) if (x) GN_TRY(on_this_device(x, "attention_paged"));
