@@ -23,6 +23,13 @@ def _refuse(message):
     raise GonanoError(message)
 
 
+def _counts(**values):
+    # a structure's 32-bit fields would take the low bits of larger numbers
+    for name, x in values.items():
+        if not -2 ** 31 <= x < 2 ** 31:
+            _refuse(f"{name}: {x} is outside 32 bits")
+
+
 def _want(name, dtype, shape, device):
     _refuse(f"{name}: want a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
 
@@ -93,6 +100,7 @@ def _address(tensor):
 
 
 def _sink_params(q, k, v, sinks, window, scale, lengths):
+    _counts(sinks=sinks, window=window)
     device = _cuda("q", q, 4)
     batch, heads, seq, dim = q.shape
     kv_heads = _shaped("k", k, 4, "[batch, kv_heads, seq, dim]")[1]
@@ -157,6 +165,7 @@ def paged_attention(q, key_pages, value_pages, page_table, query_starts, context
     Returns out (like q), lse [tokens, heads] and, when mass or mass_out is given, mass_out.  Entries behind the last row's tokens
     are left as they are (0 in tensors made here)."""
     lib = _lib.load()
+    _counts(max_query=max_query, max_context=0 if max_context is None else max_context, sinks=sinks, window=window)
     device = _cuda("q", q, 3)
     tokens, heads, dim = q.shape
     pages, kv_heads, page_size, _ = _shaped("key_pages", key_pages, 4, "[pages, kv_heads, page_size, dim]")
@@ -198,6 +207,7 @@ def evict_pages(key_pages, value_pages, mass, page_table, context_lens, budget, 
     Returns kept (int32 [rows, kv_heads, budget], the indices the keys had, -1 behind them), the new lengths (int32 [rows]) and the
     kept keys' mass [rows, kv_heads, budget]."""
     lib = _lib.load()
+    _counts(budget=budget, sinks=sinks, recent=recent, max_context=0 if max_context is None else max_context)
     device = _cuda("key_pages", key_pages, 4)
     pages, kv_heads, page_size, dim = store = key_pages.shape
     rows, width = _shaped("page_table", page_table, 2, "[rows, width]")

@@ -10,6 +10,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from gonano_b200 import _lib, streaming  # noqa: E402
+from gonano_b200._lib import GonanoError  # noqa: E402
 from test_gpu_streaming import DEVICE, Cache, evict64, evict_params, paged_params  # noqa: E402
 
 
@@ -161,3 +162,22 @@ def test_weights_that_share_a_part_are_refused(lib, shift):
     for apart in (0, 2 * 2 * 32 * 4, -2 * 2 * 32 * 4):
         p = paged_params(mass=2 ** 20, mass_out=2 ** 20 + apart)
         assert lib.gn_attention_paged(C.byref(p), C.byref(view), None, None, 0, None) == 1 and b"share a part" not in lib.gn_last_error()
+
+
+# ---------------------------------------------------------------- numbers
+
+@pytest.mark.parametrize("big", [2 ** 31, 2 ** 32, 2 ** 32 + 3, -2 ** 31 - 1, 2 ** 70])
+def test_numbers_beyond_32_bits_are_refused(big):
+    """2^32 sinks are not 0 sinks."""
+    x, table, lens = torch.zeros(1, 2, 4, 8), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for name in ("sinks", "window"):
+        with pytest.raises(GonanoError, match=f"{name}: {big} is outside"):
+            streaming.sink_attention_forward(x, x, x, **{"sinks": 0, "window": -1, name: big})
+        with pytest.raises(GonanoError, match=f"{name}: {big} is outside"):
+            streaming.sink_attention_backward(x, x, x, x, x, x[..., 0], **{"sinks": 0, "window": -1, name: big})
+    for name in ("max_query", "max_context", "sinks", "window"):
+        with pytest.raises(GonanoError, match=f"{name}: {big} is outside"):
+            streaming.paged_attention(x[0], x, x, table, lens, lens, **{"max_query": 1, name: big})
+    for name in ("budget", "sinks", "recent", "max_context"):
+        with pytest.raises(GonanoError, match=f"{name}: {big} is outside"):
+            streaming.evict_pages(x, x, x[0], table, lens, **{"budget": 1, name: big})
