@@ -23,10 +23,13 @@ def _refuse(message):
     raise GonanoError(message)
 
 
+_BEYOND = 2 ** 31
+
+
 def _counts(**values):
     # a structure's 32-bit fields would take the low bits of larger numbers
     for name, x in values.items():
-        if not -2 ** 31 <= x < 2 ** 31:
+        if not -_BEYOND <= x < _BEYOND:
             _refuse(f"{name}: {x} is outside 32 bits")
 
 
@@ -165,7 +168,8 @@ def paged_attention(q, key_pages, value_pages, page_table, query_starts, context
     Returns out (like q), lse [tokens, heads] and, when mass or mass_out is given, mass_out.  Entries behind the last row's tokens
     are left as they are (0 in tensors made here)."""
     lib = _lib.load()
-    _counts(max_query=max_query, max_context=0 if max_context is None else max_context, sinks=sinks, window=window)
+    if (max_query | sinks | (max_context or 0)) >> 31 or not -_BEYOND <= window < _BEYOND:   # a shortcut: the whole check takes 0.8 us
+        _counts(max_query=max_query, max_context=max_context or 0, sinks=sinks, window=window)
     device = _cuda("q", q, 3)
     tokens, heads, dim = q.shape
     pages, kv_heads, page_size, _ = _shaped("key_pages", key_pages, 4, "[pages, kv_heads, page_size, dim]")
@@ -207,7 +211,7 @@ def evict_pages(key_pages, value_pages, mass, page_table, context_lens, budget, 
     Returns kept (int32 [rows, kv_heads, budget], the indices the keys had, -1 behind them), the new lengths (int32 [rows]) and the
     kept keys' mass [rows, kv_heads, budget]."""
     lib = _lib.load()
-    _counts(budget=budget, sinks=sinks, recent=recent, max_context=0 if max_context is None else max_context)
+    _counts(budget=budget, sinks=sinks, recent=recent, max_context=max_context or 0)
     device = _cuda("key_pages", key_pages, 4)
     pages, kv_heads, page_size, dim = store = key_pages.shape
     rows, width = _shaped("page_table", page_table, 2, "[rows, width]")
