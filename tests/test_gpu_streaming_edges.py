@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 
 from gonano_b200 import _lib, streaming  # noqa: E402
 from gonano_b200._lib import GonanoError  # noqa: E402
-from test_gpu_streaming import DEVICE, Cache, evict64, evict_params, paged_params  # noqa: E402
+from test_gpu_streaming import DEVICE, FLOOR, PRODUCT, Cache, attend64, check_paged, close, evict64, evict_params, paged_params, score_bound, tensors, visible  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -181,3 +181,131 @@ def test_numbers_beyond_32_bits_are_refused(big):
     for name in ("budget", "sinks", "recent", "max_context"):
         with pytest.raises(GonanoError, match=f"{name}: {big} is outside"):
             streaming.evict_pages(x, x, x[0], table, lens, **{"budget": 1, name: big})
+
+
+# ---------------------------------------------------------------- values that are not finite, rows shorter than their tokens, missing pages
+
+CLEAN = 2.0 ** -16   # between two passes that differ in other queries' operands only: twice the rounding of each, as in test_gpu_streaming.py
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,heads,kv_heads", [(1, 4, 2), (12, 2, 2), (12, 1, 1), (40, 4, 2), (140, 2, 1)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("old", [False, True])
+def test_non_finite_in_the_cache(count, heads, kv_heads, value, which, old):
+    """A cached key or value (or a new token's) that is not finite reaches only the queries that see it, and the weights of the keys that those see."""
+    n, page, window, sinks, dim = 300, 16, 4, 2, 64
+    at = n - count - 3 if old else n - (count + 1) // 2
+    cache = Cache(2, kv_heads, dim, page, -(-n // page), seed=32)
+    cache.fill([n - count, n - count])
+    q = torch.randn(2 * count, heads, dim, generator=cache.gen, device=DEVICE)
+    new = [torch.randn(2 * count, kv_heads, dim, generator=cache.gen, device=DEVICE) for _ in range(2)]
+    got = []
+    for bad in (False, True):
+        k, v, nk, nv = cache.k.clone(), cache.v.clone(), *(x.clone() for x in new)
+        if bad:
+            if old:
+                (k if which == "k" else v)[int(cache.table[0, at // page]), :, at % page, 3] = value
+            else:
+                (nk if which == "k" else nv)[at - (n - count), :, 3] = value
+        got.append(streaming.paged_attention(q, k, v, cache.table, ints(0, count, 2 * count), ints(n, n), count, new_key=nk, new_value=nv, sinks=sinks, window=window,
+                                             scale=0.125, mass_out=torch.zeros(2, kv_heads, cache.table.shape[1] * page, device=DEVICE)))
+    pos, keys = torch.arange(n - count, n, device=DEVICE), torch.arange(n, device=DEVICE)
+    see = visible(pos, keys, window, sinks)
+    hit = torch.zeros(2 * count, dtype=torch.bool, device=DEVICE)
+    hit[:count] = see[:, at]
+    (clean, clean_lse, clean_mass), (out, lse, mass) = got
+    assert bool(hit.any())
+    if which == "v" or math.isnan(value):
+        assert not bool(out[hit][..., 3].isfinite().any())
+    close(out[~hit], clean[~hit].double(), CLEAN, "out")
+    close(lse[~hit], clean_lse[~hit].double(), CLEAN, "lse")
+    reached = see[hit[:count]].any(0)
+    close(mass[0, :, :n][:, ~reached], clean_mass[0, :, :n][:, ~reached].double(), CLEAN, "mass")
+    close(mass[1], clean_mass[1].double(), CLEAN, "mass of the other row")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,dim", [(1, 64), (4, 128)])
+def test_non_finite_in_a_training_pass(which, value, heads, dim):
+    """It reaches the gradients of the queries that see the key (or hold the value themselves) and of the keys that those see, no others."""
+    T, window, sinks, at = 700, 20, 2, 350
+    clean = tensors(1, heads, 1, T, dim, seed=33)
+    bad = [x.clone() for x in clean]
+    bad[("q", "k", "v", "dout").index(which)][0, 0, at, 3] = value
+    results = []
+    for q, k, v, dout in (clean, bad):
+        out, lse = streaming.sink_attention_forward(q, k, v, sinks, window, 0.1)
+        results.append((out, lse, *streaming.sink_attention_backward(q, k, v, out, dout, lse, sinks, window, 0.1)))
+    i = torch.arange(T, device=DEVICE)
+    see = visible(i, i, window, sinks)
+    queries = see[:, at] if which in ("k", "v") else i == at
+    keys = see[queries].any(0)
+    rows = torch.zeros(heads, T, dtype=torch.bool, device=DEVICE)
+    rows[:heads if which in ("k", "v") else 1] = queries
+    (out, lse, dq, dk, dv), (out2, lse2, dq2, dk2, dv2) = results
+    fine = ~rows if which != "dout" else torch.ones_like(rows)
+    # sums of up to 21 x heads terms of size 1 and the largest sinks' of T x heads: relative to the clean tensors' largest
+    for name, a, b, where in (("out", out[0], out2[0], fine), ("lse", lse[0], lse2[0], fine), ("dq", dq[0], dq2[0], ~rows), ("dk", dk[0, 0], dk2[0, 0], ~keys), ("dv", dv[0, 0], dv2[0, 0], ~keys)):
+        close(b[where], a[where].double(), CLEAN * max(1.0, float(a[a.isfinite()].abs().max())), name)
+    if math.isnan(value):
+        assert not bool(dq2[0][rows].isfinite().any())
+        if which in ("q", "dout"):
+            assert not bool(dk2[0, 0][keys].isfinite().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,lens,heads,kv_heads,dim,page,window,sinks", [
+    ([1, 0, 1, 1], [300, 20, 0, 5], 4, 2, 40, 8, 20, 4),
+    ([7, 9], [2000, 3], 2, 2, 128, 256, 30, 900),
+    ([5, 4, 8, 2], [3, 0, 8, 1], 2, 1, 64, 16, -1, 0),
+    ([16, 1], [9, 1], 1, 1, 128, 4, 3, 1),
+    ([40, 30, 12], [17, 0, 200], 4, 2, 64, 16, -1, 0),
+    ([300, 200], [150, 1999], 2, 1, 80, 24, 50, 700),
+])
+def test_rows_shorter_than_their_new_tokens(counts, lens, heads, kv_heads, dim, page, window, sinks):
+    """The first tokens then stand before the cache: they see nothing and are not written; sinks beyond most of a long row."""
+    rows, group, scale = len(counts), heads // kv_heads, 1 / math.sqrt(dim)
+    cache = Cache(rows, kv_heads, dim, page, max(1, -(-max(lens) // page)), seed=34)
+    cache.fill([max(0, n - c) for n, c in zip(lens, counts)])
+    tokens = sum(counts)
+    q = torch.randn(tokens, heads, dim, generator=cache.gen, device=DEVICE)
+    nk, nv = (torch.randn(tokens, kv_heads, dim, generator=cache.gen, device=DEVICE) for _ in range(2))
+    old = cache.k.clone()
+    starts = [sum(counts[:r]) for r in range(rows + 1)]
+    before = torch.rand(rows, kv_heads, cache.table.shape[1] * page, generator=cache.gen, device=DEVICE)
+    out, lse, mass = streaming.paged_attention(q, cache.k, cache.v, cache.table, ints(*starts), ints(*lens), max(counts), new_key=nk, new_value=nv, sinks=sinks,
+                                               window=window, scale=scale, mass=before)
+    written = torch.zeros(old.shape[:3], dtype=torch.bool, device=DEVICE)
+    for r, (c, n) in enumerate(zip(counts, lens)):
+        b, new = starts[r], min(c, n)
+        k64, v64 = cache.row(r, n)
+        assert torch.equal(k64[n - new:], nk[b + c - new:b + c].double()) and torch.equal(v64[n - new:], nv[b + c - new:b + c].double())
+        for j in range(n - new, n):
+            written[int(cache.table[r, j // page]), :, j % page] = True
+        see = visible(torch.arange(n - c, n, device=DEVICE), torch.arange(n, device=DEVICE), window, sinks)
+        for h in range(kv_heads):
+            mine = slice(h * group, (h + 1) * group)
+            qq = q[b:b + c, mine].double().transpose(0, 1)
+            o, l, w = attend64(qq, k64[:, h], v64[:, h], see, scale)
+            e = (2 * score_bound(qq, k64[:, h], scale) if qq.numel() else 0.0) + PRODUCT
+            close(out[b:b + c, mine].transpose(0, 1), o, e * torch.einsum("gnm,md->gnd", w, v64[:, h].abs()) + FLOOR * (n + 2) * float(v64.abs().max() if n else 0), f"out of row {r}")
+            close(lse[b:b + c, mine].transpose(0, 1), l, e * (1 + l.abs()), f"lse of row {r}")
+            want = w.sum((0, 1))
+            want[:max(0, n - c)] += before[r, h, :max(0, n - c)].double()
+            close(mass[r, h, :n], want, e * want + 2.0 ** -22 * want, f"mass of row {r}")
+            assert torch.equal(mass[r, :, n:], before[r, :, n:])
+    assert torch.equal(cache.k[~written].nan_to_num(9.0), old[~written].nan_to_num(9.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,group", [([1, 1], 2), ([6, 3], 2), ([6, 3], 1), ([90, 33], 2)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (60, 5)])
+def test_new_tokens_without_a_page(counts, group, window, sinks):
+    """A new token whose slot lies on a page that does not exist is neither written nor seen, its neighbours are."""
+    check_paged(counts, [400, 333], 2 * group, 2, 64, 32, window, sinks, hide=(0, 12))
+    check_paged(counts, [385, 353], 2 * group, 2, 64, 32, window, sinks, hide=(0, 12))
+    check_paged(counts, [400, 353], 2 * group, 2, 64, 32, window, sinks, hide=(1, 11))
