@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
   }
   if (norms && value) {
     top = warp_max(top);
-    if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &found[2] : norms + plane * 2, __float_as_uint(top));
+    if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &found[2] : norms + plane, __float_as_uint(top));
   }
   if (whole) {
     cluster_meet();
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(256) stream_pack_kernel(const __grid_constant_
       const uint32_t odd = cluster_largest(&found[1], ctas), norm = cluster_largest(&found[2], ctas);
       if (threadIdx.x == 0) {
         pk.amax[plane * 2 + value] = largest; pk.odd[plane * 2 + value] = odd;
-        if (norms && value) norms[plane * 2] = norm;
+        if (norms && value) norms[plane] = norm;
       }
     }
     cluster_meet();   // no CTA goes while its words are read
@@ -706,7 +706,7 @@ int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStre
     GN_CUDA(launch_cluster(stream_pack_kernel<CB, PAGED>, dim3(ctas, s.Hkv, 2 * s.rows), 256, ctas, st, s, pk, norms, vec, 1));
   } else {
     GN_CUDA(cudaMemsetAsync(pk.amax, 0, (int64_t)s.rows * s.Hkv * 4 * sizeof(uint32_t), st));   // amax and odd
-    if (norms) GN_CUDA(cudaMemsetAsync(norms, 0, (int64_t)s.rows * s.Hkv * 2 * sizeof(uint32_t), st));
+    if (norms) GN_CUDA(cudaMemsetAsync(norms, 0, (int64_t)s.rows * s.Hkv * sizeof(uint32_t), st));
     stream_amax_kernel<CB, PAGED><<<dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, vec);
     GN_LAUNCH_CHECK();
     GN_CUDA(launch_behind(!PAGED, stream_pack_kernel<CB, PAGED>, dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), dim3(256), 0, st, s, pk, norms, vec, 0));

@@ -85,8 +85,8 @@ inline cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int threa
   cfg.attrs = attr; cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
-// Packs keys and values; amax and the 2 * planes words of odd stand in one piece.  norms: null, or [plane][2]: [0] receives the bits of the
-// largest squared norm of a scaled value row.
+// Packs keys and values; amax and the 2 * planes words of odd stand in one piece.  norms: null, or [plane], which receives the bits
+// of the largest squared norm of a scaled value row.
 int stream_pack_keys(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStream_t stream);
 
 // tcgen05 forward of a call (streaming_tc.cu): the workspace it wants, and the launches.
@@ -213,6 +213,7 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 // The power of two that brings `amax` (bits of the largest finite magnitude) to [2^14, 2^15), and its inverse.
+__device__ __forceinline__ int scale_exponent(uint32_t amax) { return amax == 0 ? 0 : 14 + 127 - max((int)(amax >> 23), 27); }
 __device__ __forceinline__ void plane_scale(uint32_t amax, float& s, float& inverse) {
   const int e = max((int)(amax >> 23), 27) - 127;   // 0 and what is below 2^-100 scale like 2^-100
   s = amax == 0 ? 1.0f : __uint_as_float((uint32_t)(14 - e + 127) << 23);

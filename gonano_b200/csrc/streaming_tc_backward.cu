@@ -6,9 +6,14 @@
 // As in the forward pass the heads of a group are rows side by side (f = token * group + head), so the sum over a group's heads
 // that dK and dV want is part of the contraction, and the query rows that see key j are one run [j G, (j + window + 1) G).
 //
-// Operands are f16 pairs (streaming_tc.cuh).  dS has no bound known before the call; |dO.V - delta| <= 2 max|dO| max|V| (row norms,
-// found while packing) gives the power of two that keeps it in f16's range.  A query row with a non-finite component gets
-// NaN for its lse, which reaches exactly the gradients of what it sees.
+// Operands are f16 pairs (streaming_tc.cuh), and a pair's smallest step is absolute.  dO differs between tokens by orders of magnitude (and dS
+// by p more), so scales are as local as the sums allow.  Keys and values have one per plane.  Queries and dO have one per tile of 128 query rows: dK and dV
+// leave tensor memory after each such tile, and its factors go in where they are added.  Inside a tile a row whose dO is small moves what it has to
+// spare from one factor of a sum to the other, for i the row, 2^u_i <= 2^16 its distance from the tile's largest dO in norm, 2^h_i <= 2^6 in components:
+//   q_i 2^-u_i   against  dS_i 2^u_i    in dK (scores take 2^u_i back),         dO_i 2^h_i  against  P_i 2^-h_i  in dV.
+// dQ's rows are their own: dS_i has the scale that |dO.V - delta| <= 2 |dO_i| max|V| allows.  (With one scale per plane, dQ of rows whose dO was 1e-5
+// of the sequence's largest had a relative error of 5e-4.)  A query row with a non-finite component gets NaN for its lse, which reaches exactly the
+// gradients of what it sees.
 #include <algorithm>
 
 #include "streaming_tc.cuh"
@@ -21,18 +26,16 @@ struct BackwardTc {
   StreamRows s;
   PackedKeys pk;
   Packed q, g;                   // queries and dO, rows f
-  uint32_t* qamax;               // [plane][2]: q, dO
-  uint32_t* norms;               // [plane][2]: largest squared norm of a scaled row of V, dO
-  float* off; float* delta;      // [plane][q.rows]: 15 - lse in log2 units; delta times the scales of dO and V
+  uint32_t* norms;               // [plane]: largest squared norm of a scaled row of V
+  float* off; float* delta; float* score;   // [plane][q.rows]: 15 - h_i - lse in log2 units; delta times the scales of dO, V and dS; from products to log2 units
+  float4* own;                   // [plane][q.rows], for dQ: score, dS's scale, delta times that of dO, V and dS, from sums to dQ
+  float4* tile;                  // [plane][q_tiles], for dK and dV: (bits of) dS's scale over score's, from sums to dK, to dV
   gn_view out, dout, dq, dk, dv;
   const float* lse;
   int accumulate, vec_in, vec_dq, vec_dkv;
   int q_tiles, key_tiles, sink_tiles, parts_sink, parts, units;
   float* part;                   // [plane][unit][dV, dK][128][DP] of key tiles in several parts
 };
-
-constexpr int kAmaxRowsQ = 256;
-constexpr int kPackRowsQ = 64;   // 256 threads, 16 half warps
 
 // Half a warp per query row f: channels 4 i .. of the 64-channel blocks.
 template <int CB>
@@ -53,106 +56,110 @@ __device__ __forceinline__ void load_query_row(const StreamRows& s, const gn_vie
   }
 }
 
-// Largest finite magnitudes of q and dO.  Bound: HBM; 35 us for 2 x 69632 rows of 128 channels (143 MB, 4.1 TB/s).
-template <int CB>
-__global__ void __launch_bounds__(256) stream_query_amax_kernel(const __grid_constant__ BackwardTc p) {
-  pdl_trigger();
-  pdl_wait();
-  const StreamRows& s = p.s;
-  const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, f0 = blockIdx.x * kAmaxRowsQ;
-  const int nf = row_span<false>(s, r).q_len * s.G;
-  if (f0 >= nf) return;
-  uint32_t top[2] = {0, 0};
-#pragma unroll 4
-  for (int u = 0; u < kAmaxRowsQ / 16; ++u) {
-    const int f = f0 + u * 16 + half;
-    if (f >= nf) continue;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float x[4 * CB];
-      load_query_row<CB>(s, w ? p.dout : s.q, p.vec_in, r, hk, f, x);
-#pragma unroll
-      for (int e = 0; e < 4 * CB; ++e) if (finite_bits(x[e])) top[w] = max(top[w], __float_as_uint(x[e]) & 0x7fffffffu);
-    }
-  }
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const uint32_t x = __reduce_max_sync(0xffffffffu, top[w]);
-    if ((threadIdx.x & 31) == 0 && x) atomicMax(p.qamax + ((int64_t)r * s.Hkv + hk) * 2 + w, x);
-  }
-}
+// x 2^n, cut to what is finite.
+__device__ __forceinline__ float times_pow2(float x, int n) { return fminf(fmaxf(ldexpf(x, n), -3.4028234e38f), 3.4028234e38f); }
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }   // of x >= 0: below 2^(exponent + 1)
 
-// Packs q and dO and leaves each row's lse and delta in the form that the kernels use.  Half a warp per row, so that delta = dO.O is four
-// shuffles.  Bound: HBM, 12 D bytes a row in and 8 D out; 61 us for 2 x 69632 rows of 128 channels (215 MB read, 143 written: 5.9 TB/s).
+constexpr int kThreadsQ = 256, kTileQ = 128, kHalves = kThreadsQ / 16, kRowsEach = kTileQ / kHalves;   // half a warp per row, eight rows one after the other
+
+// Packs q and dO of a tile of query rows and leaves each row's lse, delta and scales in the form that the kernels use: one reading for magnitudes,
+// norms and delta = dO.O (four shuffles), a second, from the cache, for the halves.  Bound: HBM, 12 D bytes a row in and 8 D out; 77 us for 2 x 69632 rows of 128 channels (215 MB in, 143 out:
+// 4.6 TB/s).  Rows kept in registers between the two, one block of 512 threads an SM, took 99 us: nothing else reads while it waits and stores.
 template <int CB>
-__global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_constant__ BackwardTc p, int whole) {
+__global__ void __launch_bounds__(kThreadsQ, 4) stream_query_pack_kernel(const __grid_constant__ BackwardTc p) {
   pdl_trigger();
-  pdl_wait();
   const StreamRows& s = p.s;
-  const int hk = blockIdx.y, r = whole ? blockIdx.z : gridDim.z - 1 - blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-  const int ctas = gridDim.x, step = whole ? 16 * ctas : 16, f0 = whole ? blockIdx.x * 16 : (gridDim.x - 1 - blockIdx.x) * kPackRowsQ;
-  const int nf = row_span<false>(s, r).q_len * s.G, last = min(p.q.rows, (nf + 15) / 16 * 16 + 16);
-  if (!whole && f0 >= last) return;
+  const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15, f0 = blockIdx.x * kTileQ + half;
+  const int nf = row_span<false>(s, r).q_len * s.G, last = min(p.q.rows, (nf + 15) / 16 * 16);   // a tile is copied in 16s
+  if ((int)blockIdx.x * kTileQ >= last) { pdl_wait(); return; }
   const int64_t plane = (int64_t)r * s.Hkv + hk;
-  __shared__ uint32_t found[3];   // of this CTA's rows: largest magnitudes of q and dO, largest norm
-  uint32_t largest[2];
-  if (whole) {   // the plane is this cluster's: its largest magnitudes first
-    if (threadIdx.x < 3) found[threadIdx.x] = 0;
-    __syncthreads();
-    uint32_t top[2] = {0, 0};
-#pragma unroll 4
-    for (int f = f0 + half; f < nf; f += step)
+  __shared__ uint32_t found[3];   // largest magnitudes of q and dO, largest squared norm of a row of dO times its scale
+  if (threadIdx.x < 3) found[threadIdx.x] = 0;
+  __syncthreads();
+  // lane u of the half warp keeps what row u has: the bits of dO's largest magnitude, its squared norm over that's power of two, delta (not finite: the row is odd)
+  uint32_t top_q = 0, my_top = 0;
+  float my_sq = 0.0f, my_delta = 0.0f;
+#pragma unroll 2
+  for (int u = 0; u < kRowsEach; ++u) {
+    const int f = f0 + u * kHalves, at = min(f, nf - 1);   // loads without a condition: a row behind the last reads the last, and counts for nothing
+    float x[2][4 * CB], o[4 * CB], delta = 0.0f, sq = 0.0f;
+    load_query_row<CB>(s, s.q, p.vec_in, r, hk, at, x[0]);
+    load_query_row<CB>(s, p.dout, p.vec_in, r, hk, at, x[1]);
+    load_query_row<CB>(s, p.out, p.vec_in, r, hk, at, o);
+    uint32_t top = 0;
+    bool bad = false;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        float x[4 * CB];
-        load_query_row<CB>(s, w ? p.dout : s.q, p.vec_in, r, hk, f, x);
+    for (int e = 0; e < 4 * CB; ++e) {
 #pragma unroll
-        for (int e = 0; e < 4 * CB; ++e) if (finite_bits(x[e])) top[w] = max(top[w], __float_as_uint(x[e]) & 0x7fffffffu);
-      }
-#pragma unroll
-    for (int w = 0; w < 2; ++w) if (top[w]) atomicMax(&found[w], top[w]);
-    cluster_meet();
-    for (int w = 0; w < 2; ++w) largest[w] = cluster_largest(&found[w], ctas);
-  } else {
-    for (int w = 0; w < 2; ++w) largest[w] = p.qamax[plane * 2 + w];
-  }
-  float sc[2], inv, sv;
-  plane_scale(largest[0], sc[0], inv);
-  plane_scale(largest[1], sc[1], inv);
-  plane_scale(p.pk.amax[plane * 2 + 1], sv, inv);
-  float top = 0.0f;
-  const int end = whole ? last : min(last, f0 + kPackRowsQ);
-  // backwards: what was read last is in a cache
-#pragma unroll 1
-  for (int f16 = f0 + (end - f0 + step - 1) / step * step - step; f16 >= f0; f16 -= step) {
-    const int f = f16 + half;
-    float x[2][4 * CB], delta = 0.0f, sq = 0.0f;
-    bool odd = false;
-#pragma unroll
-    for (int e = 0; e < 4 * CB; ++e) x[0][e] = x[1][e] = 0.0f;
-    if (f < nf) {
-      load_query_row<CB>(s, s.q, p.vec_in, r, hk, f, x[0]);
-      load_query_row<CB>(s, p.dout, p.vec_in, r, hk, f, x[1]);
-      float o[4 * CB];
-      load_query_row<CB>(s, p.out, p.vec_in, r, hk, f, o);
-#pragma unroll
-      for (int e = 0; e < 4 * CB; ++e) delta = fmaf(x[1][e], o[e], delta);
+      for (int w = 0; w < 2; ++w) if (!finite_bits(x[w][e])) { bad = true; x[w][e] = 0.0f; }
+      if (f < nf) top_q = max(top_q, __float_as_uint(x[0][e]) & 0x7fffffffu);
+      top = max(top, __float_as_uint(x[1][e]) & 0x7fffffffu);
+      delta = fmaf(x[1][e], o[e], delta);
     }
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+    for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float by = ldexpf(1.0f, scale_exponent(top));
 #pragma unroll
-      for (int e = 0; e < 4 * CB; ++e) {
-        if (!finite_bits(x[w][e])) { odd = true; x[w][e] = 0.0f; }
-        x[w][e] *= sc[w];
-        if (w == 1) sq = fmaf(x[w][e], x[w][e], sq);
-      }
+    for (int e = 0; e < 4 * CB; ++e) sq = fmaf(x[1][e] * by, x[1][e] * by, sq);
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1) { delta += __shfl_xor_sync(0xffffffffu, delta, d); sq += __shfl_xor_sync(0xffffffffu, sq, d); }
-    top = fmaxf(top, sq);
-    odd = ((__ballot_sync(0xffffffffu, odd) >> (threadIdx.x & 16)) & 0xffffu) != 0;
+    if ((__ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 16)) & 0xffffu) delta = NAN;
+    if (l16 == u && f < nf) { my_top = top; my_sq = sq; my_delta = delta; }
+  }
+  const uint32_t top_g = __reduce_max_sync(0xffffffffu, my_top);
+  top_q = __reduce_max_sync(0xffffffffu, top_q);
+  if ((threadIdx.x & 31) == 0) { atomicMax(&found[0], top_q); atomicMax(&found[1], top_g); }
+  __syncthreads();
+  const int nq = scale_exponent(found[0]), ng = scale_exponent(found[1]);
+  my_sq = my_top == 0 ? 0.0f : ldexpf(my_sq, 2 * (ng - scale_exponent(my_top)));   // with the tile's scale
+  const uint32_t most_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(my_sq));
+  if ((threadIdx.x & 31) == 0) atomicMax(&found[2], most_bits);
+  __syncthreads();
+  const float most = __uint_as_float(found[2]);
+  pdl_wait();   // for what the packing of keys and values found
+  const int nk = scale_exponent(p.pk.amax[plane * 2]), nv = scale_exponent(p.pk.amax[plane * 2 + 1]);
+  const float norm_v = sqrtf(__uint_as_float(p.norms[plane]));
+  // scores below 2^-100 of the products are zeros, whatever their factor
+  const float unit = times_pow2(s.scale * kLog2e, -nq - nk), score = copysignf(fminf(fmaxf(fabsf(unit), 0x1p-100f), 0x1p100f), unit);
+  // |dO.V| and |delta| of scaled rows are at most their norms' product, below 2^37: with reach < 2^e twice that times 2^(14 - e) is below 2^15.
+  // The weights' 2^15 goes out at the same time.
+  auto above = [](float reach) { return reach > 0.0f ? exponent(reach) + 1 : 0; };
+  const int e_tile = above(sqrtf(most) * norm_v);
+  const float grad = ldexpf(1.0f, -1 - e_tile);
+  if (threadIdx.x == 0)
+    p.tile[plane * p.q_tiles + blockIdx.x] = make_float4(__uint_as_float(__float_as_uint(grad) - __float_as_uint(score)), times_pow2(s.scale, e_tile - 14 - ng - nv - nq),
+                                                         ldexpf(1.0f, -15 - ng), 0.0f);
+  const int my_up = min(max((exponent(most) - exponent(my_sq) - 1) >> 1, 0), 16);                                                  // the row's norm 2^up is at most the largest
+  const int my_lift = min(max(exponent(__uint_as_float(found[1])) - exponent(__uint_as_float(my_top)), 0), 6);   // and its components 2^lift
+  const int mine = f0 + l16 * kHalves;
+  if (l16 < kRowsEach && mine < last) {
+    const int64_t at = plane * p.q.rows + mine;
+    const int e = above(sqrtf(my_sq) * norm_v) + my_lift;
+    const bool odd = !isfinite(my_delta);
+    const float gain = ldexpf(1.0f, my_lift - 1 - e), scaled = odd ? 0.0f : times_pow2(my_delta, ng + my_lift + nv), t = ldexpf(score, my_up);
+    float off = 0.0f;
+    if (mine < nf) {
+      const int token = s.by_G.of(mine);
+      off = odd ? NAN : kWeightShift - (float)my_lift - p.lse[stat_offset<false>(s, r, hk * s.G + mine - token * s.G, token)] * kLog2e;
+    }
+    p.off[at] = off;
+    p.delta[at] = scaled * ldexpf(grad, my_up);
+    p.score[at] = t;
+    p.own[at] = make_float4(t, gain, scaled * gain, times_pow2(s.scale, e - 14 - ng - my_lift - nv - nk));
+  }
+#pragma unroll 2
+  for (int u = kRowsEach - 1; u >= 0; --u) {   // backwards: what was read last is in the cache
+    const int f = f0 + u * kHalves, from = (threadIdx.x & 16) + u;
+    const float by[2] = {ldexpf(1.0f, nq - __shfl_sync(0xffffffffu, my_up, from)), ldexpf(1.0f, ng + __shfl_sync(0xffffffffu, my_lift, from))};
+    float x[2][4 * CB];
+    load_query_row<CB>(s, s.q, p.vec_in, r, hk, min(f, nf - 1), x[0]);
+    load_query_row<CB>(s, p.dout, p.vec_in, r, hk, min(f, nf - 1), x[1]);
+    if (f >= last) continue;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const Packed& dst = w ? p.g : p.q;
+#pragma unroll
+      for (int e = 0; e < 4 * CB; ++e) x[w][e] = f < nf && finite_bits(x[w][e]) ? x[w][e] * by[w] : 0.0f;
 #pragma unroll
       for (int b = 0; b < CB; ++b) {
         uint2 hi, lo;
@@ -163,43 +170,7 @@ __global__ void __launch_bounds__(256) stream_query_pack_kernel(const __grid_con
         *reinterpret_cast<uint2*>(at + (int64_t)dst.rows * 128) = lo;
       }
     }
-    if (l16 == 0) {
-      float off = 0.0f;
-      if (f < nf) { const int t = s.by_G.of(f); off = odd ? NAN : kWeightShift - p.lse[stat_offset<false>(s, r, hk * s.G + f - t * s.G, t)] * kLog2e; }
-      p.off[plane * p.q.rows + f] = off;
-      p.delta[plane * p.q.rows + f] = delta * sc[1] * sv;
-    }
   }
-  top = warp_max(top);
-  if ((threadIdx.x & 31) == 0 && top > 0.0f) atomicMax(whole ? &found[2] : p.norms + plane * 2 + 1, __float_as_uint(top));
-  if (whole) {
-    cluster_meet();
-    if (blockIdx.x == 0 && threadIdx.x < 32) {
-      const uint32_t norm = cluster_largest(&found[2], ctas);
-      if (threadIdx.x == 0) { p.qamax[plane * 2] = largest[0]; p.qamax[plane * 2 + 1] = largest[1]; p.norms[plane * 2 + 1] = norm; }
-    }
-    cluster_meet();   // no CTA goes while its words are read
-  }
-}
-
-// Factors of a plane: scores to log2 units, dO.V - delta (scaled) into f16's range with the weights' 2^15 taken out, and the
-// results back.
-struct PlaneFactors { float score, grad, dq, dk, dv; };
-__device__ __forceinline__ PlaneFactors plane_factors(const BackwardTc& p, int64_t plane) {
-  float sq, iq, sg, ig, sk, ik, sv, iv;
-  plane_scale(p.qamax[plane * 2], sq, iq);
-  plane_scale(p.qamax[plane * 2 + 1], sg, ig);
-  plane_scale(p.pk.amax[plane * 2], sk, ik);
-  plane_scale(p.pk.amax[plane * 2 + 1], sv, iv);
-  // |dO.V| and |delta| of scaled rows are at most their norms' product, below 2^37; dS then stays below 2^15: reach < 2^e, twice that times 2^(14 - e)
-  const float reach = sqrtf(__uint_as_float(p.norms[plane * 2])) * sqrtf(__uint_as_float(p.norms[plane * 2 + 1]));
-  const int e = reach > 0.0f ? (int)(__float_as_uint(reach) >> 23) - 127 + 1 : 0;   // reach < 2^e
-  PlaneFactors f;
-  f.score = p.s.scale * kLog2e * iq * ik;
-  f.grad = exp2f((float)(14 - e) - kWeightShift);
-  const float back = exp2f((float)(e - 14)) * ig * iv * p.s.scale;
-  f.dq = back * ik; f.dk = back * iq; f.dv = exp2f(-kWeightShift) * ig;
-  return f;
 }
 
 constexpr int kThreadsB = 640;        // four warpgroups of softmax threads, one for the issuing and the copying warps
@@ -207,15 +178,15 @@ constexpr int kRegsSoftmax = 104, kRegsOther = 64;   // shares of the launch's 5
 constexpr int kFlush = 2;             // steps whose sums are left to the tensor core before they are rounded into registers: the error of
                                       // dk and dv grows with it (1: 6.9e-7 of the largest norm, 2: 8.4e-7, 4: 1.2e-6, 8: 2.0e-6)
 
-// Adds N (32 or 16) columns of an accumulator to registers.
+// Adds N (32 or 16) columns of an accumulator, times z, to registers.
 template <int N>
-__device__ __forceinline__ void add_columns(uint32_t taddr, float (&acc)[N]) {
+__device__ __forceinline__ void add_columns(uint32_t taddr, float (&acc)[N], float z) {
   uint32_t y[N];
   if constexpr (N == 32) tmem_ld32(taddr, y);
   else tmem_ld16(taddr, y);
   tmem_ld_wait();
 #pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] += __uint_as_float(y[e]);
+  for (int e = 0; e < N; ++e) acc[e] = fmaf(__uint_as_float(y[e]), z, acc[e]);
 }
 // 16 values of a row to f16 pairs in tensor memory: 8 columns of hi, 8 of lo.
 __device__ __forceinline__ void store_pairs(uint32_t taddr, const float (&x)[16]) {
@@ -272,7 +243,7 @@ __device__ __forceinline__ void write_row(float* dst, int ch, int D, float (&acc
 template <int DP>
 __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __grid_constant__ BackwardTc p) {
   constexpr int CB = DP / 64, QC = DP / 4;
-  constexpr uint32_t SLOT = CB * 16384u, OFF_KL = CB * 32768u, OFF_Q = OFF_KL + CB * 16384u, OFF_G = OFF_Q + 2 * SLOT, STATS = OFF_G + 2 * SLOT, BARS = STATS + 1024;
+  constexpr uint32_t SLOT = CB * 16384u, OFF_KL = CB * 32768u, OFF_Q = OFF_KL + CB * 16384u, OFF_G = OFF_Q + 2 * SLOT, STATS = OFF_G + 2 * SLOT, BARS = STATS + 1536, FACTORS = BARS + 208;
   constexpr uint32_t COL_S = 0, COL_DP = 128, COL_KH = 192, COL_DV = 256, COL_DK = 384;
   extern __shared__ uint8_t smem_raw[];
   const StreamRows& s = p.s;
@@ -284,8 +255,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   if (k0 >= len && parts > 1) { pdl_wait(); return; }   // the summing kernel does not look at padding
   const int nf = len * s.G;
   const int64_t t_end = (s.window < 0 || k0 < s.sinks) ? len : min((int64_t)len, (int64_t)k0 + 128 + s.window);
-  const int f_begin = (k0 * s.G) & ~7, f_end = (int)t_end * s.G;
-  const int steps = k0 < len ? (f_end - f_begin + 63) / 64 : 0, per = (steps + parts - 1) / parts;
+  const int f_begin = k0 * s.G, f_end = (int)t_end * s.G;
+  const int steps = k0 < len ? (f_end - f_begin + 63) / 64 : 0, per = (steps + parts * kFlush - 1) / (parts * kFlush) * kFlush;   // whole tiles of query rows
   const int i0 = part_i * per, n = max(0, min(steps, i0 + per) - i0);
   const int64_t plane = (int64_t)r * s.Hkv + hk;
 
@@ -303,6 +274,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   auto v_done = [&](int i) { return bars + 184u + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    static_assert(kFlush * 64 == kTileQ && FACTORS + 32 <= BARS + 256);   // a tile's sums have its factors
     mbar_init(v_full, 1); mbar_init(kh_full, 1); mbar_init(kh_ready, 512); mbar_init(dp_full, 1); mbar_init(ds_full, 512); mbar_init(acc_full, 1); mbar_init(acc_empty, 512); mbar_init(dp_free, 512);
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full(i), 1); mbar_init(g_full(i), 1); mbar_init(q_empty(i), 1); mbar_init(g_empty(i), 2); mbar_init(s_full(i), 1); mbar_init(p_full(i), 512);
@@ -341,11 +313,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         const int rows = rows16(i), f = row0(i), b2 = i & 1;
         if (i >= 2) ok = hold(q_empty(b2), ((i >> 1) - 1) & 1);
         if (!ok) break;
-        mbar_expect_tx(q_full(b2), (uint32_t)CB * 2u * rows * 128u + 2u * rows * 4u);
+        mbar_expect_tx(q_full(b2), (uint32_t)CB * 2u * rows * 128u + 3u * rows * 4u + 16u);
 #pragma unroll 1
         for (int b = 0; b < CB * 2; ++b) bulk_load(base + OFF_Q + b2 * SLOT + b * 8192, qp + ((int64_t)b * p.q.rows + f) * 128, rows * 128, q_full(b2));
-        bulk_load(base + STATS + b2 * 512, p.off + plane * p.q.rows + f, rows * 4, q_full(b2));
-        bulk_load(base + STATS + b2 * 512 + 256, p.delta + plane * p.q.rows + f, rows * 4, q_full(b2));
+        bulk_load(base + STATS + b2 * 768, p.off + plane * p.q.rows + f, rows * 4, q_full(b2));
+        bulk_load(base + STATS + b2 * 768 + 256, p.delta + plane * p.q.rows + f, rows * 4, q_full(b2));
+        bulk_load(base + STATS + b2 * 768 + 512, p.score + plane * p.q.rows + f, rows * 4, q_full(b2));
+        bulk_load(base + FACTORS + b2 * 16, p.tile + plane * p.q_tiles + (f >> 7), 16, q_full(b2));
         if (i == 1) ok = hold(kh_ready, 0);
         if (i >= 2) ok = hold(g_empty(b2), ((i >> 1) - 1) & 1);
         if (!ok) break;
@@ -442,7 +416,6 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     regs_inc<kRegsSoftmax>();
     const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane, key = k0 + row;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
-    const PlaneFactors fc = plane_factors(p, plane);
     bool ok = true;
     if (n > 0) {
       ok = hold_warp(kh_full, 0);
@@ -457,11 +430,12 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     float dv[QC], dk[QC];
 #pragma unroll
     for (int e = 0; e < QC; ++e) dv[e] = dk[e] = 0.0f;
+    float zk = 0.0f, zv = 0.0f;   // from sums to gradients, of the query rows whose sums stand in tensor memory
     auto flush = [&](int chunk) {
       ok = ok && hold_warp(acc_full, chunk & 1);
       tc_fence_after();
-      add_columns<QC>(lane_addr + COL_DV + part * QC, dv);
-      add_columns<QC>(lane_addr + COL_DK + part * QC, dk);
+      add_columns<QC>(lane_addr + COL_DV + part * QC, dv, zv);
+      add_columns<QC>(lane_addr + COL_DK + part * QC, dk, zk);
       tc_fence_before();
       mbar_arrive(acc_empty);
     };
@@ -469,7 +443,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
     for (int i = 0; i < n; ++i) {
       const int f0 = row0(i) + part * 16;
       const uint32_t see = (uint32_t)(bits_below(f_hi - f0) & ~bits_below(f_lo - f0));
-      const float4* off = reinterpret_cast<const float4*>(gen + STATS + (i & 1) * 512 + part * 64);
+      const float4* off = reinterpret_cast<const float4*>(gen + STATS + (i & 1) * 768 + part * 64);   // and delta 16 on, score 32 on
       float w[16];
       ok = ok && hold_warp(q_full(i & 1), (i >> 1) & 1) && hold_warp(s_full(i & 1), (i >> 1) & 1);
       tc_fence_after();
@@ -479,9 +453,9 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const float4 c = off[e >> 2];
-          w[e] = exp2_fast(fmaf(__uint_as_float(y[e]), fc.score, c.x)); w[e + 1] = exp2_fast(fmaf(__uint_as_float(y[e + 1]), fc.score, c.y));
-          w[e + 2] = exp2_fast(fmaf(__uint_as_float(y[e + 2]), fc.score, c.z)); w[e + 3] = exp2_fast(fmaf(__uint_as_float(y[e + 3]), fc.score, c.w));
+          const float4 c = off[e >> 2], t = off[32 + (e >> 2)];
+          w[e] = exp2_fast(fmaf(__uint_as_float(y[e]), t.x, c.x)); w[e + 1] = exp2_fast(fmaf(__uint_as_float(y[e + 1]), t.y, c.y));
+          w[e + 2] = exp2_fast(fmaf(__uint_as_float(y[e + 2]), t.z, c.z)); w[e + 3] = exp2_fast(fmaf(__uint_as_float(y[e + 3]), t.w, c.w));
         }
       }
       const bool whole = __all_sync(0xffffffffu, (see & 0xffffu) == 0xffffu);
@@ -493,6 +467,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       tc_fence_before();
       mbar_arrive(p_full(i & 1));
       if (i > 0 && i % kFlush == 0) flush(i / kFlush - 1);
+      const float4 fc = *reinterpret_cast<const float4*>(gen + FACTORS + (i & 1) * 16);
+      if (i % kFlush == 0) { zk = fc.y; zv = fc.z; }
       ok = ok && hold_warp(dp_full, i & 1);
       tc_fence_after();
       {
@@ -503,9 +479,10 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
         mbar_arrive(dp_free);
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const float4 c = off[16 + (e >> 2)];
-          w[e] *= (__uint_as_float(y[e]) - c.x) * fc.grad; w[e + 1] *= (__uint_as_float(y[e + 1]) - c.y) * fc.grad;
-          w[e + 2] *= (__uint_as_float(y[e + 2]) - c.z) * fc.grad; w[e + 3] *= (__uint_as_float(y[e + 3]) - c.w) * fc.grad;
+          const float4 c = off[16 + (e >> 2)], t = off[32 + (e >> 2)];
+          auto gain = [&](float score) { return __uint_as_float(__float_as_uint(score) + __float_as_uint(fc.x)); };   // dS's scale goes with the score's
+          w[e] *= fmaf(__uint_as_float(y[e]), gain(t.x), -c.x); w[e + 1] *= fmaf(__uint_as_float(y[e + 1]), gain(t.y), -c.y);
+          w[e + 2] *= fmaf(__uint_as_float(y[e + 2]), gain(t.z), -c.z); w[e + 3] *= fmaf(__uint_as_float(y[e + 3]), gain(t.w), -c.w);
         }
       }
       if (!whole) {
@@ -519,14 +496,14 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
       mbar_arrive(ds_full);
     }
     if (n > 0) flush((n - 1) / kFlush);
-    const float zk = ok ? fc.dk : NAN, zv = ok ? fc.dv : NAN;
+    const float z = ok ? 1.0f : NAN;
     if (parts > 1) {
       float* at = p.part + (((plane * p.units + x0) * 2) * 128 + row) * DP;
-      write_row<QC>(at, part * QC, DP, dv, zv, false, true);
-      write_row<QC>(at + 128 * DP, part * QC, DP, dk, zk, false, true);
+      write_row<QC>(at, part * QC, DP, dv, z, false, true);
+      write_row<QC>(at + 128 * DP, part * QC, DP, dk, z, false, true);
     } else {
-      write_row<QC>(key < s.seq ? p.dv.data + token_offset<false>(p.dv, r, hk, key) : nullptr, part * QC, s.D, dv, zv, p.accumulate, p.vec_dkv);
-      write_row<QC>(key < s.seq ? p.dk.data + token_offset<false>(p.dk, r, hk, key) : nullptr, part * QC, s.D, dk, zk, p.accumulate, p.vec_dkv);
+      write_row<QC>(key < s.seq ? p.dv.data + token_offset<false>(p.dv, r, hk, key) : nullptr, part * QC, s.D, dv, z, p.accumulate, p.vec_dkv);
+      write_row<QC>(key < s.seq ? p.dk.data + token_offset<false>(p.dk, r, hk, key) : nullptr, part * QC, s.D, dk, z, p.accumulate, p.vec_dkv);
     }
   }
   __syncwarp();
@@ -723,8 +700,8 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const bool live = f < nf;
     const int t = s.by_G.of(f), h = hk * s.G + f - t * s.G;
-    const PlaneFactors fc = plane_factors(p, plane);
-    float off = 0.0f, delta = 0.0f;
+    float off = 0.0f;
+    float4 fc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     bool ok = true;
     if (n > 0) {
       ok = hold_warp(hi_full, 0);
@@ -735,7 +712,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(hi_ready);
-      if (live) { off = p.off[plane * p.q.rows + f]; delta = p.delta[plane * p.q.rows + f]; }
+      if (live) { off = p.off[plane * p.q.rows + f]; fc = p.own[plane * p.q.rows + f]; }
     }
     const int s_end = live ? min(s.sinks, t + 1) : 0;
     const int lo_key = live ? (s.window < 0 ? 0 : max(0, t - s.window)) - runs.shift : 0, hi_key = live ? t - runs.shift : -1;
@@ -745,7 +722,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
     auto flush = [&](int chunk) {   // one step later, as above
       ok = ok && hold_warp(acc_full, chunk & 1);
       tc_fence_after();
-      add_columns<QC>(lane_addr + COL_DQ + part * QC, acc);
+      add_columns<QC>(lane_addr + COL_DQ + part * QC, acc, 1.0f);
       tc_fence_before();
       mbar_arrive(acc_empty);
     };
@@ -762,7 +739,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
         tmem_ld16(lane_addr + COL_DP + (j & 1) * 64 + part * 16, z);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = exp2_fast(fmaf(__uint_as_float(y[e]), fc.score, off)) * ((__uint_as_float(z[e]) - delta) * fc.grad);
+        for (int e = 0; e < 16; ++e) w[e] = exp2_fast(fmaf(__uint_as_float(y[e]), fc.x, off)) * fmaf(__uint_as_float(z[e]), fc.y, -fc.z);
       }
       if (!__all_sync(0xffffffffu, (see & 0xffffu) == 0xffffu)) {
 #pragma unroll
@@ -774,7 +751,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid
       if (j > 0 && j % kFlush == 0) flush(j / kFlush - 1);
     }
     if (n > 0) flush((n - 1) / kFlush);
-    write_row<QC>(f < s.seq * s.G ? p.dq.data + token_offset<false>(p.dq, r, h, t) : nullptr, part * QC, s.D, acc, ok ? fc.dq : NAN, p.accumulate, p.vec_dq);
+    write_row<QC>(f < s.seq * s.G ? p.dq.data + token_offset<false>(p.dq, r, h, t) : nullptr, part * QC, s.D, acc, ok ? fc.w : NAN, p.accumulate, p.vec_dq);
   }
   __syncwarp();
   tc_fence_before();
@@ -809,8 +786,7 @@ int64_t carve_backward(const StreamRows& s, void* workspace, BackwardTc* b) {
   PackedKeys& pk = b->pk;
   pk.amax = c.take<uint32_t>(planes * 4);
   pk.odd = reinterpret_cast<int*>(pk.amax + planes * 2);
-  b->qamax = c.take<uint32_t>(planes * 2);
-  b->norms = c.take<uint32_t>(planes * 2);
+  b->norms = c.take<uint32_t>(planes);
   pk.k.rows = pk.v.rows = packed_rows(s.seq);
   b->q.rows = b->g.rows = packed_rows((int64_t)s.seq * s.G);
   pk.k.data = c.take<uint8_t>(planes * pk.k.plane_bytes(CB));
@@ -821,6 +797,9 @@ int64_t carve_backward(const StreamRows& s, void* workspace, BackwardTc* b) {
   b->g.data = c.take<uint8_t>(planes * b->g.plane_bytes(CB));
   b->off = c.take<float>(planes * b->q.rows);
   b->delta = c.take<float>(planes * b->q.rows);
+  b->score = c.take<float>(planes * b->q.rows);
+  b->own = c.take<float4>(planes * b->q.rows);
+  b->tile = c.take<float4>(planes * b->q_tiles);
   if (b->parts > 1 || b->parts_sink > 1) b->part = c.take<float>(planes * b->units * 2 * 128 * DP);
   return c.used;
 }
@@ -828,23 +807,13 @@ int64_t carve_backward(const StreamRows& s, void* workspace, BackwardTc* b) {
 template <int DP>
 int backward_go(const StreamRows& s, BackwardTc& b, cudaStream_t st) {
   constexpr int CB = DP / 64;
-  constexpr int kSmemKv = CB * (32768 + 16384 + 4 * 16384) + 1024 + 256 + 1024, kSmemQ = CB * (2 * 16384 + 5 * 16384) + 256 + 1024;
+  constexpr int kSmemKv = CB * (32768 + 16384 + 4 * 16384) + 1536 + 256 + 1024, kSmemQ = CB * (2 * 16384 + 5 * 16384) + 256 + 1024;
   static std::atomic<uint64_t> ready_kv{0}, ready_q{0};
   constexpr int kShared = 512 * kRegsSoftmax + 128 * kRegsOther;
   GN_TRY(prepare_kernel(ready_kv, reinterpret_cast<const void*>(stream_tc_dkv_kernel<DP>), kSmemKv, kThreadsB, kShared));
   GN_TRY(prepare_kernel(ready_q, reinterpret_cast<const void*>(stream_tc_dq_kernel<DP>), kSmemQ, kThreadsB, kShared));
-  const int64_t planes = (int64_t)s.rows * s.Hkv;
   GN_TRY(stream_pack_keys(s, b.pk, b.norms, st));
-  const int ctas = pack_cluster(b.q.rows, planes);
-  if (ctas) {
-    GN_CUDA(launch_cluster(stream_query_pack_kernel<CB>, dim3(ctas, s.Hkv, s.rows), 256, ctas, st, b, 1));
-  } else {
-    GN_CUDA(cudaMemsetAsync(b.qamax, 0, planes * 2 * sizeof(uint32_t), st));
-    GN_CUDA(cudaMemset2DAsync(b.norms + 1, 2 * sizeof(uint32_t), 0, sizeof(uint32_t), planes, st));
-    stream_query_amax_kernel<CB><<<dim3(ceil_div(b.q.rows, kAmaxRowsQ), s.Hkv, s.rows), 256, 0, st>>>(b);
-    GN_LAUNCH_CHECK();
-    GN_CUDA(launch_pdl(stream_query_pack_kernel<CB>, dim3(ceil_div(b.q.rows, kPackRowsQ), s.Hkv, s.rows), dim3(256), 0, st, b, 0));
-  }
+  GN_CUDA(launch_pdl(stream_query_pack_kernel<CB>, dim3(b.q_tiles, s.Hkv, s.rows), dim3(kThreadsQ), 0, st, b));
   GN_CUDA(launch_pdl(stream_tc_dkv_kernel<DP>, dim3(b.units, s.Hkv, s.rows), dim3(kThreadsB), kSmemKv, st, b));
   GN_CUDA(launch_pdl(stream_tc_dq_kernel<DP>, dim3(b.q_tiles, s.Hkv, s.rows), dim3(kThreadsB), kSmemQ, st, b));
   if (b.parts > 1 || b.parts_sink > 1)

@@ -233,6 +233,11 @@ int gn_attention_windowed_backward(const float* query, const float* key, const f
  * gets zeros and lse = -inf.  A non-finite key or value reaches only the
  * queries that see it (whose channels may then all be NaN).
  *
+ * Precision: products of operands held to 22 bits, float32 sums; errors are about 1e-6 of a result's norm.  Beside that the calls that run on
+ * the tensor cores in f16 pairs (all but a few new tokens over pages) hold a key or value to 2^-39 of the largest of its sequence and kv
+ * head, a query's weight to 2^-40.  Queries and out_grad have scales of their own, row by row: gradients of tokens whose out_grad is 1e-7 of
+ * the others' are as precise as theirs.
+ *
  * Unlike the calls above these take device memory of the current device only, read and written through views with strides,
  * run asynchronously on `stream` (a cudaStream_t; NULL = the default stream), allocate nothing and may be captured into a
  * CUDA graph.  The scratch memory is the caller's: gn_*_workspace gives the bytes for a call with the same parameters

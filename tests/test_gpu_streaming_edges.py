@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 
 from gonano_b200 import _lib, streaming  # noqa: E402
 from gonano_b200._lib import GonanoError  # noqa: E402
-from test_gpu_streaming import DEVICE, FLOOR, PRODUCT, Cache, attend64, check_paged, close, evict64, evict_params, paged_params, score_bound, tensors, visible  # noqa: E402
+from test_gpu_streaming import DEVICE, FLOOR, PRODUCT, Cache, attend64, check_paged, close, evict64, evict_params, paged_params, score_bound, tensors, visible, window_reference  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -309,3 +309,55 @@ def test_new_tokens_without_a_page(counts, group, window, sinks):
     check_paged(counts, [400, 333], 2 * group, 2, 64, 32, window, sinks, hide=(0, 12))
     check_paged(counts, [385, 353], 2 * group, 2, 64, 32, window, sinks, hide=(0, 12))
     check_paged(counts, [400, 353], 2 * group, 2, 64, 32, window, sinks, hide=(1, 11))
+
+
+# ---------------------------------------------------------------- gradients of quiet tokens
+
+def norm_error(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ratio", [1.0, 1e-3, 1e-5, 1e-7])
+@pytest.mark.parametrize("heads,kv_heads,T,window,sinks,begin,end", [
+    (1, 1, 768, 512, 4, 300, 556),      # a stretch in the middle
+    (8, 1, 900, 512, 4, 301, 557),      # the heads of a group side by side
+    (6, 2, 900, 32, 0, 200, 456),       # keys that only quiet tokens see
+    (1, 1, 700, -1, 0, 444, 700),       # at the end, under a causal mask: again such keys
+    (2, 1, 2100, 100, 2, 1000, 1256),
+])
+def test_gradients_of_quiet_tokens(ratio, heads, kv_heads, T, window, sinks, begin, end):
+    """256 tokens whose dO is a small part of the others': their dQ, dK and dV are as precise as float32, relative to their own norm.
+
+    2e-6: operands of 22 bits, float32 sums and an exponential make 3e-7 to 9e-7 of the norm where all tokens are alike, in float32 too."""
+    q, k, v, dout = tensors(1, heads, kv_heads, T, 128, seed=40)
+    dout[:, :, begin:end] *= ratio
+    scale = 128 ** -0.5
+    out, lse = streaming.sink_attention_forward(q, k, v, sinks, window, scale)
+    got = dict(zip(("dq", "dk", "dv"), streaming.sink_attention_backward(q, k, v, out, dout, lse, sinks, window, scale)))
+    want, _ = window_reference(q, k, v, dout, None, window, sinks, scale)
+    errors = {n: (norm_error(g[:, :, begin:end], want[n][:, :, begin:end]), norm_error(g, want[n])) for n, g in got.items()}
+    print(ratio, errors)
+    assert all(e < 2e-6 for pair in errors.values() for e in pair), errors
+
+
+@pytest.mark.gpu
+def test_gradients_of_tokens_and_heads_of_every_size():
+    """dO of every token and head at its own power of ten, zeros and whole tiles of zeros among them: every row of dQ is precise."""
+    T, heads = 500, 4
+    q, k, v, dout = tensors(2, heads, 1, T, 64, seed=41)
+    gen = torch.Generator(device=DEVICE).manual_seed(42)
+    size = 10.0 ** torch.randint(-9, 1, (2, heads, T, 1), generator=gen, device=DEVICE).float()
+    size[:, :, ::17], size[0, :, 64:200], size[1, 2] = 0.0, 0.0, 1e-12
+    dout = dout * size
+    out, lse = streaming.sink_attention_forward(q, k, v, 3, 60, 0.125)
+    dq, dk, dv = streaming.sink_attention_backward(q, k, v, out, dout, lse, 3, 60, 0.125)
+    want, _ = window_reference(q, k, v, dout, None, 60, 3, 0.125)
+    assert bool((dq[(size == 0).expand_as(dq)] == 0).all())
+    rows = (dq.double() - want["dq"]).norm(dim=-1) / want["dq"].norm(dim=-1)
+    rows = rows[(size > 0).squeeze(-1) & (torch.arange(T, device=DEVICE) > 0)]   # the first token sees itself alone: its dQ is 0 but for roundings
+    # a component of dO is off by up to 2^-39 2^-6 of the tile's largest: 2^-45 10^12 / 1 = 0.03 for the quietest, 3e-5 at 10^-9 and below 1e-6 from 10^-7 on
+    quiet = size[(size > 0) & (torch.arange(T, device=DEVICE) > 0)[None, None, :, None]] < 2e-8
+    assert float(rows[~quiet].max()) < 1e-4 and float(rows[~quiet].median()) < 2e-6, (float(rows[~quiet].max()), float(rows[~quiet].median()))
+    for name, g in (("dk", dk), ("dv", dv)):
+        assert norm_error(g, want[name]) < 2e-6
