@@ -151,11 +151,12 @@ int gn_attention_sink_backward(const gn_sink_params* p, const gn_view* out, cons
   StreamRows s;
   GN_TRY(sink_rows(p, &s));
   if (!s.rows || !s.seq) return GN_OK;
-  GN_TRY(sink_pointers(p));
   GN_REQUIRE(out && out->data && out_grad && out_grad->data && lse && dq && dq->data && dk && dk->data && dv && dv->data, "attention_sink_backward: null tensor");
   GN_REQUIRE(strides_ok(*out) && strides_ok(*out_grad) && strides_ok(*dq) && strides_ok(*dk) && strides_ok(*dv), "attention_sink_backward: negative stride");
   GN_REQUIRE(apart(*dq, s.rows, s.Hq, s.seq, s.D) && apart(*dk, s.rows, s.Hkv, s.seq, s.D) && apart(*dv, s.rows, s.Hkv, s.seq, s.D),
              "attention_sink_backward: elements of a gradient share memory");
+  GN_REQUIRE(dq->data != dk->data && dq->data != dv->data && dk->data != dv->data, "attention_sink_backward: two gradients share memory");
+  GN_TRY(sink_pointers(p));
   const void* ptrs[] = {out->data, out_grad->data, lse, dq->data, dk->data, dv->data};
   for (const void* x : ptrs) GN_TRY(on_this_device(x, "attention_sink_backward"));
   GN_TRY(workspace_ok(workspace, workspace_bytes, sink_bytes(s, 1), "attention_sink_backward"));
@@ -188,6 +189,8 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
   GN_REQUIRE((p->new_key.data == nullptr) == (p->new_value.data == nullptr), "attention_paged: new_key and new_value come together");
   GN_REQUIRE(!p->mass || p->mass_out, "attention_paged: mass without mass_out");
   GN_REQUIRE(strides_ok(*out) && apart(*out, 1, s.Hq, s.tokens, s.D), "attention_paged: elements of out share memory");
+  // the queries are read a second time for the weights, new tokens by the blocks of other heads
+  GN_REQUIRE(out->data != p->query.data && out->data != p->new_key.data && out->data != p->new_value.data, "attention_paged: out shares memory with an input");
   const void* ptrs[] = {p->query.data, p->query_starts, p->context_lens, out->data, lse, p->key_pages, p->value_pages, p->page_table, p->new_key.data,
                         p->new_value.data, p->mass, p->mass_out};
   for (const void* x : ptrs) if (x) GN_TRY(on_this_device(x, "attention_paged"));

@@ -241,7 +241,8 @@ int gn_attention_windowed_backward(const float* query, const float* key, const f
  * Unlike the calls above these take device memory of the current device only, read and written through views with strides,
  * run asynchronously on `stream` (a cudaStream_t; NULL = the default stream), allocate nothing and may be captured into a
  * CUDA graph.  The scratch memory is the caller's: gn_*_workspace gives the bytes for a call with the same parameters
- * (of the pointers only whether mass_out is NULL counts), 16-byte aligned; calls that may overlap in time need workspaces of their own.  Data on the
+ * (of the pointers only whether mass_out is NULL counts), 16-byte aligned; calls that may overlap in time need workspaces of their own.
+ * Outputs share no memory with inputs or with one another, except where it is said (what starts at the same address is refused).  Data on the
  * device (lengths, tables) cannot be refused: what lies outside its range is cut off or skipped as stated, never read. */
 
 /* float32 tensor [batch, heads, tokens, head_dim] with strides in elements; the channels of a head are contiguous. */

@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 
 from gonano_b200 import _lib, streaming  # noqa: E402
 from gonano_b200._lib import GonanoError  # noqa: E402
-from test_gpu_streaming import DEVICE, FLOOR, PRODUCT, Cache, attend64, check_paged, close, evict64, evict_params, paged_params, score_bound, tensors, visible, window_reference  # noqa: E402
+from test_gpu_streaming import DEVICE, FLOOR, PRODUCT, Cache, attend64, check_paged, close, evict64, evict_params, paged_params, score_bound, sink_params, tensors, visible, window_reference  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -361,3 +361,40 @@ def test_gradients_of_tokens_and_heads_of_every_size():
     assert float(rows[~quiet].max()) < 1e-4 and float(rows[~quiet].median()) < 2e-6, (float(rows[~quiet].max()), float(rows[~quiet].median()))
     for name, g in (("dk", dk), ("dv", dv)):
         assert norm_error(g, want[name]) < 2e-6
+
+
+# ---------------------------------------------------------------- outputs in one place
+
+def test_outputs_that_share_memory_are_refused(lib):
+    """The same tensor as two gradients, or attention written over its own inputs."""
+    def view(at, heads):
+        return _lib.GnView(at, heads * 512, 512, 64)
+    p = sink_params(query=view(2 ** 20, 4), key=view(2 ** 21, 2), value=view(2 ** 22, 2))
+    at = [2 ** 23, 2 ** 24, 2 ** 25]
+    for i, j in ((0, 1), (0, 2), (1, 2)):
+        same = list(at)
+        same[j] = same[i]
+        grads = [view(same[0], 4), view(same[1], 2), view(same[2], 2)]
+        assert lib.gn_attention_sink_backward(C.byref(p), C.byref(view(2 ** 26, 4)), C.byref(view(2 ** 27, 4)), 2 ** 28, *map(C.byref, grads), 0, 2 ** 29, 2 ** 30, None) == 1
+        assert b"two gradients share memory" in lib.gn_last_error()
+    def token_view(at, heads):
+        return _lib.GnView(at, 0, 64, heads * 64)
+    fields = dict(query=token_view(2 ** 20, 4), new_key=token_view(2 ** 21, 2), new_value=token_view(2 ** 22, 2), key_pages=2 ** 23, value_pages=2 ** 24, page_table=2 ** 25,
+                  query_starts=2 ** 26, context_lens=2 ** 27)
+    for start in (2 ** 20, 2 ** 21, 2 ** 22):
+        assert lib.gn_attention_paged(C.byref(paged_params(**fields)), C.byref(token_view(start, 4)), 2 ** 28, 2 ** 29, 2 ** 20, None) == 1
+        assert b"out shares memory" in lib.gn_last_error()
+
+
+@pytest.mark.gpu
+def test_gradients_in_one_tensor_are_refused():
+    q, k, v, dout = tensors(1, 2, 2, 16, 32, seed=43)
+    out, lse = streaming.sink_attention_forward(q, k, v, 0, -1)
+    dq, dk = torch.zeros_like(q), torch.zeros_like(k)
+    with pytest.raises(GonanoError, match="two gradients"):
+        streaming.sink_attention_backward(q, k, v, out, dout, lse, 0, -1, dq=dq, dk=dk, dv=dk)
+    fused = torch.zeros(1, 16, 6, 32, device=DEVICE).transpose(1, 2)   # side by side in one buffer is fine
+    want = streaming.sink_attention_backward(q, k, v, out, dout, lse, 0, -1)
+    got = streaming.sink_attention_backward(q, k, v, out, dout, lse, 0, -1, dq=fused[:, :2], dk=fused[:, 2:4], dv=fused[:, 4:])
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
