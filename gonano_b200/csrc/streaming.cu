@@ -190,7 +190,7 @@ int gn_attention_paged(const gn_paged_params* p, const gn_view* out, float* lse,
   GN_REQUIRE(!p->mass || p->mass_out, "attention_paged: mass without mass_out");
   GN_REQUIRE(strides_ok(*out) && apart(*out, 1, s.Hq, s.tokens, s.D), "attention_paged: elements of out share memory");
   // the queries are read a second time for the weights, new tokens by the blocks of other heads
-  GN_REQUIRE(out->data != p->query.data && out->data != p->new_key.data && out->data != p->new_value.data, "attention_paged: out shares memory with an input");
+  GN_REQUIRE((out->data != p->query.data || !p->mass_out) && out->data != p->new_key.data && out->data != p->new_value.data, "attention_paged: out shares memory with an input");
   const void* ptrs[] = {p->query.data, p->query_starts, p->context_lens, out->data, lse, p->key_pages, p->value_pages, p->page_table, p->new_key.data,
                         p->new_value.data, p->mass, p->mass_out};
   for (const void* x : ptrs) if (x) GN_TRY(on_this_device(x, "attention_paged"));

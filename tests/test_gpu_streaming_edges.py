@@ -380,7 +380,7 @@ def test_outputs_that_share_memory_are_refused(lib):
     def token_view(at, heads):
         return _lib.GnView(at, 0, 64, heads * 64)
     fields = dict(query=token_view(2 ** 20, 4), new_key=token_view(2 ** 21, 2), new_value=token_view(2 ** 22, 2), key_pages=2 ** 23, value_pages=2 ** 24, page_table=2 ** 25,
-                  query_starts=2 ** 26, context_lens=2 ** 27)
+                  query_starts=2 ** 26, context_lens=2 ** 27, mass_out=2 ** 19)
     for start in (2 ** 20, 2 ** 21, 2 ** 22):
         assert lib.gn_attention_paged(C.byref(paged_params(**fields)), C.byref(token_view(start, 4)), 2 ** 28, 2 ** 29, 2 ** 20, None) == 1
         assert b"out shares memory" in lib.gn_last_error()
