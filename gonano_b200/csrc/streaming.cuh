@@ -73,12 +73,6 @@ template <bool PAGED>
 __device__ __forceinline__ int64_t stat_offset(const StreamRows& s, int r, int h, int token) {
   return PAGED ? (int64_t)token * s.Hq + h : ((int64_t)r * s.Hq + h) * s.seq + token;
 }
-// The keys that a query at position pos sees: [0, sink_end) and [begin, pos].
-struct Seen { int sink_end, begin; };
-__device__ __forceinline__ Seen seen_by(const StreamRows& s, int pos) {
-  const int begin = s.window < 0 ? 0 : max(0, pos - s.window);
-  return {min(s.sinks, begin), begin};
-}
 __device__ __forceinline__ bool sees(const StreamRows& s, int pos, int j) {
   return j <= pos && (s.window < 0 || pos - j <= s.window || j < s.sinks);
 }
