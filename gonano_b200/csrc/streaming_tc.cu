@@ -345,9 +345,12 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         for (int j = 0; j < n && ok; ++j, ++tile) {
           const int rows = j + 1 == n ? last16 : kRowsT, b = tile & 1;
           const uint32_t m = ring + (products ? min(2 * j + 2, 2 * n - 1) : j == 0 ? 0 : 2 * j - 1), slot = m % RING;
-          ok = hold_warp(full(slot), (m / RING) & 1);
-          if (products) ok = ok && hold_warp(p_full(b), (tile >> 1) & 1) && (tile == 0 || hold_warp(o_empty, (tile - 1) & 1));
-          else ok = ok && (tile < 2 || hold_warp(s_free(b), ((tile >> 1) - 1) & 1));
+          // The other warp's signal first, then the copy.  What stood in the slot before may have been the other warp's (K_j before V_j), which this
+          // one has not waited for; while it has not landed, the barrier is a phase behind and a wait for this copy's parity passes at once.  The
+          // weights of tile j mean that K_j landed, free scores that V_j-2 did, and nothing else stood there.
+          if (products) ok = hold_warp(p_full(b), (tile >> 1) & 1) && (tile == 0 || hold_warp(o_empty, (tile - 1) & 1));
+          else ok = tile < 2 || hold_warp(s_free(b), ((tile >> 1) - 1) & 1);
+          ok = ok && hold_warp(full(slot), (m / RING) & 1);
           if (!ok) break;
           tc_fence_after();
           if (products) {

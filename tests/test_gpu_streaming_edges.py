@@ -398,3 +398,62 @@ def test_gradients_in_one_tensor_are_refused():
     got = streaming.sink_attention_backward(q, k, v, out, dout, lse, 0, -1, dq=fused[:, :2], dk=fused[:, 2:4], dv=fused[:, 4:])
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- tiles that arrive late
+
+def cold_calls(call, times):
+    """Outputs of the first call, after others on caches filled with something else gave the same bits."""
+    room = torch.empty(256 << 20, dtype=torch.uint8, device=DEVICE)
+    first, differ = [x.clone() for x in call()], []
+    for i in range(times):
+        room.fill_(i & 127)
+        differ.append(torch.stack([(x != y).sum() for x, y in zip(call(), first)]))
+    assert int(torch.stack(differ).sum()) == 0
+    return first
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,chunk,context,heads,dim,page", [(44, 30, 5246, 4, 96, 256), (12, 64, 8704, 8, 128, 64), (90, 24, 3000, 4, 64, 64)])
+def test_long_rows_from_cold_caches(rows, chunk, context, heads, dim, page):
+    """Caches larger than L2: key tiles come from memory, more slowly than they are multiplied.  A tile used before it is there shows in the result
+    (and ended calls in a device error: its place was handed out twice)."""
+    host = torch.Generator().manual_seed(77)
+    counts = torch.randint(0, chunk + 1, (rows,), generator=host)
+    counts[0], counts[1] = chunk, 0
+    lens = torch.randint(context // 2, context + 1, (rows,), generator=host)
+    lens[0] = context
+    width = -(-context // page)
+    gen = torch.Generator(device=DEVICE).manual_seed(44)
+    k = torch.randn(rows * width, 1, page, dim, generator=gen, device=DEVICE)
+    v = torch.randn(rows * width, 1, page, dim, generator=gen, device=DEVICE)
+    table = torch.randperm(rows * width, generator=host).to(torch.int32).view(rows, width).to(DEVICE)
+    starts = [int(counts[:r].sum()) for r in range(rows + 1)]
+    q = torch.randn(starts[-1], heads, dim, generator=gen, device=DEVICE)
+    scale = dim ** -0.5
+    out, lse = cold_calls(lambda: streaming.paged_attention(q, k, v, table, ints(*starts), ints(*lens.tolist()), chunk, scale=scale), 60)
+    for r in (0, 2, rows - 1):
+        b, e, n = starts[r], starts[r + 1], int(lens[r])
+        k64, v64 = (x[table[r].long()].reshape(-1, dim)[:n].double() for x in (k, v))
+        see = visible(torch.arange(n - (e - b), n, device=DEVICE), torch.arange(n, device=DEVICE), -1, 0)
+        qq = q[b:e].double().transpose(0, 1)
+        o, l, w = attend64(qq, k64, v64, see, scale)
+        if e > b:
+            bound = 2 * score_bound(qq, k64, scale) + PRODUCT
+            close(out[b:e].transpose(0, 1), o, bound * torch.einsum("gnm,md->gnd", w, v64.abs()) + FLOOR * (n + 2) * float(v64.abs().max()), f"out of row {r}")
+            close(lse[b:e].transpose(0, 1), l, bound * (1 + l.abs()), f"lse of row {r}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hkv,T,D,window,sinks", [(64, 2, 2, 2000, 128, 256, 4), (200, 2, 2, 600, 128, 0, 0), (3, 4, 4, 6000, 128, -1, 0)])
+def test_prefill_from_cold_caches(B, H, Hkv, T, D, window, sinks):
+    """The same of padded batches: items of a few key tiles, of a single one, of many."""
+    q, k, v, _ = tensors(B, H, Hkv, T, D, seed=45)
+    out, lse = cold_calls(lambda: streaming.sink_attention_forward(q, k, v, sinks, window, 0.09), 40)
+    at = torch.arange(T, device=DEVICE)
+    for b in (0, B - 1):
+        qq, kk, vv = q[b, :1].double(), k[b, 0].double(), v[b, 0].double()
+        o, l, w = attend64(qq, kk, vv, visible(at, at, window, sinks), 0.09)
+        bound = 2 * score_bound(qq, kk, 0.09) + PRODUCT
+        close(out[b, :1], o, bound * torch.einsum("gnm,md->gnd", w, vv.abs()) + FLOOR * (T + 2) * float(vv.abs().max()), "out")
+        close(lse[b, :1], l, bound * (1 + l.abs()), "lse")
