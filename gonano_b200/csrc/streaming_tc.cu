@@ -345,12 +345,17 @@ __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __
         for (int j = 0; j < n && ok; ++j, ++tile) {
           const int rows = j + 1 == n ? last16 : kRowsT, b = tile & 1;
           const uint32_t m = ring + (products ? min(2 * j + 2, 2 * n - 1) : j == 0 ? 0 : 2 * j - 1), slot = m % RING;
-          // The other warp's signal first, then the copy.  What stood in the slot before may have been the other warp's (K_j before V_j), which this
-          // one has not waited for; while it has not landed, the barrier is a phase behind and a wait for this copy's parity passes at once.  The
-          // weights of tile j mean that K_j landed, free scores that V_j-2 did, and nothing else stood there.
-          if (products) ok = hold_warp(p_full(b), (tile >> 1) & 1) && (tile == 0 || hold_warp(o_empty, (tile - 1) & 1));
-          else ok = tile < 2 || hold_warp(s_free(b), ((tile >> 1) - 1) & 1);
-          ok = ok && hold_warp(full(slot), (m / RING) & 1);
+          // A copy is waited for only when what stood in its slot before is known to have landed: it may have been the other warp's (K_j before V_j), which
+          // this one does not wait for, and as long as it is on its way the parity of the phase before it lets a wait for this copy pass.  Scores of
+          // tile j mean that K_j landed.  Before K_j stood a tile of keys, or V of three tiles back or more, whose products freed the buffer that the last
+          // scores were issued into; only at an item's start it may be V of two tiles back, which the free buffer of these scores means.
+          if (products) {
+            ok = hold_warp(s_full(b), (tile >> 1) & 1) && hold_warp(full(slot), (m / RING) & 1) && hold_warp(p_full(b), (tile >> 1) & 1) &&
+                 (tile == 0 || hold_warp(o_empty, (tile - 1) & 1));
+          } else {
+            auto free_scores = [&]() { return tile < 2 || hold_warp(s_free(b), ((tile >> 1) - 1) & 1); };
+            ok = (j > 0 || free_scores()) && hold_warp(full(slot), (m / RING) & 1) && (j == 0 || free_scores());
+          }
           if (!ok) break;
           tc_fence_after();
           if (products) {
