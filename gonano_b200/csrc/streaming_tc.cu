@@ -717,7 +717,7 @@ int pack_go(const StreamRows& s, const PackedKeys& pk, uint32_t* norms, cudaStre
     if (norms) GN_CUDA(cudaMemsetAsync(norms, 0, (int64_t)s.rows * s.Hkv * sizeof(uint32_t), st));
     stream_amax_kernel<CB, PAGED><<<dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), 256, 0, st>>>(s, pk, vec);
     GN_LAUNCH_CHECK();
-    GN_CUDA(launch_behind(!PAGED, stream_pack_kernel<CB, PAGED>, dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), dim3(256), 0, st, s, pk, norms, vec, 0));
+    GN_CUDA(launch_pdl(stream_pack_kernel<CB, PAGED>, dim3(ceil_div(keys, kPackRows), s.Hkv, 2 * s.rows), dim3(256), 0, st, s, pk, norms, vec, 0));
   }
   return GN_OK;
 }
@@ -730,8 +730,8 @@ int forward_go(const StreamRows& s, const Plan& pl, ForwardTc& f, cudaStream_t s
   GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(stream_tc_forward_kernel<DP, PAGED>), kSmem, kThreads, 512 * kRegsSoftmax + 128 * (kRegsFetch + kRegsOther)));
   const int64_t items = pl.planes * pl.tiles * pl.splits;
   GN_REQUIRE(items < (1ll << 31) - 1024, "attention: %lld tiles of query rows", (long long)items);
-  GN_CUDA(launch_behind(!PAGED, stream_tc_forward_kernel<DP, PAGED>, dim3((unsigned)std::min<int64_t>(items, num_sms())), dim3(kThreads), kSmem, st, f));
-  if (pl.splits > 1) GN_CUDA(launch_behind(!PAGED, stream_tc_combine_kernel<DP, PAGED>, dim3(ceil_div(pl.max_q * s.G, 8), s.Hkv, s.rows), dim3(256), 0, st, f));
+  GN_CUDA(launch_pdl(stream_tc_forward_kernel<DP, PAGED>, dim3((unsigned)std::min<int64_t>(items, num_sms())), dim3(kThreads), kSmem, st, f));
+  if (pl.splits > 1) GN_CUDA(launch_pdl(stream_tc_combine_kernel<DP, PAGED>, dim3(ceil_div(pl.max_q * s.G, 8), s.Hkv, s.rows), dim3(256), 0, st, f));
   return GN_OK;
 }
 

@@ -64,17 +64,10 @@ static inline int pack_cluster(int64_t rows, int64_t planes) {
   while (ctas < 8 && (rows >= 128 * ctas || (rows > 16 * ctas && planes * ctas < 592))) ctas *= 2;
   return rows <= 1280 || planes * ctas >= 296 ? ctas : 0;
 }
-// A launch that may set up while the kernel before it on the stream still runs (launch_pdl), or, for paged calls, an ordinary one: a chunk call ended once
-// in a device error among many thousands whose cause was not found, and there nothing overlaps until it is (5 us a call, 10 with weights).
-// Each CTA of a kernel that may overlap waits for the one before to be complete before it ends (and before it reads what that one writes), so that
-// complete means complete with all before it.  A call's first kernel waits for the stream as usual; what the caller passed in is there from then on.
-template <typename... KArgs, typename... Args>
-inline cudaError_t launch_behind(bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
-  if (overlap) return launch_pdl(kernel, grid, block, smem, st, std::forward<Args>(args)...);
-  kernel<<<grid, block, smem, st>>>(static_cast<KArgs>(args)...);
-  return cudaGetLastError();
-}
-// Clusters are launched in the ordinary way for the same reason.
+// A call's first kernel waits for the stream as usual, and what the caller passed in is there from then on.  The others may set up while the one before
+// still runs (launch_pdl).  Each CTA of such a kernel waits for the one before to be complete before it ends (and before it reads what that one
+// writes), so that complete means complete with all before it.
+// Clusters pack the keys, a call's first kernel or the one behind the new tokens' copy: launched in the ordinary way.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, int ctas, cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg{};

@@ -24,6 +24,8 @@ struct MassTc {
 // Half a warp per query row f = token * group + head.
 template <int CB>
 __global__ void __launch_bounds__(256) stream_mass_pack_kernel(const __grid_constant__ MassTc p) {
+  pdl_trigger();
+  pdl_wait();
   const StreamRows& s = p.s;
   const int hk = blockIdx.y, r = blockIdx.z, half = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const RowSpan sp = row_span<true>(s, r);
@@ -87,7 +89,7 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
   const StreamRows& s = p.s;
   const int hk = blockIdx.y, r = blockIdx.z, k0 = blockIdx.x * 128;
   const RowSpan sp = row_span<true>(s, r);
-  if (k0 >= sp.ctx) return;
+  if (k0 >= sp.ctx) { pdl_wait(); return; }
   const int first = sp.ctx - sp.q_len, nf = sp.q_len * s.G;
   const int64_t plane = (int64_t)r * s.Hkv + hk;
   // the query rows that see a key of the tile
@@ -113,6 +115,7 @@ __global__ void __launch_bounds__(kThreadsM, 1) stream_tc_mass_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + BARS + 80);
+  pdl_wait();
   auto rows16 = [&](int i) { return min(128, (f_end - f_begin - i * 128 + 15) & ~15); };
 
   if (warp == 17) {
@@ -228,10 +231,8 @@ int go(const MassTc& m, cudaStream_t st) {
   const StreamRows& s = m.s;
   static std::atomic<uint64_t> ready{0};
   GN_TRY(prepare_kernel(ready, reinterpret_cast<const void*>(stream_tc_mass_kernel<DP>), kSmem, kThreadsM, 0));
-  stream_mass_pack_kernel<DP / 64><<<dim3(ceil_div(m.q.rows, 64), s.Hkv, s.rows), 256, 0, st>>>(m);
-  GN_LAUNCH_CHECK();
-  stream_tc_mass_kernel<DP><<<dim3(ceil_div(s.max_context, 128), s.Hkv, s.rows), kThreadsM, kSmem, st>>>(m);
-  GN_LAUNCH_CHECK();
+  GN_CUDA(launch_pdl(stream_mass_pack_kernel<DP / 64>, dim3(ceil_div(m.q.rows, 64), s.Hkv, s.rows), dim3(256), 0, st, m));
+  GN_CUDA(launch_pdl(stream_tc_mass_kernel<DP>, dim3(ceil_div(s.max_context, 128), s.Hkv, s.rows), dim3(kThreadsM), kSmem, st, m));
   return GN_OK;
 }
 
