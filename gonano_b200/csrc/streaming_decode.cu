@@ -367,7 +367,8 @@ __global__ void __launch_bounds__(256) stream_decode_mass_kernel(const __grid_co
 
 int queries_of(const StreamRows& s) { return s.max_query * s.G <= 8 ? 8 : 16; }
 int splits_of(const StreamRows& s) {
-  // about as many CTAs as the machine holds at once, and no range below two tiles a warp
+  // about two CTAs an SM, and no range below two tiles a warp.  (Eight queries leave room for three an SM: 32 rows of 8704 keys would take 76 us
+  // instead of 86, 100 of 1000 41 instead of 53, 512 of 384 the same 90.)
   int64_t seen = s.max_context;
   if (s.window >= 0) seen = std::min<int64_t>(seen, (int64_t)s.window + s.sinks + s.max_query);
   const int64_t ctas = (int64_t)s.rows * s.Hkv;

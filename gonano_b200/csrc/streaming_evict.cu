@@ -173,7 +173,8 @@ __device__ __forceinline__ void move_row(const Evict& e, int hk, int r, float* p
   }
 }
 
-// In place (new_table is page_table): a CTA per (32 channels, kv head, row x {key, value}).
+// In place (new_table is page_table): a CTA per (32 channels, kv head, row x {key, value}).  With the selection 53 us for 32 rows of up to 8704 keys to
+// 2048 (on other pages 49), 113 for 64 x 2 of 4096 to 2048 (104), 12 for 8 x 2 of 384 to 128 (14).
 __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ Evict e) {
   pdl_wait();
   __shared__ int64_t from[256], to[256];

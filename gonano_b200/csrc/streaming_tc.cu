@@ -244,8 +244,8 @@ __device__ __forceinline__ Item get_item(const ForwardTc& p, const int* before, 
 // long unrolled code once a tile wait for instructions most of the time.  Sixteen warps, because eight took 3360 cycles a tile
 // (read 530, meet 250, weights 1650, O 850) against the 48 instructions of 64 cycles of the tensor pipe, which is the bound of a tile.  Every wait is
 // bounded; a kernel whose wait ran out writes NaN.
-// 4 x 8192 tokens, 8 heads on one, window 512 and 64 sinks: 249 us, tensor pipe busy 47 %; a tile takes about 3400 cycles, and between two
-// items (O to memory in 6700, the next rows' bounds 2000) there are about three tiles' time.  Chunks over 8704 keys: 57 %.
+// 4 x 8192 tokens, 8 heads on one, window 512 and 64 sinks: 253 us, tensor pipe busy 46 %; a tile takes about 3400 cycles, and between two
+// items (O to memory in 6700, the next rows' bounds 2000) there are about three tiles' time.  Chunks over 8704 keys: 55 %.
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) stream_tc_forward_kernel(const __grid_constant__ ForwardTc p) {
   constexpr int CB = DP / 64, QC = DP / 4, RING = DP == 64 ? 6 : 3;

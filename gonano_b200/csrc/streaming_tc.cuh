@@ -55,10 +55,10 @@ int prepare_kernel(std::atomic<uint64_t>& ready, const void* kernel, int smem, i
 static inline bool vec_view(const gn_view& v, int D) {
   return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && D % 4 == 0 && v.batch_stride % 4 == 0 && v.head_stride % 4 == 0 && v.token_stride % 4 == 0;
 }
-// CTAs of a cluster that packs a plane of `rows` rows and finds its largest magnitude on the way (0: a launch of its own finds it).
+// CTAs of a cluster that packs a plane of `rows` keys and finds its largest magnitude on the way (0: a launch of its own finds it).
 // CTAs until the machine has four each, then until their rows (128 or fewer) still stand in a cache when they are read again.  Long planes of which
-// there are few leave SMs idle that way.  In one launch and in two: 128 planes of 383 keys and 1149 query rows 433 and 450 us (forward and
-// backward), 48 of 2000 keys 74 and 79, 8 of 63 keys and 126 rows 49 and 72; 4 of 8704 keys and 69632 rows 2095 and 830.
+// there are few leave SMs idle that way.  A forward call with one launch and with two: 16 planes of 63 keys 14.3 and 17.4 us, 256 of 383 119 and 120
+// (with the backward pass 401 and 409), 64 of 1024 94 and 91, 256 of 2000 334 and 329; 8 of 1280 63 and 57, 4 of 8704 233 and 145.
 static inline int pack_cluster(int64_t rows, int64_t planes) {
   int ctas = 1;
   while (ctas < 8 && (rows >= 128 * ctas || (rows > 16 * ctas && planes * ctas < 592))) ctas *= 2;

@@ -239,7 +239,7 @@ __device__ __forceinline__ void write_row(float* dst, int ch, int D, float (&acc
 // Tensor memory: S^T / P^T / dS^T 2 x 64 columns, dP^T 64, K hi 64, dV 128, dK 128.  Shared memory: V 64 KB, K lo 32 KB, 2 x (Q 32 KB + dO 32 KB).
 // Every kFlush steps dV and dK are added to float32 registers (32 + 32 a thread), one step later, between that step's weights and
 // its dS, while the products that end the chunk run.  Bound: tensor pipe, 48 instructions of 46 cycles and 24 of 64 a step.
-// 2 x 8704 tokens, 8 heads on one, window 512: 338 us, tensor pipe busy 46 %, 4500 to 5700 cycles a step.
+// 2 x 8704 tokens, 8 heads on one, window 512: 337 us, tensor pipe busy 47 %, 4500 to 5700 cycles a step.
 template <int DP>
 __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __grid_constant__ BackwardTc p) {
   constexpr int CB = DP / 64, QC = DP / 4;
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dkv_kernel(const __gri
   if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
-// Sums the parts of key tiles that were divided, in their order: DP / 4 threads per key row and tensor.  Bound: reading them; 25 us for 63 MB.
+// Sums the parts of key tiles that were divided, in their order: DP / 4 threads per key row and tensor.  Bound: reading them; 23 us for 63 MB.
 template <int DP>
 __global__ void __launch_bounds__(256) stream_tc_dkv_sum_kernel(const __grid_constant__ BackwardTc p) {
   pdl_wait();
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(256) stream_tc_dkv_sum_kernel(const __grid_con
 // It needs nothing from the dK and dV kernel, which stands before it on the stream: its CTAs fill the SMs that that one's last CTAs leave
 // free.  (They start once every CTA there has seen the packing kernels complete, and end after it has ended.)
 // Tensor memory: Q hi 64 columns, dO hi 64, S 2 x 64, dP 2 x 64, dQ 128.  Shared memory: Q lo, dO lo 32 KB each, 3 K and 2 V tiles of 32 KB.
-// Bound: tensor pipe; the call above 214 us, busy 39 %: 4050 cycles a step, and 5000 and 3500 for a CTA's start and end.
+// Bound: tensor pipe; the call above 205 us, busy 41 %: 4050 cycles a step, and 5000 and 3500 for a CTA's start and end.
 template <int DP>
 __global__ void __launch_bounds__(kThreadsB, 1) stream_tc_dq_kernel(const __grid_constant__ BackwardTc p) {
   constexpr int CB = DP / 64, QC = DP / 4;

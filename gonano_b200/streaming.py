@@ -7,6 +7,9 @@ j <= i and (window < 0 or i - j <= window or j < sinks).
 
 The calls run on torch's current stream of the tensors' device, do not synchronise, and may be captured into a CUDA graph.
 Tensors are float32 (lengths and tables int32) on one CUDA device; the channels of a head have to be contiguous.
+
+Nothing is recorded for autograd: outputs are tensors without a graph, also where inputs require gradients, which come from
+``sink_attention_backward``.  Outputs may not share memory with inputs or with one another, except ``mass_out`` with ``mass``.
 """
 from __future__ import annotations
 
@@ -209,7 +212,7 @@ def evict_pages(key_pages, value_pages, mass, page_table, context_lens, budget, 
     left whole; ``page_table[:, :w].contiguous()`` compacts in place too.  Rows of at most ``budget`` keys are kept whole.
 
     Returns kept (int32 [rows, kv_heads, budget], the indices the keys had, -1 behind them), the new lengths (int32 [rows]) and the
-    kept keys' mass [rows, kv_heads, budget]."""
+    kept keys' mass [rows, kv_heads, budget] (to gather further, the front of a tensor as wide as the new pages)."""
     lib = _lib.load()
     _counts(budget=budget, sinks=sinks, recent=recent, max_context=max_context or 0)
     device = _cuda("key_pages", key_pages, 4)

@@ -243,7 +243,8 @@ int gn_attention_windowed_backward(const float* query, const float* key, const f
  * CUDA graph.  The scratch memory is the caller's: gn_*_workspace gives the bytes for a call with the same parameters
  * (of the pointers only whether mass_out is NULL counts), 16-byte aligned; calls that may overlap in time need workspaces of their own.
  * Outputs share no memory with inputs or with one another, except where it is said (what starts at the same address is refused).  Data on the
- * device (lengths, tables) cannot be refused: what lies outside its range is cut off or skipped as stated, never read. */
+ * device (lengths, tables) cannot be refused: what lies outside its range is cut off or skipped as stated, never read.  Every wait inside the
+ * kernels is bounded; one whose wait ran out (about a second at most) writes NaN, after the call has returned GN_OK. */
 
 /* float32 tensor [batch, heads, tokens, head_dim] with strides in elements; the channels of a head are contiguous. */
 typedef struct gn_view {
