@@ -11,7 +11,7 @@ namespace {
 
 struct Evict {
   gn_evict_params p;
-  int32_t* kept; int32_t* new_lens; float* mass_out;
+  int32_t* kept; int32_t* new_lens; float* mass_out;   // new_lens null: written at the end, over the lengths that all kernels read
   int vec;
 };
 // Weight as an integer that orders like it: equal values (both zeros too) alike, NaN below everything.
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
     at += __popc(taken);
   }
   for (int i = keep + tid; i < p.budget; i += kSelect) { kept[i] = -1; if (e.mass_out) e.mass_out[head * p.budget + i] = 0.0f; }
-  if (hk == 0 && tid == 0) e.new_lens[r] = keep;
+  if (hk == 0 && tid == 0 && e.new_lens) e.new_lens[r] = keep;
 }
 
 // A row's kept keys to slots that may be its own: the slots are filled in ascending order, KEYS at a time, every read of a group before its
@@ -231,10 +231,16 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(const __grid_constant__
   }
 }
 
+__global__ void __launch_bounds__(256) evict_lens_kernel(const __grid_constant__ Evict e, int32_t* new_lens) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r < e.p.rows) new_lens[r] = min(evict_len(e.p, r), e.p.budget);
+}
+
 }  // namespace
 
 int stream_evict(const gn_evict_params& p, int32_t* kept, int32_t* new_lens, float* mass_out, cudaStream_t st) {
-  Evict e{p, kept, new_lens, mass_out, 0};
+  const bool over = new_lens == p.context_lens;
+  Evict e{p, kept, over ? nullptr : new_lens, mass_out, 0};
   e.vec = p.head_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.key_pages) | reinterpret_cast<uintptr_t>(p.value_pages)) & 15) == 0;
   const int cached = p.max_context <= kCached;
   static std::atomic<uint64_t> ready{0};
@@ -242,12 +248,18 @@ int stream_evict(const gn_evict_params& p, int32_t* kept, int32_t* new_lens, flo
   evict_select_kernel<<<dim3(p.n_kv_head, p.rows), kSelect, cached ? p.max_context * sizeof(uint32_t) : 0, st>>>(e, cached);
   GN_LAUNCH_CHECK();
   const int most = std::min(p.budget, p.max_context);
-  if (most == 0) return GN_OK;
-  if (p.new_table == p.page_table) GN_CUDA(launch_pdl(evict_move_kernel, dim3(ceil_div(p.head_dim, 32), p.n_kv_head, 2 * p.rows), dim3(256), 0, st, e));
-  else {
+  if (most == 0) {
+    // nothing moves
+  } else if (p.new_table == p.page_table) {
+    GN_CUDA(launch_pdl(evict_move_kernel, dim3(ceil_div(p.head_dim, 32), p.n_kv_head, 2 * p.rows), dim3(256), 0, st, e));
+  } else {
     int lanes = 1;
     while (lanes < 32 && lanes * 4 < p.head_dim) lanes *= 2;
     GN_CUDA(launch_pdl(evict_copy_kernel, dim3(ceil_div(most, 64), p.n_kv_head, 2 * p.rows), dim3(256), 0, st, e, lanes));
+  }
+  if (over) {
+    evict_lens_kernel<<<ceil_div(p.rows, 256), 256, 0, st>>>(e, new_lens);
+    GN_LAUNCH_CHECK();
   }
   return GN_OK;
 }

@@ -307,7 +307,8 @@ typedef struct gn_evict_params {
 } gn_evict_params;
 
 /* kept [rows, n_kv_head, budget]: the indices that the kept keys had (-1 behind them); new_lens [rows]; mass_out [rows, n_kv_head,
- * budget] (0 behind them), nullable.  None of the three may share memory with an input or with another (new_lens is not context_lens). */
+ * budget] (0 behind them), nullable.  None of the three may share memory with an input or with another, except that
+ * new_lens may be context_lens. */
 int gn_cache_evict(const gn_evict_params* p, int32_t* kept, int32_t* new_lens, float* mass_out, void* stream);
 
 /* ===================================================================== *

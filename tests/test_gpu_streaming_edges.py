@@ -69,7 +69,7 @@ EVICT_BUFFERS = dict(key_pages=2 ** 20, value_pages=2 ** 21, mass=2 ** 22, page_
 EVICT_OUTPUTS = [2 ** 26, 2 ** 27, 2 ** 28]   # kept, new_lens, mass_out
 
 
-@pytest.mark.parametrize("which,at", [(1, 2 ** 25), (1, 2 ** 25 + 4), (2, 2 ** 22), (2, 2 ** 22 + 64), (0, 2 ** 23), (1, 2 ** 24 + 12), (0, 2 ** 27), (2, 2 ** 26 - 4), (0, 2 ** 20 + 40),
+@pytest.mark.parametrize("which,at", [(1, 2 ** 25 - 4), (1, 2 ** 25 + 4), (2, 2 ** 22), (2, 2 ** 22 + 64), (0, 2 ** 23), (1, 2 ** 24 + 12), (0, 2 ** 27), (2, 2 ** 26 - 4), (0, 2 ** 20 + 40),
                                       (2, 2 ** 21)])
 def test_evict_refuses_shared_memory(lib, which, at):
     """Lengths written over the lengths that are read, weights over the weights, and so on: the answer would go by which block came first."""
@@ -92,6 +92,34 @@ def test_evict_buffers_side_by_side(lib):
                      context_lens=room.data_ptr())
     assert lib.gn_cache_evict(C.byref(p), room[2 * rows:].data_ptr(), room[rows:].data_ptr(), None, torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(room[rows:2 * rows], want[1]) and torch.equal(room[2 * rows:].view_as(want[0]), want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("budget", [0, 16, 100, 400])
+def test_evict_with_the_lengths_in_one_place(lib, in_place, budget):
+    """new_lens over context_lens, as a cache that is compacted in place keeps them: what two arrays give, for every head."""
+    lens, heads, page, width = [300, 90, 16, 0, 299], 6, 16, 20
+    extra = max(1, -(-budget // page))
+    cache = Cache(len(lens), heads, 32, page, width + extra, seed=46)
+    cache.fill(lens)
+    table, other = cache.table[:, :width].contiguous(), cache.table[:, width:].contiguous()
+    target = table if in_place else other
+    if in_place and budget > width * page:
+        budget = width * page
+    mass = torch.rand(len(lens), heads, width * page, generator=cache.gen, device=DEVICE)
+    sinks, recent = min(2, budget), min(7, max(0, budget - 2))
+    k, v = cache.k.clone(), cache.v.clone()
+    want = streaming.evict_pages(k, v, mass, table, ints(*lens), budget, sinks, recent, new_table=target)
+    for _ in range(5):
+        k2, v2, here = cache.k.clone(), cache.v.clone(), ints(*lens)
+        kept = torch.full((len(lens), heads, max(1, budget)), -9, dtype=torch.int32, device=DEVICE)
+        p = evict_params(rows=len(lens), n_kv_head=heads, head_dim=32, page_size=page, pages=k2.shape[0], table_width=width, new_width=target.shape[1], mass_stride=width * page,
+                         max_context=width * page, budget=budget, sinks=sinks, recent=recent, key_pages=k2.data_ptr(), value_pages=v2.data_ptr(), mass=mass.data_ptr(),
+                         page_table=table.data_ptr(), new_table=target.data_ptr(), context_lens=here.data_ptr())
+        assert lib.gn_cache_evict(C.byref(p), kept.data_ptr(), here.data_ptr(), None, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(here, want[1]) and (budget == 0 or torch.equal(kept, want[0]))
+        assert torch.equal(k2.nan_to_num(9.0), k.nan_to_num(9.0)) and torch.equal(v2.nan_to_num(9.0), v.nan_to_num(9.0))
 
 
 @pytest.mark.gpu
