@@ -428,6 +428,24 @@ def test_gradients_in_one_tensor_are_refused():
         assert torch.equal(a, b)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("a,b,c", [(0, 0, 40), (0, 0, -60), (35, 0, 0), (-35, 0, 0), (0, 50, -30), (0, -50, 60), (20, 30, 10)])
+@pytest.mark.parametrize("heads,kv_heads,T,D", [(4, 2, 300, 64), (6, 1, 200, 128)])
+def test_powers_of_two_go_through(a, b, c, heads, kv_heads, T, D):
+    """Queries times 2^a and keys over 2^a, values times 2^b, dO times 2^c: the same bits, times the powers that the formulas give."""
+    q, k, v, dout = tensors(2, heads, kv_heads, T, D, seed=47)
+    dout[:, :, 50:90] *= 1e-4
+    mask = dict(sinks=3, window=40, scale=0.11)
+
+    def run(q, k, v, dout):
+        out, lse = streaming.sink_attention_forward(q, k, v, **mask)
+        return out, lse, *streaming.sink_attention_backward(q, k, v, out, dout, lse, **mask)
+    plain = run(q, k, v, dout)
+    moved = run(q * 2.0 ** a, k * 2.0 ** -a, v * 2.0 ** b, dout * 2.0 ** c)
+    for name, x, y, power in zip(("out", "lse", "dq", "dk", "dv"), plain, moved, (b, 0, b + c - a, b + c + a, c)):
+        assert torch.equal(y, x * 2.0 ** power), name
+
+
 # ---------------------------------------------------------------- tiles that arrive late
 
 def cold_calls(call, times):
