@@ -2,8 +2,8 @@
 //
 // Precision.  kind::f16 multiplies at twice the rate of kind::tf32 with the same 11-bit significand, so a float32 operand x is
 // held as two halves of s x, s a power of two: hi = f16(s x), lo = f16(s x - hi).  Together they keep 22 bits, as the tf32 pair
-// does, in half the bytes.  What f16 lacks is range, hence s: the largest finite |x| of a plane (a sequence and key head) lands
-// in [2^14, 2^15), which leaves every x an absolute error of at most 2^-40 of that largest one (f16's smallest step is 2^-24) or
+// does, in half the bytes.  What f16 lacks is range, hence s: the largest finite |x| of a plane (a sequence and key head; queries
+// and dO have finer scales) lands in [2^14, 2^15), which leaves every x an absolute error of at most 2^-40 of that largest one (f16's smallest step is 2^-24) or
 // 2^-22 of x, whichever is more.  A product is hi*lo + lo*hi + hi*hi in float32 (lo*lo is below 2^-22), the small terms first: the tensor core
 // cuts each partial sum off instead of rounding it, and a cut of the small terms costs 2^-11 of one of the large ones.
 //
